@@ -15,6 +15,7 @@ from halo_b200.refetcher import HALORefetcher
 from halo_b200.kv_cache import HALOCache
 from halo_b200.kv_cache_chunked import HALOCacheChunked
 from halo_b200.memory_tier import MemoryTier, TieredStorage
+from halo_b200.paged_cache import PagedKVCache
 from halo_b200.preforward_peel import install_preforward_peel
 
 __all__ = [
@@ -28,6 +29,7 @@ __all__ = [
     "HALOCacheChunked",
     "MemoryTier",
     "TieredStorage",
+    "PagedKVCache",
     "install_preforward_peel",
 ]
 

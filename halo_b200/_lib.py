@@ -93,6 +93,30 @@ class PrefillOut(ctypes.Structure):
                 ("o", ctypes.c_void_p)]
 
 
+class PagePool(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_stride_p", ctypes.c_int64), ("k_stride_h", ctypes.c_int64),
+                ("k_stride_t", ctypes.c_int64),
+                ("v_stride_p", ctypes.c_int64), ("v_stride_h", ctypes.c_int64),
+                ("v_stride_t", ctypes.c_int64),
+                ("n_pages", ctypes.c_int32), ("H_kv", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("D", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+class TreeProblem(ctypes.Structure):
+    _fields_ = [("R", ctypes.c_int32), ("T", ctypes.c_int32), ("H", ctypes.c_int32),
+                ("max_nodes", ctypes.c_int32), ("max_blocks", ctypes.c_int32),
+                ("scale", ctypes.c_float),
+                ("q", ctypes.c_void_p), ("q_stride_t", ctypes.c_int64),
+                ("q_stride_h", ctypes.c_int64),
+                ("block_tables", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("context_lens", ctypes.c_void_p), ("cu_nodes", ctypes.c_void_p),
+                ("mask", ctypes.c_void_p), ("mask_stride", ctypes.c_int64),
+                ("out", ctypes.c_void_p), ("out_stride_t", ctypes.c_int64),
+                ("out_stride_h", ctypes.c_int64), ("out_dtype", ctypes.c_int32),
+                ("lse", ctypes.c_void_p)]
+
+
 # name -> (restype, argtypes); must match include/halo_b200.h
 SIGNATURES = {
     "halo_decode_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(DecodeProblem),
@@ -158,6 +182,28 @@ SIGNATURES = {
                                               ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
                                               ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p,
                                               ctypes.c_void_p]),
+    "halo_update_block_tables": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32,
+                                                  ctypes.c_int32, ctypes.c_void_p,
+                                                  ctypes.c_void_p, ctypes.c_void_p,
+                                                  ctypes.c_int32, ctypes.c_void_p,
+                                                  ctypes.c_void_p, ctypes.c_int32,
+                                                  ctypes.c_int32, ctypes.c_void_p,
+                                                  ctypes.c_void_p, ctypes.c_void_p,
+                                                  ctypes.c_void_p, ctypes.c_void_p]),
+    "halo_write_kv_pages": (ctypes.c_int32, [ctypes.POINTER(PagePool), ctypes.c_void_p,
+                                             ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
+                                             ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
+                                             ctypes.c_void_p, ctypes.c_void_p]),
+    "halo_tree_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(PagePool),
+                                                   ctypes.POINTER(TreeProblem)]),
+    "halo_tree_attention": (ctypes.c_int32, [ctypes.POINTER(PagePool),
+                                             ctypes.POINTER(TreeProblem), ctypes.c_void_p,
+                                             ctypes.c_int64, ctypes.c_void_p]),
+    "halo_commit_tree_path": (ctypes.c_int32, [ctypes.POINTER(PagePool), ctypes.c_void_p,
+                                               ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+                                               ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                               ctypes.c_int32, ctypes.c_void_p,
+                                               ctypes.c_void_p]),
     "halo_copy2d_async": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
                                            ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                            ctypes.c_void_p]),

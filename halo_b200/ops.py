@@ -512,3 +512,202 @@ def lse_merge(m_parts: torch.Tensor, l_parts: Optional[torch.Tensor], o_parts: t
                                     L.stream_handle(dev))
     L.check(rc, "halo_lse_merge")
     return out, lse
+
+
+# ------------------------------------------------------------ paged cache
+
+def _require_int32(t: torch.Tensor, name: str, shape: tuple, device: torch.device) -> None:
+    if t.dtype != torch.int32 or t.device != device:
+        raise L.HaloError(f"{name} must be int32 on {device}", L.HALO_ERR_INVALID_ARG)
+    if t.shape != shape or (shape[-1] > 1 and t.stride(-1) != 1):
+        raise L.HaloError(f"{name} must be {shape} with a contiguous last dim, got "
+                          f"{tuple(t.shape)}", L.HALO_ERR_INVALID_ARG)
+
+
+def _require_table(t: torch.Tensor, device: torch.device) -> None:
+    if t.dim() != 2 or t.dtype != torch.int32 or t.device != device or \
+            (t.shape[1] > 1 and t.stride(1) != 1):
+        raise L.HaloError(f"block_tables must be int32 (R, max_blocks) on {device} with contiguous "
+                          "rows", L.HALO_ERR_INVALID_ARG)
+
+
+def _page_pool(k: torch.Tensor, v: torch.Tensor) -> L.PagePool:
+    """The C-ABI description of page pools ``(n_pages, H_kv, page_size, D)``."""
+    _require_cuda(k, "k_pages")
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+        raise L.HaloError("k_pages and v_pages must be (n_pages, H_kv, page_size, D) of one shape, "
+                          "dtype and device", L.HALO_ERR_INVALID_ARG)
+    n, H_kv, page, D = k.shape
+    ks, vs = k.stride(), v.stride()
+    if D > 1 and (ks[3] != 1 or vs[3] != 1):
+        raise L.HaloError("page rows must be contiguous", L.HALO_ERR_INVALID_ARG)
+    return L.PagePool(k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], n, H_kv,
+                      page, D, L.halo_dtype(k.dtype))
+
+
+def update_block_tables(block_tables: torch.Tensor, old_lens: torch.Tensor, new_lens: torch.Tensor,
+                        free_pages: torch.Tensor, n_free: torch.Tensor, *, page_size: int,
+                        max_tokens: int, n_free_out: Optional[torch.Tensor] = None):
+    """Block tables, slots and positions from request lengths, on the device
+    (``halo_update_block_tables``).
+
+    ``block_tables (R, max_blocks)`` and ``free_pages`` (int32) are updated in
+    place: requests whose length shrinks from ``old_lens`` to ``new_lens``
+    ``(R,)`` give their last pages back to the end of
+    ``free_pages[:n_free]``, requests that grow then take pages off its end,
+    both in request order.  The length of the list that is left goes to
+    ``n_free_out`` (default: ``n_free (1,)`` itself).
+
+    Returns ``(slots, positions, cu_tokens, lens)``: slot and cache position
+    (int64, ``max_tokens`` entries, -1 behind the last row) of the new rows of
+    all requests packed in request order, their running count ``(R + 1,)``,
+    and the lengths the requests now have -- ``old_lens`` for one that the
+    free list or its table row cannot hold, which stays as it is."""
+    dev = block_tables.device
+    _require_cuda(block_tables, "block_tables")
+    _require_table(block_tables, dev)
+    R, max_blocks = block_tables.shape
+    _require_int32(old_lens, "old_lens", (R,), dev)
+    _require_int32(new_lens, "new_lens", (R,), dev)
+    _require_int32(free_pages, "free_pages", (free_pages.numel(),), dev)
+    _require_int32(n_free, "n_free", (1,), dev)
+    if n_free_out is None:
+        n_free_out = n_free
+    else:
+        _require_int32(n_free_out, "n_free_out", (1,), dev)
+    if max_tokens < 0:
+        raise L.HaloError("max_tokens must not be negative", L.HALO_ERR_INVALID_ARG)
+    rows = torch.empty(2, max_tokens, dtype=torch.int64, device=dev)
+    ints = torch.empty(2 * R + 1, dtype=torch.int32, device=dev)
+    slots, positions = rows[0], rows[1]
+    cu, lens = ints[:R + 1], ints[R + 1:]
+    with L.on_device(dev):
+        rc = L.lib().halo_update_block_tables(
+            block_tables.data_ptr(), block_tables.stride(0), R, max_blocks, old_lens.data_ptr(),
+            new_lens.data_ptr(), free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(),
+            n_free_out.data_ptr(), int(page_size), int(max_tokens), slots.data_ptr(),
+            positions.data_ptr(), cu.data_ptr(), lens.data_ptr(), L.stream_handle(dev))
+    L.check(rc, "halo_update_block_tables")
+    return slots, positions, cu, lens
+
+
+def write_kv_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                   slots: torch.Tensor) -> None:
+    """Copy K/V rows ``(T, H_kv, D)`` into the slots ``(T,)`` (int64) of page
+    pools ``(n_pages, H_kv, page_size, D)`` (``halo_write_kv_pages``).  Rows
+    with a slot outside the pools (-1: none) are skipped; slots are distinct."""
+    pool = _page_pool(k_pages, v_pages)
+    dev = k_pages.device
+    T = k.shape[0]
+    if k.shape != (T, pool.H_kv, pool.D) or v.shape != k.shape or k.dtype != k_pages.dtype or \
+            v.dtype != k.dtype or k.device != dev or v.device != dev:
+        raise L.HaloError("k and v must be (T, H_kv, D) of the pools' dtype and device",
+                          L.HALO_ERR_INVALID_ARG)
+    if slots.dtype != torch.int64 or slots.device != dev or slots.shape != (T,) or \
+            not slots.is_contiguous():
+        raise L.HaloError("slots must be contiguous int64 (T,) on the pools' device",
+                          L.HALO_ERR_INVALID_ARG)
+    k, v = _last_contig(k), _last_contig(v)
+    with L.on_device(dev):
+        rc = L.lib().halo_write_kv_pages(ctypes.byref(pool), k.data_ptr(), k.stride(0), k.stride(1),
+                                         v.data_ptr(), v.stride(0), v.stride(1), T,
+                                         slots.data_ptr(), L.stream_handle(dev))
+    L.check(rc, "halo_write_kv_pages")
+
+
+def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                   block_tables: torch.Tensor, context_lens: torch.Tensor, cu_nodes: torch.Tensor,
+                   tree_mask: torch.Tensor, *, scale: Optional[float] = None,
+                   out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None,
+                   lse: Optional[torch.Tensor] = None, want_lse: bool = True):
+    """Attention of drafted token trees over a paged K/V cache
+    (``halo_tree_attention``).
+
+    ``q (T, H, D)`` holds the nodes of all requests packed: request ``r``'s
+    are rows ``cu_nodes[r]`` to ``cu_nodes[r + 1] - 1``, its node ``i`` at
+    cache position ``context_lens[r] + i``, where its K/V row was written
+    before.  A node sees every position of its context and the nodes ``j``
+    with ``tree_mask[row, j]`` (bool ``(T, max_nodes)``); one that sees
+    nothing gets zeros and a log-sum-exp of -inf.  With one node a request
+    and a mask of ones this is a decode step over the paged cache.
+
+    Returns ``(out (T, H, D), lse (T, H))``; ``lse`` is ``None`` with
+    ``want_lse=False`` and none given.  Rows from ``cu_nodes[R]`` on are not
+    written.  bf16/fp16, head dim 64 or 128, a page size that is a multiple
+    of 8."""
+    _require_cuda(q, "q")
+    dev = q.device
+    pool = _page_pool(k_pages, v_pages)
+    if q.dim() != 3 or q.dtype != k_pages.dtype or k_pages.device != dev or q.shape[2] != pool.D:
+        raise L.HaloError("q must be (T, H, D) of the pools' dtype, device and head dim",
+                          L.HALO_ERR_INVALID_ARG)
+    T, H, D = q.shape
+    _require_table(block_tables, dev)
+    R, max_blocks = block_tables.shape
+    _require_int32(context_lens, "context_lens", (R,), dev)
+    _require_int32(cu_nodes, "cu_nodes", (R + 1,), dev)
+    if tree_mask.dim() != 2 or tree_mask.shape[0] != T or tree_mask.device != dev or \
+            tree_mask.dtype not in (torch.bool, torch.uint8) or \
+            (tree_mask.shape[1] > 1 and tree_mask.stride(1) != 1):
+        raise L.HaloError("tree_mask must be bool (T, max_nodes) with contiguous rows on q's device",
+                          L.HALO_ERR_INVALID_ARG)
+    q = _last_contig(q)
+    if out is None:
+        out = torch.empty(T, H, D, dtype=out_dtype or q.dtype, device=dev)
+    elif out.shape != q.shape or out.device != dev or (D > 1 and out.stride(2) != 1):
+        raise L.HaloError("out must be (T, H, D) with contiguous rows on q's device",
+                          L.HALO_ERR_INVALID_ARG)
+    if lse is None:
+        if want_lse:
+            lse = torch.empty(T, H, dtype=torch.float32, device=dev)
+    elif lse.shape != (T, H) or lse.dtype != torch.float32 or lse.device != dev or \
+            not lse.is_contiguous():
+        raise L.HaloError("lse must be contiguous fp32 (T, H) on q's device",
+                          L.HALO_ERR_INVALID_ARG)
+    prob = L.TreeProblem(R, T, H, tree_mask.shape[1], max_blocks,
+                         float(scale) if scale is not None else 1.0 / math.sqrt(D), q.data_ptr(),
+                         q.stride(0), q.stride(1), block_tables.data_ptr(), block_tables.stride(0),
+                         context_lens.data_ptr(), cu_nodes.data_ptr(), tree_mask.data_ptr(),
+                         tree_mask.stride(0), out.data_ptr(), out.stride(0), out.stride(1),
+                         L.halo_dtype(out.dtype), lse.data_ptr() if lse is not None else None)
+    lib = L.lib()
+    with L.on_device(dev):
+        need = lib.halo_tree_workspace_bytes(ctypes.byref(pool), ctypes.byref(prob))
+        if need < 0:
+            L.check(int(need), "halo_tree_workspace_bytes")
+        # a workspace of the call's own: stream-ordered by the allocator, and
+        # graphs captured on one stream never share it
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        rc = lib.halo_tree_attention(ctypes.byref(pool), ctypes.byref(prob),
+                                     ws.data_ptr() if ws is not None else None, need,
+                                     L.stream_handle(dev))
+    L.check(rc, "halo_tree_attention")
+    return out, lse
+
+
+def commit_tree_path(k_pages: torch.Tensor, v_pages: torch.Tensor, block_tables: torch.Tensor,
+                     context_lens: torch.Tensor, path: torch.Tensor,
+                     path_lens: torch.Tensor) -> None:
+    """Move the accepted nodes' K/V rows to the end of each request's context
+    (``halo_commit_tree_path``): step ``i < path_lens[r]`` moves the row at
+    position ``context_lens[r] + path[r, i]`` to ``context_lens[r] + i``.
+    ``path (R, max_depth)`` (int32) holds node indices with
+    ``path[r, i] >= i``, as paths from a root do when children are numbered
+    after their parents; other steps move nothing."""
+    pool = _page_pool(k_pages, v_pages)
+    dev = k_pages.device
+    _require_table(block_tables, dev)
+    R, max_blocks = block_tables.shape
+    if path.dim() != 2:
+        raise L.HaloError("path must be int32 (R, max_depth)", L.HALO_ERR_INVALID_ARG)
+    depth = path.shape[1]
+    _require_int32(path, "path", (R, depth), dev)
+    _require_int32(context_lens, "context_lens", (R,), dev)
+    _require_int32(path_lens, "path_lens", (R,), dev)
+    with L.on_device(dev):
+        rc = L.lib().halo_commit_tree_path(ctypes.byref(pool), block_tables.data_ptr(),
+                                           block_tables.stride(0), max_blocks, R,
+                                           context_lens.data_ptr(), path.data_ptr(),
+                                           path.stride(0), depth, path_lens.data_ptr(),
+                                           L.stream_handle(dev))
+    L.check(rc, "halo_commit_tree_path")

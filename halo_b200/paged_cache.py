@@ -1,0 +1,91 @@
+"""A paged K/V cache for batches of requests whose drafts are token trees.
+
+The cache owns one page pool per layer, the block tables and the free list,
+all on the device; nothing here reads a length back to the host, so a step
+can be captured in a CUDA graph.  One step of tree decoding:
+
+>>> rows = cache.extend(counts, max_tokens)          # room behind each context
+>>> for layer in range(n_layers):
+...     cache.write(layer, k, v, rows)
+...     out, lse = cache.attend(layer, q, rows, tree_mask)
+>>> cache.accept(path, path_lens)                    # keep one path of each tree
+
+A prompt is a step whose rows are all kept: ``extend``, ``write``, the
+prompt's own attention, then ``accept(None, counts)``.  No counterpart in the
+reference (its caches hold one tensor per layer and one token a step).
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from halo_b200 import _lib as L
+from halo_b200 import ops
+
+
+class PagedRows(NamedTuple):
+    """Rows of one step, packed in request order (``ops.update_block_tables``).
+    ``cu[r + 1] - cu[r]`` is 0 for a request whose rows the pool cannot hold."""
+    slots: torch.Tensor        # int64 (max_tokens,), -1 behind the last row
+    positions: torch.Tensor    # int64 (max_tokens,), -1 behind the last row
+    cu: torch.Tensor           # int32 (max_requests + 1,)
+
+
+class PagedKVCache:
+    def __init__(self, n_layers: int, n_pages: int, n_kv_heads: int, head_dim: int, *,
+                 max_requests: int, max_len: int, page_size: int = 64,
+                 dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        if min(n_layers, n_pages, n_kv_heads, head_dim, max_requests, max_len, page_size) < 1:
+            raise L.HaloError("cache dimensions must be positive", L.HALO_ERR_INVALID_ARG)
+        self.page_size = page_size
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(n_layers)]
+        self.v = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(n_layers)]
+        dev = self.k[0].device
+        blocks = -(-max_len // page_size)
+        self.block_tables = torch.zeros(max_requests, blocks, dtype=torch.int32, device=dev)
+        self.free_pages = torch.arange(n_pages, dtype=torch.int32, device=dev)
+        self.n_free = torch.full((1,), n_pages, dtype=torch.int32, device=dev)
+        # rows of each request's context, and with the rows of the step under way
+        self.lens = torch.zeros(max_requests, dtype=torch.int32, device=dev)
+        self.held = torch.zeros(max_requests, dtype=torch.int32, device=dev)
+
+    def extend(self, counts: torch.Tensor, max_tokens: int) -> PagedRows:
+        """Room for ``counts[r]`` (int32, at most ``max_tokens`` in all) rows
+        behind each request's context."""
+        slots, pos, cu, held = ops.update_block_tables(
+            self.block_tables, self.held, self.lens + counts, self.free_pages, self.n_free,
+            page_size=self.page_size, max_tokens=max_tokens)
+        self.held.copy_(held)
+        return PagedRows(slots, pos, cu)
+
+    def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, rows: PagedRows) -> None:
+        """Store the step's K/V rows ``(max_tokens, H_kv, D)``."""
+        ops.write_kv_pages(k, v, self.k[layer], self.v[layer], rows.slots)
+
+    def attend(self, layer: int, q: torch.Tensor, rows: PagedRows, tree_mask: torch.Tensor,
+               **kwargs):
+        """``ops.tree_attention`` of the step's rows over ``layer``."""
+        return ops.tree_attention(q, self.k[layer], self.v[layer], self.block_tables, self.lens,
+                                  rows.cu, tree_mask, **kwargs)
+
+    def accept(self, path: Optional[torch.Tensor], path_lens: torch.Tensor) -> None:
+        """End the step: request ``r`` keeps the rows ``path[r, :path_lens[r]]``
+        of its step (``None``: its first ``path_lens[r]`` rows) and gives the
+        other pages back."""
+        if path is not None:
+            for k, v in zip(self.k, self.v):
+                ops.commit_tree_path(k, v, self.block_tables, self.lens, path, path_lens)
+        self._resize(torch.minimum(self.lens + path_lens.clamp(min=0), self.held))
+
+    def release(self, ended: torch.Tensor) -> None:
+        """Empty the requests where ``ended (max_requests,)`` is true."""
+        self._resize(torch.where(ended, torch.zeros_like(self.lens), self.lens))
+
+    def _resize(self, lens: torch.Tensor) -> None:
+        _, _, _, held = ops.update_block_tables(
+            self.block_tables, self.held, lens, self.free_pages, self.n_free,
+            page_size=self.page_size, max_tokens=0)
+        self.held.copy_(held)
+        self.lens.copy_(held)

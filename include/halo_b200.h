@@ -417,6 +417,108 @@ int32_t halo_prefill_attention_ws(const halo_prefill_problem_t* problem,
                                   const halo_prefill_out_t* out, void* workspace,
                                   int64_t workspace_bytes, halo_stream_t stream);
 
+/* ------------------------------------------------------------ paged cache */
+
+/* A paged K/V cache: n_pages pages of page_size rows for each of H_kv heads;
+ * element (page, h, t, d) of K lives at
+ *   k + page*k_stride_p + h*k_stride_h + t*k_stride_t + d      (elements)
+ * and likewise for V.  A request keeps its position t in the page that entry
+ * t / page_size of its block table names, row t % page_size; slot
+ * page * page_size + row names one row of every head.  No counterpart in the
+ * reference, whose cache is one tensor per layer. */
+typedef struct halo_page_pool {
+  void* k;
+  void* v;
+  int64_t k_stride_p, k_stride_h, k_stride_t;
+  int64_t v_stride_p, v_stride_h, v_stride_t;
+  int32_t n_pages, H_kv, page_size, D;
+  int32_t dtype;
+} halo_page_pool_t;
+
+/* Block tables, slots and positions from request lengths, in one launch.
+ * block_tables (R, max_blocks) int32 rows table_stride apart.  Request r
+ * holds old_lens[r] rows and is to hold new_lens[r].  Requests that shrink
+ * give pages back: the pages of entries ceil(new/page_size) ..
+ * ceil(old/page_size) - 1 go behind free_pages[0 .. *n_free) in request
+ * order, entry order.  Requests that grow then take pages off the end of
+ * that list, in request order; their new table entries are written.  A
+ * request whose pages (with those of all growing requests before it) exceed
+ * the list, or whose length is negative or beyond max_blocks pages, stays as
+ * it is: lens[r] is new_lens[r] where granted and old_lens[r] where not.
+ * *n_free_out gets the length of the list that is left (it may be n_free
+ * itself) and free_pages its new entries; other entries of block_tables and
+ * free_pages are left as they were.  The new rows of all requests, packed in
+ * request order (cu_tokens (R + 1): their running count), get their slot
+ * and position in slots / positions (max_tokens); entries without a row get
+ * -1, and rows beyond max_tokens no entry.  R <= 8192. */
+int32_t halo_update_block_tables(int32_t* block_tables, int64_t table_stride, int32_t R,
+                                 int32_t max_blocks, const int32_t* old_lens,
+                                 const int32_t* new_lens, int32_t* free_pages,
+                                 int32_t free_capacity, const int32_t* n_free,
+                                 int32_t* n_free_out, int32_t page_size, int32_t max_tokens,
+                                 int64_t* slots, int64_t* positions, int32_t* cu_tokens,
+                                 int32_t* lens, halo_stream_t stream);
+
+/* Copy K and V rows k, v (T, H_kv, D) (element strides *_stride_t,
+ * *_stride_h) into the slots (T) of the pool.  Rows whose slot is negative
+ * or beyond the pool are skipped.  Slots are distinct: of two rows with one
+ * slot either may be kept, element by element. */
+int32_t halo_write_kv_pages(const halo_page_pool_t* pool, const void* k, int64_t k_stride_t,
+                            int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                            int64_t v_stride_h, int32_t T, const int64_t* slots,
+                            halo_stream_t stream);
+
+/* Attention of drafted token trees over the paged cache.  q is (T, H, D),
+ * the nodes of all requests packed: request r's are rows cu_nodes[r] ..
+ * cu_nodes[r + 1] - 1, its node i at cache position context_lens[r] + i
+ * (its K/V row written there before).  Node i sees the context (positions
+ * below context_lens[r]) and every node j with mask[row of i][j] != 0
+ * (mask (T, max_nodes) bytes, rows mask_stride apart).  A node that sees
+ * nothing gets zeros and lse -inf.  A K/V row that a node does not see (a
+ * hidden node's, one behind the last node) never reaches its output, whatever
+ * the row holds.  Rows of q from cu_nodes[R] on are not written.  A request has at
+ * most max_nodes nodes (others are not written) and at most max_blocks
+ * pages; a table entry that names no page reads as rows of zeros. */
+typedef struct halo_tree_problem {
+  int32_t R, T, H, max_nodes, max_blocks;
+  float scale;                   /* softmax scale, positive */
+  const void* q;                 /* in the pool's dtype */
+  int64_t q_stride_t, q_stride_h;
+  const int32_t* block_tables;
+  int64_t table_stride;
+  const int32_t* context_lens;
+  const int32_t* cu_nodes;
+  const uint8_t* mask;
+  int64_t mask_stride;
+  void* out;                     /* (T, H, D) in out_dtype (the pool's, or fp32) */
+  int64_t out_stride_t, out_stride_h;
+  int32_t out_dtype;
+  float* lse;                    /* (T, H) contiguous, natural log; optional */
+} halo_tree_problem_t;
+
+/* Bytes of workspace for halo_tree_attention (256-byte aligned; no
+ * initialisation, overwritten by the call; one call in flight per
+ * workspace).  Negative status on bad arguments. */
+int64_t halo_tree_workspace_bytes(const halo_page_pool_t* pool,
+                                  const halo_tree_problem_t* problem);
+
+/* bf16 / fp16, head_dim 64 or 128, page_size a multiple of 8, rows of K, V,
+ * q and out 16-byte aligned, max_nodes <= 1024. */
+int32_t halo_tree_attention(const halo_page_pool_t* pool, const halo_tree_problem_t* problem,
+                            void* workspace, int64_t workspace_bytes, halo_stream_t stream);
+
+/* Move the accepted nodes' K/V rows to the end of the context: for each step
+ * i < path_lens[r] of request r, the row at position context_lens[r] +
+ * path[r][i] goes to position context_lens[r] + i.  path (R, max_depth),
+ * rows path_stride apart, holds node indices with path[r][i] >= i (as every
+ * path from a root has when children come after their parents); other steps,
+ * and steps whose table entries name no page, move nothing. */
+int32_t halo_commit_tree_path(const halo_page_pool_t* pool, const int32_t* block_tables,
+                              int64_t table_stride, int32_t max_blocks, int32_t R,
+                              const int32_t* context_lens, const int32_t* path,
+                              int64_t path_stride, int32_t max_depth, const int32_t* path_lens,
+                              halo_stream_t stream);
+
 /* ------------------------------------------------------------------ tiers */
 
 /* Pitched async copy of `height` rows of `width_bytes` between any two of

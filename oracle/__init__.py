@@ -18,8 +18,11 @@ lzbaclz/HALO project root):
   bf16 rounding (``baselines/kivi_cache.py``).  numpy, cross-checked against
   the plain-C restatement in ``oracle/kivi_ref.c`` (built by
   ``oracle/Makefile`` into ``oracle/_build/liboracle_kivi.so``).
+* ``oracle.paged`` -- block tables, row moves and tree attention of the paged
+  cache (no reference counterpart: written from the definitions).  torch CPU,
+  64 bits.
 
-Pinning: every function is checked against golden vectors that were
+Pinning: every function of the reference's algorithm is checked against golden vectors that were
 generated by running the reference's own Python code in the build container
 (``tests/golden/make_golden.py``; fixtures in ``tests/golden/*.npz``).
 """

@@ -1,0 +1,151 @@
+"""Paged-cache operators: refusals of the C ABI and of the tensor wrappers (no
+GPU needed), and the oracle against independent small cases."""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from oracle import paged as O
+
+
+def _pool(L, **kw):
+    p = L.PagePool(0x10000, 0x20000, 2 * 16 * 128, 16 * 128, 128, 2 * 16 * 128, 16 * 128, 128, 10,
+                   2, 16, 128, L.DTYPE_BF16)
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return p
+
+
+def _tree(L, **kw):
+    p = L.TreeProblem(2, 8, 8, 4, 5, 0.1, 0x30000, 8 * 128, 128, 0x40000, 5, 0x50000, 0x60000,
+                      0x70000, 4, 0x80000, 8 * 128, 128, L.DTYPE_BF16, 0x90000)
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return p
+
+
+@pytest.mark.parametrize("pool,prob,code", [
+    ({"dtype": 0}, {}, "UNSUPPORTED"), ({"dtype": 9}, {}, "UNSUPPORTED"),
+    ({"D": 96}, {}, "UNSUPPORTED"), ({"D": 256}, {}, "UNSUPPORTED"),
+    ({"page_size": 12}, {}, "UNSUPPORTED"), ({"page_size": 0}, {}, "INVALID_ARG"),
+    ({"n_pages": 0}, {}, "INVALID_ARG"), ({"H_kv": 3}, {}, "INVALID_ARG"),
+    ({}, {"R": -1}, "INVALID_ARG"), ({}, {"T": -1}, "INVALID_ARG"),
+    ({}, {"max_nodes": 1025}, "UNSUPPORTED"), ({}, {"max_blocks": 2 ** 30}, "UNSUPPORTED"),
+    ({}, {"scale": 0.0}, "UNSUPPORTED"), ({}, {"scale": -1.0}, "UNSUPPORTED"),
+    ({}, {"scale": math.inf}, "UNSUPPORTED"), ({}, {"scale": math.nan}, "UNSUPPORTED"),
+    ({"k": None}, {}, "INVALID_ARG"), ({}, {"q": None}, "INVALID_ARG"),
+    ({}, {"out": None}, "INVALID_ARG"), ({}, {"mask": None}, "INVALID_ARG"),
+    ({}, {"cu_nodes": None}, "INVALID_ARG"), ({}, {"context_lens": None}, "INVALID_ARG"),
+    ({}, {"block_tables": None}, "INVALID_ARG"),
+    ({"k": 0x10008}, {}, "MISALIGNED"), ({"v_stride_t": 132}, {}, "MISALIGNED"),
+    ({"k_stride_h": 1}, {}, "MISALIGNED"), ({}, {"q": 0x30002}, "MISALIGNED"),
+    ({}, {"q_stride_h": 130}, "MISALIGNED"), ({}, {"out_stride_t": 12}, "MISALIGNED"),
+    ({}, {"out_dtype": 2}, "UNSUPPORTED")])
+def test_tree_attention_refusals(pool, prob, code):
+    from halo_b200 import _lib as L
+    lib = L.lib()
+    po, pr = _pool(L, **pool), _tree(L, **prob)
+    rc = lib.halo_tree_attention(ctypes.byref(po), ctypes.byref(pr), 0x100000, 1 << 40, None)
+    assert rc == getattr(L, "HALO_ERR_" + code), lib.halo_last_error_string()
+    assert lib.halo_last_error_string()
+
+
+def test_tree_attention_nothing_to_do_and_null_arguments():
+    from halo_b200 import _lib as L
+    lib = L.lib()
+    po = _pool(L)
+    for kw in ({"R": 0}, {"T": 0}, {"max_nodes": 0}):
+        pr = _tree(L, **kw)
+        assert lib.halo_tree_workspace_bytes(ctypes.byref(po), ctypes.byref(pr)) >= 0
+        assert lib.halo_tree_attention(ctypes.byref(po), ctypes.byref(pr), None, 0, None) == L.HALO_OK
+    assert lib.halo_tree_attention(None, ctypes.byref(_tree(L)), None, 0, None) == L.HALO_ERR_INVALID_ARG
+    assert lib.halo_tree_workspace_bytes(ctypes.byref(po), None) == L.HALO_ERR_INVALID_ARG
+
+
+def test_block_table_refusals():
+    from halo_b200 import _lib as L
+    lib = L.lib()
+
+    def call(table=0x1000, stride=8, R=4, blocks=8, old=0x2000, cap=10, n=0x4000, page=16, tok=5,
+             slots=0x5000, cu=0x7000):
+        return lib.halo_update_block_tables(table, stride, R, blocks, old, 0x2800, 0x3000, cap, n,
+                                            0x4000, page, tok, slots, 0x6000, cu, 0x8000, None)
+    for kw in ({"table": None}, {"old": None}, {"n": None}, {"slots": None}, {"cu": None},
+               {"R": -1}, {"blocks": -1}, {"cap": -1}, {"page": 0}, {"tok": -1}, {"stride": 7}):
+        assert call(**kw) == L.HALO_ERR_INVALID_ARG, kw
+    for kw in ({"R": 8193}, {"blocks": 2 ** 28, "stride": 2 ** 28}):
+        assert call(**kw) == L.HALO_ERR_UNSUPPORTED, kw
+
+
+def test_write_and_commit_refusals():
+    from halo_b200 import _lib as L
+    lib = L.lib()
+
+    def write(pool=None, k=0x1000, T=3, slots=0x2000):
+        return lib.halo_write_kv_pages(ctypes.byref(pool or _pool(L)), k, 256, 128, 0x3000, 256, 128,
+                                       T, slots, None)
+
+    def commit(pool=None, R=2, depth=3, blocks=4, path=0x2000):
+        return lib.halo_commit_tree_path(ctypes.byref(pool or _pool(L)), 0x1000, 4, blocks, R,
+                                         0x1800, path, 3, depth, 0x2800, None)
+    assert write(T=0) == L.HALO_OK and commit(R=0) == L.HALO_OK and commit(depth=0) == L.HALO_OK
+    assert write(T=-1) == write(k=None) == write(slots=None) == L.HALO_ERR_INVALID_ARG
+    assert commit(R=-1) == commit(depth=-1) == commit(path=None) == L.HALO_ERR_INVALID_ARG
+    assert commit(R=65536) == L.HALO_ERR_UNSUPPORTED
+    assert write(k=0x1001) == L.HALO_ERR_MISALIGNED
+    for call in (write, commit):
+        assert call(_pool(L, dtype=5)) == L.HALO_ERR_INVALID_ARG
+        assert call(_pool(L, D=0)) == L.HALO_ERR_INVALID_ARG
+        assert call(_pool(L, v=None)) == L.HALO_ERR_INVALID_ARG
+        assert call(_pool(L, k=0x10001)) == L.HALO_ERR_MISALIGNED
+
+
+def test_wrappers_refuse_cpu_tensors():
+    from halo_b200 import ops
+    from halo_b200._lib import HaloError
+    i = torch.zeros(2, dtype=torch.int32)
+    t = torch.zeros(2, 4, dtype=torch.int32)
+    p = torch.zeros(3, 2, 16, 64, dtype=torch.bfloat16)
+    with pytest.raises(HaloError, match="CUDA"):
+        ops.update_block_tables(t, i, i, i, i[:1], page_size=16, max_tokens=4)
+    with pytest.raises(HaloError, match="CUDA"):
+        ops.write_kv_pages(p[0], p[0], p, p, torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(HaloError, match="CUDA"):
+        ops.commit_tree_path(p, p, t, i, t, i)
+    with pytest.raises(HaloError, match="CUDA"):
+        ops.tree_attention(p[0], p, p, t, i, i, torch.ones(2, 3, dtype=torch.bool))
+
+
+def test_oracle_block_tables_by_hand():
+    # page 4: request 0 shrinks from 9 to 4 rows and gives pages 8, 9 back;
+    # request 1 grows from 3 to 10 and takes 9, then 8; request 2 wants more than is left
+    t, f, n, s, p, cu, lens = O.update_block_tables(
+        [[7, 8, 9], [1, 0, 0], [0, 0, 0]], [9, 3, 0], [4, 10, 9], [5, 6, 0, 0, 0], 2, 4, 9)
+    assert t == [[7, 8, 9], [1, 9, 8], [0, 0, 0]] and lens == [4, 10, 0]
+    assert n == 2 and f == [5, 6, 0, 0, 0]
+    assert p == [3, 4, 5, 6, 7, 8, 9, -1, -1] and cu == [0, 0, 7, 7]
+    assert s == [7, 36, 37, 38, 39, 32, 33, -1, -1]
+
+
+def test_oracle_tree_attention_by_softmax():
+    g = torch.Generator().manual_seed(0)
+    k, v = torch.randn(4, 1, 8, 16, generator=g), torch.randn(4, 1, 8, 16, generator=g)
+    q = torch.randn(3, 2, 16, generator=g)
+    mask = torch.tensor([[1, 0, 0], [1, 1, 0], [1, 0, 1]], dtype=torch.bool)
+    out, lse, _, _ = O.tree_attention(q, k, v, [[2, 0]], [9], [0, 3], mask)
+    kk = torch.cat([k[2, 0], k[0, 0]])[:12].double()
+    vv = torch.cat([v[2, 0], v[0, 0]])[:12].double()
+    seen = torch.cat([torch.ones(3, 9, dtype=torch.bool), mask], 1)
+    s = (q.double() @ kk.T / 4).masked_fill(~seen[:, None], -math.inf)
+    assert torch.allclose(out, torch.softmax(s, -1) @ vv)
+    assert torch.allclose(lse, torch.logsumexp(s, -1))
+
+
+def test_oracle_commit_reads_before_it_writes():
+    k = torch.arange(8.0).view(1, 1, 8, 1).clone()
+    v = -k.clone()
+    O.commit_tree_path(k, v, [[0]], [2], [[0, 2, 3]], [3])
+    assert k.flatten().tolist() == [0, 1, 2, 4, 5, 5, 6, 7] and torch.equal(v, -k)
