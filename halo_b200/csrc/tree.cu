@@ -6,24 +6,49 @@
 //   s_j = scale q . k_j,  m = max s_j,  l = sum e^{s_j - m},
 //   out = sum e^{s_j - m} v_j / l,  lse = m + ln l
 // (zeros and -inf where it sees nothing).
+//
+// The n_r * G query rows that share a K/V head (G = H / H_kv) go through the
+// tensor cores together, so a K/V row is read once for all of them (once for
+// each 256 of them).  Up to about 64 rows the cache's bytes bound the kernel;
+// at 256 rows bytes, products and exponentials come out about level.
+//
+// Split: a unit is 128 positions of one (request, K/V head, row group), and
+// the units of all requests, in that order, are cut into one equal run per
+// SM.  The lengths are read on the device, so the cut is even for any mix of
+// them and nothing depends on the host knowing one.  A (request, head, group)
+// that lies in one run is finished there; the parts of others go to the
+// workspace as (m, l, o) and tree_merge_kernel joins them.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
+#include <mutex>
+#include <type_traits>
+
 #include "halo_common.cuh"
+#include "umma.cuh"
 
 namespace halo {
 
 int fail(int code, const char* fmt, ...);
 int cuda_fail(cudaError_t e, const char* what);
+int device_sms();
 
 namespace tree {
 
-struct Params {
-  const char* k;
-  const char* v;
-  int64_t k_sp, k_sh, k_st, v_sp, v_sh, v_st;    // elements
+constexpr int kBN = 128;               // positions of a tile (a unit)
+constexpr int kThreads = 384;
+constexpr uint32_t kTmemCols = 512;
+constexpr float kRescaleLog2 = 8.f;    // headroom of the running maximum
+constexpr int kBadSlots = 8;
+
+struct alignas(64) Params {
+  CUtensorMap kmap;                    // {D, page, H_kv, n_pages}
+  CUtensorMap vmap;
   const char* q;
-  int64_t q_st, q_sh;
+  int64_t q_st, q_sh;                  // elements
+  const char* v;
+  int64_t v_sp, v_sh, v_st;            // elements
   const int32_t* table;
   int64_t table_stride;
   const int32_t* ctx;
@@ -33,104 +58,1062 @@ struct Params {
   char* out;
   int64_t out_st, out_sh;
   float* lse;
-  float scale_log2;
+  float scale_log2;                    // softmax scale * log2(e)
   int32_t out_f32;
-  int32_t R, T, H, G, max_nodes, max_blocks, n_pages, page;
+  int32_t R, T, H, H_kv, G, max_nodes, max_blocks, n_pages, page, box;
+  struct Desc* desc;                   // workspace: one a CTA
+  float* part;                         // workspace: two slots a CTA
+  unsigned int* err;
 };
 
-// One CTA per query row (node, head), keys dealt to its warps, a lane
-// holding D / 32 columns.
-constexpr int kWarps = 8;
+// What the merge has to know of the segment that holds a CTA's first unit.
+struct alignas(64) Desc {
+  int64_t start, end, total;           // units: the segment's, and all units
+  int32_t cu0, hk, row0, rows;         // row0: the group's first row of the request
+};
+
+// Rows of a group's slot: o[D], m (log2 units), l, padding to 16 bytes.
+template <int D>
+constexpr int kPartStride = D + 4;
+
+template <int D, int QT>
+struct Geom {
+  static constexpr int kBlocks = D / 64;                  // 128-byte column blocks
+  static constexpr int kBlockBytes = kBN * 128;
+  static constexpr int kTileBytes = kBlocks * kBlockBytes;
+  // as many K and V tiles in flight as 227 KB hold beside QT query tiles
+  static constexpr int kStK = D == 64 ? 6 : 3;
+  static constexpr int kStV = D == 64 ? 6 : (QT == 1 ? 3 : 2);
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffK = QT * kTileBytes;
+  static constexpr int kOffV = kOffK + kStK * kTileBytes;
+  static constexpr int kOffMl = kOffV + kStV * kTileBytes;   // m, l [2][128]
+  static constexpr int kOffBar = kOffMl + 2048;
+  static constexpr int kSmemBytes = kOffBar + 1024;
+  static constexpr uint32_t kColO = 256;
+};
+
+struct Bars {
+  uint64_t q_full;
+  uint64_t k_full[6], k_empty[6], v_full[6], v_ready[6], v_empty[6];
+  uint64_t s_full[2], p_full[2], pv_done[2], mma_done;
+  int64_t scan[12];
+  int64_t base0, total;
+  uint32_t tmem_base;
+  int abort_flag, r0;
+  int bad[2][kBadSlots];
+};
+static_assert(sizeof(Bars) <= 1024, "barrier block");
+
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// Bounded wait that also ends when another role gave up.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Bars* bs,
+                                         unsigned int* err) {
+  if (mbar_try_wait_hint(bar, parity, 1000)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+    for (int i = 0; i < 8; ++i)
+      if (mbar_try_wait_hint(bar, parity, 1000)) return true;
+    if (*reinterpret_cast<volatile int*>(&bs->abort_flag)) return false;
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      set_device_error(err, static_cast<unsigned int>(-HALO_ERR_TIMEOUT));
+      *reinterpret_cast<volatile int*>(&bs->abort_flag) = 1;
+      return false;
+    }
+  }
+}
+
+// ---- the units of a request
+struct Req {
+  int ctx, end, nodes, cu0, nt, ng;
+  __device__ __forceinline__ int64_t units(int H_kv) const { return (int64_t)nt * ng * H_kv; }
+};
+
+template <int RG>
+__device__ __forceinline__ Req load_req(const Params& p, int r) {
+  Req q;
+  const int lim = p.max_blocks * p.page;
+  q.cu0 = min(max(p.cu[r], 0), p.T);
+  q.nodes = min(min(max(p.cu[r + 1] - q.cu0, 0), p.max_nodes), p.T - q.cu0);
+  q.ctx = min(max(p.ctx[r], 0), lim);
+  q.end = min(q.ctx + q.nodes, lim);
+  q.ng = (q.nodes * p.G + RG - 1) / RG;
+  q.nt = q.nodes > 0 ? max(1, (q.end + kBN - 1) / kBN) : 0;
+  return q;
+}
+
+// One (request, head, group) part of a CTA's run: tiles [t0, t1) of nt.
+struct Seg {
+  int hk, row0, rows, t0, t1;
+  bool whole, first;
+};
+
+// Walks a CTA's run segment by segment; every role keeps its own.
+template <int RG>
+struct Walk {
+  int64_t u, u0, u1, base, units;
+  int r;
+  Req q;
+  __device__ __forceinline__ Walk(const Params& p, int r0, int64_t base0, int64_t a, int64_t b)
+      : u(a), u0(a), u1(b), base(base0), r(r0) {
+    q = load_req<RG>(p, r);
+    units = q.units(p.H_kv);
+  }
+  __device__ __forceinline__ bool next(const Params& p, Seg& s) {
+    if (u >= u1) return false;
+    while (u - base >= units) {
+      base += units;
+      q = load_req<RG>(p, ++r);
+      units = q.units(p.H_kv);
+    }
+    const int64_t local = u - base;
+    const int hg = (int)(local / q.nt);
+    s.t0 = (int)(local - (int64_t)hg * q.nt);
+    s.t1 = (int)min((int64_t)q.nt, s.t0 + (u1 - u));
+    s.hk = hg / q.ng;
+    s.row0 = (hg - s.hk * q.ng) * RG;
+    s.rows = min(RG, q.nodes * p.G - s.row0);
+    s.whole = s.t0 == 0 && s.t1 == q.nt;
+    s.first = u == u0;
+    u += s.t1 - s.t0;
+    return true;
+  }
+};
+
+// ---- TMEM loads of 8 / 16 columns (the 32-column form is in umma.cuh)
+__device__ __forceinline__ void tmem_ld(uint32_t a, float (&v)[8]) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                 "=r"(r[6]), "=r"(r[7])
+               : "r"(a));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_ld(uint32_t a, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(a));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_ld(uint32_t a, float (&v)[32]) { umma::tmem_ld32(a, v); }
+
+// A value the compiler cannot see through: keeps it from hoisting every
+// unrolled MMA's descriptor out of the issuer's polling loop.
+__device__ __forceinline__ uint64_t opaque(uint64_t v) {
+  asm volatile("mov.b64 %0, %0;" : "+l"(v));
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ bool bad16(uint32_t x) {   // inf or NaN in the low 16 bits
+  constexpr uint32_t e = Elem<T>::kDtype == HALO_DTYPE_BF16 ? 0x7F80u : 0x7C00u;
+  return (x & e) == e;
+}
+
+// ======================================================================
+// tree_kernel: one CTA an SM, 384 threads.
+//   warp 0      TMA producer: K and V tiles of 128 positions, each made of
+//               boxes of p.box rows (the largest power of two, up to 128,
+//               that divides the page), through two rings; the lanes issue a
+//               tile's boxes side by side.  Boxes behind the last position
+//               or without a page start outside the tensor: zeros.
+//   warp 1      TMEM owner; lane 0 issues every MMA, polling for whichever
+//               step has its inputs ready.
+//   warps 2, 3  clean V: in tiles that reach behind the context, rows behind
+//               the last node and elements that are not finite become zero
+//               (a weight of zero would turn them into NaN); a node that does
+//               see such an element gets it back in the epilogue.
+//   warps 4-7   softmax stream 0, warps 8-11 stream 1 (thread = TMEM lane).
+// Each stream has its own scores S_X (128 TMEM columns, overwritten in place
+// by the weights P_X) and output O_X: S_X = Q K^T, O_X += P_X V, both M128.
+// P is split into a 16-bit value and a 16-bit remainder (two MMAs), ~16
+// significant bits: one 16-bit P would cost up to 2^-9 |v|, as much as the
+// output's own rounding.  Sums, maxima and O are fp32.
+//
+// Row groups of more than 128 rows (QT = 2): stream X takes query tile X and
+// both take every K/V tile.  Smaller ones: both streams share the query tile
+// and take every second K/V tile, and if the rows fit 64 or 32 lanes the
+// tile holds 2 or 4 copies of them (KPT = 64, 32), copy c taking positions
+// [c KPT, (c + 1) KPT) of each tile: the exponentials of a few rows are spread
+// over all 256 softmax threads, while the MMAs, which cost the same for 1 row
+// as for 128, stay under the time the bytes take.  A copy's weights are zero
+// outside its positions.  All copies and streams are joined in shared memory
+// at the end of a segment.
+template <typename T, int D, int KPT, int QT>
+__global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ Params p) {
+  using Gm = Geom<D, QT>;
+  constexpr int COP = kBN / KPT;           // copies of the rows in a query tile
+  constexpr int RPC = 128 / COP;           // rows of a copy
+  constexpr int RG = RPC * QT;             // rows of a group
+  constexpr bool kBf16 = Elem<T>::kDtype == HALO_DTYPE_BF16;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  Bars* bs = reinterpret_cast<Bars*>(smem + Gm::kOffBar);
+  float* sm_m = reinterpret_cast<float*>(smem + Gm::kOffMl);
+  float* sm_l = sm_m + 256;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bs->q_full, 8);
+    for (int i = 0; i < 6; ++i) {
+      mbar_init(&bs->k_full[i], 1);
+      mbar_init(&bs->k_empty[i], 2);
+      mbar_init(&bs->v_full[i], 1);
+      mbar_init(&bs->v_ready[i], 2);
+      mbar_init(&bs->v_empty[i], 2);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&bs->s_full[x], 1);
+      mbar_init(&bs->p_full[x], 4);
+      mbar_init(&bs->pv_done[x], 1);
+    }
+    mbar_init(&bs->mma_done, 1);
+    bs->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    umma::tmem_alloc(&bs->tmem_base, kTmemCols);
+    umma::tmem_relinquish();
+  }
+  grid_dep_wait();                         // the caller's writes are visible
+
+  // ---- this CTA's run of units: [c U / C, (c + 1) U / C)
+  auto prefix = [&](int64_t v, int64_t& total) {   // inclusive, over the CTA
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t o = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d) v += o;
+    }
+    __syncthreads();
+    if (lane == 31) bs->scan[warp] = v;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) v += bs->scan[w];
+      total += bs->scan[w];
+    }
+    return v;
+  };
+  auto units_of = [&](int r) { return r < p.R ? load_req<RG>(p, r).units(p.H_kv) : (int64_t)0; };
+  int64_t U = 0, mine = 0, incl = 0;
+  for (int r0 = 0; r0 < p.R; r0 += kThreads) {
+    int64_t t;
+    mine = units_of(r0 + threadIdx.x);
+    incl = prefix(mine, t);
+    U += t;
+  }
+  const int64_t u0 = (int64_t)blockIdx.x * U / gridDim.x;
+  const int64_t u1 = (int64_t)(blockIdx.x + 1) * U / gridDim.x;
+  {
+    int64_t before = 0;
+    for (int r0 = 0; r0 < p.R; r0 += kThreads) {
+      int64_t t = U;
+      if (p.R > kThreads) {                // else the scan above holds
+        mine = units_of(r0 + threadIdx.x);
+        incl = prefix(mine, t);
+      }
+      const int64_t lo = before + incl - mine;
+      if (mine > 0 && lo <= u0 && u0 < lo + mine) {
+        bs->r0 = r0 + threadIdx.x;
+        bs->base0 = lo;
+      }
+      before += t;
+    }
+  }
+  umma::fence_before_sync();
+  __syncthreads();
+  umma::fence_after_sync();
+  const uint32_t tmem = bs->tmem_base;
+  if (threadIdx.x == 0) {
+    Desc d{};
+    d.total = U;
+    d.start = d.end = u0;
+    if (u0 < U) {
+      Walk<RG> w(p, bs->r0, bs->base0, u0, u0 + 1);
+      Seg s;
+      w.next(p, s);
+      d.start = u0 - s.t0;
+      d.end = d.start + w.q.nt;
+      d.cu0 = w.q.cu0;
+      d.hk = s.hk;
+      d.row0 = s.row0;
+      d.rows = s.rows;
+    }
+    p.desc[blockIdx.x] = d;
+  }
+  grid_dep_trigger();
+
+  const uint32_t sQ = smem_addr(smem + Gm::kOffQ);
+  const uint32_t sK = smem_addr(smem + Gm::kOffK);
+  const uint32_t sV = smem_addr(smem + Gm::kOffV);
+  constexpr int SK = Gm::kStK, SV = Gm::kStV;
+
+  // the swizzled tiles need 1024-byte alignment, which dynamic shared memory
+  // without static shared memory before it has
+  const bool aligned = (sQ & 1023) == 0;
+  if (!aligned && threadIdx.x == 0)
+    set_device_error(p.err, static_cast<unsigned int>(-HALO_ERR_MISALIGNED));
+
+  // Register split (128 x 88 + 256 x 208 = 384 x 168, the launch budget).
+  if (u0 < u1 && aligned) {
+  if (warp < 4) {
+    umma::regs_dec<88>();
+    Walk<RG> walk(p, bs->r0, bs->base0, u0, u1);
+    Seg s;
+    if (warp == 0) {
+      // -------------------------------------------------------- producer
+      const int n_box = kBN / p.box, n_iss = n_box * Gm::kBlocks;   // at most 32
+      const int blk = lane / n_box, bx = lane - blk * n_box;
+      const uint32_t dst = blk * Gm::kBlockBytes + bx * p.box * 128;
+      int g = 0;
+      bool ok = true;
+      while (ok && walk.next(p, s)) {
+        const int32_t* tab = p.table + (int64_t)walk.r * p.table_stride;
+        const uint32_t absent = s.rows > 128 ? 0u : 1u;   // streams that skip a tile
+        auto entry = [&](int t) {
+          const int pos = t * kBN + bx * p.box;
+          return lane < n_iss && t < s.t1 && pos < walk.q.end ? tab[pos / p.page] : -1;
+        };
+        int pg = entry(s.t0);
+        for (int t = s.t0; t < s.t1; ++t, ++g) {
+          const int pg_next = entry(t + 1);
+          const int pos = t * kBN + bx * p.box;
+          const int row = pos % p.page;
+          const int page = (uint32_t)pg < (uint32_t)p.n_pages ? pg : p.n_pages;   // outside: zeros
+          const int ik = g % SK, iv = g % SV;
+          if (g >= SK) ok = __all_sync(0xffffffffu, wait_bar(&bs->k_empty[ik], (g / SK - 1) & 1, bs, p.err));
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&bs->k_full[ik], Gm::kTileBytes);
+            if (absent) mbar_arrive_n(&bs->k_empty[ik], absent);
+          }
+          __syncwarp();
+          if (lane < n_iss)
+            tma_load_4d(smem + Gm::kOffK + ik * Gm::kTileBytes + dst, &p.kmap, blk * 64, row, s.hk,
+                        page, &bs->k_full[ik]);
+          if (g >= SV) ok = __all_sync(0xffffffffu, wait_bar(&bs->v_empty[iv], (g / SV - 1) & 1, bs, p.err));
+          if (!ok) {
+            // this tile's K is on its way: count it below
+            ++g;
+            break;
+          }
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&bs->v_full[iv], Gm::kTileBytes);
+            if (absent) mbar_arrive_n(&bs->v_empty[iv], absent);
+          }
+          __syncwarp();
+          if (lane < n_iss)
+            tma_load_4d(smem + Gm::kOffV + iv * Gm::kTileBytes + dst, &p.vmap, blk * 64, row, s.hk,
+                        page, &bs->v_full[iv]);
+          pg = pg_next;
+        }
+      }
+      // every copy issued lands before the CTA can exit
+      if (lane == 0) {
+        for (int i = 0; i < SK; ++i) {
+          const int n = (g - i + SK - 1) / SK;
+          if (n > 0) mbar_wait(&bs->k_full[i], (n - 1) & 1, p.err);
+        }
+        const int gv = ok ? g : g - 1;
+        for (int i = 0; i < SV; ++i) {
+          const int n = (gv - i + SV - 1) / SV;
+          if (gv > 0 && n > 0) mbar_wait(&bs->v_full[i], (n - 1) & 1, p.err);
+        }
+      }
+    } else if (warp == 1) {
+      // -------------------------------------------------------- MMA issuer
+      if (lane == 0) {
+        constexpr uint32_t kIdQK = umma::instr_desc_f16(128, kBN, kBf16, false, false);
+        constexpr uint32_t kIdPV = umma::instr_desc_f16(128, D, kBf16, false, true);
+        const uint64_t qdesc0 = umma::smem_desc_sw128(sQ, 16, 1024);
+        const uint64_t kdesc0 = umma::smem_desc_sw128(sK, 16, 1024);
+        const uint64_t vdesc0 = umma::smem_desc_sw128(sV, Gm::kBlockBytes, 1024);
+        // K (V) tiles below kpre (vpre) have landed: barriers are probed in
+        // tile order, so none is probed more than one phase ahead
+        int kpre = 0, vpre = 0;
+        auto landed = [&](int& pre, uint64_t* bar, int st, int g) {
+          while (pre <= g && mbar_test(&bar[pre % st], (pre / st) & 1)) ++pre;
+          return g < pre;
+        };
+        int jq[2] = {0, 0}, jp[2] = {0, 0};   // QK / PV issued a stream, all segments
+        int qseq[2] = {0, 0}, seq = 0;        // issue order of each stream's latest QK
+        int g0 = 0, si = 0;
+        bool ok = true;
+        uint64_t t_idle = 0;
+        int idle = 0;
+        while (ok && walk.next(p, s)) {
+          const bool two = s.rows > 128;
+          const int n = s.t1 - s.t0, step = two ? 1 : 2;
+          const int nx[2] = {two ? n : (n + 1) / 2, two ? n : n / 2};
+          int a[2] = {0, 0}, b[2] = {0, 0};   // QK / PV issued in this segment
+          ok = wait_bar(&bs->q_full, si & 1, bs, p.err);
+          while (ok && (b[0] < nx[0] || b[1] < nx[1])) {
+            bool did = false;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              if (b[x] < a[x]) {              // O_X += P_X V
+                const int g = g0 + (two ? 0 : x) + b[x] * step;
+                if (mbar_test(&bs->p_full[x], jp[x] & 1) && landed(vpre, bs->v_ready, SV, g)) {
+                  umma::fence_after_sync();
+                  const uint32_t pc = tmem + x * 128, oc = tmem + Gm::kColO + x * D;
+                  const int iv = g % SV;
+                  const uint64_t vd = opaque(vdesc0 + (uint64_t)((iv * Gm::kTileBytes) >> 4));
+#pragma unroll
+                  for (int kk = 0; kk < kBN / 16; ++kk)
+                    umma::mma_ts(oc, pc + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), kIdPV,
+                                 b[x] > 0 || kk > 0);
+#pragma unroll
+                  for (int kk = 0; kk < kBN / 16; ++kk)
+                    umma::mma_ts(oc, pc + 64 + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4),
+                                 kIdPV, true);
+                  umma::commit(&bs->pv_done[x]);
+                  umma::commit(&bs->v_empty[iv]);
+                  ++jp[x];
+                  ++b[x];
+                  did = true;
+                }
+              }
+              if (a[x] < nx[x] && a[x] == b[x]) {   // S_X = Q K^T, S_X free
+                const int g = g0 + (two ? 0 : x) + a[x] * step;
+                if ((jq[x] == 0 || mbar_test(&bs->pv_done[x], (jq[x] - 1) & 1)) &&
+                    landed(kpre, bs->k_full, SK, g)) {
+                  umma::fence_after_sync();
+                  const int ik = g % SK;
+                  const uint64_t qd =
+                      opaque(qdesc0 + (uint64_t)(((two ? x : 0) * Gm::kTileBytes) >> 4));
+                  const uint64_t kd = opaque(kdesc0 + (uint64_t)((ik * Gm::kTileBytes) >> 4));
+#pragma unroll
+                  for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t off = ((kk >> 2) * Gm::kBlockBytes + (kk & 3) * 32) >> 4;
+                    umma::mma_ss(tmem + x * 128, qd + off, kd + off, kIdQK, kk > 0);
+                  }
+                  umma::commit(&bs->s_full[x]);
+                  umma::commit(&bs->k_empty[ik]);
+                  qseq[x] = ++seq;
+                  ++jq[x];
+                  ++a[x];
+                  did = true;
+                }
+              }
+            }
+            if (did) {
+              idle = 0;
+              continue;
+            }
+            // Nothing ready: sleep in hardware on what is expected first: a PV
+            // about to complete, the oldest pending P, else V, else K.
+            int xo = -1, xq = -1;
+            if (b[0] < a[0]) xo = 0;
+            if (b[1] < a[1] && (xo < 0 || qseq[1] < qseq[0])) xo = 1;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              if (a[x] < nx[x] && a[x] == b[x] && jq[x] > 0 &&
+                  !mbar_test(&bs->pv_done[x], (jq[x] - 1) & 1))
+                xq = x;
+            if (xq >= 0)
+              mbar_try_wait_hint(&bs->pv_done[xq], (jq[xq] - 1) & 1, 1000);
+            else if (xo >= 0 && !mbar_test(&bs->p_full[xo], jp[xo] & 1))
+              mbar_try_wait_hint(&bs->p_full[xo], jp[xo] & 1, 1000);
+            else if (xo >= 0)
+              mbar_try_wait_hint(&bs->v_ready[vpre % SV], (vpre / SV) & 1, 1000);
+            else
+              mbar_try_wait_hint(&bs->k_full[kpre % SK], (kpre / SK) & 1, 1000);
+            if (++idle == 64) t_idle = globaltimer_ns();
+            if (idle > 64 && (idle & 63) == 0) {
+              if (*reinterpret_cast<volatile int*>(&bs->abort_flag)) {
+                ok = false;
+              } else if (globaltimer_ns() - t_idle > kWaitLimitNs) {
+                set_device_error(p.err, static_cast<unsigned int>(-HALO_ERR_TIMEOUT));
+                *reinterpret_cast<volatile int*>(&bs->abort_flag) = 1;
+                ok = false;
+              }
+            }
+          }
+          g0 += n;
+          ++si;
+        }
+        // this thread's MMAs complete before the CTA can free TMEM
+        umma::commit(&bs->mma_done);
+        mbar_wait(&bs->mma_done, 0, p.err);
+      }
+    } else {
+      // -------------------------------------------------------- V cleaners
+      int g = 0, si = 0;
+      bool ok = true;
+      volatile int* bad = &bs->bad[warp - 2][0];
+      while (ok && walk.next(p, s)) {
+        if (lane == 0) bad[si % kBadSlots] = 0;
+        __syncwarp();
+        for (int t = s.t0; t < s.t1; ++t, ++g) {
+          const int iv = g % SV;
+          ok = __all_sync(0xffffffffu, wait_bar(&bs->v_full[iv], (g / SV) & 1, bs, p.err));
+          if (!ok) break;
+          const int lo = max(0, walk.q.ctx - t * kBN), end = walk.q.end - t * kBN;
+          if (lo < kBN) {
+            bool any = false;
+            const int n = (kBN - lo) * (D / 8);
+            for (int i = (warp - 2) * 32 + lane; i < n; i += 64) {
+              const int row = lo + i / (D / 8), c = i % (D / 8);
+              uint4* w = reinterpret_cast<uint4*>(smem + Gm::kOffV + iv * Gm::kTileBytes +
+                                                  (c >> 3) * Gm::kBlockBytes + row * 128 +
+                                                  (((c & 7) ^ (row & 7)) << 4));
+              if (row >= end) {
+                *w = make_uint4(0, 0, 0, 0);
+                continue;
+              }
+              uint4 x = *w;
+              uint32_t e[4] = {x.x, x.y, x.z, x.w};
+              bool hit = false;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if (bad16<T>(e[k])) {
+                  e[k] &= 0xFFFF0000u;
+                  hit = true;
+                }
+                if (bad16<T>(e[k] >> 16)) {
+                  e[k] &= 0xFFFFu;
+                  hit = true;
+                }
+              }
+              if (hit) {
+                *w = make_uint4(e[0], e[1], e[2], e[3]);
+                any = true;
+              }
+            }
+            if (any) bad[si % kBadSlots] = 1;
+            fence_proxy_async_smem();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bs->v_ready[iv]);
+        }
+        ++si;
+      }
+    }
+  } else {
+    umma::regs_inc<208>();
+    // ------------------------------------------------------------ softmax X
+    const int x = (warp - 4) >> 2;
+    const int sub = warp & 3;
+    const int r = sub * 32 + lane;               // TMEM lane
+    const int copy = sub * 32 / RPC;             // uniform in a warp
+    const int rr = r - copy * RPC;               // row within the tile
+    const int tid = threadIdx.x - 128;           // 0..255 over both streams
+    const uint32_t trow = tmem + ((uint32_t)(sub * 32) << 16);
+    const uint32_t scol = x * 128, ocol = Gm::kColO + x * D;
+    Walk<RG> walk(p, bs->r0, bs->base0, u0, u1);
+    Seg s;
+    int j = 0, si = 0;                           // tiles of this stream; segments
+    bool ok = true;
+    while (walk.next(p, s)) {
+      const bool two = QT == 2 && s.rows > 128;
+      const int nodes = walk.q.nodes, ctx = walk.q.ctx, end = walk.q.end, cu0 = walk.q.cu0;
+      // ---- Q: the previous segment's MMAs and scratch are done with
+      named_bar_sync(1, 256);
+      {
+        constexpr int VPR = D / 8;
+        const int n = (two ? 256 : 128) * VPR;
+        for (int i0 = 0; i0 < n; i0 += 256 * 4) {
+          uint4 w[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int i = i0 + u * 256 + tid;
+            const int ql = i / VPR, c = i % VPR;             // tile row, 16-byte column
+            const int row = two ? ql : ql % RPC;
+            w[u] = make_uint4(0, 0, 0, 0);
+            if (i < n && row < s.rows) {
+              const int rq = s.row0 + row, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
+              w[u] = *reinterpret_cast<const uint4*>(
+                  reinterpret_cast<const T*>(p.q) + (int64_t)(cu0 + node) * p.q_st + hq * p.q_sh +
+                  c * 8);
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int i = i0 + u * 256 + tid;
+            const int ql = i / VPR, c = i % VPR;
+            const int qt = ql >> 7, q = ql & 127;
+            if (i < n)
+              *reinterpret_cast<uint4*>(smem + Gm::kOffQ + qt * Gm::kTileBytes +
+                                        (c >> 3) * Gm::kBlockBytes + q * 128 +
+                                        (((c & 7) ^ (q & 7)) << 4)) = w[u];
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bs->q_full);
+      }
+      const int n = s.t1 - s.t0, step = two ? 1 : 2;
+      const int nx = two ? n : (x ? n / 2 : (n + 1) / 2);
+      const int rowx = s.row0 + (two ? x * 128 : 0);   // request row of the tile's row 0
+      const int rows = min(s.row0 + s.rows - rowx, RPC);
+      float m = -INFINITY, l = 0.f;
+      for (int it = 0; it < nx; ++it, ++j) {
+        const int p0 = (s.t0 + (two ? 0 : x) + it * step) * kBN + copy * KPT;
+        // which of the thread's positions its row sees
+        const bool full = p0 + KPT <= ctx;
+        uint32_t vis[KPT / 32];
+        if (!full) {
+#pragma unroll
+          for (int w = 0; w < KPT / 32; ++w) {
+            const int b = p0 + 32 * w;
+            vis[w] = 0;
+            if (b + 32 <= ctx) {
+              vis[w] = 0xffffffffu;
+            } else if (b < end) {
+              // one mask row at a time, a lane a position
+              const int jn = b + lane - ctx;
+              const bool node_ok = jn >= 0 && b + lane < end;
+              const int first = rowx + sub * 32 - copy * RPC;
+              const uint8_t* mp = p.mask + (int64_t)cu0 * p.mask_stride + jn;
+#pragma unroll 8
+              for (int i = 0; i < 32; ++i) {
+                const int node = (first + i) / p.G;
+                const bool v = jn < 0 || (node_ok && node < nodes &&
+                                          mp[(int64_t)node * p.mask_stride] != 0);
+                const uint32_t bits = __ballot_sync(0xffffffffu, v);
+                if (lane == i) vis[w] = bits;
+              }
+            }
+          }
+        }
+        ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->s_full[x], j & 1, bs, p.err));
+        if (!ok) break;
+        umma::fence_after_sync();
+        float sv[KPT];
+#pragma unroll
+        for (int c = 0; c < KPT / 32; ++c)
+          umma::tmem_ld32(trow + scol + copy * KPT + c * 32, sv + c * 32);
+        umma::tmem_wait_ld();
+        if (!full) {
+#pragma unroll
+          for (int c = 0; c < KPT; ++c)
+            if (!((vis[c >> 5] >> (c & 31)) & 1u)) sv[c] = -INFINITY;
+        }
+        float mx8[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx8[e] = sv[e];
+#pragma unroll
+        for (int c = 8; c < KPT; ++c) mx8[c & 7] = fmaxf(mx8[c & 7], sv[c]);
+        const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
+                               fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]))) *
+                         p.scale_log2;
+        // the maximum moves only past its headroom: weights are at most 2^8
+        const bool grow = mx > m + kRescaleLog2 || (m == -INFINITY && mx > -INFINITY);
+        float fac = 1.f;
+        if (grow) {
+          fac = (m == -INFINITY) ? 0.f : ex2(m - mx);
+          l *= fac;
+          m = mx;
+        }
+        if (it > 0 && __any_sync(0xffffffffu, grow)) {
+          // O_X is quiescent: this QK was issued after the last PV completed,
+          // and the next PV waits for this P
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            float ov[32];
+            umma::tmem_ld32(trow + ocol + c * 32, ov);
+            umma::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) ov[e] *= fac;
+            umma::tmem_st32(trow + ocol + c * 32, ov);
+          }
+        }
+        const float nm = (m == -INFINITY) ? 0.f : -m;
+        float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KPT / 32; ++c) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float a = ex2(fmaf(sv[c * 32 + 2 * e], p.scale_log2, nm));
+            const float b = ex2(fmaf(sv[c * 32 + 2 * e + 1], p.scale_log2, nm));
+            rs[e & 1] += a;
+            rs[2 + (e & 1)] += b;
+            float ah, bh;
+            if constexpr (kBf16) {         // truncated: one byte permute a pair
+              hi[e] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+              ah = __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
+              bh = __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
+            } else {
+              hi[e] = Elem<T>::pack(a, b);
+              Elem<T>::unpack(hi[e], ah, bh);
+            }
+            lo[e] = Elem<T>::pack(a - ah, b - bh);
+          }
+          umma::tmem_st16u(trow + scol + copy * (KPT / 2) + c * 16, hi);
+          umma::tmem_st16u(trow + scol + 64 + copy * (KPT / 2) + c * 16, lo);
+        }
+        if constexpr (COP > 1) {           // the other copies' positions weigh nothing here
+          const uint32_t z[16] = {};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (c / (KPT / 32) != copy) {
+              umma::tmem_st16u(trow + scol + c * 16, z);
+              umma::tmem_st16u(trow + scol + 64 + c * 16, z);
+            }
+          }
+        }
+        l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+        umma::tmem_wait_st();
+        umma::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bs->p_full[x]);
+      }
+
+      // ---- epilogue.  Named barriers are passed whether or not a wait
+      // failed, so that no thread is left behind at one.
+      if (nx > 0 && ok) {
+        ok = __all_sync(0xffffffffu, wait_bar(&bs->pv_done[x], (j - 1) & 1, bs, p.err));
+        umma::fence_after_sync();
+      }
+      float* slot = p.part + ((int64_t)blockIdx.x * 2 + (s.first ? 0 : 1)) * RG * kPartStride<D>;
+      // non-finite V of nodes, which the cleaners took out, for a row that
+      // sees them: its weights are positive, so the sum is the value itself
+      auto add_bad = [&](int row, int col, float* o, int n_col) {
+        const int node = (s.row0 + row) / p.G;
+        const int a = max(ctx, s.t0 * kBN), b = min(end, s.t1 * kBN);
+        for (int pos = a; pos < b; ++pos) {
+          if (!p.mask[(int64_t)(cu0 + node) * p.mask_stride + pos - ctx]) continue;
+          const int pg = p.table[(int64_t)walk.r * p.table_stride + pos / p.page];
+          if ((uint32_t)pg >= (uint32_t)p.n_pages) continue;
+          const T* v = reinterpret_cast<const T*>(p.v) + pg * p.v_sp + s.hk * p.v_sh +
+                       (pos % p.page) * p.v_st + col;
+          for (int e = 0; e < n_col; ++e) {
+            const float y = Elem<T>::to_f32(v[e]);
+            if (!isfinite(y)) o[e] += y;
+          }
+        }
+      };
+      auto store = [&](int row, int col, float M, float L, float* o, auto n_col) {
+        constexpr int N = decltype(n_col)::value;
+        if (!s.whole) {
+          float* d = slot + (int64_t)row * kPartStride<D> + col;
+#pragma unroll
+          for (int e = 0; e < N; e += 4)
+            *reinterpret_cast<float4*>(d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          if (col == 0) *reinterpret_cast<float2*>(slot + (int64_t)row * kPartStride<D> + D) = make_float2(M, L);
+          return;
+        }
+        const int rq = s.row0 + row, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
+        const int64_t t = cu0 + node;
+        const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+        if (col == 0 && p.lse)
+          p.lse[t * p.H + hq] = L > 0.f ? (M + log2f(L)) * kLn2 : (L == L ? -INFINITY : L);
+        const int64_t at = t * p.out_st + hq * p.out_sh + col;
+        if (p.out_f32) {
+          float4* d = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at);
+#pragma unroll
+          for (int e = 0; e < N; e += 4)
+            d[e / 4] = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+        } else {
+          uint4* d = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + at);
+#pragma unroll
+          for (int e = 0; e < N; e += 8)
+            d[e / 8] = make_uint4(Elem<T>::pack(o[e] * inv, o[e + 1] * inv),
+                                  Elem<T>::pack(o[e + 2] * inv, o[e + 3] * inv),
+                                  Elem<T>::pack(o[e + 4] * inv, o[e + 5] * inv),
+                                  Elem<T>::pack(o[e + 6] * inv, o[e + 7] * inv));
+        }
+      };
+      if (two) {
+        // every row is one thread's
+        const volatile int* b0 = &bs->bad[0][0];
+        const volatile int* b1 = &bs->bad[1][0];
+        const bool fix = b0[si % kBadSlots] || b1[si % kBadSlots];
+        if (ok) {
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            float ov[32];
+            umma::tmem_ld32(trow + ocol + c * 32, ov);
+            umma::tmem_wait_ld();
+            if (rr < rows) {
+              if (fix) add_bad(rr + x * 128, c * 32, ov, 32);
+              store(rr + x * 128, c * 32, m, l, ov, std::integral_constant<int, 32>());
+            }
+          }
+        }
+      } else {
+        // join the 2 COP states of every row.  All states agree on the row's
+        // maximum through shared memory, then add their scaled outputs into
+        // one fp32 copy in the query tile's space (its MMAs have completed):
+        // in round k state i adds column slice (i + k) mod 2 COP, so all
+        // threads work at once and the order of the sum is fixed.
+        constexpr int NS = 2 * COP, HALVES = COP == 1 ? 2 : 1;
+        constexpr int DA = D / HALVES, W = DA / NS;          // columns held, of a slice
+        static_assert(RPC * DA * 4 <= Gm::kTileBytes, "scratch fits the query tile");
+        sm_m[x * 128 + r] = m;
+        sm_l[x * 128 + r] = l;
+        named_bar_sync(1, 256);
+        const volatile int* b0 = &bs->bad[0][0];
+        const volatile int* b1 = &bs->bad[1][0];
+        const bool fix = b0[si % kBadSlots] || b1[si % kBadSlots];
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) M = fmaxf(M, sm_m[(i / COP) * 128 + (i % COP) * RPC + rr]);
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          const int at = (i / COP) * 128 + (i % COP) * RPC + rr;
+          const float mi = sm_m[at], li = sm_l[at];
+          L = fmaf(li, (mi == -INFINITY) ? (li == li ? 0.f : 1.f) : ex2(mi - M), L);
+        }
+        const float w = (m == -INFINITY) ? (l == l ? 0.f : 1.f) : ex2(m - M);
+        const int state = x * COP + copy;
+        float* acc = reinterpret_cast<float*>(smem + Gm::kOffQ);
+        // float4 granule `gr` of a row: swizzled against bank conflicts
+        auto granule = [&](int row, int gr) {
+          return reinterpret_cast<float4*>(acc + row * DA + ((gr ^ (row & (DA / 4 < 8 ? DA / 4 - 1 : 7))) << 2));
+        };
+        for (int hf = 0; hf < HALVES; ++hf) {
+#pragma unroll 1
+          for (int k = 0; k < NS; ++k) {
+            const int sl = (state + k) % NS;
+            float ov[W];
+            if (nx > 0 && ok) {
+              tmem_ld(trow + ocol + hf * DA + sl * W, ov);
+              umma::tmem_wait_ld();
+            } else {
+#pragma unroll
+              for (int e = 0; e < W; ++e) ov[e] = 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < W; e += 4) {
+              float4* d = granule(rr, (sl * W + e) >> 2);
+              float4 y = k == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *d;
+              y.x = fmaf(ov[e], w, y.x);
+              y.y = fmaf(ov[e + 1], w, y.y);
+              y.z = fmaf(ov[e + 2], w, y.z);
+              y.w = fmaf(ov[e + 3], w, y.w);
+              *d = y;
+            }
+            named_bar_sync(1, 256);
+          }
+          if (hf == 0) {
+            if (state == 0) {                  // everyone has read m and l
+              sm_m[rr] = M;
+              sm_l[rr] = L;
+            }
+            named_bar_sync(1, 256);
+          }
+          if (ok) {
+            for (int i = tid; i < rows * (DA / 8); i += 256) {
+              const int row = i / (DA / 8), c = i % (DA / 8);
+              const float4 y0 = *granule(row, 2 * c), y1 = *granule(row, 2 * c + 1);
+              float o[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
+              if (fix) add_bad(row, hf * DA + c * 8, o, 8);
+              store(row, hf * DA + c * 8, sm_m[row], sm_l[row], o, std::integral_constant<int, 8>());
+            }
+          }
+          if (HALVES > 1 && hf == 0) named_bar_sync(1, 256);   // before the second half
+        }
+      }
+      ++si;
+    }
+  }
+  }
+
+  // ---- teardown: every TMEM access and MMA has completed
+  umma::fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    umma::fence_after_sync();
+    umma::tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// ======================================================================
+// tree_merge_kernel: joins the parts of segments that were cut.  Block
+// (c - 1, y) looks at the cut between CTAs c - 1 and c; the first cut inside
+// a segment owns it, y takes 8 of its rows, a warp each.
+constexpr int kMergeWarps = 8;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32) tree_rows_kernel(const Params p) {
+__global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
+    const __grid_constant__ Params p, int n_cta, int RG) {
   constexpr int C = D / 32;
-  __shared__ float s_m[kWarps], s_l[kWarps], s_o[kWarps][D];
-  const int t = (int)blockIdx.x, h = (int)blockIdx.y, hk = h / p.G;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (t >= p.cu[p.R]) return;
-  int lo = 0, n = p.R;                 // the request of row t
-  while (n > 1) {
-    const int half = n >> 1;
-    if (p.cu[lo + half] <= t) {
-      lo += half;
-      n -= half;
-    } else {
-      n = half;
+  grid_dep_wait();
+  const int c = (int)blockIdx.x + 1;
+  const Desc d = p.desc[c];
+  auto cut = [&](int i) { return (int64_t)i * d.total / n_cta; };
+  const int64_t uc = cut(c);
+  if (uc >= d.total || d.start >= uc || cut(c - 1) > d.start) return;
+  const int row = (int)blockIdx.y * kMergeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= d.rows) return;
+  auto part = [&](int i) {      // CTA i's rows of this segment
+    const int sl = i == c - 1 && cut(c - 1) < d.start ? 1 : 0;
+    return p.part + (((int64_t)i * 2 + sl) * RG + row) * kPartStride<D>;
+  };
+  // the CTAs that hold a part: c - 1, then those that begin before the end
+  int last = c;
+  while (last + 1 < n_cta && cut(last + 1) < d.end) ++last;
+  float M = -INFINITY, L = 0.f, acc[C];
+#pragma unroll
+  for (int e = 0; e < C; ++e) acc[e] = 0.f;
+  constexpr int B = 8;
+  for (int i0 = c - 1; i0 <= last; i0 += B) {
+    float mi[B], li[B], o[B][C];
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      const int i = i0 + u;
+      mi[u] = -INFINITY;
+      li[u] = 0.f;
+#pragma unroll
+      for (int e = 0; e < C; ++e) o[u][e] = 0.f;
+      if (i <= last && cut(i) < cut(i + 1)) {
+        const float* s = part(i);
+        const float2 ml = *reinterpret_cast<const float2*>(s + D);
+        mi[u] = ml.x;
+        li[u] = ml.y;
+        if constexpr (C == 4) {
+          const float4 y = *reinterpret_cast<const float4*>(s + lane * 4);
+          o[u][0] = y.x;
+          o[u][1] = y.y;
+          o[u][2] = y.z;
+          o[u][3] = y.w;
+        } else {
+          const float2 y = *reinterpret_cast<const float2*>(s + lane * 2);
+          o[u][0] = y.x;
+          o[u][1] = y.y;
+        }
+      }
     }
-  }
-  const int r = lo, node = t - p.cu[r];
-  const int nodes = min(p.cu[r + 1] - p.cu[r], p.max_nodes);
-  if (node < 0 || node >= nodes) return;
-  const int64_t ctx = max(p.ctx[r], 0);
-  const int64_t end = min(ctx + nodes, (int64_t)p.max_blocks * p.page);
-  const T* q = reinterpret_cast<const T*>(p.q) + t * p.q_st + h * p.q_sh + lane * C;
-  const uint8_t* mask = p.mask + t * p.mask_stride;
-  const int32_t* tab = p.table + r * p.table_stride;
-  float qf[C], o[C], m = -INFINITY, l = 0.f;
+    float Mn = M;
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    qf[c] = Elem<T>::to_f32(q[c]);
-    o[c] = 0.f;
-  }
-  for (int64_t j = warp; j < end; j += kWarps) {
-    if (j >= ctx && !mask[j - ctx]) continue;
-    const int32_t pg = tab[j / p.page];
-    const int row = (int)(j % p.page);
-    const bool in = (uint32_t)pg < (uint32_t)p.n_pages;
-    float s = 0.f;
-    if (in) {
-      const T* k = reinterpret_cast<const T*>(p.k) + pg * p.k_sp + hk * p.k_sh + row * p.k_st + lane * C;
+    for (int u = 0; u < B; ++u) Mn = fmaxf(Mn, mi[u]);
+    const float a = (M == -INFINITY) ? (L == L ? 0.f : 1.f) : ex2(M - Mn);
+    L *= a;
 #pragma unroll
-      for (int c = 0; c < C; ++c) s = fmaf(qf[c], Elem<T>::to_f32(k[c]), s);
+    for (int e = 0; e < C; ++e) acc[e] *= a;
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      const float w = (mi[u] == -INFINITY) ? (li[u] == li[u] ? 0.f : 1.f) : ex2(mi[u] - Mn);
+      L = fmaf(li[u], w, L);
+#pragma unroll
+      for (int e = 0; e < C; ++e) acc[e] = fmaf(o[u][e], w, acc[e]);
     }
+    M = Mn;
+  }
+  const int rq = d.row0 + row, node = rq / p.G, hq = d.hk * p.G + rq - node * p.G;
+  const int64_t t = d.cu0 + node;
+  const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+  if (lane == 0 && p.lse)
+    p.lse[t * p.H + hq] = L > 0.f ? (M + log2f(L)) * kLn2 : (L == L ? -INFINITY : L);
+  const int64_t at = t * p.out_st + hq * p.out_sh + lane * C;
+  if (p.out_f32) {
+    float* o = reinterpret_cast<float*>(p.out) + at;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    s *= p.scale_log2;
-    const float mn = fmaxf(m, s);
-    const float a = m == -INFINITY ? 0.f : exp2f(m - mn);
-    const float w = s == -INFINITY ? 0.f : exp2f(s - mn);
-    l = l * a + w;
-    const T* v = reinterpret_cast<const T*>(p.v) + (in ? pg * p.v_sp + hk * p.v_sh + row * p.v_st + lane * C : 0);
+    for (int e = 0; e < C; ++e) o[e] = acc[e] * inv;
+  } else {
+    uint32_t* o = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + at);
 #pragma unroll
-    for (int c = 0; c < C; ++c) o[c] = o[c] * a + (in ? w * Elem<T>::to_f32(v[c]) : 0.f);
-    m = mn;
+    for (int e = 0; e < C; e += 2) o[e / 2] = Elem<T>::pack(acc[e] * inv, acc[e + 1] * inv);
   }
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
-  }
-#pragma unroll
-  for (int c = 0; c < C; ++c) s_o[warp][lane * C + c] = o[c];
-  __syncthreads();
-  float M = -INFINITY, L = 0.f;
-  for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w]);
-  const int d = threadIdx.x;
-  float acc = 0.f;
-  for (int w = 0; w < kWarps; ++w) {
-    const float e = s_m[w] == -INFINITY ? 0.f : exp2f(s_m[w] - M);
-    L = fmaf(s_l[w], e, L);
-    if (d < D) acc = fmaf(s_o[w][d], e, acc);
-  }
-  if (d < D) {
-    const float x = L > 0.f ? acc / L : (L == L ? 0.f : L);
-    const int64_t at = t * p.out_st + h * p.out_sh + d;
-    if (p.out_f32) reinterpret_cast<float*>(p.out)[at] = x;
-    else reinterpret_cast<T*>(p.out)[at] = Elem<T>::from_f32(x);
-  }
-  if (d == 0 && p.lse)
-    p.lse[(int64_t)t * p.H + h] = L > 0.f ? (M + log2f(L)) * kLn2 : (L == L ? -INFINITY : L);
 }
 
 }  // namespace tree
 
 // ================================================================ host side
+namespace tree {
+
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                             const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeFn encode_fn() {
+  static EncodeFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
+            cudaSuccess && q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(ptr);
+  });
+  return fn;
+}
+
+// The tensor map of a pool's K or V: {D, page, H_kv, n_pages}, boxes of 64
+// elements x `box` rows, 128-byte swizzle, zeros outside.  A map depends on
+// the description alone; the last ones made are kept.
+struct MapKey {
+  const void* ptr;
+  int64_t sp, sh, st;
+  int32_t n_pages, H_kv, page, D, dtype, box;
+};
+
+static int encode_pool(const MapKey& key, CUtensorMap* out) {
+  struct Slot {
+    MapKey key;
+    CUtensorMap map;
+    bool used;
+  };
+  constexpr int kSlots = 256;
+  static std::mutex mu;
+  static Slot cache[kSlots];
+  uint64_t h = reinterpret_cast<uint64_t>(key.ptr) >> 8;
+  for (uint64_t v : {(uint64_t)key.sp, (uint64_t)key.sh, (uint64_t)key.st, (uint64_t)key.n_pages,
+                     (uint64_t)key.page})
+    h = (h ^ v) * 0x9E3779B97F4A7C15ull;
+  Slot& s = cache[(h >> 32) % kSlots];
+  std::lock_guard<std::mutex> lk(mu);
+  const bool same = s.used && s.key.ptr == key.ptr && s.key.sp == key.sp && s.key.sh == key.sh &&
+                    s.key.st == key.st && s.key.n_pages == key.n_pages && s.key.H_kv == key.H_kv &&
+                    s.key.page == key.page && s.key.D == key.D && s.key.dtype == key.dtype &&
+                    s.key.box == key.box;
+  if (!same) {
+    EncodeFn fn = encode_fn();
+    if (!fn) return fail(HALO_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+    // the stride of a dimension of one is never used, but has to be legal
+    const int64_t st = key.st * 2;
+    const int64_t sh = key.H_kv > 1 ? key.sh * 2 : st;
+    const int64_t sp = key.n_pages > 1 ? key.sp * 2 : st;
+    cuuint64_t dims[4] = {(cuuint64_t)key.D, (cuuint64_t)key.page, (cuuint64_t)key.H_kv,
+                          (cuuint64_t)key.n_pages};
+    cuuint64_t str[3] = {(cuuint64_t)st, (cuuint64_t)sh, (cuuint64_t)sp};
+    cuuint32_t box[4] = {64, (cuuint32_t)key.box, 1, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r =
+        fn(&s.map, key.dtype == HALO_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+           4, const_cast<void*>(key.ptr), dims, str, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    s.used = r == CUDA_SUCCESS;
+    if (r != CUDA_SUCCESS)
+      return fail(HALO_ERR_INVALID_ARG,
+                  "page pool tensor map encode failed (%d): %d pages, page %d, strides %lld %lld "
+                  "%lld bytes", (int)r, key.n_pages, key.page, (long long)sp, (long long)sh,
+                  (long long)st);
+    s.key = key;
+  }
+  *out = s.map;
+  return HALO_OK;
+}
+
 static bool rows16(const void* p, int64_t a, int64_t b, int64_t c, int elt) {
   return ((reinterpret_cast<uintptr_t>(p) | (uint64_t)(a * elt) | (uint64_t)(b * elt) |
            (uint64_t)(c * elt)) & 15) == 0;
 }
 
-static int tree_check(const halo_page_pool_t* pool, const halo_tree_problem_t* pb) {
+static int check(const halo_page_pool_t* pool, const halo_tree_problem_t* pb) {
   if (!pool || !pb) return fail(HALO_ERR_INVALID_ARG, "page pool/problem is NULL");
   if (pool->dtype != HALO_DTYPE_BF16 && pool->dtype != HALO_DTYPE_F16)
     return fail(HALO_ERR_UNSUPPORTED, "tree attention needs bf16 or fp16 (dtype %d)", pool->dtype);
@@ -148,7 +1131,8 @@ static int tree_check(const halo_page_pool_t* pool, const halo_tree_problem_t* p
     return fail(HALO_ERR_INVALID_ARG, "H=%d not divisible by H_kv=%d", pb->H, pool->H_kv);
   if (pb->max_nodes > 1024)
     return fail(HALO_ERR_UNSUPPORTED, "%d nodes a request (at most 1024)", pb->max_nodes);
-  if ((int64_t)pb->max_blocks * pool->page_size + 1024 > INT_MAX)
+  if (pb->H > 65535) return fail(HALO_ERR_UNSUPPORTED, "%d heads", pb->H);
+  if ((int64_t)pb->max_blocks * pool->page_size + 2048 > INT_MAX)
     return fail(HALO_ERR_UNSUPPORTED, "block tables of %d pages of %d are too long", pb->max_blocks,
                 pool->page_size);
   if (!(pb->scale > 0.f) || !std::isfinite(pb->scale))
@@ -156,23 +1140,62 @@ static int tree_check(const halo_page_pool_t* pool, const halo_tree_problem_t* p
   return HALO_OK;
 }
 
-}  // namespace halo
-
-using namespace halo;
-
-extern "C" int64_t halo_tree_workspace_bytes(const halo_page_pool_t* pool,
-                                             const halo_tree_problem_t* pb) {
-  const int rc = tree_check(pool, pb);
-  return rc != HALO_OK ? rc : 0;
+// Rows of a group, from the most rows a request can have on one K/V head:
+// the smallest of 32, 64, 128 and 256 that holds them (256 at most).
+static int group_rows(const halo_page_pool_t* pool, const halo_tree_problem_t* pb) {
+  const int64_t rows = (int64_t)pb->max_nodes * (pb->H / pool->H_kv);
+  return rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
 }
 
-extern "C" int32_t halo_tree_attention(const halo_page_pool_t* pool, const halo_tree_problem_t* pb,
-                                       void* workspace, int64_t workspace_bytes,
-                                       halo_stream_t stream) {
-  int rc = tree_check(pool, pb);
+static int64_t desc_bytes(int n_cta) { return ((int64_t)n_cta * sizeof(Desc) + 255) & ~int64_t(255); }
+
+static int64_t ws_bytes(const halo_page_pool_t* pool, const halo_tree_problem_t* pb) {
+  const int n = device_sms();
+  return desc_bytes(n) + (int64_t)n * 2 * group_rows(pool, pb) * (pool->D + 4) * sizeof(float);
+}
+
+template <typename T, int D, int KPT, int QT>
+static int launch(const Params& p, int n_cta, cudaStream_t st) {
+  using Gm = Geom<D, QT>;
+  constexpr int RG = KPT * QT == 256 ? 256 : KPT;     // copies x rows = 128
+  auto kernel = tree_kernel<T, D, KPT, QT>;
+  static std::once_flag once[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  cudaError_t e = cudaSuccess;
+  std::call_once(once[dev & 63], [&] {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Gm::kSmemBytes);
+  });
+  if (e != cudaSuccess) return cuda_fail(e, "tree_kernel shared-memory attribute");
+  e = launch_dependent(kernel, dim3((unsigned)n_cta), dim3(kThreads), Gm::kSmemBytes, st, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "tree_kernel launch");
+  count_launches();
+  if (n_cta > 1) {
+    e = launch_dependent(tree_merge_kernel<T, D>,
+                         dim3((unsigned)n_cta - 1, (RG + kMergeWarps - 1) / kMergeWarps),
+                         dim3(kMergeWarps * 32), 0, st, p, n_cta, (int)RG);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "tree_merge_kernel launch");
+    count_launches();
+  }
+  return HALO_OK;
+}
+
+template <typename T, int D>
+static int dispatch(int rows, const Params& p, int n_cta, cudaStream_t st) {
+  switch (rows) {
+    case 32: return launch<T, D, 32, 1>(p, n_cta, st);
+    case 64: return launch<T, D, 64, 1>(p, n_cta, st);
+    case 128: return launch<T, D, 128, 1>(p, n_cta, st);
+    default: return launch<T, D, 128, 2>(p, n_cta, st);
+  }
+}
+
+static int run(const halo_page_pool_t* pool, const halo_tree_problem_t* pb, void* workspace,
+               int64_t workspace_bytes, halo_stream_t stream) {
+  int rc = check(pool, pb);
   if (rc != HALO_OK) return rc;
-  (void)workspace;
-  (void)workspace_bytes;
   if (pb->R == 0 || pb->T == 0 || pb->max_nodes == 0) return HALO_OK;
   if (!pool->k || !pool->v || !pb->q || !pb->out || !pb->context_lens || !pb->cu_nodes ||
       !pb->mask || (pb->max_blocks > 0 && !pb->block_tables))
@@ -181,26 +1204,38 @@ extern "C" int32_t halo_tree_attention(const halo_page_pool_t* pool, const halo_
     return fail(HALO_ERR_UNSUPPORTED, "out dtype must be fp32 or the pool's dtype");
   if (!rows16(pool->k, pool->k_stride_p, pool->k_stride_h, pool->k_stride_t, 2) ||
       !rows16(pool->v, pool->v_stride_p, pool->v_stride_h, pool->v_stride_t, 2) ||
-      pool->k_stride_t <= 0 || pool->v_stride_t <= 0)
-    return fail(HALO_ERR_MISALIGNED, "page rows must be 16-byte aligned");
+      pool->k_stride_t <= 0 || pool->v_stride_t <= 0 ||
+      (pool->H_kv > 1 && (pool->k_stride_h <= 0 || pool->v_stride_h <= 0)) ||
+      (pool->n_pages > 1 && (pool->k_stride_p <= 0 || pool->v_stride_p <= 0)))
+    return fail(HALO_ERR_MISALIGNED, "page rows must be 16-byte aligned, strides positive");
   if (!rows16(pb->q, pb->q_stride_t, pb->q_stride_h, 0, 2))
     return fail(HALO_ERR_MISALIGNED, "q rows must be 16-byte aligned");
   if (!rows16(pb->out, pb->out_stride_t, pb->out_stride_h, 0,
               pb->out_dtype == HALO_DTYPE_F32 ? 4 : 2))
     return fail(HALO_ERR_MISALIGNED, "out rows must be 16-byte aligned");
-  if (pb->H > 65535) return fail(HALO_ERR_UNSUPPORTED, "%d heads", pb->H);
-  tree::Params p{};
-  p.k = static_cast<const char*>(pool->k);
-  p.v = static_cast<const char*>(pool->v);
-  p.k_sp = pool->k_stride_p;
-  p.k_sh = pool->k_stride_h;
-  p.k_st = pool->k_stride_t;
-  p.v_sp = pool->v_stride_p;
-  p.v_sh = pool->v_stride_h;
-  p.v_st = pool->v_stride_t;
+  const int64_t need = ws_bytes(pool, pb);
+  if (!workspace || workspace_bytes < need)
+    return fail(HALO_ERR_WORKSPACE, "tree workspace has %lld bytes, needs %lld",
+                (long long)(workspace ? workspace_bytes : 0), (long long)need);
+  if (reinterpret_cast<uintptr_t>(workspace) & 255)
+    return fail(HALO_ERR_MISALIGNED, "tree workspace must be 256-byte aligned");
+
+  Params p{};
+  p.box = 8;
+  while (p.box < kBN && pool->page_size % (2 * p.box) == 0) p.box *= 2;
+  rc = encode_pool({pool->k, pool->k_stride_p, pool->k_stride_h, pool->k_stride_t, pool->n_pages,
+                    pool->H_kv, pool->page_size, pool->D, pool->dtype, p.box}, &p.kmap);
+  if (rc != HALO_OK) return rc;
+  rc = encode_pool({pool->v, pool->v_stride_p, pool->v_stride_h, pool->v_stride_t, pool->n_pages,
+                    pool->H_kv, pool->page_size, pool->D, pool->dtype, p.box}, &p.vmap);
+  if (rc != HALO_OK) return rc;
   p.q = static_cast<const char*>(pb->q);
   p.q_st = pb->q_stride_t;
   p.q_sh = pb->q_stride_h;
+  p.v = static_cast<const char*>(pool->v);
+  p.v_sp = pool->v_stride_p;
+  p.v_sh = pool->v_stride_h;
+  p.v_st = pool->v_stride_t;
   p.table = pb->block_tables;
   p.table_stride = pb->table_stride;
   p.ctx = pb->context_lens;
@@ -216,23 +1251,39 @@ extern "C" int32_t halo_tree_attention(const halo_page_pool_t* pool, const halo_
   p.R = pb->R;
   p.T = pb->T;
   p.H = pb->H;
+  p.H_kv = pool->H_kv;
   p.G = pb->H / pool->H_kv;
   p.max_nodes = pb->max_nodes;
   p.max_blocks = pb->max_blocks;
   p.n_pages = pool->n_pages;
   p.page = pool->page_size;
+  const int n_cta = device_sms();
+  p.desc = static_cast<Desc*>(workspace);
+  p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + desc_bytes(n_cta));
+  p.err = device_error_ptr();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid((unsigned)pb->T, (unsigned)pb->H);
-  const int threads = tree::kWarps * 32;
-  if (pool->dtype == HALO_DTYPE_BF16) {
-    if (pool->D == 128) tree::tree_rows_kernel<__nv_bfloat16, 128><<<grid, threads, 0, st>>>(p);
-    else tree::tree_rows_kernel<__nv_bfloat16, 64><<<grid, threads, 0, st>>>(p);
-  } else {
-    if (pool->D == 128) tree::tree_rows_kernel<__half, 128><<<grid, threads, 0, st>>>(p);
-    else tree::tree_rows_kernel<__half, 64><<<grid, threads, 0, st>>>(p);
-  }
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "tree_rows_kernel launch");
-  count_launches();
-  return HALO_OK;
+  const int rows = group_rows(pool, pb);
+  if (pool->dtype == HALO_DTYPE_BF16)
+    return pool->D == 128 ? dispatch<__nv_bfloat16, 128>(rows, p, n_cta, st)
+                          : dispatch<__nv_bfloat16, 64>(rows, p, n_cta, st);
+  return pool->D == 128 ? dispatch<__half, 128>(rows, p, n_cta, st)
+                        : dispatch<__half, 64>(rows, p, n_cta, st);
+}
+
+}  // namespace tree
+}  // namespace halo
+
+using namespace halo;
+
+extern "C" int64_t halo_tree_workspace_bytes(const halo_page_pool_t* pool,
+                                             const halo_tree_problem_t* pb) {
+  const int rc = tree::check(pool, pb);
+  if (rc != HALO_OK) return rc;
+  return pb->R == 0 || pb->T == 0 || pb->max_nodes == 0 ? 0 : tree::ws_bytes(pool, pb);
+}
+
+extern "C" int32_t halo_tree_attention(const halo_page_pool_t* pool, const halo_tree_problem_t* pb,
+                                       void* workspace, int64_t workspace_bytes,
+                                       halo_stream_t stream) {
+  return tree::run(pool, pb, workspace, workspace_bytes, stream);
 }

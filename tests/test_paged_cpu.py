@@ -53,6 +53,20 @@ def test_tree_attention_refusals(pool, prob, code):
     assert lib.halo_last_error_string()
 
 
+def test_tree_attention_workspace():
+    from halo_b200 import _lib as L
+    lib = L.lib()
+    po, pr = _pool(L), _tree(L)
+    need = lib.halo_tree_workspace_bytes(ctypes.byref(po), ctypes.byref(pr))
+    assert need > 0
+    for ws, n, code in ((None, need, L.HALO_ERR_WORKSPACE), (0x100000, need - 1, L.HALO_ERR_WORKSPACE),
+                        (0x100010, need, L.HALO_ERR_MISALIGNED)):
+        assert lib.halo_tree_attention(ctypes.byref(po), ctypes.byref(pr), ws, n, None) == code
+    # more rows a K/V head, larger parts
+    wide = lib.halo_tree_workspace_bytes(ctypes.byref(po), ctypes.byref(_tree(L, max_nodes=1000)))
+    assert wide > need
+
+
 def test_tree_attention_nothing_to_do_and_null_arguments():
     from halo_b200 import _lib as L
     lib = L.lib()
