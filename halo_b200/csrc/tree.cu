@@ -96,26 +96,14 @@ struct Geom {
 struct Bars {
   uint64_t q_full;
   uint64_t k_full[6], k_empty[6], v_full[6], v_ready[6], v_empty[6];
-  uint64_t s_full[2], p_full[2], pv_done[2], mma_done;
+  uint64_t s_full[2], p_full[2], pv_done[2], mma_done[2];
   int64_t scan[12];
   int64_t base0, total;
   uint32_t tmem_base;
   int abort_flag, r0;
-  int bad[2][kBadSlots];
+  int bad[kBadSlots];
 };
 static_assert(sizeof(Bars) <= 1024, "barrier block");
-
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_addr(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
 
 // Bounded wait that also ends when another role gave up.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Bars* bs,
@@ -215,8 +203,8 @@ __device__ __forceinline__ void tmem_ld(uint32_t a, float (&v)[16]) {
 }
 __device__ __forceinline__ void tmem_ld(uint32_t a, float (&v)[32]) { umma::tmem_ld32(a, v); }
 
-// A value the compiler cannot see through: keeps it from hoisting every
-// unrolled MMA's descriptor out of the issuer's polling loop.
+// A value the compiler cannot see through: keeps it from holding every
+// unrolled MMA's descriptor in a register across the loop.
 __device__ __forceinline__ uint64_t opaque(uint64_t v) {
   asm volatile("mov.b64 %0, %0;" : "+l"(v));
   return v;
@@ -235,15 +223,16 @@ __device__ __forceinline__ bool bad16(uint32_t x) {   // inf or NaN in the low 1
 //               that divides the page), through two rings; the lanes issue a
 //               tile's boxes side by side.  Boxes behind the last position
 //               or without a page start outside the tensor: zeros.
-//   warp 1      TMEM owner; lane 0 issues every MMA, polling for whichever
-//               step has its inputs ready.
-//   warps 2, 3  clean V: in tiles that reach behind the context, rows behind
+//   warps 1, 3  lane 0 issues the MMAs of stream 0 / 1; warp 1 owns TMEM.
+//   warp 2      cleans V: in tiles that reach behind the context, rows behind
 //               the last node and elements that are not finite become zero
 //               (a weight of zero would turn them into NaN); a node that does
 //               see such an element gets it back in the epilogue.
 //   warps 4-7   softmax stream 0, warps 8-11 stream 1 (thread = TMEM lane).
 // Each stream has its own scores S_X (128 TMEM columns, overwritten in place
 // by the weights P_X) and output O_X: S_X = Q K^T, O_X += P_X V, both M128.
+// One thread issues a stream's MMAs, which execute in that order: the QK that
+// overwrites P_X follows the PV that reads it without waiting for its end.
 // P is split into a 16-bit value and a 16-bit remainder (two MMAs), ~16
 // significant bits: one 16-bit P would cost up to 2^-9 |v|, as much as the
 // output's own rounding.  Sums, maxima and O are fp32.
@@ -276,15 +265,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       mbar_init(&bs->k_full[i], 1);
       mbar_init(&bs->k_empty[i], 2);
       mbar_init(&bs->v_full[i], 1);
-      mbar_init(&bs->v_ready[i], 2);
+      mbar_init(&bs->v_ready[i], 1);
       mbar_init(&bs->v_empty[i], 2);
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&bs->s_full[x], 1);
       mbar_init(&bs->p_full[x], 4);
       mbar_init(&bs->pv_done[x], 1);
+      mbar_init(&bs->mma_done[x], 1);
     }
-    mbar_init(&bs->mma_done, 1);
     bs->abort_flag = 0;
     fence_mbar_init();
   }
@@ -438,127 +427,73 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           if (gv > 0 && n > 0) mbar_wait(&bs->v_full[i], (n - 1) & 1, p.err);
         }
       }
-    } else if (warp == 1) {
-      // -------------------------------------------------------- MMA issuer
+    } else if (warp & 1) {
+      // -------------------------------------------------------- MMA issuer X
       if (lane == 0) {
+        const int x = warp >> 1;
         constexpr uint32_t kIdQK = umma::instr_desc_f16(128, kBN, kBf16, false, false);
         constexpr uint32_t kIdPV = umma::instr_desc_f16(128, D, kBf16, false, true);
         const uint64_t qdesc0 = umma::smem_desc_sw128(sQ, 16, 1024);
         const uint64_t kdesc0 = umma::smem_desc_sw128(sK, 16, 1024);
         const uint64_t vdesc0 = umma::smem_desc_sw128(sV, Gm::kBlockBytes, 1024);
-        // K (V) tiles below kpre (vpre) have landed: barriers are probed in
-        // tile order, so none is probed more than one phase ahead
-        int kpre = 0, vpre = 0;
-        auto landed = [&](int& pre, uint64_t* bar, int st, int g) {
-          while (pre <= g && mbar_test(&bar[pre % st], (pre / st) & 1)) ++pre;
-          return g < pre;
-        };
-        int jq[2] = {0, 0}, jp[2] = {0, 0};   // QK / PV issued a stream, all segments
-        int qseq[2] = {0, 0}, seq = 0;        // issue order of each stream's latest QK
-        int g0 = 0, si = 0;
+        const uint32_t pc = tmem + x * 128, oc = tmem + Gm::kColO + x * D;
+        int g0 = 0, si = 0, j = 0;            // tiles before the segment; segments; P waits
         bool ok = true;
-        uint64_t t_idle = 0;
-        int idle = 0;
         while (ok && walk.next(p, s)) {
           const bool two = s.rows > 128;
           const int n = s.t1 - s.t0, step = two ? 1 : 2;
-          const int nx[2] = {two ? n : (n + 1) / 2, two ? n : n / 2};
-          int a[2] = {0, 0}, b[2] = {0, 0};   // QK / PV issued in this segment
+          const int nx = two ? n : (x ? n / 2 : (n + 1) / 2);
+          const uint64_t qd0 = qdesc0 + (uint64_t)(((two ? x : 0) * Gm::kTileBytes) >> 4);
+          int g = g0 + (two ? 0 : x);
+          auto qk = [&]() {                   // S_X = Q K(g)^T
+            const int ik = g % SK;
+            if (!wait_bar(&bs->k_full[ik], (g / SK) & 1, bs, p.err)) return false;
+            umma::fence_after_sync();
+            const uint64_t qd = opaque(qd0);
+            const uint64_t kd = opaque(kdesc0 + (uint64_t)((ik * Gm::kTileBytes) >> 4));
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = ((kk >> 2) * Gm::kBlockBytes + (kk & 3) * 32) >> 4;
+              umma::mma_ss(pc, qd + off, kd + off, kIdQK, kk > 0);
+            }
+            umma::commit(&bs->s_full[x]);
+            umma::commit(&bs->k_empty[ik]);
+            return true;
+          };
           ok = wait_bar(&bs->q_full, si & 1, bs, p.err);
-          while (ok && (b[0] < nx[0] || b[1] < nx[1])) {
-            bool did = false;
+          if (ok && nx > 0) ok = qk();
+          for (int it = 0; ok && it < nx; ++it, ++j) {
+            const int iv = g % SV;
+            ok = wait_bar(&bs->p_full[x], j & 1, bs, p.err) &&
+                 wait_bar(&bs->v_ready[iv], (g / SV) & 1, bs, p.err);
+            if (!ok) break;
+            umma::fence_after_sync();
+            const uint64_t vd = opaque(vdesc0 + (uint64_t)((iv * Gm::kTileBytes) >> 4));
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              if (b[x] < a[x]) {              // O_X += P_X V
-                const int g = g0 + (two ? 0 : x) + b[x] * step;
-                if (mbar_test(&bs->p_full[x], jp[x] & 1) && landed(vpre, bs->v_ready, SV, g)) {
-                  umma::fence_after_sync();
-                  const uint32_t pc = tmem + x * 128, oc = tmem + Gm::kColO + x * D;
-                  const int iv = g % SV;
-                  const uint64_t vd = opaque(vdesc0 + (uint64_t)((iv * Gm::kTileBytes) >> 4));
+            for (int kk = 0; kk < kBN / 16; ++kk)   // O_X += P_X V(g)
+              umma::mma_ts(oc, pc + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), kIdPV,
+                           it > 0 || kk > 0);
 #pragma unroll
-                  for (int kk = 0; kk < kBN / 16; ++kk)
-                    umma::mma_ts(oc, pc + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), kIdPV,
-                                 b[x] > 0 || kk > 0);
-#pragma unroll
-                  for (int kk = 0; kk < kBN / 16; ++kk)
-                    umma::mma_ts(oc, pc + 64 + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4),
-                                 kIdPV, true);
-                  umma::commit(&bs->pv_done[x]);
-                  umma::commit(&bs->v_empty[iv]);
-                  ++jp[x];
-                  ++b[x];
-                  did = true;
-                }
-              }
-              if (a[x] < nx[x] && a[x] == b[x]) {   // S_X = Q K^T, S_X free
-                const int g = g0 + (two ? 0 : x) + a[x] * step;
-                if ((jq[x] == 0 || mbar_test(&bs->pv_done[x], (jq[x] - 1) & 1)) &&
-                    landed(kpre, bs->k_full, SK, g)) {
-                  umma::fence_after_sync();
-                  const int ik = g % SK;
-                  const uint64_t qd =
-                      opaque(qdesc0 + (uint64_t)(((two ? x : 0) * Gm::kTileBytes) >> 4));
-                  const uint64_t kd = opaque(kdesc0 + (uint64_t)((ik * Gm::kTileBytes) >> 4));
-#pragma unroll
-                  for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = ((kk >> 2) * Gm::kBlockBytes + (kk & 3) * 32) >> 4;
-                    umma::mma_ss(tmem + x * 128, qd + off, kd + off, kIdQK, kk > 0);
-                  }
-                  umma::commit(&bs->s_full[x]);
-                  umma::commit(&bs->k_empty[ik]);
-                  qseq[x] = ++seq;
-                  ++jq[x];
-                  ++a[x];
-                  did = true;
-                }
-              }
-            }
-            if (did) {
-              idle = 0;
-              continue;
-            }
-            // Nothing ready: sleep in hardware on what is expected first: a PV
-            // about to complete, the oldest pending P, else V, else K.
-            int xo = -1, xq = -1;
-            if (b[0] < a[0]) xo = 0;
-            if (b[1] < a[1] && (xo < 0 || qseq[1] < qseq[0])) xo = 1;
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-              if (a[x] < nx[x] && a[x] == b[x] && jq[x] > 0 &&
-                  !mbar_test(&bs->pv_done[x], (jq[x] - 1) & 1))
-                xq = x;
-            if (xq >= 0)
-              mbar_try_wait_hint(&bs->pv_done[xq], (jq[xq] - 1) & 1, 1000);
-            else if (xo >= 0 && !mbar_test(&bs->p_full[xo], jp[xo] & 1))
-              mbar_try_wait_hint(&bs->p_full[xo], jp[xo] & 1, 1000);
-            else if (xo >= 0)
-              mbar_try_wait_hint(&bs->v_ready[vpre % SV], (vpre / SV) & 1, 1000);
-            else
-              mbar_try_wait_hint(&bs->k_full[kpre % SK], (kpre / SK) & 1, 1000);
-            if (++idle == 64) t_idle = globaltimer_ns();
-            if (idle > 64 && (idle & 63) == 0) {
-              if (*reinterpret_cast<volatile int*>(&bs->abort_flag)) {
-                ok = false;
-              } else if (globaltimer_ns() - t_idle > kWaitLimitNs) {
-                set_device_error(p.err, static_cast<unsigned int>(-HALO_ERR_TIMEOUT));
-                *reinterpret_cast<volatile int*>(&bs->abort_flag) = 1;
-                ok = false;
-              }
-            }
+            for (int kk = 0; kk < kBN / 16; ++kk)
+              umma::mma_ts(oc, pc + 64 + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), kIdPV,
+                           true);
+            umma::commit(&bs->v_empty[iv]);
+            if (it + 1 == nx) umma::commit(&bs->pv_done[x]);
+            g += step;
+            if (it + 1 < nx) ok = qk();
           }
           g0 += n;
           ++si;
         }
         // this thread's MMAs complete before the CTA can free TMEM
-        umma::commit(&bs->mma_done);
-        mbar_wait(&bs->mma_done, 0, p.err);
+        umma::commit(&bs->mma_done[x]);
+        mbar_wait(&bs->mma_done[x], 0, p.err);
       }
     } else {
-      // -------------------------------------------------------- V cleaners
+      // -------------------------------------------------------- V cleaner
       int g = 0, si = 0;
       bool ok = true;
-      volatile int* bad = &bs->bad[warp - 2][0];
+      volatile int* bad = &bs->bad[0];
       while (ok && walk.next(p, s)) {
         if (lane == 0) bad[si % kBadSlots] = 0;
         __syncwarp();
@@ -570,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           if (lo < kBN) {
             bool any = false;
             const int n = (kBN - lo) * (D / 8);
-            for (int i = (warp - 2) * 32 + lane; i < n; i += 64) {
+            for (int i = lane; i < n; i += 32) {
               const int row = lo + i / (D / 8), c = i % (D / 8);
               uint4* w = reinterpret_cast<uint4*>(smem + Gm::kOffV + iv * Gm::kTileBytes +
                                                   (c >> 3) * Gm::kBlockBytes + row * 128 +
@@ -620,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     const uint32_t scol = x * 128, ocol = Gm::kColO + x * D;
     Walk<RG> walk(p, bs->r0, bs->base0, u0, u1);
     Seg s;
-    int j = 0, si = 0;                           // tiles of this stream; segments
+    int j = 0, si = 0, sx = 0;                   // tiles of this stream; segments; with tiles
     bool ok = true;
     while (walk.next(p, s)) {
       const bool two = QT == 2 && s.rows > 128;
@@ -724,8 +659,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           m = mx;
         }
         if (it > 0 && __any_sync(0xffffffffu, grow)) {
-          // O_X is quiescent: this QK was issued after the last PV completed,
-          // and the next PV waits for this P
+          // O_X is quiescent: the last PV was issued before this QK, so it has
+          // completed, and the next PV waits for this P
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             float ov[32];
@@ -781,7 +716,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       // ---- epilogue.  Named barriers are passed whether or not a wait
       // failed, so that no thread is left behind at one.
       if (nx > 0 && ok) {
-        ok = __all_sync(0xffffffffu, wait_bar(&bs->pv_done[x], (j - 1) & 1, bs, p.err));
+        ok = __all_sync(0xffffffffu, wait_bar(&bs->pv_done[x], sx & 1, bs, p.err));
+        ++sx;
         umma::fence_after_sync();
       }
       float* slot = p.part + ((int64_t)blockIdx.x * 2 + (s.first ? 0 : 1)) * RG * kPartStride<D>;
@@ -835,9 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       };
       if (two) {
         // every row is one thread's
-        const volatile int* b0 = &bs->bad[0][0];
-        const volatile int* b1 = &bs->bad[1][0];
-        const bool fix = b0[si % kBadSlots] || b1[si % kBadSlots];
+        const bool fix = *reinterpret_cast<volatile int*>(&bs->bad[si % kBadSlots]) != 0;
         if (ok) {
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
@@ -862,9 +796,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         sm_m[x * 128 + r] = m;
         sm_l[x * 128 + r] = l;
         named_bar_sync(1, 256);
-        const volatile int* b0 = &bs->bad[0][0];
-        const volatile int* b1 = &bs->bad[1][0];
-        const bool fix = b0[si % kBadSlots] || b1[si % kBadSlots];
+        const bool fix = *reinterpret_cast<volatile int*>(&bs->bad[si % kBadSlots]) != 0;
         float M = -INFINITY, L = 0.f;
 #pragma unroll
         for (int i = 0; i < NS; ++i) M = fmaxf(M, sm_m[(i / COP) * 128 + (i % COP) * RPC + rr]);
