@@ -37,7 +37,8 @@ int device_sms();
 namespace tree {
 
 constexpr int kBN = 128;               // positions of a tile (a unit)
-constexpr int kThreads = 384;
+constexpr int kThreads = 384;          // tree_kernel
+constexpr int kFewThreads = 256;       // tree_few_kernel
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.f;    // headroom of the running maximum
 constexpr int kBadSlots = 8;
@@ -76,6 +77,7 @@ struct alignas(64) Desc {
 template <int D>
 constexpr int kPartStride = D + 4;
 
+// tree_kernel: QT query tiles of 128 rows.
 template <int D, int QT>
 struct Geom {
   static constexpr int kBlocks = D / 64;                  // 128-byte column blocks
@@ -93,8 +95,39 @@ struct Geom {
   static constexpr uint32_t kColO = 256;
 };
 
+// tree_few_kernel: NR (16, 32 or 64) query rows.
+template <int D, int NR>
+struct FewGeom {
+  static constexpr int kBlocks = D / 64;
+  static constexpr int kBlockBytes = kBN * 128;
+  static constexpr int kTileBytes = kBlocks * kBlockBytes;
+  static constexpr int kQBytes = NR * D * 2;
+  static constexpr int kPBytes = (NR == 64 ? 2 : 1) * kBlockBytes;
+  static constexpr int kStK = D == 64 ? (NR == 64 ? 5 : 6) : 3;
+  static constexpr int kStV = D == 64 ? (NR == 64 ? 5 : 6) : (NR == 64 ? 2 : 3);
+  static constexpr int kOffK = 0;
+  static constexpr int kOffV = kStK * kTileBytes;
+  static constexpr int kOffP = kOffV + kStV * kTileBytes;
+  static constexpr int kOffQ = kOffP + kPBytes;                // two buffers
+  static constexpr int kOffRed = kOffQ + 2 * kQBytes;          // see FewShared
+  static constexpr int kOffBar = kOffRed + 2048;
+  static constexpr int kSmemBytes = kOffBar + 1024;
+  static constexpr uint32_t kColO = 2 * NR;                    // S 2 x NR, O 2 NR
+};
+static_assert(FewGeom<128, 64>::kSmemBytes <= 232448 && FewGeom<128, 32>::kSmemBytes <= 232448 &&
+              FewGeom<64, 64>::kSmemBytes <= 232448 && FewGeom<64, 32>::kSmemBytes <= 232448 &&
+              Geom<128, 1>::kSmemBytes <= 232448 && Geom<128, 2>::kSmemBytes <= 232448 &&
+              Geom<64, 2>::kSmemBytes <= 232448, "227 KB of shared memory");
+
+struct FewShared {
+  float red[4][64];                    // per warp and row
+  float m[64], fac[64];                // running maximum; its latest rescale, or 1 / l
+  int64_t off[64];                     // output element of each row
+};
+static_assert(sizeof(FewShared) <= 2048, "scratch of tree_few_kernel");
+
 struct Bars {
-  uint64_t q_full;
+  uint64_t q_full[2], q_empty[2];
   uint64_t k_full[6], k_empty[6], v_full[6], v_ready[6], v_empty[6];
   uint64_t s_full[2], p_full[2], pv_done[2], mma_done[2];
   int64_t scan[12];
@@ -216,18 +249,239 @@ __device__ __forceinline__ bool bad16(uint32_t x) {   // inf or NaN in the low 1
   return (x & e) == e;
 }
 
+// ---- parts of both kernels
+
+// The CTA's run [c U / C, (c + 1) U / C) of the U units of all requests, and
+// the request (bs->r0, beginning at unit bs->base0) that holds its first.
+// Ends without a barrier: bs->r0 holds after the caller's next one.
+template <int RG, int NT>
+__device__ __forceinline__ void find_run(const Params& p, Bars* bs, int64_t& u0, int64_t& u1,
+                                         int64_t& U) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto prefix = [&](int64_t v, int64_t& total) {   // inclusive, over the CTA
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t o = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d) v += o;
+    }
+    __syncthreads();
+    if (lane == 31) bs->scan[warp] = v;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) {
+      if (w < warp) v += bs->scan[w];
+      total += bs->scan[w];
+    }
+    return v;
+  };
+  auto units_of = [&](int r) { return r < p.R ? load_req<RG>(p, r).units(p.H_kv) : (int64_t)0; };
+  int64_t mine = 0, incl = 0;
+  U = 0;
+  for (int r0 = 0; r0 < p.R; r0 += NT) {
+    int64_t t;
+    mine = units_of(r0 + threadIdx.x);
+    incl = prefix(mine, t);
+    U += t;
+  }
+  u0 = (int64_t)blockIdx.x * U / gridDim.x;
+  u1 = (int64_t)(blockIdx.x + 1) * U / gridDim.x;
+  {
+    int64_t before = 0;
+    for (int r0 = 0; r0 < p.R; r0 += NT) {
+      int64_t t = U;
+      if (p.R > NT) {                // else the scan above holds
+        mine = units_of(r0 + threadIdx.x);
+        incl = prefix(mine, t);
+      }
+      const int64_t lo = before + incl - mine;
+      if (mine > 0 && lo <= u0 && u0 < lo + mine) {
+        bs->r0 = r0 + threadIdx.x;
+        bs->base0 = lo;
+      }
+      before += t;
+    }
+  }
+}
+
+// Thread 0: the segment of the run's first unit, for the merge.
+template <int RG>
+__device__ __forceinline__ void write_desc(const Params& p, const Bars* bs, int64_t u0, int64_t U) {
+  Desc d{};
+  d.total = U;
+  d.start = d.end = u0;
+  if (u0 < U) {
+    Walk<RG> w(p, bs->r0, bs->base0, u0, u0 + 1);
+    Seg s;
+    w.next(p, s);
+    d.start = u0 - s.t0;
+    d.end = d.start + w.q.nt;
+    d.cu0 = w.q.cu0;
+    d.hk = s.hk;
+    d.row0 = s.row0;
+    d.rows = s.rows;
+  }
+  p.desc[blockIdx.x] = d;
+}
+
+// Producer warp: the run's K and V tiles through the two rings.  SKIP: in
+// segments of at most 128 rows only one of the two streams reads a tile.
+template <int RG, class Gm, bool SKIP>
+__device__ __forceinline__ void produce(const Params& p, Bars* bs, unsigned char* smem,
+                                        Walk<RG>& walk) {
+  constexpr int SK = Gm::kStK, SV = Gm::kStV;
+  const int lane = threadIdx.x & 31;
+  Seg s;
+  const int n_box = kBN / p.box, n_iss = n_box * Gm::kBlocks;   // at most 32
+  const int blk = lane / n_box, bx = lane - blk * n_box;
+  const uint32_t dst = blk * Gm::kBlockBytes + bx * p.box * 128;
+  int nk = 0, nv = 0;             // K and V tiles issued
+  bool ok = true;
+  while (ok && walk.next(p, s)) {
+    const int32_t* tab = p.table + (int64_t)walk.r * p.table_stride;
+    const uint32_t absent = SKIP && s.rows <= 128 ? 1u : 0u;   // streams that skip a tile
+    auto entry = [&](int t) {
+      const int pos = t * kBN + bx * p.box;
+      return lane < n_iss && t < s.t1 && pos < walk.q.end ? tab[pos / p.page] : -1;
+    };
+    int pg = entry(s.t0);
+    for (int t = s.t0; t < s.t1; ++t) {
+      const int pg_next = entry(t + 1);
+      const int pos = t * kBN + bx * p.box;
+      const int row = pos % p.page;
+      const int page = (uint32_t)pg < (uint32_t)p.n_pages ? pg : p.n_pages;   // outside: zeros
+      const int ik = nk % SK, iv = nv % SV;
+      if (nk >= SK)
+        ok = __all_sync(0xffffffffu,
+                        wait_bar(&bs->k_empty[ik], (nk / SK - 1) & 1, bs, p.err));
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bs->k_full[ik], Gm::kTileBytes);
+        if (absent) mbar_arrive_n(&bs->k_empty[ik], absent);
+      }
+      __syncwarp();
+      if (lane < n_iss)
+        tma_load_4d(smem + Gm::kOffK + ik * Gm::kTileBytes + dst, &p.kmap, blk * 64, row, s.hk,
+                    page, &bs->k_full[ik]);
+      ++nk;
+      if (nv >= SV)
+        ok = __all_sync(0xffffffffu,
+                        wait_bar(&bs->v_empty[iv], (nv / SV - 1) & 1, bs, p.err));
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bs->v_full[iv], Gm::kTileBytes);
+        if (absent) mbar_arrive_n(&bs->v_empty[iv], absent);
+      }
+      __syncwarp();
+      if (lane < n_iss)
+        tma_load_4d(smem + Gm::kOffV + iv * Gm::kTileBytes + dst, &p.vmap, blk * 64, row, s.hk,
+                    page, &bs->v_full[iv]);
+      ++nv;
+      pg = pg_next;
+    }
+  }
+  // every copy issued lands before the CTA can exit
+  if (lane == 0) {
+    for (int i = 0; i < SK; ++i) {
+      const int n = (nk - i + SK - 1) / SK;
+      if (n > 0) mbar_wait(&bs->k_full[i], (n - 1) & 1, p.err);
+    }
+    for (int i = 0; i < SV; ++i) {
+      const int n = (nv - i + SV - 1) / SV;
+      if (n > 0) mbar_wait(&bs->v_full[i], (n - 1) & 1, p.err);
+    }
+  }
+}
+
+// Cleaner warp: passes every V tile on, cleaned where it reaches behind the
+// context: rows behind the last node and elements that are not finite become
+// zero (a weight of zero would turn them into NaN).  bs->bad[segment] tells
+// whether a node's element was taken out; bad_sum gives it back.
+template <typename T, int D, int RG, class Gm>
+__device__ __forceinline__ void clean(const Params& p, Bars* bs, unsigned char* smem,
+                                      Walk<RG>& walk) {
+  constexpr int SV = Gm::kStV;
+  const int lane = threadIdx.x & 31;
+  Seg s;
+  int g = 0, si = 0;
+  bool ok = true;
+  volatile int* bad = &bs->bad[0];
+  while (ok && walk.next(p, s)) {
+    if (lane == 0) bad[si % kBadSlots] = 0;
+    __syncwarp();
+    for (int t = s.t0; t < s.t1; ++t, ++g) {
+      const int iv = g % SV;
+      ok = __all_sync(0xffffffffu, wait_bar(&bs->v_full[iv], (g / SV) & 1, bs, p.err));
+      if (!ok) break;
+      const int lo = max(0, walk.q.ctx - t * kBN), end = walk.q.end - t * kBN;
+      if (lo < kBN) {
+        bool any = false;
+        const int n = (kBN - lo) * (D / 8);
+        for (int i = lane; i < n; i += 32) {
+          const int row = lo + i / (D / 8), c = i % (D / 8);
+          uint4* w = reinterpret_cast<uint4*>(smem + Gm::kOffV + iv * Gm::kTileBytes +
+                                              (c >> 3) * Gm::kBlockBytes + row * 128 +
+                                              (((c & 7) ^ (row & 7)) << 4));
+          if (row >= end) {
+            *w = make_uint4(0, 0, 0, 0);
+            continue;
+          }
+          uint4 x = *w;
+          uint32_t e[4] = {x.x, x.y, x.z, x.w};
+          bool hit = false;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (bad16<T>(e[k])) {
+              e[k] &= 0xFFFF0000u;
+              hit = true;
+            }
+            if (bad16<T>(e[k] >> 16)) {
+              e[k] &= 0xFFFFu;
+              hit = true;
+            }
+          }
+          if (hit) {
+            *w = make_uint4(e[0], e[1], e[2], e[3]);
+            any = true;
+          }
+        }
+        if (any) bad[si % kBadSlots] = 1;
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bs->v_ready[iv]);
+    }
+    ++si;
+  }
+}
+
+// Sum of the non-finite V elements, in column `col`, of the nodes at positions
+// [a, b) that query row t sees: its weights are positive, so each adds itself
+// to the row's output.
+template <typename T>
+__device__ __noinline__ float bad_sum(const Params& p, int r, int t, int ctx, int a, int b, int hk,
+                                      int col) {
+  float o = 0.f;
+  for (int pos = a; pos < b; ++pos) {
+    if (!p.mask[(int64_t)t * p.mask_stride + pos - ctx]) continue;
+    const int pg = p.table[(int64_t)r * p.table_stride + pos / p.page];
+    if ((uint32_t)pg >= (uint32_t)p.n_pages) continue;
+    const float y = Elem<T>::to_f32(reinterpret_cast<const T*>(
+        p.v)[pg * p.v_sp + hk * p.v_sh + (pos % p.page) * p.v_st + col]);
+    if (!isfinite(y)) o += y;
+  }
+  return o;
+}
+
 // ======================================================================
-// tree_kernel: one CTA an SM, 384 threads.
+// tree_kernel: groups of more than 64 rows.  One CTA an SM, 384 threads.
 //   warp 0      TMA producer: K and V tiles of 128 positions, each made of
 //               boxes of p.box rows (the largest power of two, up to 128,
 //               that divides the page), through two rings; the lanes issue a
 //               tile's boxes side by side.  Boxes behind the last position
 //               or without a page start outside the tensor: zeros.
 //   warps 1, 3  lane 0 issues the MMAs of stream 0 / 1; warp 1 owns TMEM.
-//   warp 2      cleans V: in tiles that reach behind the context, rows behind
-//               the last node and elements that are not finite become zero
-//               (a weight of zero would turn them into NaN); a node that does
-//               see such an element gets it back in the epilogue.
+//   warp 2      cleans V.
 //   warps 4-7   softmax stream 0, warps 8-11 stream 1 (thread = TMEM lane).
 // Each stream has its own scores S_X (128 TMEM columns, overwritten in place
 // by the weights P_X) and output O_X: S_X = Q K^T, O_X += P_X V, both M128.
@@ -239,19 +493,12 @@ __device__ __forceinline__ bool bad16(uint32_t x) {   // inf or NaN in the low 1
 //
 // Row groups of more than 128 rows (QT = 2): stream X takes query tile X and
 // both take every K/V tile.  Smaller ones: both streams share the query tile
-// and take every second K/V tile, and if the rows fit 64 or 32 lanes the
-// tile holds 2 or 4 copies of them (KPT = 64, 32), copy c taking positions
-// [c KPT, (c + 1) KPT) of each tile: the exponentials of a few rows are spread
-// over all 256 softmax threads, while the MMAs, which cost the same for 1 row
-// as for 128, stay under the time the bytes take.  A copy's weights are zero
-// outside its positions.  All copies and streams are joined in shared memory
-// at the end of a segment.
-template <typename T, int D, int KPT, int QT>
+// and take every second K/V tile; the two are joined in shared memory at the
+// end of a segment.
+template <typename T, int D, int QT>
 __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ Params p) {
   using Gm = Geom<D, QT>;
-  constexpr int COP = kBN / KPT;           // copies of the rows in a query tile
-  constexpr int RPC = 128 / COP;           // rows of a copy
-  constexpr int RG = RPC * QT;             // rows of a group
+  constexpr int RG = 128 * QT;             // rows of a group
   constexpr bool kBf16 = Elem<T>::kDtype == HALO_DTYPE_BF16;
   extern __shared__ __align__(1024) unsigned char smem[];
   Bars* bs = reinterpret_cast<Bars*>(smem + Gm::kOffBar);
@@ -260,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    mbar_init(&bs->q_full, 8);
+    mbar_init(&bs->q_full[0], 8);
     for (int i = 0; i < 6; ++i) {
       mbar_init(&bs->k_full[i], 1);
       mbar_init(&bs->k_empty[i], 2);
@@ -283,71 +530,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   }
   grid_dep_wait();                         // the caller's writes are visible
 
-  // ---- this CTA's run of units: [c U / C, (c + 1) U / C)
-  auto prefix = [&](int64_t v, int64_t& total) {   // inclusive, over the CTA
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t o = __shfl_up_sync(0xffffffffu, v, d);
-      if (lane >= d) v += o;
-    }
-    __syncthreads();
-    if (lane == 31) bs->scan[warp] = v;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) v += bs->scan[w];
-      total += bs->scan[w];
-    }
-    return v;
-  };
-  auto units_of = [&](int r) { return r < p.R ? load_req<RG>(p, r).units(p.H_kv) : (int64_t)0; };
-  int64_t U = 0, mine = 0, incl = 0;
-  for (int r0 = 0; r0 < p.R; r0 += kThreads) {
-    int64_t t;
-    mine = units_of(r0 + threadIdx.x);
-    incl = prefix(mine, t);
-    U += t;
-  }
-  const int64_t u0 = (int64_t)blockIdx.x * U / gridDim.x;
-  const int64_t u1 = (int64_t)(blockIdx.x + 1) * U / gridDim.x;
-  {
-    int64_t before = 0;
-    for (int r0 = 0; r0 < p.R; r0 += kThreads) {
-      int64_t t = U;
-      if (p.R > kThreads) {                // else the scan above holds
-        mine = units_of(r0 + threadIdx.x);
-        incl = prefix(mine, t);
-      }
-      const int64_t lo = before + incl - mine;
-      if (mine > 0 && lo <= u0 && u0 < lo + mine) {
-        bs->r0 = r0 + threadIdx.x;
-        bs->base0 = lo;
-      }
-      before += t;
-    }
-  }
+  int64_t u0, u1, U;
+  find_run<RG, kThreads>(p, bs, u0, u1, U);
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
   const uint32_t tmem = bs->tmem_base;
-  if (threadIdx.x == 0) {
-    Desc d{};
-    d.total = U;
-    d.start = d.end = u0;
-    if (u0 < U) {
-      Walk<RG> w(p, bs->r0, bs->base0, u0, u0 + 1);
-      Seg s;
-      w.next(p, s);
-      d.start = u0 - s.t0;
-      d.end = d.start + w.q.nt;
-      d.cu0 = w.q.cu0;
-      d.hk = s.hk;
-      d.row0 = s.row0;
-      d.rows = s.rows;
-    }
-    p.desc[blockIdx.x] = d;
-  }
+  if (threadIdx.x == 0) write_desc<RG>(p, bs, u0, U);
   grid_dep_trigger();
 
   const uint32_t sQ = smem_addr(smem + Gm::kOffQ);
@@ -368,65 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     Walk<RG> walk(p, bs->r0, bs->base0, u0, u1);
     Seg s;
     if (warp == 0) {
-      // -------------------------------------------------------- producer
-      const int n_box = kBN / p.box, n_iss = n_box * Gm::kBlocks;   // at most 32
-      const int blk = lane / n_box, bx = lane - blk * n_box;
-      const uint32_t dst = blk * Gm::kBlockBytes + bx * p.box * 128;
-      int g = 0;
-      bool ok = true;
-      while (ok && walk.next(p, s)) {
-        const int32_t* tab = p.table + (int64_t)walk.r * p.table_stride;
-        const uint32_t absent = s.rows > 128 ? 0u : 1u;   // streams that skip a tile
-        auto entry = [&](int t) {
-          const int pos = t * kBN + bx * p.box;
-          return lane < n_iss && t < s.t1 && pos < walk.q.end ? tab[pos / p.page] : -1;
-        };
-        int pg = entry(s.t0);
-        for (int t = s.t0; t < s.t1; ++t, ++g) {
-          const int pg_next = entry(t + 1);
-          const int pos = t * kBN + bx * p.box;
-          const int row = pos % p.page;
-          const int page = (uint32_t)pg < (uint32_t)p.n_pages ? pg : p.n_pages;   // outside: zeros
-          const int ik = g % SK, iv = g % SV;
-          if (g >= SK) ok = __all_sync(0xffffffffu, wait_bar(&bs->k_empty[ik], (g / SK - 1) & 1, bs, p.err));
-          if (!ok) break;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&bs->k_full[ik], Gm::kTileBytes);
-            if (absent) mbar_arrive_n(&bs->k_empty[ik], absent);
-          }
-          __syncwarp();
-          if (lane < n_iss)
-            tma_load_4d(smem + Gm::kOffK + ik * Gm::kTileBytes + dst, &p.kmap, blk * 64, row, s.hk,
-                        page, &bs->k_full[ik]);
-          if (g >= SV) ok = __all_sync(0xffffffffu, wait_bar(&bs->v_empty[iv], (g / SV - 1) & 1, bs, p.err));
-          if (!ok) {
-            // this tile's K is on its way: count it below
-            ++g;
-            break;
-          }
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&bs->v_full[iv], Gm::kTileBytes);
-            if (absent) mbar_arrive_n(&bs->v_empty[iv], absent);
-          }
-          __syncwarp();
-          if (lane < n_iss)
-            tma_load_4d(smem + Gm::kOffV + iv * Gm::kTileBytes + dst, &p.vmap, blk * 64, row, s.hk,
-                        page, &bs->v_full[iv]);
-          pg = pg_next;
-        }
-      }
-      // every copy issued lands before the CTA can exit
-      if (lane == 0) {
-        for (int i = 0; i < SK; ++i) {
-          const int n = (g - i + SK - 1) / SK;
-          if (n > 0) mbar_wait(&bs->k_full[i], (n - 1) & 1, p.err);
-        }
-        const int gv = ok ? g : g - 1;
-        for (int i = 0; i < SV; ++i) {
-          const int n = (gv - i + SV - 1) / SV;
-          if (gv > 0 && n > 0) mbar_wait(&bs->v_full[i], (n - 1) & 1, p.err);
-        }
-      }
+      produce<RG, Gm, true>(p, bs, smem, walk);
     } else if (warp & 1) {
       // -------------------------------------------------------- MMA issuer X
       if (lane == 0) {
@@ -460,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             umma::commit(&bs->k_empty[ik]);
             return true;
           };
-          ok = wait_bar(&bs->q_full, si & 1, bs, p.err);
+          ok = wait_bar(&bs->q_full[0], si & 1, bs, p.err);
           if (ok && nx > 0) ok = qk();
           for (int it = 0; ok && it < nx; ++it, ++j) {
             const int iv = g % SV;
@@ -490,57 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         mbar_wait(&bs->mma_done[x], 0, p.err);
       }
     } else {
-      // -------------------------------------------------------- V cleaner
-      int g = 0, si = 0;
-      bool ok = true;
-      volatile int* bad = &bs->bad[0];
-      while (ok && walk.next(p, s)) {
-        if (lane == 0) bad[si % kBadSlots] = 0;
-        __syncwarp();
-        for (int t = s.t0; t < s.t1; ++t, ++g) {
-          const int iv = g % SV;
-          ok = __all_sync(0xffffffffu, wait_bar(&bs->v_full[iv], (g / SV) & 1, bs, p.err));
-          if (!ok) break;
-          const int lo = max(0, walk.q.ctx - t * kBN), end = walk.q.end - t * kBN;
-          if (lo < kBN) {
-            bool any = false;
-            const int n = (kBN - lo) * (D / 8);
-            for (int i = lane; i < n; i += 32) {
-              const int row = lo + i / (D / 8), c = i % (D / 8);
-              uint4* w = reinterpret_cast<uint4*>(smem + Gm::kOffV + iv * Gm::kTileBytes +
-                                                  (c >> 3) * Gm::kBlockBytes + row * 128 +
-                                                  (((c & 7) ^ (row & 7)) << 4));
-              if (row >= end) {
-                *w = make_uint4(0, 0, 0, 0);
-                continue;
-              }
-              uint4 x = *w;
-              uint32_t e[4] = {x.x, x.y, x.z, x.w};
-              bool hit = false;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                if (bad16<T>(e[k])) {
-                  e[k] &= 0xFFFF0000u;
-                  hit = true;
-                }
-                if (bad16<T>(e[k] >> 16)) {
-                  e[k] &= 0xFFFFu;
-                  hit = true;
-                }
-              }
-              if (hit) {
-                *w = make_uint4(e[0], e[1], e[2], e[3]);
-                any = true;
-              }
-            }
-            if (any) bad[si % kBadSlots] = 1;
-            fence_proxy_async_smem();
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bs->v_ready[iv]);
-        }
-        ++si;
-      }
+      clean<T, D, RG, Gm>(p, bs, smem, walk);
     }
   } else {
     umma::regs_inc<208>();
@@ -548,8 +629,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     const int x = (warp - 4) >> 2;
     const int sub = warp & 3;
     const int r = sub * 32 + lane;               // TMEM lane
-    const int copy = sub * 32 / RPC;             // uniform in a warp
-    const int rr = r - copy * RPC;               // row within the tile
     const int tid = threadIdx.x - 128;           // 0..255 over both streams
     const uint32_t trow = tmem + ((uint32_t)(sub * 32) << 16);
     const uint32_t scol = x * 128, ocol = Gm::kColO + x * D;
@@ -571,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           for (int u = 0; u < 4; ++u) {
             const int i = i0 + u * 256 + tid;
             const int ql = i / VPR, c = i % VPR;             // tile row, 16-byte column
-            const int row = two ? ql : ql % RPC;
+            const int row = ql;
             w[u] = make_uint4(0, 0, 0, 0);
             if (i < n && row < s.rows) {
               const int rq = s.row0 + row, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
@@ -593,21 +672,21 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bs->q_full);
+        if (lane == 0) mbar_arrive(&bs->q_full[0]);
       }
       const int n = s.t1 - s.t0, step = two ? 1 : 2;
       const int nx = two ? n : (x ? n / 2 : (n + 1) / 2);
       const int rowx = s.row0 + (two ? x * 128 : 0);   // request row of the tile's row 0
-      const int rows = min(s.row0 + s.rows - rowx, RPC);
+      const int rows = min(s.row0 + s.rows - rowx, 128);
       float m = -INFINITY, l = 0.f;
       for (int it = 0; it < nx; ++it, ++j) {
-        const int p0 = (s.t0 + (two ? 0 : x) + it * step) * kBN + copy * KPT;
+        const int p0 = (s.t0 + (two ? 0 : x) + it * step) * kBN;
         // which of the thread's positions its row sees
-        const bool full = p0 + KPT <= ctx;
-        uint32_t vis[KPT / 32];
+        const bool full = p0 + kBN <= ctx;
+        uint32_t vis[kBN / 32];
         if (!full) {
 #pragma unroll
-          for (int w = 0; w < KPT / 32; ++w) {
+          for (int w = 0; w < kBN / 32; ++w) {
             const int b = p0 + 32 * w;
             vis[w] = 0;
             if (b + 32 <= ctx) {
@@ -616,7 +695,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
               // one mask row at a time, a lane a position
               const int jn = b + lane - ctx;
               const bool node_ok = jn >= 0 && b + lane < end;
-              const int first = rowx + sub * 32 - copy * RPC;
+              const int first = rowx + sub * 32;
               const uint8_t* mp = p.mask + (int64_t)cu0 * p.mask_stride + jn;
 #pragma unroll 8
               for (int i = 0; i < 32; ++i) {
@@ -632,21 +711,21 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->s_full[x], j & 1, bs, p.err));
         if (!ok) break;
         umma::fence_after_sync();
-        float sv[KPT];
+        float sv[kBN];
 #pragma unroll
-        for (int c = 0; c < KPT / 32; ++c)
-          umma::tmem_ld32(trow + scol + copy * KPT + c * 32, sv + c * 32);
+        for (int c = 0; c < kBN / 32; ++c)
+          umma::tmem_ld32(trow + scol + c * 32, sv + c * 32);
         umma::tmem_wait_ld();
         if (!full) {
 #pragma unroll
-          for (int c = 0; c < KPT; ++c)
+          for (int c = 0; c < kBN; ++c)
             if (!((vis[c >> 5] >> (c & 31)) & 1u)) sv[c] = -INFINITY;
         }
         float mx8[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) mx8[e] = sv[e];
 #pragma unroll
-        for (int c = 8; c < KPT; ++c) mx8[c & 7] = fmaxf(mx8[c & 7], sv[c]);
+        for (int c = 8; c < kBN; ++c) mx8[c & 7] = fmaxf(mx8[c & 7], sv[c]);
         const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
                                fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]))) *
                          p.scale_log2;
@@ -674,7 +753,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         const float nm = (m == -INFINITY) ? 0.f : -m;
         float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < KPT / 32; ++c) {
+        for (int c = 0; c < kBN / 32; ++c) {
           uint32_t hi[16], lo[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -693,18 +772,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             }
             lo[e] = Elem<T>::pack(a - ah, b - bh);
           }
-          umma::tmem_st16u(trow + scol + copy * (KPT / 2) + c * 16, hi);
-          umma::tmem_st16u(trow + scol + 64 + copy * (KPT / 2) + c * 16, lo);
-        }
-        if constexpr (COP > 1) {           // the other copies' positions weigh nothing here
-          const uint32_t z[16] = {};
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (c / (KPT / 32) != copy) {
-              umma::tmem_st16u(trow + scol + c * 16, z);
-              umma::tmem_st16u(trow + scol + 64 + c * 16, z);
-            }
-          }
+          umma::tmem_st16u(trow + scol + c * 16, hi);
+          umma::tmem_st16u(trow + scol + 64 + c * 16, lo);
         }
         l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
         umma::tmem_wait_st();
@@ -721,22 +790,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         umma::fence_after_sync();
       }
       float* slot = p.part + ((int64_t)blockIdx.x * 2 + (s.first ? 0 : 1)) * RG * kPartStride<D>;
-      // non-finite V of nodes, which the cleaners took out, for a row that
-      // sees them: its weights are positive, so the sum is the value itself
-      auto add_bad = [&](int row, int col, float* o, int n_col) {
-        const int node = (s.row0 + row) / p.G;
-        const int a = max(ctx, s.t0 * kBN), b = min(end, s.t1 * kBN);
-        for (int pos = a; pos < b; ++pos) {
-          if (!p.mask[(int64_t)(cu0 + node) * p.mask_stride + pos - ctx]) continue;
-          const int pg = p.table[(int64_t)walk.r * p.table_stride + pos / p.page];
-          if ((uint32_t)pg >= (uint32_t)p.n_pages) continue;
-          const T* v = reinterpret_cast<const T*>(p.v) + pg * p.v_sp + s.hk * p.v_sh +
-                       (pos % p.page) * p.v_st + col;
-          for (int e = 0; e < n_col; ++e) {
-            const float y = Elem<T>::to_f32(v[e]);
-            if (!isfinite(y)) o[e] += y;
-          }
-        }
+      auto bad = [&](int row, int col) {
+        return bad_sum<T>(p, walk.r, cu0 + (s.row0 + row) / p.G, ctx, max(ctx, s.t0 * kBN),
+                          min(end, s.t1 * kBN), s.hk, col);
       };
       auto store = [&](int row, int col, float M, float L, float* o, auto n_col) {
         constexpr int N = decltype(n_col)::value;
@@ -778,45 +834,42 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             float ov[32];
             umma::tmem_ld32(trow + ocol + c * 32, ov);
             umma::tmem_wait_ld();
-            if (rr < rows) {
-              if (fix) add_bad(rr + x * 128, c * 32, ov, 32);
-              store(rr + x * 128, c * 32, m, l, ov, std::integral_constant<int, 32>());
+            if (r < rows) {
+              if (fix)
+                for (int e = 0; e < 32; ++e) ov[e] += bad(r + x * 128, c * 32 + e);
+              store(r + x * 128, c * 32, m, l, ov, std::integral_constant<int, 32>());
             }
           }
         }
       } else {
-        // join the 2 COP states of every row.  All states agree on the row's
+        // join the two streams' states of every row.  Both agree on the row's
         // maximum through shared memory, then add their scaled outputs into
-        // one fp32 copy in the query tile's space (its MMAs have completed):
-        // in round k state i adds column slice (i + k) mod 2 COP, so all
-        // threads work at once and the order of the sum is fixed.
-        constexpr int NS = 2 * COP, HALVES = COP == 1 ? 2 : 1;
-        constexpr int DA = D / HALVES, W = DA / NS;          // columns held, of a slice
-        static_assert(RPC * DA * 4 <= Gm::kTileBytes, "scratch fits the query tile");
+        // one fp32 copy in the query tile's space (its MMAs have completed),
+        // half the columns at a time: in round k stream x adds quarter
+        // (x + k) mod 2 of that half, so both work at once and the order of
+        // the sum is fixed.
+        constexpr int DA = D / 2, W = DA / 2;                // columns held, of a quarter
+        static_assert(128 * DA * 4 <= Gm::kTileBytes, "scratch fits the query tile");
         sm_m[x * 128 + r] = m;
         sm_l[x * 128 + r] = l;
         named_bar_sync(1, 256);
         const bool fix = *reinterpret_cast<volatile int*>(&bs->bad[si % kBadSlots]) != 0;
-        float M = -INFINITY, L = 0.f;
-#pragma unroll
-        for (int i = 0; i < NS; ++i) M = fmaxf(M, sm_m[(i / COP) * 128 + (i % COP) * RPC + rr]);
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-          const int at = (i / COP) * 128 + (i % COP) * RPC + rr;
-          const float mi = sm_m[at], li = sm_l[at];
-          L = fmaf(li, (mi == -INFINITY) ? (li == li ? 0.f : 1.f) : ex2(mi - M), L);
-        }
-        const float w = (m == -INFINITY) ? (l == l ? 0.f : 1.f) : ex2(m - M);
-        const int state = x * COP + copy;
+        // a row that saw only NaN has m = -inf and l = NaN: weight 1 keeps the NaN
+        const float m0 = sm_m[r], m1 = sm_m[128 + r], l0 = sm_l[r], l1 = sm_l[128 + r];
+        const float M = fmaxf(m0, m1);
+        const float w0 = (m0 == -INFINITY) ? (l0 == l0 ? 0.f : 1.f) : ex2(m0 - M);
+        const float w1 = (m1 == -INFINITY) ? (l1 == l1 ? 0.f : 1.f) : ex2(m1 - M);
+        const float L = fmaf(l1, w1, l0 * w0);
+        const float w = x ? w1 : w0;
         float* acc = reinterpret_cast<float*>(smem + Gm::kOffQ);
         // float4 granule `gr` of a row: swizzled against bank conflicts
         auto granule = [&](int row, int gr) {
-          return reinterpret_cast<float4*>(acc + row * DA + ((gr ^ (row & (DA / 4 < 8 ? DA / 4 - 1 : 7))) << 2));
+          return reinterpret_cast<float4*>(acc + row * DA + ((gr ^ (row & 7)) << 2));
         };
-        for (int hf = 0; hf < HALVES; ++hf) {
+        for (int hf = 0; hf < 2; ++hf) {
 #pragma unroll 1
-          for (int k = 0; k < NS; ++k) {
-            const int sl = (state + k) % NS;
+          for (int k = 0; k < 2; ++k) {
+            const int sl = x ^ k;
             float ov[W];
             if (nx > 0 && ok) {
               tmem_ld(trow + ocol + hf * DA + sl * W, ov);
@@ -827,7 +880,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             }
 #pragma unroll
             for (int e = 0; e < W; e += 4) {
-              float4* d = granule(rr, (sl * W + e) >> 2);
+              float4* d = granule(r, (sl * W + e) >> 2);
               float4 y = k == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *d;
               y.x = fmaf(ov[e], w, y.x);
               y.y = fmaf(ov[e + 1], w, y.y);
@@ -838,9 +891,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             named_bar_sync(1, 256);
           }
           if (hf == 0) {
-            if (state == 0) {                  // everyone has read m and l
-              sm_m[rr] = M;
-              sm_l[rr] = L;
+            if (x == 0) {                      // everyone has read m and l
+              sm_m[r] = M;
+              sm_l[r] = L;
             }
             named_bar_sync(1, 256);
           }
@@ -849,11 +902,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
               const int row = i / (DA / 8), c = i % (DA / 8);
               const float4 y0 = *granule(row, 2 * c), y1 = *granule(row, 2 * c + 1);
               float o[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
-              if (fix) add_bad(row, hf * DA + c * 8, o, 8);
+              if (fix)
+                for (int e = 0; e < 8; ++e) o[e] += bad(row, hf * DA + c * 8 + e);
               store(row, hf * DA + c * 8, sm_m[row], sm_l[row], o, std::integral_constant<int, 8>());
             }
           }
-          if (HALVES > 1 && hf == 0) named_bar_sync(1, 256);   // before the second half
+          if (hf == 0) named_bar_sync(1, 256);   // before the second half
         }
       }
       ++si;
@@ -867,6 +921,440 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   if (warp == 1) {
     umma::fence_after_sync();
     umma::tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// ======================================================================
+// tree_few_kernel: groups of at most 64 rows (NR = 16, 32 or 64).  One CTA an
+// SM, 256 threads.
+//   warp 0      TMA producer (as in tree_kernel)
+//   warp 1      TMEM owner; lane 0 issues every MMA
+//   warp 2      cleans V
+//   warp 3      query rows of the next segment (two buffers)
+//   warps 4-7   softmax (thread = position of the tile) and epilogue (thread =
+//               output column)
+// Both products have the K/V tile as the 128-row operand and the query rows
+// as the columns: S^T = K Q^T (M = positions, N = NR) and O^T += V^T P^T
+// (M = columns of V, N = 2 NR: the weights' 16-bit values and, beside them,
+// their 16-bit remainders, so V goes through the tensor pipe once).  With the
+// rows on the 128-row side, as in tree_kernel, the MMAs of 8 rows would cost
+// the energy of 128, and what bounds a long context is the clock that the
+// power limit leaves beside the memory's own draw: one request of a million
+// tokens ran at 1.33 GHz that way.  An MMA takes 60 to 70 clocks for any N up
+// to 128 (its 4 KB of K or V from shared memory), 1000 a tile, well under the
+// 2800 that the tile's bytes take at 1.9 GHz.
+// The row maximum lies across threads here, but it moves only past its
+// headroom of 2^8, so a tile costs one barrier with a vote; the reduction runs
+// in a segment's first tile and in the rare tile that raises it.
+constexpr float kNoMax = -1e30f;           // nothing seen yet: any score raises it
+
+// Sum or maximum over the warp of NR columns, one a row.  Lane i ends with row
+// i % NR in v[0] (NR = 64: rows i and 32 + i in v[0], v[1]).
+template <int NR, class Op>
+__device__ __forceinline__ void warp_columns(float (&v)[NR], Op op) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (NR == 16) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = op(v[i], __shfl_xor_sync(0xffffffffu, v[i], 16));
+  }
+  constexpr int W = NR < 32 ? NR : 32;
+#pragma unroll
+  for (int o = W / 2; o >= 1; o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int b = 0; b < NR; b += W) {
+#pragma unroll
+      for (int i = 0; i < o; ++i) {
+        const float keep = up ? v[b + i + o] : v[b + i], give = up ? v[b + i] : v[b + i + o];
+        v[b + i] = op(keep, __shfl_xor_sync(0xffffffffu, give, o));
+      }
+    }
+  }
+  if constexpr (NR == 64) v[1] = v[32];
+}
+
+// Barrier of the four softmax warps that tells whether any thread voted.
+__device__ __forceinline__ bool vote_bar(bool vote) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(vote ? 1u : 0u)
+      : "memory");
+  return any != 0;
+}
+
+template <typename T, int D, int NR>
+__global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_constant__ Params p) {
+  using Gm = FewGeom<D, NR>;
+  constexpr int RG = NR;
+  constexpr bool kBf16 = Elem<T>::kDtype == HALO_DTYPE_BF16;
+  constexpr int SK = Gm::kStK, SV = Gm::kStV;
+  constexpr uint32_t kCols = 4 * NR;             // TMEM: S twice, O
+  extern __shared__ __align__(1024) unsigned char smem[];
+  Bars* bs = reinterpret_cast<Bars*>(smem + Gm::kOffBar);
+  FewShared* sh = reinterpret_cast<FewShared*>(smem + Gm::kOffRed);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bs->q_full[i], 1);
+      mbar_init(&bs->q_empty[i], 1);
+      mbar_init(&bs->s_full[i], 1);
+    }
+    for (int i = 0; i < 6; ++i) {
+      mbar_init(&bs->k_full[i], 1);
+      mbar_init(&bs->k_empty[i], 1);
+      mbar_init(&bs->v_full[i], 1);
+      mbar_init(&bs->v_ready[i], 1);
+      mbar_init(&bs->v_empty[i], 1);
+    }
+    mbar_init(&bs->p_full[0], 4);
+    mbar_init(&bs->pv_done[0], 1);
+    mbar_init(&bs->mma_done[0], 1);
+    bs->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    umma::tmem_alloc(&bs->tmem_base, kCols);
+    umma::tmem_relinquish();
+  }
+  grid_dep_wait();                         // the caller's writes are visible
+  int64_t u0, u1, U;
+  find_run<RG, kFewThreads>(p, bs, u0, u1, U);
+  umma::fence_before_sync();
+  __syncthreads();
+  umma::fence_after_sync();
+  const uint32_t tmem = bs->tmem_base;
+  if (threadIdx.x == 96) write_desc<RG>(p, bs, u0, U);
+  grid_dep_trigger();
+
+  const uint32_t sQ = smem_addr(smem + Gm::kOffQ);
+  const uint32_t sK = smem_addr(smem + Gm::kOffK);
+  const uint32_t sV = smem_addr(smem + Gm::kOffV);
+  const uint32_t sP = smem_addr(smem + Gm::kOffP);
+  const bool aligned = (sK & 1023) == 0;   // as in tree_kernel
+  if (!aligned && threadIdx.x == 0)
+    set_device_error(p.err, static_cast<unsigned int>(-HALO_ERR_MISALIGNED));
+
+  if (u0 < u1 && aligned) {
+    Walk<RG> walk(p, bs->r0, bs->base0, u0, u1);
+    Seg s;
+    if (warp == 0) {
+      produce<RG, Gm, false>(p, bs, smem, walk);
+    } else if (warp == 1) {
+      // -------------------------------------------------------- MMA issuer
+      if (lane == 0) {
+        constexpr uint32_t kIdQK = umma::instr_desc_f16(kBN, NR, kBf16, false, false);
+        constexpr uint32_t kIdPV = umma::instr_desc_f16(128, 2 * NR, kBf16, true, true);
+        const uint64_t kdesc0 = umma::smem_desc_sw128(sK, 16, 1024);
+        // V^T has 128 rows; 64 columns of V fill them twice (the same block
+        // again), and the second half of O^T is not read
+        const uint64_t vdesc0 =
+            umma::smem_desc_sw128(sV, D == 64 ? 0 : Gm::kBlockBytes, 1024);
+        const uint64_t pdesc0 = umma::smem_desc_sw128(sP, Gm::kBlockBytes, 1024);
+        int g = 0, si = 0;                  // tiles; segments
+        bool ok = true;
+        while (ok && walk.next(p, s)) {
+          const int n = s.t1 - s.t0;
+          const uint64_t qd0 = umma::smem_desc_sw128(sQ + (si & 1) * Gm::kQBytes, 16, 1024);
+          auto qk = [&](int t, bool last) {          // S^T = K(t) Q^T
+            const int ik = t % SK;
+            if (!wait_bar(&bs->k_full[ik], (t / SK) & 1, bs, p.err)) return false;
+            umma::fence_after_sync();
+            const uint64_t qd = opaque(qd0);
+            const uint64_t kd = opaque(kdesc0 + (uint64_t)((ik * Gm::kTileBytes) >> 4));
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+              umma::mma_ss(tmem + (t & 1) * NR,
+                           kd + (uint64_t)(((kk >> 2) * Gm::kBlockBytes + (kk & 3) * 32) >> 4),
+                           qd + (uint64_t)(((kk >> 2) * NR * 128 + (kk & 3) * 32) >> 4), kIdQK,
+                           kk > 0);
+            umma::commit(&bs->s_full[t & 1]);
+            umma::commit(&bs->k_empty[ik]);
+            if (last) umma::commit(&bs->q_empty[si & 1]);
+            return true;
+          };
+          ok = wait_bar(&bs->q_full[si & 1], (si >> 1) & 1, bs, p.err) && qk(g, n == 1);
+          for (int it = 0; ok && it < n; ++it, ++g) {
+            // S(g + 1)'s buffer held S(g - 1), which P(g - 1) says was read
+            if (it + 1 < n && !(ok = qk(g + 1, it + 2 == n))) break;
+            const int iv = g % SV;
+            ok = wait_bar(&bs->p_full[0], g & 1, bs, p.err) &&
+                 wait_bar(&bs->v_ready[iv], (g / SV) & 1, bs, p.err);
+            if (!ok) break;
+            umma::fence_after_sync();
+            const uint64_t vd = opaque(vdesc0 + (uint64_t)((iv * Gm::kTileBytes) >> 4));
+            const uint64_t pd = opaque(pdesc0);
+#pragma unroll
+            for (int kk = 0; kk < kBN / 16; ++kk)    // O^T += V(g)^T P^T
+              umma::mma_ss(tmem + Gm::kColO, vd + (uint64_t)((kk * 16 * 128) >> 4),
+                           pd + (uint64_t)((kk * 16 * 128) >> 4), kIdPV, it > 0 || kk > 0);
+            umma::commit(&bs->pv_done[0]);
+            umma::commit(&bs->v_empty[iv]);
+          }
+          ++si;
+        }
+        umma::commit(&bs->mma_done[0]);
+        mbar_wait(&bs->mma_done[0], 0, p.err);
+      }
+    } else if (warp == 2) {
+      clean<T, D, RG, Gm>(p, bs, smem, walk);
+    } else if (warp == 3) {
+      // -------------------------------------------------------- query rows
+      int si = 0;
+      bool ok = true;
+      while (ok && walk.next(p, s)) {
+        if (si >= 2)
+          ok = __all_sync(0xffffffffu,
+                          wait_bar(&bs->q_empty[si & 1], ((si >> 1) - 1) & 1, bs, p.err));
+        if (!ok) break;
+        constexpr int VPR = D / 8, N = NR * VPR;   // a multiple of 128
+        for (int i0 = 0; i0 < N; i0 += 128) {
+          uint4 w[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int i = i0 + u * 32 + lane, row = i / VPR, c = i % VPR;
+            w[u] = make_uint4(0, 0, 0, 0);
+            if (row < s.rows) {
+              const int rq = s.row0 + row, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
+              w[u] = *reinterpret_cast<const uint4*>(
+                  reinterpret_cast<const T*>(p.q) + (int64_t)(walk.q.cu0 + node) * p.q_st +
+                  hq * p.q_sh + c * 8);
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int i = i0 + u * 32 + lane, row = i / VPR, c = i % VPR;
+            *reinterpret_cast<uint4*>(smem + Gm::kOffQ + (si & 1) * Gm::kQBytes +
+                                      (c >> 3) * NR * 128 + row * 128 +
+                                      (((c & 7) ^ (row & 7)) << 4)) = w[u];
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bs->q_full[si & 1]);
+        ++si;
+      }
+    } else {
+      // -------------------------------------------------------- softmax
+      const int sub = warp & 3, tid = threadIdx.x - 128;
+      const uint32_t trow = tmem + ((uint32_t)(sub * 32) << 16);
+      auto load_s = [&](int g, float (&x)[NR]) {
+        const uint32_t a = trow + (g & 1) * NR;
+        if constexpr (NR == 16) {
+          tmem_ld(a, x);
+        } else {
+#pragma unroll
+          for (int c = 0; c < NR / 32; ++c) umma::tmem_ld32(a + c * 32, x + c * 32);
+        }
+        umma::tmem_wait_ld();
+      };
+      int g = 0, si = 0;
+      bool ok = true;
+      while (walk.next(p, s)) {
+        const int ctx = walk.q.ctx, end = walk.q.end;
+        float l[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) l[r] = 0.f;
+        if (tid < NR) sh->m[tid] = kNoMax;
+        named_bar_sync(1, 128);
+        for (int t = s.t0; t < s.t1; ++t, ++g) {
+          // rows that see this thread's position
+          const bool full = (t + 1) * kBN <= ctx;
+          uint32_t vis[(NR + 31) / 32];
+          if (!full) {
+            const int pos = t * kBN + tid, jn = pos - ctx;
+#pragma unroll
+            for (int w = 0; w < (NR + 31) / 32; ++w) vis[w] = pos < ctx ? 0xffffffffu : 0u;
+            if (jn >= 0 && pos < end) {
+              int node = s.row0 / p.G, rem = s.row0 - node * p.G;
+              const uint8_t* mp = p.mask + (int64_t)walk.q.cu0 * p.mask_stride + jn;
+#pragma unroll
+              for (int r = 0; r < NR; ++r) {
+                const bool v = r < s.rows && mp[(int64_t)node * p.mask_stride] != 0;
+                vis[r >> 5] |= (v ? 1u : 0u) << (r & 31);
+                if (++rem == p.G) {
+                  rem = 0;
+                  ++node;
+                }
+              }
+            }
+          }
+          ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->s_full[g & 1], (g >> 1) & 1, bs, p.err));
+          umma::fence_after_sync();
+          float x[NR];
+          auto load_x = [&]() {            // raw scores
+            load_s(g, x);
+            if (!full) {
+#pragma unroll
+              for (int r = 0; r < NR; ++r)
+                if (!((vis[r >> 5] >> (r & 31)) & 1u)) x[r] = -INFINITY;
+            }
+          };
+          auto shift_x = [&]() {           // against the running maxima, log2 units
+#pragma unroll
+            for (int r = 0; r < NR; r += 4) {
+              const float4 m = *reinterpret_cast<const float4*>(&sh->m[r]);
+              x[r] = fmaf(x[r], p.scale_log2, -m.x);
+              x[r + 1] = fmaf(x[r + 1], p.scale_log2, -m.y);
+              x[r + 2] = fmaf(x[r + 2], p.scale_log2, -m.z);
+              x[r + 3] = fmaf(x[r + 3], p.scale_log2, -m.w);
+            }
+          };
+          load_x();
+          shift_x();
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int r = 0; r < NR; ++r) top[r & 3] = fmaxf(top[r & 3], x[r]);
+          if (vote_bar(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > kRescaleLog2)) {
+            // some row's maximum rises
+            load_x();
+            warp_columns<NR>(x, [](float a, float b) { return fmaxf(a, b); });
+            if (lane < NR) sh->red[sub][lane] = x[0];
+            if constexpr (NR == 64) sh->red[sub][32 + lane] = x[1];
+            named_bar_sync(1, 128);
+            if (tid < NR) {
+              const float mx = fmaxf(fmaxf(sh->red[0][tid], sh->red[1][tid]),
+                                     fmaxf(sh->red[2][tid], sh->red[3][tid])) * p.scale_log2;
+              const float mo = sh->m[tid];
+              const bool grow = mx > mo + kRescaleLog2;
+              sh->fac[tid] = grow ? ex2(mo - mx) : 1.f;
+              sh->m[tid] = grow ? mx : mo;
+            }
+            named_bar_sync(1, 128);
+            float fac[NR];
+#pragma unroll
+            for (int r = 0; r < NR; r += 4) {
+              const float4 b = *reinterpret_cast<const float4*>(&sh->fac[r]);
+              fac[r] = b.x, fac[r + 1] = b.y, fac[r + 2] = b.z, fac[r + 3] = b.w;
+            }
+#pragma unroll
+            for (int r = 0; r < NR; ++r) l[r] *= fac[r];
+            if (t > s.t0) {
+              // O^T: every PV issued so far has to be done
+              ok = ok && __all_sync(0xffffffffu,
+                                    wait_bar(&bs->pv_done[0], (g - 1) & 1, bs, p.err));
+              umma::fence_after_sync();
+#pragma unroll
+              for (int c = 0; c < 2 * NR / 32; ++c) {
+                float ov[32];
+                umma::tmem_ld32(trow + Gm::kColO + c * 32, ov);
+                umma::tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) ov[e] *= fac[(c * 32 + e) % NR];
+                umma::tmem_st32(trow + Gm::kColO + c * 32, ov);
+              }
+              umma::tmem_wait_st();
+            }
+            load_x();
+            shift_x();
+          }
+          uint32_t hi[NR / 2], lo[NR / 2];
+#pragma unroll
+          for (int r = 0; r < NR; r += 2) {
+            const float a = ex2(x[r]), b = ex2(x[r + 1]);
+            l[r] += a;
+            l[r + 1] += b;
+            float ah, bh;
+            if constexpr (kBf16) {         // truncated: one byte permute a pair
+              hi[r / 2] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+              ah = __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
+              bh = __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
+            } else {
+              hi[r / 2] = Elem<T>::pack(a, b);
+              Elem<T>::unpack(hi[r / 2], ah, bh);
+            }
+            lo[r / 2] = Elem<T>::pack(a - ah, b - bh);
+          }
+          // P's buffer is free once the last PV is done
+          if (g > 0)
+            ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->pv_done[0], (g - 1) & 1, bs, p.err));
+          // row `position` of P^T: NR values, NR remainders
+          unsigned char* pr = smem + Gm::kOffP + tid * 128;
+          const int sw = tid & 7;
+#pragma unroll
+          for (int c = 0; c < NR / 8; ++c) {
+            *reinterpret_cast<uint4*>(pr + ((c ^ sw) << 4)) =
+                make_uint4(hi[4 * c], hi[4 * c + 1], hi[4 * c + 2], hi[4 * c + 3]);
+            unsigned char* q = NR == 64 ? pr + Gm::kBlockBytes + ((c ^ sw) << 4)
+                                        : pr + (((NR / 8 + c) ^ sw) << 4);
+            *reinterpret_cast<uint4*>(q) =
+                make_uint4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
+          }
+          fence_proxy_async_smem();
+          umma::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bs->p_full[0]);
+        }
+
+        // ---- epilogue; barriers are passed whether or not a wait failed
+        ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->pv_done[0], (g - 1) & 1, bs, p.err));
+        umma::fence_after_sync();
+        warp_columns<NR>(l, [](float a, float b) { return a + b; });
+        if (lane < NR) sh->red[sub][lane] = l[0];
+        if constexpr (NR == 64) sh->red[sub][32 + lane] = l[1];
+        named_bar_sync(1, 128);
+        float* slot = p.part + ((int64_t)blockIdx.x * 2 + (s.first ? 0 : 1)) * RG * kPartStride<D>;
+        if (tid < s.rows && ok) {
+          const float L = (sh->red[0][tid] + sh->red[1][tid]) + (sh->red[2][tid] + sh->red[3][tid]);
+          const float M = sh->m[tid] == kNoMax ? -INFINITY : sh->m[tid];
+          if (!s.whole) {
+            *reinterpret_cast<float2*>(slot + (int64_t)tid * kPartStride<D> + D) = make_float2(M, L);
+          } else {
+            const int rq = s.row0 + tid, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
+            const int64_t row = walk.q.cu0 + node;
+            if (p.lse)
+              p.lse[row * p.H + hq] =
+                  L > 0.f ? (M + log2f(L)) * kLn2 : (L == L ? -INFINITY : L);
+            sh->fac[tid] = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+            sh->off[tid] = row * p.out_st + hq * p.out_sh;
+          }
+        }
+        named_bar_sync(1, 128);
+        const bool fix = *reinterpret_cast<volatile int*>(&bs->bad[si % kBadSlots]) != 0;
+#pragma unroll 1
+        for (int c = 0; c < NR; c += 16) {
+          if (c >= s.rows || !ok) break;
+          float a[16], b[16];
+          tmem_ld(trow + Gm::kColO + c, a);
+          tmem_ld(trow + Gm::kColO + NR + c, b);
+          umma::tmem_wait_ld();
+          if (tid < D) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int r = c + e;
+              if (r < s.rows) {
+                float o = a[e] + b[e];
+                if (fix)
+                  o += bad_sum<T>(p, walk.r, walk.q.cu0 + (s.row0 + r) / p.G, ctx,
+                                  max(ctx, s.t0 * kBN), min(end, s.t1 * kBN), s.hk, tid);
+                if (!s.whole) {
+                  slot[(int64_t)r * kPartStride<D> + tid] = o;
+                } else {
+                  o *= sh->fac[r];
+                  if (p.out_f32) reinterpret_cast<float*>(p.out)[sh->off[r] + tid] = o;
+                  else reinterpret_cast<T*>(p.out)[sh->off[r] + tid] = Elem<T>::from_f32(o);
+                }
+              }
+            }
+          }
+        }
+        umma::fence_before_sync();
+        ++si;
+      }
+    }
+  }
+
+  // ---- teardown: every TMEM access and MMA has completed
+  umma::fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    umma::fence_after_sync();
+    umma::tmem_dealloc(tmem, kCols);
   }
 }
 
@@ -1073,10 +1561,10 @@ static int check(const halo_page_pool_t* pool, const halo_tree_problem_t* pb) {
 }
 
 // Rows of a group, from the most rows a request can have on one K/V head:
-// the smallest of 32, 64, 128 and 256 that holds them (256 at most).
+// the smallest of 16, 32, 64, 128 and 256 that holds them (256 at most).
 static int group_rows(const halo_page_pool_t* pool, const halo_tree_problem_t* pb) {
   const int64_t rows = (int64_t)pb->max_nodes * (pb->H / pool->H_kv);
-  return rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
 }
 
 static int64_t desc_bytes(int n_cta) { return ((int64_t)n_cta * sizeof(Desc) + 255) & ~int64_t(255); }
@@ -1086,22 +1574,30 @@ static int64_t ws_bytes(const halo_page_pool_t* pool, const halo_tree_problem_t*
   return desc_bytes(n) + (int64_t)n * 2 * group_rows(pool, pb) * (pool->D + 4) * sizeof(float);
 }
 
-template <typename T, int D, int KPT, int QT>
+template <typename T, int D, int RG>
 static int launch(const Params& p, int n_cta, cudaStream_t st) {
-  using Gm = Geom<D, QT>;
-  constexpr int RG = KPT * QT == 256 ? 256 : KPT;     // copies x rows = 128
-  auto kernel = tree_kernel<T, D, KPT, QT>;
+  void (*kernel)(const Params);
+  int smem, threads;
+  if constexpr (RG <= 64) {
+    kernel = tree_few_kernel<T, D, RG>;
+    smem = FewGeom<D, RG>::kSmemBytes;
+    threads = kFewThreads;
+  } else {
+    kernel = tree_kernel<T, D, RG / 128>;
+    smem = Geom<D, RG / 128>::kSmemBytes;
+    threads = kThreads;
+  }
   static std::once_flag once[64];
   int dev = 0;
   cudaGetDevice(&dev);
   cudaError_t e = cudaSuccess;
   std::call_once(once[dev & 63], [&] {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Gm::kSmemBytes);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   });
-  if (e != cudaSuccess) return cuda_fail(e, "tree_kernel shared-memory attribute");
-  e = launch_dependent(kernel, dim3((unsigned)n_cta), dim3(kThreads), Gm::kSmemBytes, st, p);
+  if (e != cudaSuccess) return cuda_fail(e, "tree kernel shared-memory attribute");
+  e = launch_dependent(kernel, dim3((unsigned)n_cta), dim3((unsigned)threads), (size_t)smem, st, p);
   if (e == cudaSuccess) e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "tree_kernel launch");
+  if (e != cudaSuccess) return cuda_fail(e, "tree kernel launch");
   count_launches();
   if (n_cta > 1) {
     e = launch_dependent(tree_merge_kernel<T, D>,
@@ -1117,10 +1613,11 @@ static int launch(const Params& p, int n_cta, cudaStream_t st) {
 template <typename T, int D>
 static int dispatch(int rows, const Params& p, int n_cta, cudaStream_t st) {
   switch (rows) {
-    case 32: return launch<T, D, 32, 1>(p, n_cta, st);
-    case 64: return launch<T, D, 64, 1>(p, n_cta, st);
-    case 128: return launch<T, D, 128, 1>(p, n_cta, st);
-    default: return launch<T, D, 128, 2>(p, n_cta, st);
+    case 16: return launch<T, D, 16>(p, n_cta, st);
+    case 32: return launch<T, D, 32>(p, n_cta, st);
+    case 64: return launch<T, D, 64>(p, n_cta, st);
+    case 128: return launch<T, D, 128>(p, n_cta, st);
+    default: return launch<T, D, 256>(p, n_cta, st);
   }
 }
 
