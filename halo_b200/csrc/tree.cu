@@ -38,7 +38,7 @@ namespace tree {
 
 constexpr int kBN = 128;               // positions of a tile (a unit)
 constexpr int kThreads = 384;          // tree_kernel
-constexpr int kFewThreads = 256;       // tree_few_kernel
+constexpr int kFewThreads = 384;       // tree_few_kernel
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.f;    // headroom of the running maximum
 constexpr int kBadSlots = 8;
@@ -69,13 +69,19 @@ struct alignas(64) Params {
 
 // What the merge has to know of the segment that holds a CTA's first unit.
 struct alignas(64) Desc {
-  int64_t start, end, total;           // units: the segment's, and all units
+  int64_t start;                       // units before the segment's first tile
+  int64_t quot;                        // all units: quot * CTAs + rem
+  int32_t rem;
+  int32_t nt;                          // the segment's tiles
   int32_t cu0, hk, row0, rows;         // row0: the group's first row of the request
 };
 
-// Rows of a group's slot: o[D], m (log2 units), l, padding to 16 bytes.
+// A part of a cut segment in the workspace: o [RG][D], then (m in log2 units,
+// l) [RG][2], fp32.
 template <int D>
-constexpr int kPartStride = D + 4;
+__host__ __device__ constexpr int64_t part_floats(int RG) {
+  return (int64_t)RG * (D + 2);
+}
 
 // tree_kernel: QT query tiles of 128 rows.
 template <int D, int QT>
@@ -126,6 +132,12 @@ struct FewShared {
 };
 static_assert(sizeof(FewShared) <= 2048, "scratch of tree_few_kernel");
 
+
+// ---- the units of a request
+struct Req {
+  int ctx, end, nodes, cu0, nt, ng;
+};
+
 struct Bars {
   uint64_t q_full[2], q_empty[2];
   uint64_t k_full[6], k_empty[6], v_full[6], v_ready[6], v_empty[6];
@@ -134,6 +146,7 @@ struct Bars {
   int64_t base0, total;
   uint32_t tmem_base;
   int abort_flag, r0;
+  Req req0;
   int bad[kBadSlots];
 };
 static_assert(sizeof(Bars) <= 1024, "barrier block");
@@ -155,11 +168,10 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Bars* b
   }
 }
 
-// ---- the units of a request
-struct Req {
-  int ctx, end, nodes, cu0, nt, ng;
-  __device__ __forceinline__ int64_t units(int H_kv) const { return (int64_t)nt * ng * H_kv; }
-};
+// Units that a segment weighs beside its tiles: query rows, first maxima,
+// epilogue.  They come before its tiles, so a cut among them cuts nothing.
+template <int RG>
+constexpr int kSetup = RG <= 64 ? 2 : 1;
 
 template <int RG>
 __device__ __forceinline__ Req load_req(const Params& p, int r) {
@@ -173,6 +185,10 @@ __device__ __forceinline__ Req load_req(const Params& p, int r) {
   q.nt = q.nodes > 0 ? max(1, (q.end + kBN - 1) / kBN) : 0;
   return q;
 }
+template <int RG>
+__device__ __forceinline__ int64_t units_of(const Req& q, int H_kv) {
+  return (int64_t)(q.nt + kSetup<RG>) * (q.ng * H_kv);
+}
 
 // One (request, head, group) part of a CTA's run: tiles [t0, t1) of nt.
 struct Seg {
@@ -183,32 +199,43 @@ struct Seg {
 // Walks a CTA's run segment by segment; every role keeps its own.
 template <int RG>
 struct Walk {
-  int64_t u, u0, u1, base, units;
+  int64_t u, u1, base, units;
   int r;
+  bool begun;
   Req q;
-  __device__ __forceinline__ Walk(const Params& p, int r0, int64_t base0, int64_t a, int64_t b)
-      : u(a), u0(a), u1(b), base(base0), r(r0) {
-    q = load_req<RG>(p, r);
-    units = q.units(p.H_kv);
+  __device__ __forceinline__ Walk(const Params& p, int r0, const Req& q0, int64_t base0, int64_t a,
+                                  int64_t b)
+      : u(a), u1(b), base(base0), r(r0), begun(false), q(q0) {
+    units = units_of<RG>(q, p.H_kv);
   }
   __device__ __forceinline__ bool next(const Params& p, Seg& s) {
-    if (u >= u1) return false;
-    while (u - base >= units) {
-      base += units;
-      q = load_req<RG>(p, ++r);
-      units = q.units(p.H_kv);
+    constexpr int W = kSetup<RG>;
+    while (u < u1) {
+      while (u - base >= units) {
+        base += units;
+        q = load_req<RG>(p, ++r);
+        units = units_of<RG>(q, p.H_kv);
+      }
+      const int64_t local = u - base;
+      const int len = q.nt + W;
+      // 32-bit division where it serves
+      const int hg = (local >> 31) == 0 ? (int)((uint32_t)local / (uint32_t)len)
+                                        : (int)(local / len);
+      const int a = (int)(local - (int64_t)hg * len);
+      const int b = (int)min((int64_t)len, a + (u1 - u));
+      u += b - a;
+      s.t0 = max(a - W, 0);
+      s.t1 = b - W;
+      if (s.t1 <= s.t0) continue;          // set-up units alone
+      s.hk = hg / q.ng;
+      s.row0 = (hg - s.hk * q.ng) * RG;
+      s.rows = min(RG, q.nodes * p.G - s.row0);
+      s.whole = s.t0 == 0 && s.t1 == q.nt;
+      s.first = !begun;
+      begun = true;
+      return true;
     }
-    const int64_t local = u - base;
-    const int hg = (int)(local / q.nt);
-    s.t0 = (int)(local - (int64_t)hg * q.nt);
-    s.t1 = (int)min((int64_t)q.nt, s.t0 + (u1 - u));
-    s.hk = hg / q.ng;
-    s.row0 = (hg - s.hk * q.ng) * RG;
-    s.rows = min(RG, q.nodes * p.G - s.row0);
-    s.whole = s.t0 == 0 && s.t1 == q.nt;
-    s.first = u == u0;
-    u += s.t1 - s.t0;
-    return true;
+    return false;
   }
 };
 
@@ -235,6 +262,29 @@ __device__ __forceinline__ void tmem_ld(uint32_t a, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 __device__ __forceinline__ void tmem_ld(uint32_t a, float (&v)[32]) { umma::tmem_ld32(a, v); }
+
+__device__ __forceinline__ void tmem_st(uint32_t a, const float (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a),
+               "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
+               "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])),
+               "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st(uint32_t a, const float (&v)[16]) {
+  umma::tmem_st16u(a, reinterpret_cast<const uint32_t*>(v));
+}
+__device__ __forceinline__ void tmem_st(uint32_t a, const float (&v)[32]) { umma::tmem_st32(a, v); }
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
+// Asynchronous 16-byte copy to shared memory; zeros where `in` is false.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(in ? 16 : 0)
+               : "memory");
+}
 
 // A value the compiler cannot see through: keeps it from holding every
 // unrolled MMA's descriptor in a register across the loop.
@@ -275,28 +325,39 @@ __device__ __forceinline__ void find_run(const Params& p, Bars* bs, int64_t& u0,
     }
     return v;
   };
-  auto units_of = [&](int r) { return r < p.R ? load_req<RG>(p, r).units(p.H_kv) : (int64_t)0; };
+  Req q;
+  auto units = [&](int r) -> int64_t {
+    if (r >= p.R) return 0;
+    q = load_req<RG>(p, r);
+    return units_of<RG>(q, p.H_kv);
+  };
   int64_t mine = 0, incl = 0;
   U = 0;
   for (int r0 = 0; r0 < p.R; r0 += NT) {
     int64_t t;
-    mine = units_of(r0 + threadIdx.x);
+    mine = units(r0 + threadIdx.x);
     incl = prefix(mine, t);
     U += t;
   }
-  u0 = (int64_t)blockIdx.x * U / gridDim.x;
-  u1 = (int64_t)(blockIdx.x + 1) * U / gridDim.x;
+  if ((U >> 20) == 0) {                // 32-bit divisions (a grid has < 2^12 CTAs)
+    u0 = (uint32_t)(blockIdx.x * (uint32_t)U) / gridDim.x;
+    u1 = (uint32_t)((blockIdx.x + 1) * (uint32_t)U) / gridDim.x;
+  } else {
+    u0 = (int64_t)blockIdx.x * U / gridDim.x;
+    u1 = (int64_t)(blockIdx.x + 1) * U / gridDim.x;
+  }
   {
     int64_t before = 0;
     for (int r0 = 0; r0 < p.R; r0 += NT) {
       int64_t t = U;
       if (p.R > NT) {                // else the scan above holds
-        mine = units_of(r0 + threadIdx.x);
+        mine = units(r0 + threadIdx.x);
         incl = prefix(mine, t);
       }
       const int64_t lo = before + incl - mine;
       if (mine > 0 && lo <= u0 && u0 < lo + mine) {
         bs->r0 = r0 + threadIdx.x;
+        bs->req0 = q;
         bs->base0 = lo;
       }
       before += t;
@@ -304,22 +365,22 @@ __device__ __forceinline__ void find_run(const Params& p, Bars* bs, int64_t& u0,
   }
 }
 
-// Thread 0: the segment of the run's first unit, for the merge.
+// One thread: the segment that holds the run's first unit, for the merge.
 template <int RG>
 __device__ __forceinline__ void write_desc(const Params& p, const Bars* bs, int64_t u0, int64_t U) {
   Desc d{};
-  d.total = U;
-  d.start = d.end = u0;
+  d.quot = U / gridDim.x;
+  d.rem = (int32_t)(U - d.quot * gridDim.x);
   if (u0 < U) {
-    Walk<RG> w(p, bs->r0, bs->base0, u0, u0 + 1);
-    Seg s;
-    w.next(p, s);
-    d.start = u0 - s.t0;
-    d.end = d.start + w.q.nt;
-    d.cu0 = w.q.cu0;
-    d.hk = s.hk;
-    d.row0 = s.row0;
-    d.rows = s.rows;
+    const Req& q = bs->req0;
+    const int len = q.nt + kSetup<RG>;
+    const int hg = (int)((u0 - bs->base0) / len);
+    d.start = bs->base0 + (int64_t)hg * len + kSetup<RG>;
+    d.nt = q.nt;
+    d.cu0 = q.cu0;
+    d.hk = hg / q.ng;
+    d.row0 = (hg - d.hk * q.ng) * RG;
+    d.rows = min(RG, q.nodes * p.G - d.row0);
   }
   p.desc[blockIdx.x] = d;
 }
@@ -523,6 +584,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     }
     bs->abort_flag = 0;
     fence_mbar_init();
+    prefetch_map(&p.kmap);
+    prefetch_map(&p.vmap);
   }
   if (warp == 1) {
     umma::tmem_alloc(&bs->tmem_base, kTmemCols);
@@ -554,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   if (u0 < u1 && aligned) {
   if (warp < 4) {
     umma::regs_dec<88>();
-    Walk<RG> walk(p, bs->r0, bs->base0, u0, u1);
+    Walk<RG> walk(p, bs->r0, bs->req0, bs->base0, u0, u1);
     Seg s;
     if (warp == 0) {
       produce<RG, Gm, true>(p, bs, smem, walk);
@@ -632,7 +695,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     const int tid = threadIdx.x - 128;           // 0..255 over both streams
     const uint32_t trow = tmem + ((uint32_t)(sub * 32) << 16);
     const uint32_t scol = x * 128, ocol = Gm::kColO + x * D;
-    Walk<RG> walk(p, bs->r0, bs->base0, u0, u1);
+    Walk<RG> walk(p, bs->r0, bs->req0, bs->base0, u0, u1);
     Seg s;
     int j = 0, si = 0, sx = 0;                   // tiles of this stream; segments; with tiles
     bool ok = true;
@@ -789,7 +852,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         ++sx;
         umma::fence_after_sync();
       }
-      float* slot = p.part + ((int64_t)blockIdx.x * 2 + (s.first ? 0 : 1)) * RG * kPartStride<D>;
+      float* slot = p.part + ((int64_t)blockIdx.x * 2 + (s.first ? 0 : 1)) * part_floats<D>(RG);
       auto bad = [&](int row, int col) {
         return bad_sum<T>(p, walk.r, cu0 + (s.row0 + row) / p.G, ctx, max(ctx, s.t0 * kBN),
                           min(end, s.t1 * kBN), s.hk, col);
@@ -797,11 +860,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       auto store = [&](int row, int col, float M, float L, float* o, auto n_col) {
         constexpr int N = decltype(n_col)::value;
         if (!s.whole) {
-          float* d = slot + (int64_t)row * kPartStride<D> + col;
+          float* d = slot + row * D + col;
 #pragma unroll
           for (int e = 0; e < N; e += 4)
             *reinterpret_cast<float4*>(d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          if (col == 0) *reinterpret_cast<float2*>(slot + (int64_t)row * kPartStride<D> + D) = make_float2(M, L);
+          if (col == 0) *reinterpret_cast<float2*>(slot + RG * D + 2 * row) = make_float2(M, L);
           return;
         }
         const int rq = s.row0 + row, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
@@ -926,13 +989,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
 
 // ======================================================================
 // tree_few_kernel: groups of at most 64 rows (NR = 16, 32 or 64).  One CTA an
-// SM, 256 threads.
+// SM, 384 threads.
 //   warp 0      TMA producer (as in tree_kernel)
 //   warp 1      TMEM owner; lane 0 issues every MMA
 //   warp 2      cleans V
 //   warp 3      query rows of the next segment (two buffers)
-//   warps 4-7   softmax (thread = position of the tile) and epilogue (thread =
-//               output column)
+//   warps 4-11  softmax (thread = position of the tile) and epilogue (thread =
+//               output column), warps 4-7 the first NR / 2 rows, warps 8-11 the
+//               others
 // Both products have the K/V tile as the 128-row operand and the query rows
 // as the columns: S^T = K Q^T (M = positions, N = NR) and O^T += V^T P^T
 // (M = columns of V, N = 2 NR: the weights' 16-bit values and, beside them,
@@ -948,41 +1012,37 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
 // in a segment's first tile and in the rare tile that raises it.
 constexpr float kNoMax = -1e30f;           // nothing seen yet: any score raises it
 
-// Sum or maximum over the warp of NR columns, one a row.  Lane i ends with row
-// i % NR in v[0] (NR = 64: rows i and 32 + i in v[0], v[1]).
-template <int NR, class Op>
-__device__ __forceinline__ void warp_columns(float (&v)[NR], Op op) {
+// Sum or maximum over the warp of N (8, 16 or 32) columns, one a row: lane i
+// ends with row i % N in v[0].
+template <int N, class Op>
+__device__ __forceinline__ void warp_columns(float (&v)[N], Op op) {
   const int lane = threadIdx.x & 31;
-  if constexpr (NR == 16) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = op(v[i], __shfl_xor_sync(0xffffffffu, v[i], 16));
+  for (int o = 16; o >= N; o >>= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = op(v[i], __shfl_xor_sync(0xffffffffu, v[i], o));
   }
-  constexpr int W = NR < 32 ? NR : 32;
 #pragma unroll
-  for (int o = W / 2; o >= 1; o >>= 1) {
+  for (int o = N / 2; o >= 1; o >>= 1) {
     const bool up = lane & o;
 #pragma unroll
-    for (int b = 0; b < NR; b += W) {
-#pragma unroll
-      for (int i = 0; i < o; ++i) {
-        const float keep = up ? v[b + i + o] : v[b + i], give = up ? v[b + i] : v[b + i + o];
-        v[b + i] = op(keep, __shfl_xor_sync(0xffffffffu, give, o));
-      }
+    for (int i = 0; i < o; ++i) {
+      const float keep = up ? v[i + o] : v[i], give = up ? v[i] : v[i + o];
+      v[i] = op(keep, __shfl_xor_sync(0xffffffffu, give, o));
     }
   }
-  if constexpr (NR == 64) v[1] = v[32];
 }
 
-// Barrier of the four softmax warps that tells whether any thread voted.
-__device__ __forceinline__ bool vote_bar(bool vote) {
+// Barrier `id` of four softmax warps that tells whether any thread voted.
+__device__ __forceinline__ bool vote_bar(int id, bool vote) {
   uint32_t any;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+      "barrier.cta.red.or.pred q, %2, 128, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(any)
-      : "r"(vote ? 1u : 0u)
+      : "r"(vote ? 1u : 0u), "r"(id)
       : "memory");
   return any != 0;
 }
@@ -1012,11 +1072,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
       mbar_init(&bs->v_ready[i], 1);
       mbar_init(&bs->v_empty[i], 1);
     }
-    mbar_init(&bs->p_full[0], 4);
+    mbar_init(&bs->p_full[0], 8);
     mbar_init(&bs->pv_done[0], 1);
     mbar_init(&bs->mma_done[0], 1);
     bs->abort_flag = 0;
     fence_mbar_init();
+    prefetch_map(&p.kmap);
+    prefetch_map(&p.vmap);
   }
   if (warp == 1) {
     umma::tmem_alloc(&bs->tmem_base, kCols);
@@ -1041,7 +1103,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
     set_device_error(p.err, static_cast<unsigned int>(-HALO_ERR_MISALIGNED));
 
   if (u0 < u1 && aligned) {
-    Walk<RG> walk(p, bs->r0, bs->base0, u0, u1);
+    Walk<RG> walk(p, bs->r0, bs->req0, bs->base0, u0, u1);
     Seg s;
     if (warp == 0) {
       produce<RG, Gm, false>(p, bs, smem, walk);
@@ -1112,28 +1174,18 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
           ok = __all_sync(0xffffffffu,
                           wait_bar(&bs->q_empty[si & 1], ((si >> 1) - 1) & 1, bs, p.err));
         if (!ok) break;
-        constexpr int VPR = D / 8, N = NR * VPR;   // a multiple of 128
-        for (int i0 = 0; i0 < N; i0 += 128) {
-          uint4 w[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int i = i0 + u * 32 + lane, row = i / VPR, c = i % VPR;
-            w[u] = make_uint4(0, 0, 0, 0);
-            if (row < s.rows) {
-              const int rq = s.row0 + row, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
-              w[u] = *reinterpret_cast<const uint4*>(
-                  reinterpret_cast<const T*>(p.q) + (int64_t)(walk.q.cu0 + node) * p.q_st +
-                  hq * p.q_sh + c * 8);
-            }
-          }
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int i = i0 + u * 32 + lane, row = i / VPR, c = i % VPR;
-            *reinterpret_cast<uint4*>(smem + Gm::kOffQ + (si & 1) * Gm::kQBytes +
-                                      (c >> 3) * NR * 128 + row * 128 +
-                                      (((c & 7) ^ (row & 7)) << 4)) = w[u];
-          }
+        constexpr int VPR = D / 8;
+        const T* qb = reinterpret_cast<const T*>(p.q) + (int64_t)walk.q.cu0 * p.q_st +
+                      (int64_t)s.hk * p.G * p.q_sh;
+        for (int i = lane; i < NR * VPR; i += 32) {    // 16-byte copies, all in flight
+          const int row = i / VPR, c = i % VPR;
+          const int rq = s.row0 + row, node = rq / p.G;
+          const bool in = row < s.rows;
+          copy16(sQ + (si & 1) * Gm::kQBytes + (c >> 3) * NR * 128 + row * 128 +
+                     (((c & 7) ^ (row & 7)) << 4),
+                 in ? qb + node * p.q_st + (rq - node * p.G) * p.q_sh + c * 8 : qb, in);
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bs->q_full[si & 1]);
@@ -1141,42 +1193,32 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
       }
     } else {
       // -------------------------------------------------------- softmax
-      const int sub = warp & 3, tid = threadIdx.x - 128;
+      // two groups of four warps, each RT of the NR rows; thread = position
+      constexpr int RT = NR / 2;
+      const int sub = warp & 3, grp = (warp - 4) >> 2, bar = 1 + grp;
+      const int tid = threadIdx.x & 127, r0 = grp * RT;
       const uint32_t trow = tmem + ((uint32_t)(sub * 32) << 16);
-      auto load_s = [&](int g, float (&x)[NR]) {
-        const uint32_t a = trow + (g & 1) * NR;
-        if constexpr (NR == 16) {
-          tmem_ld(a, x);
-        } else {
-#pragma unroll
-          for (int c = 0; c < NR / 32; ++c) umma::tmem_ld32(a + c * 32, x + c * 32);
-        }
-        umma::tmem_wait_ld();
-      };
       int g = 0, si = 0;
       bool ok = true;
       while (walk.next(p, s)) {
         const int ctx = walk.q.ctx, end = walk.q.end;
-        float l[NR];
+        float l[RT];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) l[r] = 0.f;
-        if (tid < NR) sh->m[tid] = kNoMax;
-        named_bar_sync(1, 128);
+        for (int r = 0; r < RT; ++r) l[r] = 0.f;
         for (int t = s.t0; t < s.t1; ++t, ++g) {
           // rows that see this thread's position
           const bool full = (t + 1) * kBN <= ctx;
-          uint32_t vis[(NR + 31) / 32];
+          uint32_t vis = 0;                // a bit a row
           if (!full) {
             const int pos = t * kBN + tid, jn = pos - ctx;
-#pragma unroll
-            for (int w = 0; w < (NR + 31) / 32; ++w) vis[w] = pos < ctx ? 0xffffffffu : 0u;
+            vis = pos < ctx ? 0xffffffffu : 0u;
             if (jn >= 0 && pos < end) {
-              int node = s.row0 / p.G, rem = s.row0 - node * p.G;
+              int node = (s.row0 + r0) / p.G, rem = s.row0 + r0 - node * p.G;
               const uint8_t* mp = p.mask + (int64_t)walk.q.cu0 * p.mask_stride + jn;
 #pragma unroll
-              for (int r = 0; r < NR; ++r) {
-                const bool v = r < s.rows && mp[(int64_t)node * p.mask_stride] != 0;
-                vis[r >> 5] |= (v ? 1u : 0u) << (r & 31);
+              for (int r = 0; r < RT; ++r) {
+                const bool v = r0 + r < s.rows && mp[(int64_t)node * p.mask_stride] != 0;
+                vis |= (v ? 1u : 0u) << r;
                 if (++rem == p.G) {
                   rem = 0;
                   ++node;
@@ -1186,76 +1228,78 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
           }
           ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->s_full[g & 1], (g >> 1) & 1, bs, p.err));
           umma::fence_after_sync();
-          float x[NR];
-          auto load_x = [&]() {            // raw scores
-            load_s(g, x);
+          // Scores against the running maxima, in log2 units; where a row's
+          // maximum has to rise (always in the first tile) the raw scores are
+          // reduced and the loop runs again.
+          float x[RT];
+          bool rise = t == s.t0;
+          while (true) {
+            tmem_ld(trow + (g & 1) * NR + r0, x);
+            umma::tmem_wait_ld();
             if (!full) {
 #pragma unroll
-              for (int r = 0; r < NR; ++r)
-                if (!((vis[r >> 5] >> (r & 31)) & 1u)) x[r] = -INFINITY;
+              for (int r = 0; r < RT; ++r)
+                if (!((vis >> r) & 1u)) x[r] = -INFINITY;
             }
-          };
-          auto shift_x = [&]() {           // against the running maxima, log2 units
+            if (!rise) {
+              float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int r = 0; r < NR; r += 4) {
-              const float4 m = *reinterpret_cast<const float4*>(&sh->m[r]);
-              x[r] = fmaf(x[r], p.scale_log2, -m.x);
-              x[r + 1] = fmaf(x[r + 1], p.scale_log2, -m.y);
-              x[r + 2] = fmaf(x[r + 2], p.scale_log2, -m.z);
-              x[r + 3] = fmaf(x[r + 3], p.scale_log2, -m.w);
+              for (int r = 0; r < RT; r += 4) {
+                const float4 m = *reinterpret_cast<const float4*>(&sh->m[r0 + r]);
+                x[r] = fmaf(x[r], p.scale_log2, -m.x);
+                x[r + 1] = fmaf(x[r + 1], p.scale_log2, -m.y);
+                x[r + 2] = fmaf(x[r + 2], p.scale_log2, -m.z);
+                x[r + 3] = fmaf(x[r + 3], p.scale_log2, -m.w);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], x[r + e]);
+              }
+              rise = vote_bar(bar, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > kRescaleLog2);
+              if (!rise) break;
+              continue;
             }
-          };
-          load_x();
-          shift_x();
-          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int r = 0; r < NR; ++r) top[r & 3] = fmaxf(top[r & 3], x[r]);
-          if (vote_bar(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > kRescaleLog2)) {
-            // some row's maximum rises
-            load_x();
-            warp_columns<NR>(x, [](float a, float b) { return fmaxf(a, b); });
-            if (lane < NR) sh->red[sub][lane] = x[0];
-            if constexpr (NR == 64) sh->red[sub][32 + lane] = x[1];
-            named_bar_sync(1, 128);
-            if (tid < NR) {
-              const float mx = fmaxf(fmaxf(sh->red[0][tid], sh->red[1][tid]),
-                                     fmaxf(sh->red[2][tid], sh->red[3][tid])) * p.scale_log2;
-              const float mo = sh->m[tid];
+            warp_columns<RT>(x, [](float a, float b) { return fmaxf(a, b); });
+            if (lane < RT) sh->red[sub][r0 + lane] = x[0];
+            named_bar_sync(bar, 128);
+            if (tid < RT) {
+              const int r = r0 + tid;
+              const float mx = fmaxf(fmaxf(sh->red[0][r], sh->red[1][r]),
+                                     fmaxf(sh->red[2][r], sh->red[3][r])) * p.scale_log2;
+              const float mo = t == s.t0 ? kNoMax : sh->m[r];
               const bool grow = mx > mo + kRescaleLog2;
-              sh->fac[tid] = grow ? ex2(mo - mx) : 1.f;
-              sh->m[tid] = grow ? mx : mo;
+              sh->fac[r] = grow ? ex2(mo - mx) : 1.f;
+              sh->m[r] = grow ? mx : mo;
             }
-            named_bar_sync(1, 128);
-            float fac[NR];
-#pragma unroll
-            for (int r = 0; r < NR; r += 4) {
-              const float4 b = *reinterpret_cast<const float4*>(&sh->fac[r]);
-              fac[r] = b.x, fac[r + 1] = b.y, fac[r + 2] = b.z, fac[r + 3] = b.w;
-            }
-#pragma unroll
-            for (int r = 0; r < NR; ++r) l[r] *= fac[r];
+            named_bar_sync(bar, 128);
             if (t > s.t0) {
               // O^T: every PV issued so far has to be done
               ok = ok && __all_sync(0xffffffffu,
                                     wait_bar(&bs->pv_done[0], (g - 1) & 1, bs, p.err));
               umma::fence_after_sync();
+              float fac[RT];
 #pragma unroll
-              for (int c = 0; c < 2 * NR / 32; ++c) {
-                float ov[32];
-                umma::tmem_ld32(trow + Gm::kColO + c * 32, ov);
+              for (int r = 0; r < RT; r += 4) {
+                const float4 b = *reinterpret_cast<const float4*>(&sh->fac[r0 + r]);
+                fac[r] = b.x, fac[r + 1] = b.y, fac[r + 2] = b.z, fac[r + 3] = b.w;
+              }
+#pragma unroll
+              for (int r = 0; r < RT; ++r) l[r] *= fac[r];
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                float ov[RT];
+                const uint32_t oc = trow + Gm::kColO + c * NR + r0;
+                tmem_ld(oc, ov);
                 umma::tmem_wait_ld();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) ov[e] *= fac[(c * 32 + e) % NR];
-                umma::tmem_st32(trow + Gm::kColO + c * 32, ov);
+                for (int e = 0; e < RT; ++e) ov[e] *= fac[e];
+                tmem_st(oc, ov);
               }
               umma::tmem_wait_st();
             }
-            load_x();
-            shift_x();
+            rise = false;
           }
-          uint32_t hi[NR / 2], lo[NR / 2];
+          uint32_t hi[RT / 2], lo[RT / 2];
 #pragma unroll
-          for (int r = 0; r < NR; r += 2) {
+          for (int r = 0; r < RT; r += 2) {
             const float a = ex2(x[r]), b = ex2(x[r + 1]);
             l[r] += a;
             l[r + 1] += b;
@@ -1275,13 +1319,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
             ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->pv_done[0], (g - 1) & 1, bs, p.err));
           // row `position` of P^T: NR values, NR remainders
           unsigned char* pr = smem + Gm::kOffP + tid * 128;
-          const int sw = tid & 7;
+          const int sw = tid & 7, c0 = grp * (RT / 8);
 #pragma unroll
-          for (int c = 0; c < NR / 8; ++c) {
-            *reinterpret_cast<uint4*>(pr + ((c ^ sw) << 4)) =
+          for (int c = 0; c < RT / 8; ++c) {
+            *reinterpret_cast<uint4*>(pr + (((c0 + c) ^ sw) << 4)) =
                 make_uint4(hi[4 * c], hi[4 * c + 1], hi[4 * c + 2], hi[4 * c + 3]);
-            unsigned char* q = NR == 64 ? pr + Gm::kBlockBytes + ((c ^ sw) << 4)
-                                        : pr + (((NR / 8 + c) ^ sw) << 4);
+            unsigned char* q = NR == 64 ? pr + Gm::kBlockBytes + (((c0 + c) ^ sw) << 4)
+                                        : pr + (((NR / 8 + c0 + c) ^ sw) << 4);
             *reinterpret_cast<uint4*>(q) =
                 make_uint4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
           }
@@ -1294,53 +1338,65 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
         // ---- epilogue; barriers are passed whether or not a wait failed
         ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->pv_done[0], (g - 1) & 1, bs, p.err));
         umma::fence_after_sync();
-        warp_columns<NR>(l, [](float a, float b) { return a + b; });
-        if (lane < NR) sh->red[sub][lane] = l[0];
-        if constexpr (NR == 64) sh->red[sub][32 + lane] = l[1];
-        named_bar_sync(1, 128);
-        float* slot = p.part + ((int64_t)blockIdx.x * 2 + (s.first ? 0 : 1)) * RG * kPartStride<D>;
-        if (tid < s.rows && ok) {
-          const float L = (sh->red[0][tid] + sh->red[1][tid]) + (sh->red[2][tid] + sh->red[3][tid]);
-          const float M = sh->m[tid] == kNoMax ? -INFINITY : sh->m[tid];
+        warp_columns<RT>(l, [](float a, float b) { return a + b; });
+        if (lane < RT) sh->red[sub][r0 + lane] = l[0];
+        named_bar_sync(bar, 128);
+        // where each row goes and what it is scaled by: the output, or as it
+        // is to the workspace
+        float* part = p.part + ((int64_t)blockIdx.x * 2 + (s.first ? 0 : 1)) * part_floats<D>(RG);
+        if (tid < RT && r0 + tid < s.rows) {
+          const int r = r0 + tid;
+          const float L = (sh->red[0][r] + sh->red[1][r]) + (sh->red[2][r] + sh->red[3][r]);
+          const float M = sh->m[r] == kNoMax ? -INFINITY : sh->m[r];
           if (!s.whole) {
-            *reinterpret_cast<float2*>(slot + (int64_t)tid * kPartStride<D> + D) = make_float2(M, L);
+            *reinterpret_cast<float2*>(part + RG * D + 2 * r) = make_float2(M, L);
+            sh->fac[r] = 1.f;
+            sh->off[r] = r * D;
           } else {
-            const int rq = s.row0 + tid, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
+            const int rq = s.row0 + r, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
             const int64_t row = walk.q.cu0 + node;
             if (p.lse)
               p.lse[row * p.H + hq] =
                   L > 0.f ? (M + log2f(L)) * kLn2 : (L == L ? -INFINITY : L);
-            sh->fac[tid] = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
-            sh->off[tid] = row * p.out_st + hq * p.out_sh;
+            sh->fac[r] = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+            sh->off[r] = row * p.out_st + hq * p.out_sh;
           }
         }
-        named_bar_sync(1, 128);
+        named_bar_sync(bar, 128);
         const bool fix = *reinterpret_cast<volatile int*>(&bs->bad[si % kBadSlots]) != 0;
+        float* of = !s.whole ? part : p.out_f32 ? reinterpret_cast<float*>(p.out) : nullptr;
 #pragma unroll 1
-        for (int c = 0; c < NR; c += 16) {
-          if (c >= s.rows || !ok) break;
-          float a[16], b[16];
+        for (int c = r0; c < min(r0 + RT, s.rows); c += 8) {
+          float a[8], b[8];
           tmem_ld(trow + Gm::kColO + c, a);
           tmem_ld(trow + Gm::kColO + NR + c, b);
-          umma::tmem_wait_ld();
-          if (tid < D) {
+          float fac[8];
+          int64_t off[8];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int r = c + e;
-              if (r < s.rows) {
-                float o = a[e] + b[e];
-                if (fix)
-                  o += bad_sum<T>(p, walk.r, walk.q.cu0 + (s.row0 + r) / p.G, ctx,
-                                  max(ctx, s.t0 * kBN), min(end, s.t1 * kBN), s.hk, tid);
-                if (!s.whole) {
-                  slot[(int64_t)r * kPartStride<D> + tid] = o;
-                } else {
-                  o *= sh->fac[r];
-                  if (p.out_f32) reinterpret_cast<float*>(p.out)[sh->off[r] + tid] = o;
-                  else reinterpret_cast<T*>(p.out)[sh->off[r] + tid] = Elem<T>::from_f32(o);
-                }
-              }
-            }
+          for (int e = 0; e < 8; ++e) {
+            fac[e] = sh->fac[c + e];
+            off[e] = sh->off[c + e] + tid;
+          }
+          umma::tmem_wait_ld();
+          if (tid >= D || !ok) continue;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) a[e] += b[e];
+          if (fix) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (c + e < s.rows)
+                a[e] += bad_sum<T>(p, walk.r, walk.q.cu0 + (s.row0 + c + e) / p.G, ctx,
+                                   max(ctx, s.t0 * kBN), min(end, s.t1 * kBN), s.hk, tid);
+          }
+          if (of) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (c + e < s.rows) of[off[e]] = a[e] * fac[e];
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (c + e < s.rows)
+                reinterpret_cast<T*>(p.out)[off[e]] = Elem<T>::from_f32(a[e] * fac[e]);
           }
         }
         umma::fence_before_sync();
@@ -1361,7 +1417,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
 // ======================================================================
 // tree_merge_kernel: joins the parts of segments that were cut.  Block
 // (c - 1, y) looks at the cut between CTAs c - 1 and c; the first cut inside
-// a segment owns it, y takes 8 of its rows, a warp each.
+// a segment owns it, y takes 8 of its rows, a warp each.  Latency-bound: the
+// lanes find the CTAs that hold a part side by side.
 constexpr int kMergeWarps = 8;
 
 template <typename T, int D>
@@ -1369,66 +1426,75 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
     const __grid_constant__ Params p, int n_cta, int RG) {
   constexpr int C = D / 32;
   grid_dep_wait();
+  grid_dep_trigger();                      // the next kernel may begin its set-up
   const int c = (int)blockIdx.x + 1;
   const Desc d = p.desc[c];
-  auto cut = [&](int i) { return (int64_t)i * d.total / n_cta; };
-  const int64_t uc = cut(c);
-  if (uc >= d.total || d.start >= uc || cut(c - 1) > d.start) return;
   const int row = (int)blockIdx.y * kMergeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (row >= d.rows) return;
-  auto part = [&](int i) {      // CTA i's rows of this segment
-    const int sl = i == c - 1 && cut(c - 1) < d.start ? 1 : 0;
-    return p.part + (((int64_t)i * 2 + sl) * RG + row) * kPartStride<D>;
+  // the cut before CTA i, in tiles of this segment (a cut in its set-up units
+  // or before it: 0); i U / n = i (U / n) + i (U mod n) / n
+  auto cut = [&](int i) {
+    const int64_t t = i * d.quot + (uint32_t)(i * d.rem) / (uint32_t)n_cta - d.start;
+    return (int)min(max(t, (int64_t)0), (int64_t)d.nt);
   };
-  // the CTAs that hold a part: c - 1, then those that begin before the end
-  int last = c;
-  while (last + 1 < n_cta && cut(last + 1) < d.end) ++last;
+  const int own = cut(c);
+  if (own <= 0 || own >= d.nt || cut(c - 1) > 0) return;
+  const int64_t before = (c - 1) * d.quot + (uint32_t)((c - 1) * d.rem) / (uint32_t)n_cta;
   float M = -INFINITY, L = 0.f, acc[C];
 #pragma unroll
   for (int e = 0; e < C; ++e) acc[e] = 0.f;
-  constexpr int B = 8;
-  for (int i0 = c - 1; i0 <= last; i0 += B) {
-    float mi[B], li[B], o[B][C];
+  for (int i0 = c - 1; i0 < n_cta && cut(i0) < d.nt; i0 += 32) {
+    const int a = cut(i0 + lane), b = cut(i0 + lane + 1);
+    uint32_t has = __ballot_sync(0xffffffffu, i0 + lane < n_cta && a < b);
+    while (has) {
+      constexpr int B = 4;
+      float2 ml[B];
+      float o[B][C];
 #pragma unroll
-    for (int u = 0; u < B; ++u) {
-      const int i = i0 + u;
-      mi[u] = -INFINITY;
-      li[u] = 0.f;
+      for (int u = 0; u < B; ++u) {
+        ml[u] = make_float2(-INFINITY, 0.f);
 #pragma unroll
-      for (int e = 0; e < C; ++e) o[u][e] = 0.f;
-      if (i <= last && cut(i) < cut(i + 1)) {
-        const float* s = part(i);
-        const float2 ml = *reinterpret_cast<const float2*>(s + D);
-        mi[u] = ml.x;
-        li[u] = ml.y;
-        if constexpr (C == 4) {
-          const float4 y = *reinterpret_cast<const float4*>(s + lane * 4);
-          o[u][0] = y.x;
-          o[u][1] = y.y;
-          o[u][2] = y.z;
-          o[u][3] = y.w;
-        } else {
-          const float2 y = *reinterpret_cast<const float2*>(s + lane * 2);
-          o[u][0] = y.x;
-          o[u][1] = y.y;
+        for (int e = 0; e < C; ++e) o[u][e] = 0.f;
+        if (has) {
+          const int i = i0 + __ffs(has) - 1;
+          has &= has - 1;
+          // CTA c - 1 may have begun before the segment's set-up units: then
+          // this is its second part
+          const int sl = i == c - 1 && before < d.start - (RG <= 64 ? kSetup<64> : kSetup<128>) ? 1 : 0;
+          const float* s = p.part + ((int64_t)i * 2 + sl) * part_floats<D>(RG);
+          ml[u] = *reinterpret_cast<const float2*>(s + RG * D + 2 * row);
+          s += row * D;
+          if constexpr (C == 4) {
+            const float4 y = *reinterpret_cast<const float4*>(s + lane * 4);
+            o[u][0] = y.x;
+            o[u][1] = y.y;
+            o[u][2] = y.z;
+            o[u][3] = y.w;
+          } else {
+            const float2 y = *reinterpret_cast<const float2*>(s + lane * 2);
+            o[u][0] = y.x;
+            o[u][1] = y.y;
+          }
         }
       }
+      float Mn = M;
+#pragma unroll
+      for (int u = 0; u < B; ++u) Mn = fmaxf(Mn, ml[u].x);
+      // a part that saw only NaN has m = -inf and l = NaN: weight 1 keeps it
+      const float a0 = (M == -INFINITY) ? (L == L ? 0.f : 1.f) : ex2(M - Mn);
+      L *= a0;
+#pragma unroll
+      for (int e = 0; e < C; ++e) acc[e] *= a0;
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        const float w = (ml[u].x == -INFINITY) ? (ml[u].y == ml[u].y ? 0.f : 1.f)
+                                               : ex2(ml[u].x - Mn);
+        L = fmaf(ml[u].y, w, L);
+#pragma unroll
+        for (int e = 0; e < C; ++e) acc[e] = fmaf(o[u][e], w, acc[e]);
+      }
+      M = Mn;
     }
-    float Mn = M;
-#pragma unroll
-    for (int u = 0; u < B; ++u) Mn = fmaxf(Mn, mi[u]);
-    const float a = (M == -INFINITY) ? (L == L ? 0.f : 1.f) : ex2(M - Mn);
-    L *= a;
-#pragma unroll
-    for (int e = 0; e < C; ++e) acc[e] *= a;
-#pragma unroll
-    for (int u = 0; u < B; ++u) {
-      const float w = (mi[u] == -INFINITY) ? (li[u] == li[u] ? 0.f : 1.f) : ex2(mi[u] - Mn);
-      L = fmaf(li[u], w, L);
-#pragma unroll
-      for (int e = 0; e < C; ++e) acc[e] = fmaf(o[u][e], w, acc[e]);
-    }
-    M = Mn;
   }
   const int rq = d.row0 + row, node = rq / p.G, hq = d.hk * p.G + rq - node * p.G;
   const int64_t t = d.cu0 + node;
@@ -1571,7 +1637,7 @@ static int64_t desc_bytes(int n_cta) { return ((int64_t)n_cta * sizeof(Desc) + 2
 
 static int64_t ws_bytes(const halo_page_pool_t* pool, const halo_tree_problem_t* pb) {
   const int n = device_sms();
-  return desc_bytes(n) + (int64_t)n * 2 * group_rows(pool, pb) * (pool->D + 4) * sizeof(float);
+  return desc_bytes(n) + (int64_t)n * 2 * group_rows(pool, pb) * (pool->D + 2) * sizeof(float);
 }
 
 template <typename T, int D, int RG>
