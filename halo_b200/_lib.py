@@ -300,6 +300,13 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def stream_handle_of(index: int) -> int:
+    """The raw handle of the current CUDA stream of device ``index``."""
+    if _raw_current_stream is not None:
+        return _raw_current_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
+
+
 def on_device(device: torch.device):
     """``torch.cuda.device(device)``, or a no-op context when ``device`` is
     already the current device (entering the torch context costs ~2 us of

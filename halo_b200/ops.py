@@ -515,34 +515,60 @@ def lse_merge(m_parts: torch.Tensor, l_parts: Optional[torch.Tensor], o_parts: t
 
 
 # ------------------------------------------------------------ paged cache
+# These calls are a few microseconds of device time, so their host path is
+# kept short: one test of everything that has to hold, and the reasons looked
+# up only where it fails.
 
-def _require_int32(t: torch.Tensor, name: str, shape: tuple, device: torch.device) -> None:
-    if t.dtype != torch.int32 or t.device != device:
-        raise L.HaloError(f"{name} must be int32 on {device}", L.HALO_ERR_INVALID_ARG)
-    if t.shape != shape or (shape[-1] > 1 and t.stride(-1) != 1):
-        raise L.HaloError(f"{name} must be {shape} with a contiguous last dim, got "
-                          f"{tuple(t.shape)}", L.HALO_ERR_INVALID_ARG)
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _require_table(t: torch.Tensor, device: torch.device) -> None:
-    if t.dim() != 2 or t.dtype != torch.int32 or t.device != device or \
+def _call(fn, index: int, *args) -> int:
+    """``fn(*args, stream)`` on device ``index`` and its current stream."""
+    if _get_device() == index:
+        return fn(*args, L.stream_handle_of(index))
+    with torch.cuda.device(index):
+        return fn(*args, L.stream_handle_of(index))
+
+
+def _refuse(what: str) -> None:
+    raise L.HaloError(what, L.HALO_ERR_INVALID_ARG)
+
+
+def _int32s(index: int, tensors: dict) -> None:
+    """Raise for the first of ``{name: (tensor, entries)}`` that is not
+    contiguous int32 of that many entries on device ``index``."""
+    for name, (t, n) in tensors.items():
+        if not t.is_cuda:
+            _refuse(f"{name} must be a CUDA tensor (no CPU path)")
+        if t.get_device() != index or t.dtype != torch.int32:
+            _refuse(f"{name} must be int32 on device {index}, got {t.dtype} on {t.device}")
+        if t.numel() != n or not t.is_contiguous():
+            _refuse(f"{name} must hold {n} contiguous entries, got shape {tuple(t.shape)}, "
+                    f"strides {t.stride()}")
+
+
+def _require_table(t: torch.Tensor, index: int) -> None:
+    if t.dim() != 2 or t.dtype != torch.int32 or t.get_device() != index or \
             (t.shape[1] > 1 and t.stride(1) != 1):
-        raise L.HaloError(f"block_tables must be int32 (R, max_blocks) on {device} with contiguous "
-                          "rows", L.HALO_ERR_INVALID_ARG)
+        _refuse(f"block_tables must be int32 (R, max_blocks) with contiguous rows on device {index}")
 
 
 def _page_pool(k: torch.Tensor, v: torch.Tensor) -> L.PagePool:
     """The C-ABI description of page pools ``(n_pages, H_kv, page_size, D)``."""
-    _require_cuda(k, "k_pages")
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
-        raise L.HaloError("k_pages and v_pages must be (n_pages, H_kv, page_size, D) of one shape, "
-                          "dtype and device", L.HALO_ERR_INVALID_ARG)
-    n, H_kv, page, D = k.shape
-    ks, vs = k.stride(), v.stride()
-    if D > 1 and (ks[3] != 1 or vs[3] != 1):
-        raise L.HaloError("page rows must be contiguous", L.HALO_ERR_INVALID_ARG)
-    return L.PagePool(k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], n, H_kv,
-                      page, D, L.halo_dtype(k.dtype))
+    if not k.is_cuda:
+        _refuse("k_pages must be a CUDA tensor (no CPU path)")
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape or v.dtype is not k.dtype or \
+            v.get_device() != k.get_device():
+        _refuse("k_pages and v_pages must be (n_pages, H_kv, page_size, D) of one shape, dtype and "
+                "device")
+    n, H_kv, page, D = shape
+    ks, kh, kt, kd = k.stride()
+    vs, vh, vt, vd = v.stride()
+    if D > 1 and (kd != 1 or vd != 1):
+        _refuse("page rows must be contiguous")
+    return L.PagePool(k.data_ptr(), v.data_ptr(), ks, kh, kt, vs, vh, vt, n, H_kv, page, D,
+                      L.halo_dtype(k.dtype))
 
 
 def update_block_tables(block_tables: torch.Tensor, old_lens: torch.Tensor, new_lens: torch.Tensor,
@@ -563,31 +589,38 @@ def update_block_tables(block_tables: torch.Tensor, old_lens: torch.Tensor, new_
     all requests packed in request order, their running count ``(R + 1,)``,
     and the lengths the requests now have -- ``old_lens`` for one that the
     free list or its table row cannot hold, which stays as it is."""
-    dev = block_tables.device
-    _require_cuda(block_tables, "block_tables")
-    _require_table(block_tables, dev)
+    if not block_tables.is_cuda:
+        _refuse("block_tables must be a CUDA tensor (no CPU path)")
+    i32, dev = torch.int32, block_tables.device
+    index = dev.index
+    _require_table(block_tables, index)
     R, max_blocks = block_tables.shape
-    _require_int32(old_lens, "old_lens", (R,), dev)
-    _require_int32(new_lens, "new_lens", (R,), dev)
-    _require_int32(free_pages, "free_pages", (free_pages.numel(),), dev)
-    _require_int32(n_free, "n_free", (1,), dev)
     if n_free_out is None:
         n_free_out = n_free
-    else:
-        _require_int32(n_free_out, "n_free_out", (1,), dev)
+    if not (old_lens.dtype is i32 and new_lens.dtype is i32 and free_pages.dtype is i32 and
+            n_free.dtype is i32 and n_free_out.dtype is i32 and
+            old_lens.get_device() == index and new_lens.get_device() == index and
+            free_pages.get_device() == index and n_free.get_device() == index and
+            n_free_out.get_device() == index and
+            old_lens.numel() == R and new_lens.numel() == R and n_free.numel() == 1 and
+            n_free_out.numel() == 1 and old_lens.is_contiguous() and new_lens.is_contiguous() and
+            free_pages.is_contiguous()):
+        _int32s(index, {"old_lens": (old_lens, R), "new_lens": (new_lens, R),
+                        "free_pages": (free_pages, free_pages.numel()), "n_free": (n_free, 1),
+                        "n_free_out": (n_free_out, 1)})
     if max_tokens < 0:
-        raise L.HaloError("max_tokens must not be negative", L.HALO_ERR_INVALID_ARG)
-    rows = torch.empty(2, max_tokens, dtype=torch.int64, device=dev)
-    ints = torch.empty(2 * R + 1, dtype=torch.int32, device=dev)
-    slots, positions = rows[0], rows[1]
-    cu, lens = ints[:R + 1], ints[R + 1:]
-    with L.on_device(dev):
-        rc = L.lib().halo_update_block_tables(
-            block_tables.data_ptr(), block_tables.stride(0), R, max_blocks, old_lens.data_ptr(),
-            new_lens.data_ptr(), free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(),
-            n_free_out.data_ptr(), int(page_size), int(max_tokens), slots.data_ptr(),
-            positions.data_ptr(), cu.data_ptr(), lens.data_ptr(), L.stream_handle(dev))
-    L.check(rc, "halo_update_block_tables")
+        _refuse("max_tokens must not be negative")
+    slots = torch.empty(max_tokens, dtype=torch.int64, device=dev)
+    positions = torch.empty(max_tokens, dtype=torch.int64, device=dev)
+    cu = torch.empty(R + 1, dtype=i32, device=dev)
+    lens = torch.empty(R, dtype=i32, device=dev)
+    rc = _call(L.lib().halo_update_block_tables, index, block_tables.data_ptr(),
+               block_tables.stride(0), R, max_blocks, old_lens.data_ptr(), new_lens.data_ptr(),
+               free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(), n_free_out.data_ptr(),
+               page_size, max_tokens, slots.data_ptr(), positions.data_ptr(), cu.data_ptr(),
+               lens.data_ptr())
+    if rc:
+        L.check(rc, "halo_update_block_tables")
     return slots, positions, cu, lens
 
 
@@ -597,22 +630,29 @@ def write_kv_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     pools ``(n_pages, H_kv, page_size, D)`` (``halo_write_kv_pages``).  Rows
     with a slot outside the pools (-1: none) are skipped; slots are distinct."""
     pool = _page_pool(k_pages, v_pages)
-    dev = k_pages.device
-    T = k.shape[0]
-    if k.shape != (T, pool.H_kv, pool.D) or v.shape != k.shape or k.dtype != k_pages.dtype or \
-            v.dtype != k.dtype or k.device != dev or v.device != dev:
-        raise L.HaloError("k and v must be (T, H_kv, D) of the pools' dtype and device",
-                          L.HALO_ERR_INVALID_ARG)
-    if slots.dtype != torch.int64 or slots.device != dev or slots.shape != (T,) or \
+    index, shape = k_pages.get_device(), k.shape
+    if len(shape) != 3 or shape[1] != pool.H_kv or shape[2] != pool.D or v.shape != shape or \
+            k.dtype is not k_pages.dtype or v.dtype is not k.dtype or \
+            k.get_device() != index or v.get_device() != index:
+        _refuse("k and v must be (T, H_kv, D) of the pools' dtype and device")
+    T = shape[0]
+    if slots.dtype is not torch.int64 or slots.get_device() != index or slots.numel() != T or \
             not slots.is_contiguous():
-        raise L.HaloError("slots must be contiguous int64 (T,) on the pools' device",
-                          L.HALO_ERR_INVALID_ARG)
-    k, v = _last_contig(k), _last_contig(v)
-    with L.on_device(dev):
-        rc = L.lib().halo_write_kv_pages(ctypes.byref(pool), k.data_ptr(), k.stride(0), k.stride(1),
-                                         v.data_ptr(), v.stride(0), v.stride(1), T,
-                                         slots.data_ptr(), L.stream_handle(dev))
-    L.check(rc, "halo_write_kv_pages")
+        _refuse("slots must be contiguous int64 (T,) on the pools' device")
+    kt, kh, kd = k.stride()
+    vt, vh, vd = v.stride()
+    if shape[2] > 1 and (kd != 1 or vd != 1):
+        k, v = k.contiguous(), v.contiguous()
+        kt, kh, _ = k.stride()
+        vt, vh, _ = v.stride()
+    rc = _call(L.lib().halo_write_kv_pages, index, ctypes.byref(pool), k.data_ptr(), kt, kh,
+               v.data_ptr(), vt, vh, T, slots.data_ptr())
+    if rc:
+        L.check(rc, "halo_write_kv_pages")
+
+
+# workspace bytes of halo_tree_attention by what they depend on
+_TREE_BYTES: dict = {}
 
 
 def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -635,53 +675,70 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     ``want_lse=False`` and none given.  Rows from ``cu_nodes[R]`` on are not
     written.  bf16/fp16, head dim 64 or 128, a page size that is a multiple
     of 8."""
-    _require_cuda(q, "q")
+    if not q.is_cuda:
+        _refuse("q must be a CUDA tensor (no CPU path)")
     dev = q.device
+    index = dev.index
     pool = _page_pool(k_pages, v_pages)
-    if q.dim() != 3 or q.dtype != k_pages.dtype or k_pages.device != dev or q.shape[2] != pool.D:
-        raise L.HaloError("q must be (T, H, D) of the pools' dtype, device and head dim",
-                          L.HALO_ERR_INVALID_ARG)
-    T, H, D = q.shape
-    _require_table(block_tables, dev)
+    dtype, qshape = q.dtype, q.shape
+    if len(qshape) != 3 or dtype is not k_pages.dtype or k_pages.get_device() != index or \
+            qshape[2] != pool.D:
+        _refuse("q must be (T, H, D) of the pools' dtype, device and head dim")
+    T, H, D = qshape
+    _require_table(block_tables, index)
     R, max_blocks = block_tables.shape
-    _require_int32(context_lens, "context_lens", (R,), dev)
-    _require_int32(cu_nodes, "cu_nodes", (R + 1,), dev)
-    if tree_mask.dim() != 2 or tree_mask.shape[0] != T or tree_mask.device != dev or \
-            tree_mask.dtype not in (torch.bool, torch.uint8) or \
-            (tree_mask.shape[1] > 1 and tree_mask.stride(1) != 1):
-        raise L.HaloError("tree_mask must be bool (T, max_nodes) with contiguous rows on q's device",
-                          L.HALO_ERR_INVALID_ARG)
-    q = _last_contig(q)
+    if not (context_lens.dtype is torch.int32 and cu_nodes.dtype is torch.int32 and
+            context_lens.get_device() == index and cu_nodes.get_device() == index and
+            context_lens.numel() == R and cu_nodes.numel() == R + 1 and
+            context_lens.is_contiguous() and cu_nodes.is_contiguous()):
+        _int32s(index, {"context_lens": (context_lens, R), "cu_nodes": (cu_nodes, R + 1)})
+    mshape, mstride = tree_mask.shape, tree_mask.stride()
+    if len(mshape) != 2 or mshape[0] != T or tree_mask.get_device() != index or \
+            tree_mask.dtype not in (torch.bool, torch.uint8) or (mshape[1] > 1 and mstride[1] != 1):
+        _refuse("tree_mask must be bool (T, max_nodes) with contiguous rows on q's device")
+    qt, qh, qd = q.stride()
+    if qd != 1 and D > 1:
+        q = q.contiguous()
+        qt, qh, _ = q.stride()
     if out is None:
-        out = torch.empty(T, H, D, dtype=out_dtype or q.dtype, device=dev)
-    elif out.shape != q.shape or out.device != dev or (D > 1 and out.stride(2) != 1):
-        raise L.HaloError("out must be (T, H, D) with contiguous rows on q's device",
-                          L.HALO_ERR_INVALID_ARG)
+        out = torch.empty(qshape, dtype=out_dtype or dtype, device=dev)
+        ot, oh = H * D, D
+    else:
+        ot, oh, od = out.stride()
+        if out.shape != qshape or out.get_device() != index or (D > 1 and od != 1):
+            _refuse("out must be (T, H, D) with contiguous rows on q's device")
     if lse is None:
         if want_lse:
             lse = torch.empty(T, H, dtype=torch.float32, device=dev)
-    elif lse.shape != (T, H) or lse.dtype != torch.float32 or lse.device != dev or \
+    elif lse.shape != (T, H) or lse.dtype is not torch.float32 or lse.get_device() != index or \
             not lse.is_contiguous():
-        raise L.HaloError("lse must be contiguous fp32 (T, H) on q's device",
-                          L.HALO_ERR_INVALID_ARG)
-    prob = L.TreeProblem(R, T, H, tree_mask.shape[1], max_blocks,
-                         float(scale) if scale is not None else 1.0 / math.sqrt(D), q.data_ptr(),
-                         q.stride(0), q.stride(1), block_tables.data_ptr(), block_tables.stride(0),
-                         context_lens.data_ptr(), cu_nodes.data_ptr(), tree_mask.data_ptr(),
-                         tree_mask.stride(0), out.data_ptr(), out.stride(0), out.stride(1),
-                         L.halo_dtype(out.dtype), lse.data_ptr() if lse is not None else None)
+        _refuse("lse must be contiguous fp32 (T, H) on q's device")
+    prob = L.TreeProblem(R, T, H, mshape[1], max_blocks,
+                         scale if scale is not None else 1.0 / math.sqrt(D), q.data_ptr(), qt, qh,
+                         block_tables.data_ptr(), block_tables.stride(0), context_lens.data_ptr(),
+                         cu_nodes.data_ptr(), tree_mask.data_ptr(), mstride[0], out.data_ptr(), ot,
+                         oh, L.halo_dtype(out.dtype), lse.data_ptr() if lse is not None else None)
+    return _tree_launch(pool, prob, index, dev, out, lse)
+
+
+def _tree_launch(pool, prob, index, dev, out, lse):
     lib = L.lib()
-    with L.on_device(dev):
-        need = lib.halo_tree_workspace_bytes(ctypes.byref(pool), ctypes.byref(prob))
+    a, b = ctypes.byref(pool), ctypes.byref(prob)
+    key = (index, pool.D, pool.H_kv, prob.H, prob.max_nodes)
+    need = _TREE_BYTES.get(key) if prob.R and prob.T else None
+    if need is None:
+        with torch.cuda.device(index):
+            need = int(lib.halo_tree_workspace_bytes(a, b))
         if need < 0:
-            L.check(int(need), "halo_tree_workspace_bytes")
-        # a workspace of the call's own: stream-ordered by the allocator, and
-        # graphs captured on one stream never share it
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        rc = lib.halo_tree_attention(ctypes.byref(pool), ctypes.byref(prob),
-                                     ws.data_ptr() if ws is not None else None, need,
-                                     L.stream_handle(dev))
-    L.check(rc, "halo_tree_attention")
+            L.check(need, "halo_tree_workspace_bytes")
+        if prob.R and prob.T:
+            _TREE_BYTES[key] = need
+    # a workspace of the call's own: ordered by the allocator's stream, and
+    # graphs captured on one stream never share it
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    rc = _call(lib.halo_tree_attention, index, a, b, ws.data_ptr() if need else None, need)
+    if rc:
+        L.check(rc, "halo_tree_attention")
     return out, lse
 
 
@@ -695,19 +752,20 @@ def commit_tree_path(k_pages: torch.Tensor, v_pages: torch.Tensor, block_tables:
     ``path[r, i] >= i``, as paths from a root do when children are numbered
     after their parents; other steps move nothing."""
     pool = _page_pool(k_pages, v_pages)
-    dev = k_pages.device
-    _require_table(block_tables, dev)
+    index = k_pages.get_device()
+    _require_table(block_tables, index)
     R, max_blocks = block_tables.shape
-    if path.dim() != 2:
-        raise L.HaloError("path must be int32 (R, max_depth)", L.HALO_ERR_INVALID_ARG)
-    depth = path.shape[1]
-    _require_int32(path, "path", (R, depth), dev)
-    _require_int32(context_lens, "context_lens", (R,), dev)
-    _require_int32(path_lens, "path_lens", (R,), dev)
-    with L.on_device(dev):
-        rc = L.lib().halo_commit_tree_path(ctypes.byref(pool), block_tables.data_ptr(),
-                                           block_tables.stride(0), max_blocks, R,
-                                           context_lens.data_ptr(), path.data_ptr(),
-                                           path.stride(0), depth, path_lens.data_ptr(),
-                                           L.stream_handle(dev))
-    L.check(rc, "halo_commit_tree_path")
+    pshape, pstride = path.shape, path.stride()
+    if len(pshape) != 2 or pshape[0] != R or path.dtype is not torch.int32 or \
+            path.get_device() != index or (pshape[1] > 1 and pstride[1] != 1):
+        _refuse("path must be int32 (R, max_depth) with contiguous rows on the pools' device")
+    if not (context_lens.dtype is torch.int32 and path_lens.dtype is torch.int32 and
+            context_lens.get_device() == index and path_lens.get_device() == index and
+            context_lens.numel() == R and path_lens.numel() == R and
+            context_lens.is_contiguous() and path_lens.is_contiguous()):
+        _int32s(index, {"context_lens": (context_lens, R), "path_lens": (path_lens, R)})
+    rc = _call(L.lib().halo_commit_tree_path, index, ctypes.byref(pool), block_tables.data_ptr(),
+               block_tables.stride(0), max_blocks, R, context_lens.data_ptr(), path.data_ptr(),
+               pstride[0], pshape[1], path_lens.data_ptr())
+    if rc:
+        L.check(rc, "halo_commit_tree_path")

@@ -524,3 +524,59 @@ def test_tree_decoding_loop(cuda_device):
     assert cache.held.tolist()[1] == n[1]
     cache.accept(None, _i32([0, 0, 0]))
     assert cache.lens.tolist() == n
+
+
+# ------------------------------------------------------------ refusals
+
+def test_wrappers_refuse_what_does_not_fit(cuda_device):
+    from halo_b200 import ops
+    from halo_b200._lib import HaloError
+    c = Case(70, [20], [3], 4, 2, 64, 8, torch.bfloat16)
+    good = dict(q=c.q.to(DEV), k_pages=c.k.to(DEV), v_pages=c.v.to(DEV),
+                block_tables=_i32(c.table), context_lens=_i32(c.ctx), cu_nodes=_i32(c.cu),
+                tree_mask=c.mask.to(DEV))
+    ops.tree_attention(**good)
+    T = c.cu[-1]
+    for bad in ({"q": good["q"].half()}, {"q": good["q"][:, :, :32]}, {"q": good["q"][0]},
+                {"q": good["q"].cpu()}, {"k_pages": good["k_pages"][:1]},
+                {"v_pages": good["v_pages"].half()}, {"k_pages": good["k_pages"].cpu()},
+                {"block_tables": good["block_tables"].long()},
+                {"block_tables": good["block_tables"][0]},
+                {"block_tables": good["block_tables"].cpu()},
+                {"context_lens": good["context_lens"].long()}, {"context_lens": _i32([1, 2])},
+                {"cu_nodes": good["cu_nodes"][:1]}, {"cu_nodes": good["cu_nodes"].cpu()},
+                {"tree_mask": good["tree_mask"].float()}, {"tree_mask": good["tree_mask"][:2]},
+                {"tree_mask": good["tree_mask"].T.contiguous().T},
+                {"out": torch.empty(T, 4, 32, device=DEV, dtype=torch.bfloat16)},
+                {"out": torch.empty(T, 4, 64, device=DEV, dtype=torch.float64)},
+                {"out": torch.empty(T, 4, 64, dtype=torch.bfloat16)},
+                {"lse": torch.empty(T, 4, device=DEV, dtype=torch.float64)},
+                {"lse": torch.empty(4, T, device=DEV).T}, {"scale": 0.0}):
+        with pytest.raises(HaloError):
+            ops.tree_attention(**{**good, **bad})
+    t, o, f, n = _i32([[0, 0]]), _i32([0]), _i32([1, 2, 3]), _i32([3])
+    ops.update_block_tables(t, o, o, f, n, page_size=4, max_tokens=2)
+    for args, kw in (((t.long(), o, o, f, n), {}), ((t, o.long(), o, f, n), {}),
+                     ((t, o, _i32([1, 2]), f, n), {}), ((t, o, o, f.cpu(), n), {}),
+                     ((t, o, o, f[::2], n), {}), ((t, o, o, f, f), {}),
+                     ((t.T, o, o, f, n), {}), ((t, o, o, f, n), {"page_size": 0}),
+                     ((t, o, o, f, n), {"max_tokens": -1}),
+                     ((t, o, o, f, n), {"n_free_out": n.cpu()})):
+        with pytest.raises(HaloError):
+            ops.update_block_tables(*args, **{"page_size": 4, "max_tokens": 2, **kw})
+    k = torch.zeros(2, 2, 64, dtype=torch.bfloat16, device=DEV)
+    s = torch.zeros(2, dtype=torch.int64, device=DEV) - 1
+    kp, vp = good["k_pages"], good["v_pages"]
+    ops.write_kv_pages(k, k, kp, vp, s)
+    for args in ((k.half(), k, kp, vp, s), (k[:1], k, kp, vp, s), (k, k, kp, vp, s.int()),
+                 (k, k, kp, vp, s[:1]), (k.cpu(), k, kp, vp, s), (k[:, :1], k[:, :1], kp, vp, s),
+                 (k, k, kp.transpose(2, 3), vp.transpose(2, 3), s)):
+        with pytest.raises(HaloError):
+            ops.write_kv_pages(*args)
+    tb, x = good["block_tables"], _i32([[0, 1]])
+    ops.commit_tree_path(kp, vp, tb, _i32([20]), x, _i32([2]))
+    for args in ((tb, _i32([20]), x.long(), _i32([2])), (tb, _i32([20]), x[0], _i32([2])),
+                 (tb, _i32([20, 1]), x, _i32([2])), (tb, _i32([20]), x, _i32([2]).cpu()),
+                 (tb.long(), _i32([20]), x, _i32([2])), (tb, _i32([20]), _i32([[1], [2]]), _i32([2]))):
+        with pytest.raises(HaloError):
+            ops.commit_tree_path(kp, vp, *args)
