@@ -34,14 +34,18 @@ namespace paged {
 // found from two prefix sums and nothing is popped one at a time.
 //
 // Every CTA forms the prefix sums of all requests for itself (two passes of
-// shuffles over shared memory; R is at most 8192) and takes a share of the
-// tokens, new table entries and pages given back: no CTA waits for what
-// another computed.  The one hazard is n_free, which n_free_out may alias:
-// it is written behind a cluster barrier that every CTA reaches after
-// reading it.  Latency-bound: a few integers a request and 16 B a token.
+// shuffles over shared memory; R is at most 8192) and takes a share of the new
+// table entries, of the pages given back and, behind a cluster barrier, of the
+// tokens, whose pages are then all in the tables.  n_free_out may alias n_free:
+// it is written behind the same barrier.  A warp takes 32 consecutive pages or
+// tokens: one search for all of them.  Latency-bound: a few integers a request
+// and 16 B a token.  8 requests: 5.6 us on the device; 1024 requests with 42000
+// new tokens: 15.4 us (22.5 us with a binary search a thread; 1.8 us each for
+// the two passes over the requests, 1.7 us for the new entries, 4 us for the
+// pages given back, 5 us for the tokens).
 constexpr int kTabThreads = 1024;
 constexpr int kTabMaxReq = 8192;
-constexpr int kTabArrays = 5;      // shared int arrays of R entries
+constexpr int kTabArrays = 7;      // shared int arrays of R entries
 
 struct TablesParams {
   int32_t* table;
@@ -56,6 +60,7 @@ struct TablesParams {
   int32_t* cu;
   int32_t* lens;
   int32_t R, max_blocks, page, cap, T;
+  uint32_t page_magic;                   // ceil(2^32 / page)
 };
 
 // Inclusive block scan of one 64-bit value a thread; *total gets the sum.
@@ -80,17 +85,23 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* s_warp, int64_
   return v + (warp > 0 ? before : 0);
 }
 
-// First i in [0, n) with a[i] > x (a ascending), or n.
-__device__ __forceinline__ int upper_bound(const int32_t* a, int n, int x) {
+// Pages of n rows (any value for a negative n, which is refused).
+__device__ __forceinline__ int blocks(int n, int page) {
+  const uint32_t b = (uint32_t)n / (uint32_t)page;
+  return (int)(b + ((uint32_t)n - b * (uint32_t)page != 0 ? 1u : 0u));
+}
+
+// First i in [0, n) with a[i] > k (running sums, k < a[n - 1]) for the warp's
+// smallest k, found by all lanes together: 32 probes a step.
+__device__ __forceinline__ int warp_find(const int32_t* a, int n, int k) {
+  const int lane = threadIdx.x & 31;
   int lo = 0;
-  while (n > 0) {
-    const int h = n >> 1;
-    if (a[lo + h] > x) {
-      n = h;
-    } else {
-      lo += h + 1;
-      n -= h + 1;
-    }
+  while (n > 1) {
+    const int step = n <= 32 ? 1 : (n + 31) >> 5 | 1;   // odd: 32 banks
+    const int at = min((lane + 1) * step, n) - 1;
+    const int f = __ffs(__ballot_sync(0xffffffffu, a[lo + at] > k)) - 1;
+    lo += f * step;
+    n = min(step, n - f * step);
   }
   return lo;
 }
@@ -104,6 +115,8 @@ __global__ void __launch_bounds__(kTabThreads) tables_kernel(const TablesParams 
   int32_t* s_tok = sm + 2 * p.R;
   int32_t* s_old = sm + 3 * p.R;
   int32_t* s_new = sm + 4 * p.R;
+  int32_t* s_ob = sm + 5 * p.R;          // pages held before, and asked for
+  int32_t* s_nb = sm + 6 * p.R;
   namespace cg = cooperative_groups;
   cg::cluster_group cl = cg::this_cluster();
   const int n_cta = (int)cl.num_blocks(), rank = (int)cl.block_rank();
@@ -117,14 +130,16 @@ __global__ void __launch_bounds__(kTabThreads) tables_kernel(const TablesParams 
     const int r = base + threadIdx.x;
     int64_t v = 0;
     if (r < p.R) {
-      const int64_t o = p.old_lens[r], n = p.new_lens[r];
-      const int64_t ob = (o + p.page - 1) / p.page, nb = (n + p.page - 1) / p.page;
+      const int o = p.old_lens[r], n = p.new_lens[r];
+      const int ob = blocks(o, p.page), nb = blocks(n, p.page);
       // a length that is negative or that the table cannot hold is refused:
       // the request stays as it is (new = old)
       const bool ok = o >= 0 && n >= 0 && ob <= p.max_blocks && nb <= p.max_blocks;
-      if (ok) v = nb > ob ? nb - ob : (ob - nb) << 32;
-      s_old[r] = (int32_t)o;
-      s_new[r] = (int32_t)(ok ? n : o);
+      if (ok) v = nb > ob ? nb - ob : (int64_t)(ob - nb) << 32;
+      s_old[r] = o;
+      s_ob[r] = ob;
+      s_nb[r] = nb;
+      s_new[r] = ok ? n : o;
     }
     const int64_t s = carry + block_scan(v, s_warp, &total);
     carry += total;
@@ -165,44 +180,75 @@ __global__ void __launch_bounds__(kTabThreads) tables_kernel(const TablesParams 
   __syncthreads();
   used = s_used;
   if (rank == 0 && threadIdx.x == 0) p.cu[0] = 0;
-  // entry k of the stack: the free list, then the pages given back
-  auto stack = [&](int k) -> int32_t {
-    if (k < n_free) return p.free_pages[k];
-    const int g = k - n_free;
-    const int r = upper_bound(s_give, p.R, g);
-    const int b = (s_new[r] + p.page - 1) / p.page + (g - (r > 0 ? s_give[r - 1] : 0));
-    return p.table[(int64_t)r * p.table_stride + b];
-  };
   const int n_tok = (int)min(carry, (int64_t)p.T);
   const int i0 = rank * kTabThreads + threadIdx.x, di = n_cta * kTabThreads;
+  const int lane = threadIdx.x & 31;
+  // Entry k of the stack: the free list, then the pages given back.  `low` is
+  // the smallest k of the warp's lanes that ask (all lanes come here).
+  auto stack = [&](int k, int low, bool ask) -> int32_t {
+    int r = 0;
+    if (__any_sync(0xffffffffu, ask && k >= n_free))
+      r = warp_find(s_give, p.R, max(low - n_free, 0));
+    if (!ask) return 0;
+    if (k < n_free) return p.free_pages[k];
+    const int g = k - n_free;
+    while (g >= s_give[r]) ++r;
+    return p.table[(int64_t)r * p.table_stride + s_nb[r] + (g - (r > 0 ? s_give[r - 1] : 0))];
+  };
 
-  // the slots of the new tokens (a row without a token gets -1)
-  for (int t = i0; t < p.T; t += di) {
-    int64_t slot = -1, pos = -1;
-    if (t < n_tok) {
-      const int r = upper_bound(s_tok, p.R, t);
-      const int o = s_old[r];
-      const int at = o + (t - (r > 0 ? s_tok[r - 1] : 0));
-      const int ob = (o + p.page - 1) / p.page, b = at / p.page;
-      const int32_t pg = b < ob ? p.table[(int64_t)r * p.table_stride + b]
-                                : stack(have - 1 - ((r > 0 ? s_need[r - 1] : 0) + b - ob));
-      slot = (int64_t)pg * p.page + (at - b * p.page);
-      pos = at;
-    }
-    p.slots[t] = slot;
-    p.positions[t] = pos;
-  }
   // the new entries of the block tables
-  for (int k = i0; k < used; k += di) {
-    const int r = upper_bound(s_need, p.R, k);
-    const int b = (s_old[r] + p.page - 1) / p.page + (k - (r > 0 ? s_need[r - 1] : 0));
-    p.table[(int64_t)r * p.table_stride + b] = stack(have - 1 - k);
+  for (int k0 = i0 - lane; k0 < used; k0 += di) {
+    const int k = k0 + lane, last = min(k0 + 31, used - 1);
+    const int32_t pg = stack(have - 1 - k, have - 1 - last, k < used);
+    int r = warp_find(s_need, p.R, k0);
+    if (k < used) {
+      while (k >= s_need[r]) ++r;
+      p.table[(int64_t)r * p.table_stride + s_ob[r] + (k - (r > 0 ? s_need[r - 1] : 0))] = pg;
+    }
   }
   // pages given back that nobody took join the free list
-  for (int k = n_free + i0; k < have - used; k += di) p.free_pages[k] = stack(k);
+  const int left = have - used;
+  for (int k0 = n_free + i0 - lane; k0 < left; k0 += di) {
+    const int k = k0 + lane;
+    const int32_t pg = stack(k, k0, k < left);
+    if (k < left) p.free_pages[k] = pg;
+  }
 
-  cl.sync();                             // every CTA has read n_free
-  if (rank == 0 && threadIdx.x == 0) *p.n_free_out = have - used;
+  cl.sync();                             // all table entries are written, n_free was read
+  if (rank == 0 && threadIdx.x == 0) *p.n_free_out = left;
+
+  // the slots of the new tokens (a row without a token gets -1), two of them
+  // kTabThreads apart in flight
+  for (int64_t t0 = i0 - lane; t0 < p.T; t0 += 2 * (int64_t)di) {
+    int64_t slot[2];
+    int pos[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int64_t te = t0 + (int64_t)e * di;
+      slot[e] = pos[e] = -1;
+      if (te < n_tok) {                    // uniform in the warp
+        int r = warp_find(s_tok, p.R, (int)te);
+        const int t = (int)te + lane;
+        if (t < n_tok) {
+          while (t >= s_tok[r]) ++r;
+          pos[e] = s_old[r] + (t - (r > 0 ? s_tok[r - 1] : 0));
+          int b = (int)__umulhi((uint32_t)pos[e], p.page_magic);   // exact or one more
+          if (p.page == 1) b = pos[e];
+          b -= (uint32_t)b * (uint32_t)p.page > (uint32_t)pos[e] ? 1 : 0;
+          slot[e] = (int64_t)p.table[(int64_t)r * p.table_stride + b] * p.page +
+                    (pos[e] - b * p.page);
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int64_t t = t0 + (int64_t)e * di + lane;
+      if (t < p.T) {
+        p.slots[t] = slot[e];
+        p.positions[t] = pos[e];
+      }
+    }
+  }
 }
 
 // ======================================================================
@@ -408,6 +454,7 @@ extern "C" int32_t halo_update_block_tables(int32_t* block_tables, int64_t table
   if (R < 0 || max_blocks < 0 || free_capacity < 0 || max_tokens < 0 || page_size <= 0)
     return fail(HALO_ERR_INVALID_ARG, "bad size (R=%d max_blocks=%d free=%d max_tokens=%d page_size=%d)",
                 R, max_blocks, free_capacity, max_tokens, page_size);
+  if (max_tokens > (1 << 30)) return fail(HALO_ERR_UNSUPPORTED, "%d tokens", max_tokens);
   if (R > kTabMaxReq) return fail(HALO_ERR_UNSUPPORTED, "%d requests (at most %d)", R, kTabMaxReq);
   if ((int64_t)R * max_blocks > INT_MAX || ((int64_t)max_blocks + 1) * page_size > INT_MAX)
     return fail(HALO_ERR_UNSUPPORTED, "block tables of %d x %d pages of %d are too large", R,
@@ -431,7 +478,8 @@ extern "C" int32_t halo_update_block_tables(int32_t* block_tables, int64_t table
   if (e != cudaSuccess) return cuda_fail(e, "tables_kernel shared-memory attribute");
   const TablesParams p{block_tables, table_stride, old_lens, new_lens, free_pages, n_free,
                        n_free_out, slots, positions, cu_tokens, lens, R, max_blocks, page_size,
-                       free_capacity, max_tokens};
+                       free_capacity, max_tokens,
+                       (uint32_t)(((1ull << 32) + page_size - 1) / page_size)};
   // two tokens a thread before another CTA joins
   const int n_cta = std::min(8, std::max(1, max_tokens / (2 * kTabThreads)));
   cudaLaunchConfig_t cfg = {};
