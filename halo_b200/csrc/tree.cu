@@ -37,7 +37,7 @@ int device_sms();
 namespace tree {
 
 constexpr int kBN = 128;               // positions of a tile (a unit)
-constexpr int kThreads = 384;          // tree_kernel
+constexpr int kThreads = 640;          // tree_kernel
 constexpr int kFewThreads = 384;       // tree_few_kernel
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.f;    // headroom of the running maximum
@@ -95,7 +95,7 @@ struct Geom {
   static constexpr int kOffQ = 0;
   static constexpr int kOffK = QT * kTileBytes;
   static constexpr int kOffV = kOffK + kStK * kTileBytes;
-  static constexpr int kOffMl = kOffV + kStV * kTileBytes;   // m, l [2][128]
+  static constexpr int kOffMl = kOffV + kStV * kTileBytes;   // maxima [2][2][128]
   static constexpr int kOffBar = kOffMl + 2048;
   static constexpr int kSmemBytes = kOffBar + 1024;
   static constexpr uint32_t kColO = 256;
@@ -141,8 +141,8 @@ struct Req {
 struct Bars {
   uint64_t q_full[2], q_empty[2];
   uint64_t k_full[6], k_empty[6], v_full[6], v_ready[6], v_empty[6];
-  uint64_t s_full[2], p_full[2], pv_done[2], mma_done[2];
-  int64_t scan[12];
+  uint64_t s_full[2], p_full[4], pv_done[2], mma_done[2];
+  int64_t scan[20];
   int64_t base0, total;
   uint32_t tmem_base;
   int abort_flag, r0;
@@ -275,6 +275,61 @@ __device__ __forceinline__ void tmem_st(uint32_t a, const float (&v)[16]) {
 }
 __device__ __forceinline__ void tmem_st(uint32_t a, const float (&v)[32]) { umma::tmem_st32(a, v); }
 
+// ---- packed fp32 pairs, three-way maximum
+__device__ __forceinline__ uint64_t f2pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2unpack(uint64_t r, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t ffma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Weights of a pair of scores, e^(s - m) in log2 units: their 16-bit values
+// (hi) and remainders (lo); the fp32 pair is returned for the row sum.
+template <typename T>
+__device__ __forceinline__ uint64_t weigh(float s0, float s1, uint64_t sc2, uint64_t nm2,
+                                          uint32_t& hi, uint32_t& lo) {
+  float x0, x1, h0, h1;
+  f2unpack(ffma2(f2pack(s0, s1), sc2, nm2), x0, x1);
+  const float a = ex2(x0), b = ex2(x1);
+  if constexpr (Elem<T>::kDtype == HALO_DTYPE_BF16) {   // truncated: one byte permute a pair
+    hi = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+    h0 = __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
+    h1 = __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
+  } else {
+    hi = Elem<T>::pack(a, b);
+    Elem<T>::unpack(hi, h0, h1);
+  }
+  const uint64_t p2 = f2pack(a, b);
+  float r0, r1;
+  f2unpack(ffma2(f2pack(h0, h1), f2pack(-1.f, -1.f), p2), r0, r1);
+  lo = Elem<T>::pack(r0, r1);
+  return p2;
+}
+
+__device__ __forceinline__ void tmem_st8u(uint32_t a, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a),
+               "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+               "r"(v[7])
+               : "memory");
+}
+
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -297,6 +352,23 @@ template <typename T>
 __device__ __forceinline__ bool bad16(uint32_t x) {   // inf or NaN in the low 16 bits
   constexpr uint32_t e = Elem<T>::kDtype == HALO_DTYPE_BF16 ? 0x7F80u : 0x7C00u;
   return (x & e) == e;
+}
+
+constexpr float kNoMax = -1e30f;           // nothing seen yet: any score raises it
+
+// Barrier `id` of N softmax threads that tells whether any of them voted.
+template <int N>
+__device__ __forceinline__ bool vote_bar(int id, bool vote) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(vote ? 1u : 0u), "r"(id), "n"(N)
+      : "memory");
+  return any != 0;
 }
 
 // ---- parts of both kernels
@@ -535,7 +607,7 @@ __device__ __noinline__ float bad_sum(const Params& p, int r, int t, int ctx, in
 }
 
 // ======================================================================
-// tree_kernel: groups of more than 64 rows.  One CTA an SM, 384 threads.
+// tree_kernel: groups of more than 64 rows.  One CTA an SM, 640 threads.
 //   warp 0      TMA producer: K and V tiles of 128 positions, each made of
 //               boxes of p.box rows (the largest power of two, up to 128,
 //               that divides the page), through two rings; the lanes issue a
@@ -543,7 +615,10 @@ __device__ __noinline__ float bad_sum(const Params& p, int r, int t, int ctx, in
 //               or without a page start outside the tensor: zeros.
 //   warps 1, 3  lane 0 issues the MMAs of stream 0 / 1; warp 1 owns TMEM.
 //   warp 2      cleans V.
-//   warps 4-7   softmax stream 0, warps 8-11 stream 1 (thread = TMEM lane).
+//   warps 4-11  softmax stream 0, warps 12-19 stream 1: thread = row and half
+//               of each tile's positions.  16 warps, since the chain of a tile
+//               (QK, exponentials, PV) is longer than its parts: with 8 warps
+//               of whole rows it took 7400 clocks for 256 rows.
 // Each stream has its own scores S_X (128 TMEM columns, overwritten in place
 // by the weights P_X) and output O_X: S_X = Q K^T, O_X += P_X V, both M128.
 // One thread issues a stream's MMAs, which execute in that order: the QK that
@@ -554,8 +629,7 @@ __device__ __noinline__ float bad_sum(const Params& p, int r, int t, int ctx, in
 //
 // Row groups of more than 128 rows (QT = 2): stream X takes query tile X and
 // both take every K/V tile.  Smaller ones: both streams share the query tile
-// and take every second K/V tile; the two are joined in shared memory at the
-// end of a segment.
+// and take every second K/V tile; the two are joined at the end of a segment.
 template <typename T, int D, int QT>
 __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ Params p) {
   using Gm = Geom<D, QT>;
@@ -563,12 +637,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   constexpr bool kBf16 = Elem<T>::kDtype == HALO_DTYPE_BF16;
   extern __shared__ __align__(1024) unsigned char smem[];
   Bars* bs = reinterpret_cast<Bars*>(smem + Gm::kOffBar);
-  float* sm_m = reinterpret_cast<float*>(smem + Gm::kOffMl);
-  float* sm_l = sm_m + 256;
+  float* sm_mx = reinterpret_cast<float*>(smem + Gm::kOffMl);   // [stream][half][128]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    mbar_init(&bs->q_full[0], 8);
+    mbar_init(&bs->q_full[0], 16);
     for (int i = 0; i < 6; ++i) {
       mbar_init(&bs->k_full[i], 1);
       mbar_init(&bs->k_empty[i], 2);
@@ -578,7 +651,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&bs->s_full[x], 1);
-      mbar_init(&bs->p_full[x], 4);
+      mbar_init(&bs->p_full[2 * x], 4);
+      mbar_init(&bs->p_full[2 * x + 1], 4);
       mbar_init(&bs->pv_done[x], 1);
       mbar_init(&bs->mma_done[x], 1);
     }
@@ -613,10 +687,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   if (!aligned && threadIdx.x == 0)
     set_device_error(p.err, static_cast<unsigned int>(-HALO_ERR_MISALIGNED));
 
-  // Register split (128 x 88 + 256 x 208 = 384 x 168, the launch budget).
+  // Register split: 128 x 56 + 512 x 104 <= 640 x 96, the launch budget.
   if (u0 < u1 && aligned) {
   if (warp < 4) {
-    umma::regs_dec<88>();
+    umma::regs_dec<56>();
     Walk<RG> walk(p, bs->r0, bs->req0, bs->base0, u0, u1);
     Seg s;
     if (warp == 0) {
@@ -658,19 +732,20 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           if (ok && nx > 0) ok = qk();
           for (int it = 0; ok && it < nx; ++it, ++j) {
             const int iv = g % SV;
-            ok = wait_bar(&bs->p_full[x], j & 1, bs, p.err) &&
-                 wait_bar(&bs->v_ready[iv], (g / SV) & 1, bs, p.err);
-            if (!ok) break;
-            umma::fence_after_sync();
+            ok = wait_bar(&bs->v_ready[iv], (g / SV) & 1, bs, p.err);
             const uint64_t vd = opaque(vdesc0 + (uint64_t)((iv * Gm::kTileBytes) >> 4));
 #pragma unroll
-            for (int kk = 0; kk < kBN / 16; ++kk)   // O_X += P_X V(g)
-              umma::mma_ts(oc, pc + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), kIdPV,
-                           it > 0 || kk > 0);
+            for (int h = 0; h < 2; ++h) {           // O_X += P_X V(g), half the positions
+              ok = ok && wait_bar(&bs->p_full[2 * x + h], j & 1, bs, p.err);
+              if (!ok) break;
+              umma::fence_after_sync();
 #pragma unroll
-            for (int kk = 0; kk < kBN / 16; ++kk)
-              umma::mma_ts(oc, pc + 64 + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), kIdPV,
-                           true);
+              for (int kk = 0; kk < 8; ++kk)        // 16 positions: values, remainders
+                umma::mma_ts(oc, pc + h * 64 + (kk >> 2) * 32 + (kk & 1) * 16 + ((kk >> 1) & 1) * 8,
+                             vd + (uint64_t)(((h * 4 + (kk >> 1)) * 16 * 128) >> 4), kIdPV,
+                             it > 0 || h > 0 || kk > 0);
+            }
+            if (!ok) break;
             umma::commit(&bs->v_empty[iv]);
             if (it + 1 == nx) umma::commit(&bs->pv_done[x]);
             g += step;
@@ -687,82 +762,65 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       clean<T, D, RG, Gm>(p, bs, smem, walk);
     }
   } else {
-    umma::regs_inc<208>();
-    // ------------------------------------------------------------ softmax X
-    const int x = (warp - 4) >> 2;
-    const int sub = warp & 3;
-    const int r = sub * 32 + lane;               // TMEM lane
-    const int tid = threadIdx.x - 128;           // 0..255 over both streams
+    umma::regs_inc<104>();
+    // ------------------------------------------------------------ softmax
+    // Thread: row r of stream x's scores, positions [64 h, 64 h + 64) of each
+    // tile.  Both halves of a row keep one maximum.
+    const int x = (warp - 4) >> 3, h = ((warp - 4) >> 2) & 1;
+    const int sub = warp & 3, r = sub * 32 + lane;       // TMEM lane
+    const int tid = threadIdx.x - 128;                   // 0..511
     const uint32_t trow = tmem + ((uint32_t)(sub * 32) << 16);
-    const uint32_t scol = x * 128, ocol = Gm::kColO + x * D;
+    const uint32_t scol = trow + x * 128 + h * 64;
     Walk<RG> walk(p, bs->r0, bs->req0, bs->base0, u0, u1);
     Seg s;
-    int j = 0, si = 0, sx = 0;                   // tiles of this stream; segments; with tiles
+    int j = 0, si = 0, s1 = 0;             // this stream's tiles; segments; those of stream 1
     bool ok = true;
     while (walk.next(p, s)) {
       const bool two = QT == 2 && s.rows > 128;
       const int nodes = walk.q.nodes, ctx = walk.q.ctx, end = walk.q.end, cu0 = walk.q.cu0;
       // ---- Q: the previous segment's MMAs and scratch are done with
-      named_bar_sync(1, 256);
+      named_bar_sync(1, 512);
       {
         constexpr int VPR = D / 8;
-        const int n = (two ? 256 : 128) * VPR;
-        for (int i0 = 0; i0 < n; i0 += 256 * 4) {
-          uint4 w[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int i = i0 + u * 256 + tid;
-            const int ql = i / VPR, c = i % VPR;             // tile row, 16-byte column
-            const int row = ql;
-            w[u] = make_uint4(0, 0, 0, 0);
-            if (i < n && row < s.rows) {
-              const int rq = s.row0 + row, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
-              w[u] = *reinterpret_cast<const uint4*>(
-                  reinterpret_cast<const T*>(p.q) + (int64_t)(cu0 + node) * p.q_st + hq * p.q_sh +
-                  c * 8);
-            }
-          }
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int i = i0 + u * 256 + tid;
-            const int ql = i / VPR, c = i % VPR;
-            const int qt = ql >> 7, q = ql & 127;
-            if (i < n)
-              *reinterpret_cast<uint4*>(smem + Gm::kOffQ + qt * Gm::kTileBytes +
-                                        (c >> 3) * Gm::kBlockBytes + q * 128 +
-                                        (((c & 7) ^ (q & 7)) << 4)) = w[u];
-          }
+        const T* qb = reinterpret_cast<const T*>(p.q) + (int64_t)cu0 * p.q_st +
+                      (int64_t)s.hk * p.G * p.q_sh;
+        for (int i = tid; i < (two ? 256 : 128) * VPR; i += 512) {
+          const int row = i / VPR, c = i % VPR, q = row & 127;
+          const int rq = s.row0 + row, node = rq / p.G;
+          const bool in = row < s.rows;
+          copy16(sQ + (row >> 7) * Gm::kTileBytes + (c >> 3) * Gm::kBlockBytes + q * 128 +
+                     (((c & 7) ^ (q & 7)) << 4),
+                 in ? qb + node * p.q_st + (rq - node * p.G) * p.q_sh + c * 8 : qb, in);
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bs->q_full[0]);
       }
       const int n = s.t1 - s.t0, step = two ? 1 : 2;
-      const int nx = two ? n : (x ? n / 2 : (n + 1) / 2);
-      const int rowx = s.row0 + (two ? x * 128 : 0);   // request row of the tile's row 0
+      const int n1 = two ? n : n / 2;                    // tiles of stream 1
+      const int nx = x ? n1 : (two ? n : (n + 1) / 2);
+      const int rowx = s.row0 + (two ? x * 128 : 0);     // request row of lane 0
       const int rows = min(s.row0 + s.rows - rowx, 128);
-      float m = -INFINITY, l = 0.f;
+      float m = kNoMax, l = 0.f;
       for (int it = 0; it < nx; ++it, ++j) {
-        const int p0 = (s.t0 + (two ? 0 : x) + it * step) * kBN;
+        const int p0 = (s.t0 + (two ? 0 : x) + it * step) * kBN + h * 64;
         // which of the thread's positions its row sees
-        const bool full = p0 + kBN <= ctx;
-        uint32_t vis[kBN / 32];
+        const bool full = p0 + 64 <= ctx;
+        uint32_t vis[2];
         if (!full) {
 #pragma unroll
-          for (int w = 0; w < kBN / 32; ++w) {
+          for (int w = 0; w < 2; ++w) {
             const int b = p0 + 32 * w;
-            vis[w] = 0;
-            if (b + 32 <= ctx) {
-              vis[w] = 0xffffffffu;
-            } else if (b < end) {
+            vis[w] = b + 32 <= ctx ? 0xffffffffu : 0u;
+            if (b + 32 > ctx && b < end) {
               // one mask row at a time, a lane a position
               const int jn = b + lane - ctx;
               const bool node_ok = jn >= 0 && b + lane < end;
-              const int first = rowx + sub * 32;
               const uint8_t* mp = p.mask + (int64_t)cu0 * p.mask_stride + jn;
 #pragma unroll 8
               for (int i = 0; i < 32; ++i) {
-                const int node = (first + i) / p.G;
+                const int node = (rowx + sub * 32 + i) / p.G;
                 const bool v = jn < 0 || (node_ok && node < nodes &&
                                           mp[(int64_t)node * p.mask_stride] != 0);
                 const uint32_t bits = __ballot_sync(0xffffffffu, v);
@@ -772,99 +830,118 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           }
         }
         ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->s_full[x], j & 1, bs, p.err));
-        if (!ok) break;
         umma::fence_after_sync();
-        float sv[kBN];
+        // 32 positions at a time, read once for the maximum and again for the
+        // weights: 64 of them held would spill
+        float sv[32];
+        auto scores = [&](int c) {
+          umma::tmem_ld32(scol + c * 32, sv);
+          umma::tmem_wait_ld();
+          if (!full) {
 #pragma unroll
-        for (int c = 0; c < kBN / 32; ++c)
-          umma::tmem_ld32(trow + scol + c * 32, sv + c * 32);
-        umma::tmem_wait_ld();
-        if (!full) {
+            for (int e = 0; e < 32; ++e)
+              if (!((vis[c] >> e) & 1u)) sv[e] = -INFINITY;
+          }
+        };
+        float mx = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < kBN; ++c)
-            if (!((vis[c >> 5] >> (c & 31)) & 1u)) sv[c] = -INFINITY;
+        for (int c = 0; c < 2; ++c) {
+          scores(c);
+          float mx4[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx4[e] = fmaxf(sv[e], sv[4 + e]);
+#pragma unroll
+          for (int e = 8; e < 32; ++e) {
+            if ((e & 4) == 0) mx4[e & 3] = fmax3(mx4[e & 3], sv[e], sv[e + 4]);
+          }
+          mx = fmaxf(mx, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
         }
-        float mx8[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) mx8[e] = sv[e];
-#pragma unroll
-        for (int c = 8; c < kBN; ++c) mx8[c & 7] = fmaxf(mx8[c & 7], sv[c]);
-        const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
-                               fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]))) *
-                         p.scale_log2;
-        // the maximum moves only past its headroom: weights are at most 2^8
-        const bool grow = mx > m + kRescaleLog2 || (m == -INFINITY && mx > -INFINITY);
-        float fac = 1.f;
-        if (grow) {
-          fac = (m == -INFINITY) ? 0.f : ex2(m - mx);
+        mx *= p.scale_log2;
+        // the maximum moves only past its headroom (weights are at most 2^8),
+        // for both halves of a row at once
+        bool rise = it == 0;
+        if (it > 0) rise = vote_bar<256>(2 + x, mx > m + kRescaleLog2);
+        if (rise) {
+          sm_mx[(x * 2 + h) * 128 + r] = mx;
+          named_bar_sync(2 + x, 256);
+          mx = fmaxf(mx, sm_mx[(x * 2 + 1 - h) * 128 + r]);
+          const bool grow = mx > m + kRescaleLog2;
+          const float fac = grow ? ex2(m - mx) : 1.f;
+          m = grow ? mx : m;
           l *= fac;
-          m = mx;
-        }
-        if (it > 0 && __any_sync(0xffffffffu, grow)) {
-          // O_X is quiescent: the last PV was issued before this QK, so it has
-          // completed, and the next PV waits for this P
+          if (it > 0) {
+            // this half's columns of O_X, which is quiescent: the last PV was
+            // issued before this QK, so it has completed, and the next PV
+            // waits for this P
+#pragma unroll 1
+            for (int c = 0; c < D / 2; c += 16) {
+              float ov[16];
+              const uint32_t oc = trow + Gm::kColO + x * D + h * (D / 2) + c;
+              tmem_ld(oc, ov);
+              umma::tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            float ov[32];
-            umma::tmem_ld32(trow + ocol + c * 32, ov);
-            umma::tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) ov[e] *= fac;
-            umma::tmem_st32(trow + ocol + c * 32, ov);
-          }
-        }
-        const float nm = (m == -INFINITY) ? 0.f : -m;
-        float rs[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < kBN / 32; ++c) {
-          uint32_t hi[16], lo[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float a = ex2(fmaf(sv[c * 32 + 2 * e], p.scale_log2, nm));
-            const float b = ex2(fmaf(sv[c * 32 + 2 * e + 1], p.scale_log2, nm));
-            rs[e & 1] += a;
-            rs[2 + (e & 1)] += b;
-            float ah, bh;
-            if constexpr (kBf16) {         // truncated: one byte permute a pair
-              hi[e] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
-              ah = __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
-              bh = __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
-            } else {
-              hi[e] = Elem<T>::pack(a, b);
-              Elem<T>::unpack(hi[e], ah, bh);
+              for (int e = 0; e < 16; ++e) ov[e] *= fac;
+              tmem_st(oc, ov);
             }
-            lo[e] = Elem<T>::pack(a - ah, b - bh);
           }
-          umma::tmem_st16u(trow + scol + c * 16, hi);
-          umma::tmem_st16u(trow + scol + 64 + c * 16, lo);
         }
-        l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+        const uint64_t sc2 = f2pack(p.scale_log2, p.scale_log2), nm2 = f2pack(-m, -m);
+        uint64_t rs2 = 0;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {      // 16 columns of values, 16 of remainders
+          scores(c);
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              rs2 = fadd2(rs2, weigh<T>(sv[b * 16 + 2 * e], sv[b * 16 + 2 * e + 1], sc2, nm2, hi[e],
+                                        lo[e]));
+            tmem_st8u(scol + c * 32 + b * 8, hi);
+            tmem_st8u(scol + c * 32 + 16 + b * 8, lo);
+          }
+        }
+        float rs0, rs1;
+        f2unpack(rs2, rs0, rs1);
+        l += rs0 + rs1;
         umma::tmem_wait_st();
         umma::fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bs->p_full[x]);
+        if (lane == 0) mbar_arrive(&bs->p_full[2 * x + h]);
       }
 
       // ---- epilogue.  Named barriers are passed whether or not a wait
-      // failed, so that no thread is left behind at one.
-      if (nx > 0 && ok) {
-        ok = __all_sync(0xffffffffu, wait_bar(&bs->pv_done[x], sx & 1, bs, p.err));
-        ++sx;
-        umma::fence_after_sync();
+      // failed, so that no thread is left behind at one.  Both streams'
+      // products are done before the query tile's space is scratch.
+      ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->pv_done[0], si & 1, bs, p.err));
+      if (n1 > 0) {
+        ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->pv_done[1], s1 & 1, bs, p.err));
+        ++s1;
       }
-      float* slot = p.part + ((int64_t)blockIdx.x * 2 + (s.first ? 0 : 1)) * part_floats<D>(RG);
+      umma::fence_after_sync();
+      float* sm_l = reinterpret_cast<float*>(smem + Gm::kOffQ);   // [stream][half][128]
+      float* sm_m = sm_l + 512;                                   // [stream][128]
+      sm_l[(x * 2 + h) * 128 + r] = l;
+      if (h == 0) sm_m[x * 128 + r] = m;
+      named_bar_sync(1, 512);
+      const bool fix = *reinterpret_cast<volatile int*>(&bs->bad[si % kBadSlots]) != 0;
+      float* part = p.part + ((int64_t)blockIdx.x * 2 + (s.first ? 0 : 1)) * part_floats<D>(RG);
       auto bad = [&](int row, int col) {
         return bad_sum<T>(p, walk.r, cu0 + (s.row0 + row) / p.G, ctx, max(ctx, s.t0 * kBN),
                           min(end, s.t1 * kBN), s.hk, col);
       };
-      auto store = [&](int row, int col, float M, float L, float* o, auto n_col) {
-        constexpr int N = decltype(n_col)::value;
+      // N columns from col of a row of the group: o scaled by 1 / L, or as it
+      // is to the workspace
+      auto store = [&](int row, int col, float M, float L, auto& o) {
+        constexpr int N = sizeof(o) / sizeof(float);
+        if (fix)
+          for (int e = 0; e < N; ++e) o[e] += bad(row, col + e);
+        M = M == kNoMax ? -INFINITY : M;
         if (!s.whole) {
-          float* d = slot + row * D + col;
+          float4* d = reinterpret_cast<float4*>(part + row * D + col);
 #pragma unroll
-          for (int e = 0; e < N; e += 4)
-            *reinterpret_cast<float4*>(d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          if (col == 0) *reinterpret_cast<float2*>(slot + RG * D + 2 * row) = make_float2(M, L);
+          for (int e = 0; e < N; e += 4) d[e / 4] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          if (col == 0) *reinterpret_cast<float2*>(part + RG * D + 2 * row) = make_float2(M, L);
           return;
         }
         const int rq = s.row0 + row, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
@@ -889,90 +966,38 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         }
       };
       if (two) {
-        // every row is one thread's
-        const bool fix = *reinterpret_cast<volatile int*>(&bs->bad[si % kBadSlots]) != 0;
-        if (ok) {
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            float ov[32];
-            umma::tmem_ld32(trow + ocol + c * 32, ov);
-            umma::tmem_wait_ld();
-            if (r < rows) {
-              if (fix)
-                for (int e = 0; e < 32; ++e) ov[e] += bad(r + x * 128, c * 32 + e);
-              store(r + x * 128, c * 32, m, l, ov, std::integral_constant<int, 32>());
-            }
-          }
+        // stream x's rows, half the columns a thread
+        const float L = sm_l[x * 256 + r] + sm_l[x * 256 + 128 + r];
+#pragma unroll 1
+        for (int c = 0; c < D / 2; c += 16) {
+          float ov[16];
+          tmem_ld(trow + Gm::kColO + x * D + h * (D / 2) + c, ov);
+          umma::tmem_wait_ld();
+          if (r < rows && ok) store(r + x * 128, h * (D / 2) + c, m, L, ov);
         }
       } else {
-        // join the two streams' states of every row.  Both agree on the row's
-        // maximum through shared memory, then add their scaled outputs into
-        // one fp32 copy in the query tile's space (its MMAs have completed),
-        // half the columns at a time: in round k stream x adds quarter
-        // (x + k) mod 2 of that half, so both work at once and the order of
-        // the sum is fixed.
-        constexpr int DA = D / 2, W = DA / 2;                // columns held, of a quarter
-        static_assert(128 * DA * 4 <= Gm::kTileBytes, "scratch fits the query tile");
-        sm_m[x * 128 + r] = m;
-        sm_l[x * 128 + r] = l;
-        named_bar_sync(1, 256);
-        const bool fix = *reinterpret_cast<volatile int*>(&bs->bad[si % kBadSlots]) != 0;
-        // a row that saw only NaN has m = -inf and l = NaN: weight 1 keeps the NaN
-        const float m0 = sm_m[r], m1 = sm_m[128 + r], l0 = sm_l[r], l1 = sm_l[128 + r];
+        // the two streams' states of a row are both in its TMEM lane: every
+        // thread joins a quarter of the columns.  A state that saw only NaN
+        // has no maximum and l = NaN: weight 1 keeps the NaN.
+        const float m0 = sm_m[r], m1 = n1 > 0 ? sm_m[128 + r] : kNoMax;
+        const float l0 = sm_l[r] + sm_l[128 + r], l1 = n1 > 0 ? sm_l[256 + r] + sm_l[384 + r] : 0.f;
         const float M = fmaxf(m0, m1);
-        const float w0 = (m0 == -INFINITY) ? (l0 == l0 ? 0.f : 1.f) : ex2(m0 - M);
-        const float w1 = (m1 == -INFINITY) ? (l1 == l1 ? 0.f : 1.f) : ex2(m1 - M);
+        const float w0 = m0 == kNoMax ? (l0 == l0 ? 0.f : 1.f) : ex2(m0 - M);
+        const float w1 = m1 == kNoMax ? (l1 == l1 ? 0.f : 1.f) : ex2(m1 - M);
         const float L = fmaf(l1, w1, l0 * w0);
-        const float w = x ? w1 : w0;
-        float* acc = reinterpret_cast<float*>(smem + Gm::kOffQ);
-        // float4 granule `gr` of a row: swizzled against bank conflicts
-        auto granule = [&](int row, int gr) {
-          return reinterpret_cast<float4*>(acc + row * DA + ((gr ^ (row & 7)) << 2));
-        };
-        for (int hf = 0; hf < 2; ++hf) {
+        const int col = (x * 2 + h) * (D / 4);
 #pragma unroll 1
-          for (int k = 0; k < 2; ++k) {
-            const int sl = x ^ k;
-            float ov[W];
-            if (nx > 0 && ok) {
-              tmem_ld(trow + ocol + hf * DA + sl * W, ov);
-              umma::tmem_wait_ld();
-            } else {
+        for (int c = 0; c < D / 4; c += 16) {
+          float a[16], b[16];
+          tmem_ld(trow + Gm::kColO + col + c, a);
+          if (n1 > 0) tmem_ld(trow + Gm::kColO + D + col + c, b);
+          umma::tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < W; ++e) ov[e] = 0.f;
-            }
-#pragma unroll
-            for (int e = 0; e < W; e += 4) {
-              float4* d = granule(r, (sl * W + e) >> 2);
-              float4 y = k == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *d;
-              y.x = fmaf(ov[e], w, y.x);
-              y.y = fmaf(ov[e + 1], w, y.y);
-              y.z = fmaf(ov[e + 2], w, y.z);
-              y.w = fmaf(ov[e + 3], w, y.w);
-              *d = y;
-            }
-            named_bar_sync(1, 256);
-          }
-          if (hf == 0) {
-            if (x == 0) {                      // everyone has read m and l
-              sm_m[r] = M;
-              sm_l[r] = L;
-            }
-            named_bar_sync(1, 256);
-          }
-          if (ok) {
-            for (int i = tid; i < rows * (DA / 8); i += 256) {
-              const int row = i / (DA / 8), c = i % (DA / 8);
-              const float4 y0 = *granule(row, 2 * c), y1 = *granule(row, 2 * c + 1);
-              float o[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
-              if (fix)
-                for (int e = 0; e < 8; ++e) o[e] += bad(row, hf * DA + c * 8 + e);
-              store(row, hf * DA + c * 8, sm_m[row], sm_l[row], o, std::integral_constant<int, 8>());
-            }
-          }
-          if (hf == 0) named_bar_sync(1, 256);   // before the second half
+          for (int e = 0; e < 16; ++e) a[e] = n1 > 0 ? fmaf(b[e], w1, a[e] * w0) : a[e] * w0;
+          if (r < rows && ok) store(r, col + c, M, L, a);
         }
       }
+      umma::fence_before_sync();
       ++si;
     }
   }
@@ -1010,8 +1035,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
 // The row maximum lies across threads here, but it moves only past its
 // headroom of 2^8, so a tile costs one barrier with a vote; the reduction runs
 // in a segment's first tile and in the rare tile that raises it.
-constexpr float kNoMax = -1e30f;           // nothing seen yet: any score raises it
-
 // Sum or maximum over the warp of N (8, 16 or 32) columns, one a row: lane i
 // ends with row i % N in v[0].
 template <int N, class Op>
@@ -1031,20 +1054,6 @@ __device__ __forceinline__ void warp_columns(float (&v)[N], Op op) {
       v[i] = op(keep, __shfl_xor_sync(0xffffffffu, give, o));
     }
   }
-}
-
-// Barrier `id` of four softmax warps that tells whether any thread voted.
-__device__ __forceinline__ bool vote_bar(int id, bool vote) {
-  uint32_t any;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, %2, 128, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(any)
-      : "r"(vote ? 1u : 0u), "r"(id)
-      : "memory");
-  return any != 0;
 }
 
 template <typename T, int D, int NR>
@@ -1253,7 +1262,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
 #pragma unroll
                 for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], x[r + e]);
               }
-              rise = vote_bar(bar, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > kRescaleLog2);
+              rise = vote_bar<128>(bar, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > kRescaleLog2);
               if (!rise) break;
               continue;
             }
