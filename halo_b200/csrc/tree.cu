@@ -141,7 +141,7 @@ struct Req {
 struct Bars {
   uint64_t q_full[2], q_empty[2];
   uint64_t k_full[6], k_empty[6], v_full[6], v_ready[6], v_empty[6];
-  uint64_t s_full[2], p_full[4], pv_done[2], mma_done[2];
+  uint64_t s_full[2], p_full[4], pv_done[2], mma_done[2], turn[2];
   int64_t scan[20];
   int64_t base0, total;
   uint32_t tmem_base;
@@ -653,6 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       mbar_init(&bs->s_full[x], 1);
       mbar_init(&bs->p_full[2 * x], 4);
       mbar_init(&bs->p_full[2 * x + 1], 4);
+      mbar_init(&bs->turn[x], 8);
       mbar_init(&bs->pv_done[x], 1);
       mbar_init(&bs->mma_done[x], 1);
     }
@@ -774,6 +775,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     Walk<RG> walk(p, bs->r0, bs->req0, bs->base0, u0, u1);
     Seg s;
     int j = 0, si = 0, s1 = 0;             // this stream's tiles; segments; those of stream 1
+    int turns = 0;                         // waited for
     bool ok = true;
     while (walk.next(p, s)) {
       const bool two = QT == 2 && s.rows > 128;
@@ -800,6 +802,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       const int n = s.t1 - s.t0, step = two ? 1 : 2;
       const int n1 = two ? n : n / 2;                    // tiles of stream 1
       const int nx = x ? n1 : (two ? n : (n + 1) / 2);
+      const int ny = x ? (two ? n : (n + 1) / 2) : n1;   // of the other stream
       const int rowx = s.row0 + (two ? x * 128 : 0);     // request row of lane 0
       const int rows = min(s.row0 + s.rows - rowx, 128);
       float m = kNoMax, l = 0.f;
@@ -830,6 +833,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           }
         }
         ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->s_full[x], j & 1, bs, p.err));
+        // The streams take turns, 0 first, so that one's softmax runs beside
+        // the other's MMAs: left alone they fall into step, both softmaxes and
+        // then both streams' MMAs (7000 clocks for 256 rows).
+        if (x == 1 || (it > 0 && it <= ny)) {
+          ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->turn[x], turns & 1, bs, p.err));
+          ++turns;
+        }
         umma::fence_after_sync();
         // 32 positions at a time, read once for the maximum and again for the
         // weights: 64 of them held would spill
@@ -904,6 +914,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         float rs0, rs1;
         f2unpack(rs2, rs0, rs1);
         l += rs0 + rs1;
+        if (lane == 0 && (x == 0 ? it < ny : it + 1 < ny)) mbar_arrive(&bs->turn[1 - x]);
         umma::tmem_wait_st();
         umma::fence_before_sync();
         __syncwarp();
