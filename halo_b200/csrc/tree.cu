@@ -651,8 +651,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&bs->s_full[x], 1);
-      mbar_init(&bs->p_full[2 * x], 4);
-      mbar_init(&bs->p_full[2 * x + 1], 4);
+      mbar_init(&bs->p_full[2 * x], 8);
+      mbar_init(&bs->p_full[2 * x + 1], 8);
       mbar_init(&bs->turn[x], 8);
       mbar_init(&bs->pv_done[x], 1);
       mbar_init(&bs->mma_done[x], 1);
@@ -714,10 +714,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           const int nx = two ? n : (x ? n / 2 : (n + 1) / 2);
           const uint64_t qd0 = qdesc0 + (uint64_t)(((two ? x : 0) * Gm::kTileBytes) >> 4);
           int g = g0 + (two ? 0 : x);
-          auto qk = [&]() {                   // S_X = Q K(g)^T
-            const int ik = g % SK;
-            if (!wait_bar(&bs->k_full[ik], (g / SK) & 1, bs, p.err)) return false;
-            umma::fence_after_sync();
+          auto k_landed = [&](int t) {
+            return wait_bar(&bs->k_full[t % SK], (t / SK) & 1, bs, p.err);
+          };
+          auto qk = [&](int t) {              // S_X = Q K(t)^T, K(t) has landed
+            const int ik = t % SK;
             const uint64_t qd = opaque(qd0);
             const uint64_t kd = opaque(kdesc0 + (uint64_t)((ik * Gm::kTileBytes) >> 4));
 #pragma unroll
@@ -727,30 +728,37 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             }
             umma::commit(&bs->s_full[x]);
             umma::commit(&bs->k_empty[ik]);
-            return true;
           };
           ok = wait_bar(&bs->q_full[0], si & 1, bs, p.err);
-          if (ok && nx > 0) ok = qk();
+          if (ok && nx > 0 && (ok = k_landed(g))) {
+            umma::fence_after_sync();
+            qk(g);
+          }
           for (int it = 0; ok && it < nx; ++it, ++j) {
             const int iv = g % SV;
-            ok = wait_bar(&bs->v_ready[iv], (g / SV) & 1, bs, p.err);
+            // everything but P is waited for ahead of it: the next QK follows
+            // this PV at once
+            ok = wait_bar(&bs->v_ready[iv], (g / SV) & 1, bs, p.err) &&
+                 (it + 1 == nx || k_landed(g + step));
             const uint64_t vd = opaque(vdesc0 + (uint64_t)((iv * Gm::kTileBytes) >> 4));
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {           // O_X += P_X V(g), half the positions
-              ok = ok && wait_bar(&bs->p_full[2 * x + h], j & 1, bs, p.err);
+            for (int c = 0; c < 2; ++c) {           // O_X += P_X V(g), as the halves of P come
+              ok = ok && wait_bar(&bs->p_full[2 * x + c], j & 1, bs, p.err);
               if (!ok) break;
               umma::fence_after_sync();
 #pragma unroll
-              for (int kk = 0; kk < 8; ++kk)        // 16 positions: values, remainders
-                umma::mma_ts(oc, pc + h * 64 + (kk >> 2) * 32 + (kk & 1) * 16 + ((kk >> 1) & 1) * 8,
-                             vd + (uint64_t)(((h * 4 + (kk >> 1)) * 16 * 128) >> 4), kIdPV,
-                             it > 0 || h > 0 || kk > 0);
+              for (int kk = 0; kk < 8; ++kk) {      // 16 positions: values, remainders
+                const int h = kk >> 2, b = (kk >> 1) & 1;
+                umma::mma_ts(oc, pc + h * 64 + c * 32 + (kk & 1) * 16 + b * 8,
+                             vd + (uint64_t)(((h * 4 + c * 2 + b) * 16 * 128) >> 4), kIdPV,
+                             it > 0 || c > 0 || kk > 0);
+              }
             }
             if (!ok) break;
-            umma::commit(&bs->v_empty[iv]);
-            if (it + 1 == nx) umma::commit(&bs->pv_done[x]);
             g += step;
-            if (it + 1 < nx) ok = qk();
+            if (it + 1 < nx) qk(g);
+            else umma::commit(&bs->pv_done[x]);
+            umma::commit(&bs->v_empty[iv]);
           }
           g0 += n;
           ++si;
@@ -910,15 +918,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             tmem_st8u(scol + c * 32 + b * 8, hi);
             tmem_st8u(scol + c * 32 + 16 + b * 8, lo);
           }
+          umma::tmem_wait_st();
+          umma::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bs->p_full[2 * x + c]);
         }
         float rs0, rs1;
         f2unpack(rs2, rs0, rs1);
         l += rs0 + rs1;
         if (lane == 0 && (x == 0 ? it < ny : it + 1 < ny)) mbar_arrive(&bs->turn[1 - x]);
-        umma::tmem_wait_st();
-        umma::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bs->p_full[2 * x + h]);
       }
 
       // ---- epilogue.  Named barriers are passed whether or not a wait
