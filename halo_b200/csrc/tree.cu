@@ -921,12 +921,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           umma::tmem_wait_st();
           umma::fence_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bs->p_full[2 * x + c]);
+          if (lane == 0) {
+            mbar_arrive(&bs->p_full[2 * x + c]);
+            // passed on halfway: the other stream's scores are read meanwhile
+            if (c == 0 && (x == 0 ? it < ny : it + 1 < ny)) mbar_arrive(&bs->turn[1 - x]);
+          }
         }
         float rs0, rs1;
         f2unpack(rs2, rs0, rs1);
         l += rs0 + rs1;
-        if (lane == 0 && (x == 0 ? it < ny : it + 1 < ny)) mbar_arrive(&bs->turn[1 - x]);
       }
 
       // ---- epilogue.  Named barriers are passed whether or not a wait
