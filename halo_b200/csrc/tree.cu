@@ -1040,7 +1040,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
 //   warp 0      TMA producer (as in tree_kernel)
 //   warp 1      TMEM owner; lane 0 issues every MMA
 //   warp 2      cleans V
-//   warp 3      query rows of the next segment (two buffers)
+//   warp 3      query rows of the next segment (two buffers; the first
+//               segment's are loaded by the softmax warps)
 //   warps 4-11  softmax (thread = position of the tile) and epilogue (thread =
 //               output column), warps 4-7 the first NR / 2 rows, warps 8-11 the
 //               others
@@ -1122,7 +1123,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
   __syncthreads();
   umma::fence_after_sync();
   const uint32_t tmem = bs->tmem_base;
-  if (threadIdx.x == 96) write_desc<RG>(p, bs, u0, U);
+  if (threadIdx.x == 64) write_desc<RG>(p, bs, u0, U);
   grid_dep_trigger();
 
   const uint32_t sQ = smem_addr(smem + Gm::kOffQ);
@@ -1136,6 +1137,22 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
   if (u0 < u1 && aligned) {
     Walk<RG> walk(p, bs->r0, bs->req0, bs->base0, u0, u1);
     Seg s;
+    // Segment si's query rows by threads 0 .. nt - 1: 16-byte copies, all in
+    // flight.
+    auto copy_q = [&](int t, int nt, int si) {
+      constexpr int VPR = D / 8;
+      const char* qb = p.q + 2 * (walk.q.cu0 * p.q_st + (int64_t)s.hk * p.G * p.q_sh);
+      const uint32_t dst = sQ + (si & 1) * Gm::kQBytes;
+#pragma unroll 1
+      for (int i = t; i < NR * VPR; i += nt) {
+        const int row = i / VPR, c = i % VPR;
+        const int rq = s.row0 + row, node = rq / p.G;
+        const bool in = row < s.rows;
+        const char* src = qb + 2 * (node * p.q_st + (rq - node * p.G) * p.q_sh + c * 8);
+        copy16(dst + (c >> 3) * NR * 128 + row * 128 + (((c & 7) ^ (row & 7)) << 4),
+               in ? src : p.q, in);
+      }
+    };
     if (warp == 0) {
       produce<RG, Gm, false>(p, bs, smem, walk);
     } else if (warp == 1) {
@@ -1198,24 +1215,15 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
       clean<T, D, RG, Gm>(p, bs, smem, walk);
     } else if (warp == 3) {
       // -------------------------------------------------------- query rows
-      int si = 0;
-      bool ok = true;
+      // (the first segment's are the softmax warps')
+      int si = 1;
+      bool ok = walk.next(p, s);
       while (ok && walk.next(p, s)) {
         if (si >= 2)
           ok = __all_sync(0xffffffffu,
                           wait_bar(&bs->q_empty[si & 1], ((si >> 1) - 1) & 1, bs, p.err));
         if (!ok) break;
-        constexpr int VPR = D / 8;
-        const T* qb = reinterpret_cast<const T*>(p.q) + (int64_t)walk.q.cu0 * p.q_st +
-                      (int64_t)s.hk * p.G * p.q_sh;
-        for (int i = lane; i < NR * VPR; i += 32) {    // 16-byte copies, all in flight
-          const int row = i / VPR, c = i % VPR;
-          const int rq = s.row0 + row, node = rq / p.G;
-          const bool in = row < s.rows;
-          copy16(sQ + (si & 1) * Gm::kQBytes + (c >> 3) * NR * 128 + row * 128 +
-                     (((c & 7) ^ (row & 7)) << 4),
-                 in ? qb + node * p.q_st + (rq - node * p.G) * p.q_sh + c * 8 : qb, in);
-        }
+        copy_q(lane, 32, si);
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async_smem();
         __syncwarp();
@@ -1233,6 +1241,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
       bool ok = true;
       while (walk.next(p, s)) {
         const int ctx = walk.q.ctx, end = walk.q.end;
+        if (si == 0) {                     // later ones come from warp 3, ahead
+          copy_q(threadIdx.x - 128, 256, 0);
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          fence_proxy_async_smem();
+          named_bar_sync(3, 256);
+          if (threadIdx.x == 128) mbar_arrive(&bs->q_full[0]);
+        }
         float l[RT];
 #pragma unroll
         for (int r = 0; r < RT; ++r) l[r] = 0.f;
@@ -1244,15 +1259,30 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
             const int pos = t * kBN + tid, jn = pos - ctx;
             vis = pos < ctx ? 0xffffffffu : 0u;
             if (jn >= 0 && pos < end) {
-              int node = (s.row0 + r0) / p.G, rem = s.row0 + r0 - node * p.G;
-              const uint8_t* mp = p.mask + (int64_t)walk.q.cu0 * p.mask_stride + jn;
+              // the nodes of this group's rows that see node jn, eight loads
+              // in flight, then a bit for each of their rows
+              const int first = s.row0 + r0, n0 = first / p.G;
+              const int n1 = min((first + RT - 1) / p.G + 1, walk.q.nodes);
+              const uint8_t* mp = p.mask + (walk.q.cu0 + n0) * p.mask_stride + jn;
+              uint32_t sees = 0;
+#pragma unroll 1
+              for (int k = 0; k < RT && n0 + k < n1; k += 8) {
+                uint8_t b[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  b[e] = n0 + k + e < n1 ? *mp : 0;
+                  mp += p.mask_stride;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sees |= (b[e] != 0 ? 1u : 0u) << (k + e);
+              }
+              int rem = first - n0 * p.G;
 #pragma unroll
               for (int r = 0; r < RT; ++r) {
-                const bool v = r0 + r < s.rows && mp[(int64_t)node * p.mask_stride] != 0;
-                vis |= (v ? 1u : 0u) << r;
+                vis |= (sees & 1u) << r;
                 if (++rem == p.G) {
                   rem = 0;
-                  ++node;
+                  sees >>= 1;
                 }
               }
             }
