@@ -8,6 +8,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 import threading
 
 import torch  # noqa: F401  -- loads the CUDA runtime the library shares with torch
@@ -117,6 +118,12 @@ class TreeProblem(ctypes.Structure):
                 ("lse", ctypes.c_void_p)]
 
 
+# The two descriptions above as packed bytes, which cost a call a fraction of
+# what filling the ctypes structures does; entry points take either.
+pack_page_pool = struct.Struct("=QQ6q5i4x").pack
+pack_tree_problem = struct.Struct("=5ifQ2qQqQQQqQ2qi4xQ").pack
+
+
 # name -> (restype, argtypes); must match include/halo_b200.h
 SIGNATURES = {
     "halo_decode_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(DecodeProblem),
@@ -190,16 +197,16 @@ SIGNATURES = {
                                                   ctypes.c_int32, ctypes.c_void_p,
                                                   ctypes.c_void_p, ctypes.c_void_p,
                                                   ctypes.c_void_p, ctypes.c_void_p]),
-    "halo_write_kv_pages": (ctypes.c_int32, [ctypes.POINTER(PagePool), ctypes.c_void_p,
+    "halo_write_kv_pages": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p,
                                              ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
                                              ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
                                              ctypes.c_void_p, ctypes.c_void_p]),
-    "halo_tree_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(PagePool),
-                                                   ctypes.POINTER(TreeProblem)]),
-    "halo_tree_attention": (ctypes.c_int32, [ctypes.POINTER(PagePool),
-                                             ctypes.POINTER(TreeProblem), ctypes.c_void_p,
+    "halo_tree_workspace_bytes": (ctypes.c_int64, [ctypes.c_void_p,
+                                                   ctypes.c_void_p]),
+    "halo_tree_attention": (ctypes.c_int32, [ctypes.c_void_p,
+                                             ctypes.c_void_p, ctypes.c_void_p,
                                              ctypes.c_int64, ctypes.c_void_p]),
-    "halo_commit_tree_path": (ctypes.c_int32, [ctypes.POINTER(PagePool), ctypes.c_void_p,
+    "halo_commit_tree_path": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p,
                                                ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
                                                ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
                                                ctypes.c_int32, ctypes.c_void_p,

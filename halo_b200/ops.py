@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 from typing import Optional, Sequence
 
 import torch
@@ -547,28 +548,30 @@ def _int32s(index: int, tensors: dict) -> None:
                     f"strides {t.stride()}")
 
 
-def _require_table(t: torch.Tensor, index: int) -> None:
-    if t.dim() != 2 or t.dtype != torch.int32 or t.get_device() != index or \
-            (t.shape[1] > 1 and t.stride(1) != 1):
+def _table(t: torch.Tensor, index: int) -> tuple:
+    """``(R, max_blocks, row stride)`` of block tables on device ``index``."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or t.dtype is not torch.int32 or t.get_device() != index or \
+            (shape[1] > 1 and stride[1] != 1):
         _refuse(f"block_tables must be int32 (R, max_blocks) with contiguous rows on device {index}")
+    return shape[0], shape[1], stride[0]
 
 
-def _page_pool(k: torch.Tensor, v: torch.Tensor) -> L.PagePool:
-    """The C-ABI description of page pools ``(n_pages, H_kv, page_size, D)``."""
-    if not k.is_cuda:
-        _refuse("k_pages must be a CUDA tensor (no CPU path)")
+def _page_pool(k: torch.Tensor, v: torch.Tensor, index: int, dtype: torch.dtype):
+    """The packed C-ABI description of page pools ``(n_pages, H_kv, page_size,
+    D)`` on device ``index``, with ``H_kv`` and ``D``."""
     shape = k.shape
-    if len(shape) != 4 or v.shape != shape or v.dtype is not k.dtype or \
-            v.get_device() != k.get_device():
+    if len(shape) != 4 or v.shape != shape or k.dtype is not dtype or v.dtype is not dtype or \
+            k.get_device() != index or v.get_device() != index:
         _refuse("k_pages and v_pages must be (n_pages, H_kv, page_size, D) of one shape, dtype and "
-                "device")
+                "device, those of the rows")
     n, H_kv, page, D = shape
     ks, kh, kt, kd = k.stride()
     vs, vh, vt, vd = v.stride()
     if D > 1 and (kd != 1 or vd != 1):
         _refuse("page rows must be contiguous")
-    return L.PagePool(k.data_ptr(), v.data_ptr(), ks, kh, kt, vs, vh, vt, n, H_kv, page, D,
-                      L.halo_dtype(k.dtype))
+    return L.pack_page_pool(k.data_ptr(), v.data_ptr(), ks, kh, kt, vs, vh, vt, n, H_kv, page, D,
+                            L.halo_dtype(dtype)), H_kv, D
 
 
 def update_block_tables(block_tables: torch.Tensor, old_lens: torch.Tensor, new_lens: torch.Tensor,
@@ -593,8 +596,7 @@ def update_block_tables(block_tables: torch.Tensor, old_lens: torch.Tensor, new_
         _refuse("block_tables must be a CUDA tensor (no CPU path)")
     i32, dev = torch.int32, block_tables.device
     index = dev.index
-    _require_table(block_tables, index)
-    R, max_blocks = block_tables.shape
+    R, max_blocks, tstride = _table(block_tables, index)
     if n_free_out is None:
         n_free_out = n_free
     if not (old_lens.dtype is i32 and new_lens.dtype is i32 and free_pages.dtype is i32 and
@@ -615,7 +617,7 @@ def update_block_tables(block_tables: torch.Tensor, old_lens: torch.Tensor, new_
     cu = torch.empty(R + 1, dtype=i32, device=dev)
     lens = torch.empty(R, dtype=i32, device=dev)
     rc = _call(L.lib().halo_update_block_tables, index, block_tables.data_ptr(),
-               block_tables.stride(0), R, max_blocks, old_lens.data_ptr(), new_lens.data_ptr(),
+               tstride, R, max_blocks, old_lens.data_ptr(), new_lens.data_ptr(),
                free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(), n_free_out.data_ptr(),
                page_size, max_tokens, slots.data_ptr(), positions.data_ptr(), cu.data_ptr(),
                lens.data_ptr())
@@ -629,10 +631,12 @@ def write_kv_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     """Copy K/V rows ``(T, H_kv, D)`` into the slots ``(T,)`` (int64) of page
     pools ``(n_pages, H_kv, page_size, D)`` (``halo_write_kv_pages``).  Rows
     with a slot outside the pools (-1: none) are skipped; slots are distinct."""
-    pool = _page_pool(k_pages, v_pages)
-    index, shape = k_pages.get_device(), k.shape
-    if len(shape) != 3 or shape[1] != pool.H_kv or shape[2] != pool.D or v.shape != shape or \
-            k.dtype is not k_pages.dtype or v.dtype is not k.dtype or \
+    if not k_pages.is_cuda:
+        _refuse("k_pages must be a CUDA tensor (no CPU path)")
+    index, dtype, shape = k_pages.get_device(), k_pages.dtype, k.shape
+    pool, H_kv, D = _page_pool(k_pages, v_pages, index, dtype)
+    if len(shape) != 3 or shape[1] != H_kv or shape[2] != D or v.shape != shape or \
+            k.dtype is not dtype or v.dtype is not dtype or \
             k.get_device() != index or v.get_device() != index:
         _refuse("k and v must be (T, H_kv, D) of the pools' dtype and device")
     T = shape[0]
@@ -641,18 +645,34 @@ def write_kv_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
         _refuse("slots must be contiguous int64 (T,) on the pools' device")
     kt, kh, kd = k.stride()
     vt, vh, vd = v.stride()
-    if shape[2] > 1 and (kd != 1 or vd != 1):
+    if D > 1 and (kd != 1 or vd != 1):
         k, v = k.contiguous(), v.contiguous()
         kt, kh, _ = k.stride()
         vt, vh, _ = v.stride()
-    rc = _call(L.lib().halo_write_kv_pages, index, ctypes.byref(pool), k.data_ptr(), kt, kh,
-               v.data_ptr(), vt, vh, T, slots.data_ptr())
+    rc = _call(L.lib().halo_write_kv_pages, index, pool, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+               T, slots.data_ptr())
     if rc:
         L.check(rc, "halo_write_kv_pages")
 
 
-# workspace bytes of halo_tree_attention by what they depend on
+# workspace bytes of halo_tree_attention by what they depend on, and the
+# workspaces of calls outside a capture, which need no initial contents
 _TREE_BYTES: dict = {}
+_TREE_LOCAL = threading.local()
+
+
+def _tree_workspace(index: int, stream: int, need: int) -> torch.Tensor:
+    """``need`` bytes for a call on ``stream``.  A thread's calls on one stream
+    follow one another and share a buffer that grows; a captured call gets one
+    of its own from the graph's pool, so that no two graphs share one."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(need, dtype=torch.uint8, device=f"cuda:{index}")
+    bufs = _TREE_LOCAL.__dict__
+    ws = bufs.get((index, stream))
+    if ws is None or ws.numel() < need:
+        ws = torch.empty(need, dtype=torch.uint8, device=f"cuda:{index}")
+        bufs[index, stream] = ws
+    return ws
 
 
 def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -677,16 +697,12 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     of 8."""
     if not q.is_cuda:
         _refuse("q must be a CUDA tensor (no CPU path)")
-    dev = q.device
-    index = dev.index
-    pool = _page_pool(k_pages, v_pages)
-    dtype, qshape = q.dtype, q.shape
-    if len(qshape) != 3 or dtype is not k_pages.dtype or k_pages.get_device() != index or \
-            qshape[2] != pool.D:
+    index, dtype, qshape = q.get_device(), q.dtype, q.shape
+    pool, H_kv, D = _page_pool(k_pages, v_pages, index, dtype)
+    if len(qshape) != 3 or qshape[2] != D:
         _refuse("q must be (T, H, D) of the pools' dtype, device and head dim")
-    T, H, D = qshape
-    _require_table(block_tables, index)
-    R, max_blocks = block_tables.shape
+    T, H, _ = qshape
+    R, max_blocks, tstride = _table(block_tables, index)
     if not (context_lens.dtype is torch.int32 and cu_nodes.dtype is torch.int32 and
             context_lens.get_device() == index and cu_nodes.get_device() == index and
             context_lens.numel() == R and cu_nodes.numel() == R + 1 and
@@ -701,42 +717,40 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         q = q.contiguous()
         qt, qh, _ = q.stride()
     if out is None:
-        out = torch.empty(qshape, dtype=out_dtype or dtype, device=dev)
+        out = torch.empty_like(q) if (out_dtype is None or out_dtype is dtype) and \
+            q.is_contiguous() else torch.empty(T, H, D, dtype=out_dtype or dtype, device=q.device)
         ot, oh = H * D, D
     else:
-        ot, oh, od = out.stride()
-        if out.shape != qshape or out.get_device() != index or (D > 1 and od != 1):
+        if out.shape != qshape or out.get_device() != index or (D > 1 and out.stride(2) != 1):
             _refuse("out must be (T, H, D) with contiguous rows on q's device")
+        ot, oh, _ = out.stride()
     if lse is None:
         if want_lse:
-            lse = torch.empty(T, H, dtype=torch.float32, device=dev)
+            lse = torch.empty(T, H, dtype=torch.float32, device=q.device)
     elif lse.shape != (T, H) or lse.dtype is not torch.float32 or lse.get_device() != index or \
             not lse.is_contiguous():
         _refuse("lse must be contiguous fp32 (T, H) on q's device")
-    prob = L.TreeProblem(R, T, H, mshape[1], max_blocks,
-                         scale if scale is not None else 1.0 / math.sqrt(D), q.data_ptr(), qt, qh,
-                         block_tables.data_ptr(), block_tables.stride(0), context_lens.data_ptr(),
-                         cu_nodes.data_ptr(), tree_mask.data_ptr(), mstride[0], out.data_ptr(), ot,
-                         oh, L.halo_dtype(out.dtype), lse.data_ptr() if lse is not None else None)
-    return _tree_launch(pool, prob, index, dev, out, lse)
-
-
-def _tree_launch(pool, prob, index, dev, out, lse):
-    lib = L.lib()
-    a, b = ctypes.byref(pool), ctypes.byref(prob)
-    key = (index, pool.D, pool.H_kv, prob.H, prob.max_nodes)
-    need = _TREE_BYTES.get(key) if prob.R and prob.T else None
-    if need is None:
+    if _get_device() != index:
         with torch.cuda.device(index):
-            need = int(lib.halo_tree_workspace_bytes(a, b))
+            return tree_attention(q, k_pages, v_pages, block_tables, context_lens, cu_nodes,
+                                  tree_mask, scale=scale, out=out, lse=lse, want_lse=want_lse)
+    max_nodes = mshape[1]
+    prob = L.pack_tree_problem(R, T, H, max_nodes, max_blocks,
+                               scale if scale is not None else 1.0 / math.sqrt(D), q.data_ptr(), qt,
+                               qh, block_tables.data_ptr(), tstride, context_lens.data_ptr(),
+                               cu_nodes.data_ptr(), tree_mask.data_ptr(), mstride[0],
+                               out.data_ptr(), ot, oh, L.halo_dtype(out.dtype),
+                               lse.data_ptr() if lse is not None else 0)
+    lib, stream = L.lib(), L.stream_handle_of(index)
+    key = (index, D, H_kv, H, max_nodes, R > 0 and T > 0)
+    need = _TREE_BYTES.get(key)
+    if need is None:
+        need = int(lib.halo_tree_workspace_bytes(pool, prob))
         if need < 0:
             L.check(need, "halo_tree_workspace_bytes")
-        if prob.R and prob.T:
-            _TREE_BYTES[key] = need
-    # a workspace of the call's own: ordered by the allocator's stream, and
-    # graphs captured on one stream never share it
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    rc = _call(lib.halo_tree_attention, index, a, b, ws.data_ptr() if need else None, need)
+        _TREE_BYTES[key] = need
+    ws = _tree_workspace(index, stream, need) if need else None
+    rc = lib.halo_tree_attention(pool, prob, ws.data_ptr() if need else None, need, stream)
     if rc:
         L.check(rc, "halo_tree_attention")
     return out, lse
@@ -751,10 +765,11 @@ def commit_tree_path(k_pages: torch.Tensor, v_pages: torch.Tensor, block_tables:
     ``path (R, max_depth)`` (int32) holds node indices with
     ``path[r, i] >= i``, as paths from a root do when children are numbered
     after their parents; other steps move nothing."""
-    pool = _page_pool(k_pages, v_pages)
+    if not k_pages.is_cuda:
+        _refuse("k_pages must be a CUDA tensor (no CPU path)")
     index = k_pages.get_device()
-    _require_table(block_tables, index)
-    R, max_blocks = block_tables.shape
+    pool, _, _ = _page_pool(k_pages, v_pages, index, k_pages.dtype)
+    R, max_blocks, tstride = _table(block_tables, index)
     pshape, pstride = path.shape, path.stride()
     if len(pshape) != 2 or pshape[0] != R or path.dtype is not torch.int32 or \
             path.get_device() != index or (pshape[1] > 1 and pstride[1] != 1):
@@ -764,8 +779,8 @@ def commit_tree_path(k_pages: torch.Tensor, v_pages: torch.Tensor, block_tables:
             context_lens.numel() == R and path_lens.numel() == R and
             context_lens.is_contiguous() and path_lens.is_contiguous()):
         _int32s(index, {"context_lens": (context_lens, R), "path_lens": (path_lens, R)})
-    rc = _call(L.lib().halo_commit_tree_path, index, ctypes.byref(pool), block_tables.data_ptr(),
-               block_tables.stride(0), max_blocks, R, context_lens.data_ptr(), path.data_ptr(),
+    rc = _call(L.lib().halo_commit_tree_path, index, pool, block_tables.data_ptr(), tstride,
+               max_blocks, R, context_lens.data_ptr(), path.data_ptr(),
                pstride[0], pshape[1], path_lens.data_ptr())
     if rc:
         L.check(rc, "halo_commit_tree_path")

@@ -163,3 +163,14 @@ def test_oracle_commit_reads_before_it_writes():
     v = -k.clone()
     O.commit_tree_path(k, v, [[0]], [2], [[0, 2, 3]], [3])
     assert k.flatten().tolist() == [0, 1, 2, 4, 5, 5, 6, 7] and torch.equal(v, -k)
+
+
+def test_packed_descriptions_match_the_structures():
+    from halo_b200 import _lib as L
+    po, pr = _pool(L), _tree(L)
+    fields = lambda x: [getattr(x, n) or 0 for n, _ in x._fields_]      # noqa: E731
+    assert L.pack_page_pool(*fields(po)) == bytes(po)
+    assert L.pack_tree_problem(*fields(pr)) == bytes(pr)
+    assert L.lib().halo_tree_workspace_bytes(L.pack_page_pool(*fields(po)),
+                                             L.pack_tree_problem(*fields(pr))) == \
+        L.lib().halo_tree_workspace_bytes(ctypes.byref(po), ctypes.byref(pr))
