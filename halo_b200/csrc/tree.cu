@@ -109,12 +109,14 @@ struct FewGeom {
   static constexpr int kTileBytes = kBlocks * kBlockBytes;
   static constexpr int kQBytes = NR * D * 2;
   static constexpr int kPBytes = (NR == 64 ? 2 : 1) * kBlockBytes;
-  static constexpr int kStK = D == 64 ? (NR == 64 ? 5 : 6) : 3;
-  static constexpr int kStV = D == 64 ? (NR == 64 ? 5 : 6) : (NR == 64 ? 2 : 3);
+  // two buffers of P where a tile's bytes take less than P V and its waits
+  static constexpr int kPBuf = D == 64 && NR <= 32 ? 2 : 1;
+  static constexpr int kStK = D == 64 ? 5 : 3;
+  static constexpr int kStV = D == 64 ? 5 : (NR == 64 ? 2 : 3);
   static constexpr int kOffK = 0;
   static constexpr int kOffV = kStK * kTileBytes;
   static constexpr int kOffP = kOffV + kStV * kTileBytes;
-  static constexpr int kOffQ = kOffP + kPBytes;                // two buffers
+  static constexpr int kOffQ = kOffP + kPBuf * kPBytes;        // two buffers
   static constexpr int kOffRed = kOffQ + 2 * kQBytes;          // see FewShared
   static constexpr int kOffBar = kOffRed + 2048;
   static constexpr int kSmemBytes = kOffBar + 1024;
@@ -457,9 +459,12 @@ __device__ __forceinline__ void write_desc(const Params& p, const Bars* bs, int6
   p.desc[blockIdx.x] = d;
 }
 
-// Producer warp: the run's K and V tiles through the two rings.  SKIP: in
-// segments of at most 128 rows only one of the two streams reads a tile.
-template <int RG, class Gm, bool SKIP>
+// Producer warp: the run's tiles through a ring, K's (KIND 1), V's (KIND 2)
+// or both (KIND 3).  A warp for each where tiles are short: issuing one takes
+// 500 to 1000 clocks (8 boxes of 16 rows), as long as its bytes at 64 columns.
+// SKIP: in segments of at most 128 rows only one of the two streams reads a
+// tile.
+template <int RG, class Gm, bool SKIP, int KIND>
 __device__ __forceinline__ void produce(const Params& p, Bars* bs, unsigned char* smem,
                                         Walk<RG>& walk) {
   constexpr int SK = Gm::kStK, SV = Gm::kStV;
@@ -468,49 +473,52 @@ __device__ __forceinline__ void produce(const Params& p, Bars* bs, unsigned char
   const int n_box = kBN / p.box, n_iss = n_box * Gm::kBlocks;   // at most 32
   const int blk = lane / n_box, bx = lane - blk * n_box;
   const uint32_t dst = blk * Gm::kBlockBytes + bx * p.box * 128;
+  const int step_page = kBN / p.page, step_row = kBN - step_page * p.page;
   int nk = 0, nv = 0;             // K and V tiles issued
   bool ok = true;
+  // one tile's boxes into a ring stage, after its previous use
+  auto issue = [&](int n, int st, uint64_t* full, uint64_t* empty, int off, const CUtensorMap* map,
+                   int row, int page, uint32_t absent) {
+    const int i = n % st;
+    if (n >= st) ok = __all_sync(0xffffffffu, wait_bar(&empty[i], (n / st - 1) & 1, bs, p.err));
+    if (!ok) return;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&full[i], Gm::kTileBytes);
+      if (absent) mbar_arrive_n(&empty[i], absent);
+    }
+    __syncwarp();
+    if (lane < n_iss)
+      tma_load_4d(smem + off + i * Gm::kTileBytes + dst, map, blk * 64, row, s.hk, page, &full[i]);
+  };
   while (ok && walk.next(p, s)) {
     const int32_t* tab = p.table + (int64_t)walk.r * p.table_stride;
     const uint32_t absent = SKIP && s.rows <= 128 ? 1u : 0u;   // streams that skip a tile
-    auto entry = [&](int t) {
-      const int pos = t * kBN + bx * p.box;
-      return lane < n_iss && t < s.t1 && pos < walk.q.end ? tab[pos / p.page] : -1;
-    };
-    int pg = entry(s.t0);
-    for (int t = s.t0; t < s.t1; ++t) {
-      const int pg_next = entry(t + 1);
-      const int pos = t * kBN + bx * p.box;
-      const int row = pos % p.page;
+    // this lane's box: position, table entry and row in the page
+    int pos = s.t0 * kBN + bx * p.box;
+    int idx = pos / p.page, row = pos - idx * p.page;
+    auto entry = [&]() { return lane < n_iss && pos < walk.q.end ? tab[idx] : -1; };
+    int pg = entry();
+    for (int t = s.t0; t < s.t1 && ok; ++t) {
       const int page = (uint32_t)pg < (uint32_t)p.n_pages ? pg : p.n_pages;   // outside: zeros
-      const int ik = nk % SK, iv = nv % SV;
-      if (nk >= SK)
-        ok = __all_sync(0xffffffffu,
-                        wait_bar(&bs->k_empty[ik], (nk / SK - 1) & 1, bs, p.err));
-      if (!ok) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&bs->k_full[ik], Gm::kTileBytes);
-        if (absent) mbar_arrive_n(&bs->k_empty[ik], absent);
+      const int this_row = row;
+      pos += kBN;
+      idx += step_page;
+      row += step_row;
+      if (row >= p.page) {
+        row -= p.page;
+        ++idx;
       }
-      __syncwarp();
-      if (lane < n_iss)
-        tma_load_4d(smem + Gm::kOffK + ik * Gm::kTileBytes + dst, &p.kmap, blk * 64, row, s.hk,
-                    page, &bs->k_full[ik]);
-      ++nk;
-      if (nv >= SV)
-        ok = __all_sync(0xffffffffu,
-                        wait_bar(&bs->v_empty[iv], (nv / SV - 1) & 1, bs, p.err));
-      if (!ok) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&bs->v_full[iv], Gm::kTileBytes);
-        if (absent) mbar_arrive_n(&bs->v_empty[iv], absent);
+      if (t + 1 < s.t1) pg = entry();      // the next tile's page, ahead of the waits
+      if (KIND & 1) {
+        issue(nk, SK, bs->k_full, bs->k_empty, Gm::kOffK, &p.kmap, this_row, page, absent);
+        if (!ok) break;
+        ++nk;
       }
-      __syncwarp();
-      if (lane < n_iss)
-        tma_load_4d(smem + Gm::kOffV + iv * Gm::kTileBytes + dst, &p.vmap, blk * 64, row, s.hk,
-                    page, &bs->v_full[iv]);
-      ++nv;
-      pg = pg_next;
+      if (KIND & 2) {
+        issue(nv, SV, bs->v_full, bs->v_empty, Gm::kOffV, &p.vmap, this_row, page, absent);
+        if (!ok) break;
+        ++nv;
+      }
     }
   }
   // every copy issued lands before the CTA can exit
@@ -530,9 +538,10 @@ __device__ __forceinline__ void produce(const Params& p, Bars* bs, unsigned char
 // context: rows behind the last node and elements that are not finite become
 // zero (a weight of zero would turn them into NaN).  bs->bad[segment] tells
 // whether a node's element was taken out; bad_sum gives it back.
-template <typename T, int D, int RG, class Gm>
+// `begin` runs at the start of every segment.
+template <typename T, int D, int RG, class Gm, class F>
 __device__ __forceinline__ void clean(const Params& p, Bars* bs, unsigned char* smem,
-                                      Walk<RG>& walk) {
+                                      Walk<RG>& walk, F begin) {
   constexpr int SV = Gm::kStV;
   const int lane = threadIdx.x & 31;
   Seg s;
@@ -542,6 +551,7 @@ __device__ __forceinline__ void clean(const Params& p, Bars* bs, unsigned char* 
   while (ok && walk.next(p, s)) {
     if (lane == 0) bad[si % kBadSlots] = 0;
     __syncwarp();
+    if (!(ok = begin())) break;
     for (int t = s.t0; t < s.t1; ++t, ++g) {
       const int iv = g % SV;
       ok = __all_sync(0xffffffffu, wait_bar(&bs->v_full[iv], (g / SV) & 1, bs, p.err));
@@ -695,7 +705,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     Walk<RG> walk(p, bs->r0, bs->req0, bs->base0, u0, u1);
     Seg s;
     if (warp == 0) {
-      produce<RG, Gm, true>(p, bs, smem, walk);
+      produce<RG, Gm, true, 3>(p, bs, smem, walk);
     } else if (warp & 1) {
       // -------------------------------------------------------- MMA issuer X
       if (lane == 0) {
@@ -768,7 +778,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         mbar_wait(&bs->mma_done[x], 0, p.err);
       }
     } else {
-      clean<T, D, RG, Gm>(p, bs, smem, walk);
+      clean<T, D, RG, Gm>(p, bs, smem, walk, [] { return true; });
     }
   } else {
     umma::regs_inc<104>();
@@ -1037,11 +1047,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
 // ======================================================================
 // tree_few_kernel: groups of at most 64 rows (NR = 16, 32 or 64).  One CTA an
 // SM, 384 threads.
-//   warp 0      TMA producer (as in tree_kernel)
+//   warps 0, 3  TMA producers of K and V (as in tree_kernel)
 //   warp 1      TMEM owner; lane 0 issues every MMA
-//   warp 2      cleans V
-//   warp 3      query rows of the next segment (two buffers; the first
-//               segment's are loaded by the softmax warps)
+//   warp 2      cleans V; query rows of the next segment (two buffers; the
+//               first segment's are loaded by the softmax warps)
 //   warps 4-11  softmax (thread = position of the tile) and epilogue (thread =
 //               output column), warps 4-7 the first NR / 2 rows, warps 8-11 the
 //               others
@@ -1084,7 +1093,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
   using Gm = FewGeom<D, NR>;
   constexpr int RG = NR;
   constexpr bool kBf16 = Elem<T>::kDtype == HALO_DTYPE_BF16;
-  constexpr int SK = Gm::kStK, SV = Gm::kStV;
+  constexpr int SK = Gm::kStK, SV = Gm::kStV, PB = Gm::kPBuf;
   constexpr uint32_t kCols = 4 * NR;             // TMEM: S twice, O
   extern __shared__ __align__(1024) unsigned char smem[];
   Bars* bs = reinterpret_cast<Bars*>(smem + Gm::kOffBar);
@@ -1106,6 +1115,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
     }
     mbar_init(&bs->p_full[0], 8);
     mbar_init(&bs->pv_done[0], 1);
+    mbar_init(&bs->pv_done[1], 1);
     mbar_init(&bs->mma_done[0], 1);
     bs->abort_flag = 0;
     fence_mbar_init();
@@ -1139,9 +1149,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
     Seg s;
     // Segment si's query rows by threads 0 .. nt - 1: 16-byte copies, all in
     // flight.
-    auto copy_q = [&](int t, int nt, int si) {
+    auto copy_q = [&](const Walk<RG>& w, const Seg& s, int t, int nt, int si) {
       constexpr int VPR = D / 8;
-      const char* qb = p.q + 2 * (walk.q.cu0 * p.q_st + (int64_t)s.hk * p.G * p.q_sh);
+      const char* qb = p.q + 2 * (w.q.cu0 * p.q_st + (int64_t)s.hk * p.G * p.q_sh);
       const uint32_t dst = sQ + (si & 1) * Gm::kQBytes;
 #pragma unroll 1
       for (int i = t; i < NR * VPR; i += nt) {
@@ -1154,7 +1164,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
       }
     };
     if (warp == 0) {
-      produce<RG, Gm, false>(p, bs, smem, walk);
+      produce<RG, Gm, false, 1>(p, bs, smem, walk);
     } else if (warp == 1) {
       // -------------------------------------------------------- MMA issuer
       if (lane == 0) {
@@ -1198,12 +1208,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
             if (!ok) break;
             umma::fence_after_sync();
             const uint64_t vd = opaque(vdesc0 + (uint64_t)((iv * Gm::kTileBytes) >> 4));
-            const uint64_t pd = opaque(pdesc0);
+            const uint64_t pd = opaque(pdesc0 + (uint64_t)(((g % PB) * Gm::kPBytes) >> 4));
 #pragma unroll
             for (int kk = 0; kk < kBN / 16; ++kk)    // O^T += V(g)^T P^T
               umma::mma_ss(tmem + Gm::kColO, vd + (uint64_t)((kk * 16 * 128) >> 4),
                            pd + (uint64_t)((kk * 16 * 128) >> 4), kIdPV, it > 0 || kk > 0);
-            umma::commit(&bs->pv_done[0]);
+            umma::commit(&bs->pv_done[g % PB]);
             umma::commit(&bs->v_empty[iv]);
           }
           ++si;
@@ -1212,24 +1222,29 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
         mbar_wait(&bs->mma_done[0], 0, p.err);
       }
     } else if (warp == 2) {
-      clean<T, D, RG, Gm>(p, bs, smem, walk);
-    } else if (warp == 3) {
-      // -------------------------------------------------------- query rows
-      // (the first segment's are the softmax warps')
-      int si = 1;
-      bool ok = walk.next(p, s);
-      while (ok && walk.next(p, s)) {
-        if (si >= 2)
-          ok = __all_sync(0xffffffffu,
-                          wait_bar(&bs->q_empty[si & 1], ((si >> 1) - 1) & 1, bs, p.err));
-        if (!ok) break;
-        copy_q(lane, 32, si);
+      // cleans V, and before a segment's first tile loads the next segment's
+      // query rows (the first segment's are the softmax warps'): their buffer
+      // was read by products that need nothing more from this warp
+      Walk<RG> ahead = walk;
+      Seg sa;
+      bool more = ahead.next(p, sa);
+      int sq = 0;
+      clean<T, D, RG, Gm>(p, bs, smem, walk, [&]() {
+        more = more && ahead.next(p, sa);
+        ++sq;
+        if (!more) return true;
+        if (sq >= 2 && !__all_sync(0xffffffffu, wait_bar(&bs->q_empty[sq & 1],
+                                                         ((sq >> 1) - 1) & 1, bs, p.err)))
+          return false;
+        copy_q(ahead, sa, lane, 32, sq);
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bs->q_full[si & 1]);
-        ++si;
-      }
+        if (lane == 0) mbar_arrive(&bs->q_full[sq & 1]);
+        return true;
+      });
+    } else if (warp == 3) {
+      produce<RG, Gm, false, 2>(p, bs, smem, walk);
     } else {
       // -------------------------------------------------------- softmax
       // two groups of four warps, each RT of the NR rows; thread = position
@@ -1239,10 +1254,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
       const uint32_t trow = tmem + ((uint32_t)(sub * 32) << 16);
       int g = 0, si = 0;
       bool ok = true;
+      auto pv_waited = [&](int t) {        // P V of tile t is done
+        return __all_sync(0xffffffffu, wait_bar(&bs->pv_done[t % PB], (t / PB) & 1, bs, p.err));
+      };
       while (walk.next(p, s)) {
         const int ctx = walk.q.ctx, end = walk.q.end;
         if (si == 0) {                     // later ones come from warp 3, ahead
-          copy_q(threadIdx.x - 128, 256, 0);
+          copy_q(walk, s, threadIdx.x - 128, 256, 0);
           asm volatile("cp.async.wait_all;" ::: "memory");
           fence_proxy_async_smem();
           named_bar_sync(3, 256);
@@ -1333,8 +1351,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
             named_bar_sync(bar, 128);
             if (t > s.t0) {
               // O^T: every PV issued so far has to be done
-              ok = ok && __all_sync(0xffffffffu,
-                                    wait_bar(&bs->pv_done[0], (g - 1) & 1, bs, p.err));
+              ok = ok && pv_waited(g - 1);
               umma::fence_after_sync();
               float fac[RT];
 #pragma unroll
@@ -1375,11 +1392,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
             }
             lo[r / 2] = Elem<T>::pack(a - ah, b - bh);
           }
-          // P's buffer is free once the last PV is done
-          if (g > 0)
-            ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->pv_done[0], (g - 1) & 1, bs, p.err));
+          // P's buffer is free once the PV that read it is done
+          if (g >= PB) ok = ok && pv_waited(g - PB);
           // row `position` of P^T: NR values, NR remainders
-          unsigned char* pr = smem + Gm::kOffP + tid * 128;
+          unsigned char* pr = smem + Gm::kOffP + (g % PB) * Gm::kPBytes + tid * 128;
           const int sw = tid & 7, c0 = grp * (RT / 8);
 #pragma unroll
           for (int c = 0; c < RT / 8; ++c) {
@@ -1397,7 +1413,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
         }
 
         // ---- epilogue; barriers are passed whether or not a wait failed
-        ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->pv_done[0], (g - 1) & 1, bs, p.err));
+        ok = ok && pv_waited(g - 1);
         umma::fence_after_sync();
         warp_columns<RT>(l, [](float a, float b) { return a + b; });
         if (lane < RT) sh->red[sub][r0 + lane] = l[0];
