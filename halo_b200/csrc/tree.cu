@@ -143,7 +143,7 @@ struct Req {
 struct Bars {
   uint64_t q_full[2], q_empty[2];
   uint64_t k_full[6], k_empty[6], v_full[6], v_ready[6], v_empty[6];
-  uint64_t s_full[2], p_full[4], pv_done[2], mma_done[2], turn[2];
+  uint64_t s_full[2], s_free[2], p_full[4], pv_done[2], mma_done[2], turn[2];
   int64_t scan[20];
   int64_t base0, total;
   uint32_t tmem_base;
@@ -1047,8 +1047,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
 // ======================================================================
 // tree_few_kernel: groups of at most 64 rows (NR = 16, 32 or 64).  One CTA an
 // SM, 384 threads.
-//   warps 0, 3  TMA producers of K and V (as in tree_kernel)
-//   warp 1      TMEM owner; lane 0 issues every MMA
+//   warp 0      TMA producer (as in tree_kernel)
+//   warps 1, 3  lane 0 issues the QK / PV MMAs (one thread for both took 1950
+//               clocks a tile, most of them in commits); warp 1 owns TMEM
 //   warp 2      cleans V; query rows of the next segment (two buffers; the
 //               first segment's are loaded by the softmax warps)
 //   warps 4-11  softmax (thread = position of the tile) and epilogue (thread =
@@ -1105,6 +1106,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
       mbar_init(&bs->q_full[i], 1);
       mbar_init(&bs->q_empty[i], 1);
       mbar_init(&bs->s_full[i], 1);
+      mbar_init(&bs->s_free[i], 8);
     }
     for (int i = 0; i < 6; ++i) {
       mbar_init(&bs->k_full[i], 1);
@@ -1114,9 +1116,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
       mbar_init(&bs->v_empty[i], 1);
     }
     mbar_init(&bs->p_full[0], 8);
+    mbar_init(&bs->p_full[1], 8);
     mbar_init(&bs->pv_done[0], 1);
     mbar_init(&bs->pv_done[1], 1);
     mbar_init(&bs->mma_done[0], 1);
+    mbar_init(&bs->mma_done[1], 1);
     bs->abort_flag = 0;
     fence_mbar_init();
     prefetch_map(&p.kmap);
@@ -1164,62 +1168,70 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
       }
     };
     if (warp == 0) {
-      produce<RG, Gm, false, 1>(p, bs, smem, walk);
+      produce<RG, Gm, false, 3>(p, bs, smem, walk);
     } else if (warp == 1) {
-      // -------------------------------------------------------- MMA issuer
+      // -------------------------------------------------------- QK issuer
       if (lane == 0) {
         constexpr uint32_t kIdQK = umma::instr_desc_f16(kBN, NR, kBf16, false, false);
-        constexpr uint32_t kIdPV = umma::instr_desc_f16(128, 2 * NR, kBf16, true, true);
         const uint64_t kdesc0 = umma::smem_desc_sw128(sK, 16, 1024);
-        // V^T has 128 rows; 64 columns of V fill them twice (the same block
-        // again), and the second half of O^T is not read
-        const uint64_t vdesc0 =
-            umma::smem_desc_sw128(sV, D == 64 ? 0 : Gm::kBlockBytes, 1024);
-        const uint64_t pdesc0 = umma::smem_desc_sw128(sP, Gm::kBlockBytes, 1024);
         int g = 0, si = 0;                  // tiles; segments
         bool ok = true;
         while (ok && walk.next(p, s)) {
-          const int n = s.t1 - s.t0;
           const uint64_t qd0 = umma::smem_desc_sw128(sQ + (si & 1) * Gm::kQBytes, 16, 1024);
-          auto qk = [&](int t, bool last) {          // S^T = K(t) Q^T
-            const int ik = t % SK;
-            if (!wait_bar(&bs->k_full[ik], (t / SK) & 1, bs, p.err)) return false;
+          ok = wait_bar(&bs->q_full[si & 1], (si >> 1) & 1, bs, p.err);
+          for (int t = s.t0; ok && t < s.t1; ++t, ++g) {   // S^T = K(g) Q^T
+            const int ik = g % SK;
+            ok = wait_bar(&bs->k_full[ik], (g / SK) & 1, bs, p.err) &&
+                 (g < 2 || wait_bar(&bs->s_free[g & 1], ((g >> 1) - 1) & 1, bs, p.err));
+            if (!ok) break;
             umma::fence_after_sync();
             const uint64_t qd = opaque(qd0);
             const uint64_t kd = opaque(kdesc0 + (uint64_t)((ik * Gm::kTileBytes) >> 4));
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk)
-              umma::mma_ss(tmem + (t & 1) * NR,
+              umma::mma_ss(tmem + (g & 1) * NR,
                            kd + (uint64_t)(((kk >> 2) * Gm::kBlockBytes + (kk & 3) * 32) >> 4),
                            qd + (uint64_t)(((kk >> 2) * NR * 128 + (kk & 3) * 32) >> 4), kIdQK,
                            kk > 0);
-            umma::commit(&bs->s_full[t & 1]);
+            umma::commit(&bs->s_full[g & 1]);
             umma::commit(&bs->k_empty[ik]);
-            if (last) umma::commit(&bs->q_empty[si & 1]);
-            return true;
-          };
-          ok = wait_bar(&bs->q_full[si & 1], (si >> 1) & 1, bs, p.err) && qk(g, n == 1);
-          for (int it = 0; ok && it < n; ++it, ++g) {
-            // S(g + 1)'s buffer held S(g - 1), which P(g - 1) says was read
-            if (it + 1 < n && !(ok = qk(g + 1, it + 2 == n))) break;
+          }
+          umma::commit(&bs->q_empty[si & 1]);
+          ++si;
+        }
+        umma::commit(&bs->mma_done[0]);
+        mbar_wait(&bs->mma_done[0], 0, p.err);
+      }
+    } else if (warp == 3) {
+      // -------------------------------------------------------- PV issuer
+      if (lane == 0) {
+        constexpr uint32_t kIdPV = umma::instr_desc_f16(128, 2 * NR, kBf16, true, true);
+        // V^T has 128 rows; 64 columns of V fill them twice (the same block
+        // again), and the second half of O^T is not read
+        const uint64_t vdesc0 =
+            umma::smem_desc_sw128(sV, D == 64 ? 0 : Gm::kBlockBytes, 1024);
+        const uint64_t pdesc0 = umma::smem_desc_sw128(sP, Gm::kBlockBytes, 1024);
+        int g = 0;
+        bool ok = true;
+        while (ok && walk.next(p, s)) {
+          for (int t = s.t0; ok && t < s.t1; ++t, ++g) {   // O^T += V(g)^T P^T
             const int iv = g % SV;
-            ok = wait_bar(&bs->p_full[0], g & 1, bs, p.err) &&
-                 wait_bar(&bs->v_ready[iv], (g / SV) & 1, bs, p.err);
+            ok = wait_bar(&bs->v_ready[iv], (g / SV) & 1, bs, p.err) &&
+                 wait_bar(&bs->p_full[g % PB], (g / PB) & 1, bs, p.err);
             if (!ok) break;
             umma::fence_after_sync();
             const uint64_t vd = opaque(vdesc0 + (uint64_t)((iv * Gm::kTileBytes) >> 4));
             const uint64_t pd = opaque(pdesc0 + (uint64_t)(((g % PB) * Gm::kPBytes) >> 4));
 #pragma unroll
-            for (int kk = 0; kk < kBN / 16; ++kk)    // O^T += V(g)^T P^T
+            for (int kk = 0; kk < kBN / 16; ++kk)
               umma::mma_ss(tmem + Gm::kColO, vd + (uint64_t)((kk * 16 * 128) >> 4),
-                           pd + (uint64_t)((kk * 16 * 128) >> 4), kIdPV, it > 0 || kk > 0);
+                           pd + (uint64_t)((kk * 16 * 128) >> 4), kIdPV, t > s.t0 || kk > 0);
             umma::commit(&bs->pv_done[g % PB]);
             umma::commit(&bs->v_empty[iv]);
           }
-          ++si;
         }
-        umma::commit(&bs->mma_done[0]);
-        mbar_wait(&bs->mma_done[0], 0, p.err);
+        umma::commit(&bs->mma_done[1]);
+        mbar_wait(&bs->mma_done[1], 0, p.err);
       }
     } else if (warp == 2) {
       // cleans V, and before a segment's first tile loads the next segment's
@@ -1243,8 +1255,6 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
         if (lane == 0) mbar_arrive(&bs->q_full[sq & 1]);
         return true;
       });
-    } else if (warp == 3) {
-      produce<RG, Gm, false, 2>(p, bs, smem, walk);
     } else {
       // -------------------------------------------------------- softmax
       // two groups of four warps, each RT of the NR rows; thread = position
@@ -1375,6 +1385,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
             }
             rise = false;
           }
+          // the scores are in registers: S's buffer is free
+          umma::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bs->s_free[g & 1]);
           uint32_t hi[RT / 2], lo[RT / 2];
 #pragma unroll
           for (int r = 0; r < RT; r += 2) {
@@ -1409,7 +1423,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
           fence_proxy_async_smem();
           umma::fence_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bs->p_full[0]);
+          if (lane == 0) mbar_arrive(&bs->p_full[g % PB]);
         }
 
         // ---- epilogue; barriers are passed whether or not a wait failed
