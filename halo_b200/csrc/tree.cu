@@ -38,7 +38,6 @@ namespace tree {
 
 constexpr int kBN = 128;               // positions of a tile (a unit)
 constexpr int kThreads = 640;          // tree_kernel
-constexpr int kFewThreads = 384;       // tree_few_kernel
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.f;    // headroom of the running maximum
 constexpr int kBadSlots = 8;
@@ -104,6 +103,8 @@ struct Geom {
 // tree_few_kernel: NR (16, 32 or 64) query rows.
 template <int D, int NR>
 struct FewGeom {
+  // a warp more for V's copies where the registers of 64 rows leave room
+  static constexpr int kThreads = NR == 64 ? 384 : 416;
   static constexpr int kBlocks = D / 64;
   static constexpr int kBlockBytes = kBN * 128;
   static constexpr int kTileBytes = kBlocks * kBlockBytes;
@@ -469,7 +470,7 @@ __device__ __forceinline__ void produce(const Params& p, Bars* bs, unsigned char
                                         Walk<RG>& walk) {
   constexpr int SK = Gm::kStK, SV = Gm::kStV;
   const int lane = threadIdx.x & 31;
-  Seg s;
+  Seg s{};
   const int n_box = kBN / p.box, n_iss = n_box * Gm::kBlocks;   // at most 32
   const int blk = lane / n_box, bx = lane - blk * n_box;
   const uint32_t dst = blk * Gm::kBlockBytes + bx * p.box * 128;
@@ -1046,8 +1047,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
 
 // ======================================================================
 // tree_few_kernel: groups of at most 64 rows (NR = 16, 32 or 64).  One CTA an
-// SM, 384 threads.
-//   warp 0      TMA producer (as in tree_kernel)
+// SM, 384 threads (NR = 64) or 416.
+//   warp 0      TMA producer (as in tree_kernel); warp 12, if there, V's
 //   warps 1, 3  lane 0 issues the QK / PV MMAs (one thread for both took 1950
 //               clocks a tile, most of them in commits); warp 1 owns TMEM
 //   warp 2      cleans V; query rows of the next segment (two buffers; the
@@ -1090,7 +1091,7 @@ __device__ __forceinline__ void warp_columns(float (&v)[N], Op op) {
 }
 
 template <typename T, int D, int NR>
-__global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(FewGeom<D, NR>::kThreads, 1) tree_few_kernel(const __grid_constant__ Params p) {
   using Gm = FewGeom<D, NR>;
   constexpr int RG = NR;
   constexpr bool kBf16 = Elem<T>::kDtype == HALO_DTYPE_BF16;
@@ -1132,7 +1133,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
   }
   grid_dep_wait();                         // the caller's writes are visible
   int64_t u0, u1, U;
-  find_run<RG, kFewThreads>(p, bs, u0, u1, U);
+  find_run<RG, Gm::kThreads>(p, bs, u0, u1, U);
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
@@ -1168,7 +1169,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
       }
     };
     if (warp == 0) {
-      produce<RG, Gm, false, 3>(p, bs, smem, walk);
+      produce<RG, Gm, false, NR == 64 ? 3 : 1>(p, bs, smem, walk);
+    } else if (NR < 64 && warp == 12) {
+      produce<RG, Gm, false, 2>(p, bs, smem, walk);
     } else if (warp == 1) {
       // -------------------------------------------------------- QK issuer
       if (lane == 0) {
@@ -1738,7 +1741,7 @@ static int launch(const Params& p, int n_cta, cudaStream_t st) {
   if constexpr (RG <= 64) {
     kernel = tree_few_kernel<T, D, RG>;
     smem = FewGeom<D, RG>::kSmemBytes;
-    threads = kFewThreads;
+    threads = FewGeom<D, RG>::kThreads;
   } else {
     kernel = tree_kernel<T, D, RG / 128>;
     smem = Geom<D, RG / 128>::kSmemBytes;

@@ -442,6 +442,49 @@ def test_long_context_of_one_request(cuda_device):
     c.check(*c.run(out_dtype=torch.float32))
 
 
+@pytest.mark.parametrize("D,page", [(64, 8), (64, 48), (128, 16), (128, 256)])
+@pytest.mark.parametrize("nodes", [1, 3, 7, 20, 40, 70])
+def test_long_contexts_at_every_row_count(cuda_device, D, page, nodes):
+    """Hundreds of tiles a CTA: every ring, buffer and phase goes round many
+    times (G = 4: 4 to 280 rows a K/V head); a second run gives the same bits."""
+    dtype = torch.bfloat16 if page % 16 else torch.float16
+    c = Case(nodes + D, [18000, 9001], [nodes, max(1, nodes // 3)], 4, 1, D, page, dtype)
+    q, k, v, t = c.q.to(DEV), c.k.to(DEV), c.v.to(DEV), _i32(c.table)
+    from halo_b200 import ops
+    args = (q, k, v, t, _i32(c.ctx), _i32(c.cu), c.mask.to(DEV))
+    out, lse = ops.tree_attention(*args, out_dtype=torch.float32)
+    c.check(out, lse)
+    again, lse2 = ops.tree_attention(*args, out_dtype=torch.float32)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+def test_calls_from_two_threads_and_streams(cuda_device):
+    """Each thread's calls have a workspace of their own."""
+    import threading
+    from halo_b200 import ops
+    cases = [Case(80 + i, [3000, 700], [5 + 20 * i, 3], 8, 2, 64, 16, torch.bfloat16)
+             for i in range(2)]
+    args = [(c.q.to(DEV), c.k.to(DEV), c.v.to(DEV), _i32(c.table), _i32(c.ctx), _i32(c.cu),
+             c.mask.to(DEV)) for c in cases]
+    want = [ops.tree_attention(*a, out_dtype=torch.float32) for a in args]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i, stream):
+        with torch.cuda.stream(stream):
+            for _ in range(50):
+                o, l = ops.tree_attention(*args[i], out_dtype=torch.float32)
+                if not (torch.equal(o, want[i][0]) and torch.equal(l, want[i][1])):
+                    wrong.append(i)
+    for streams in ([torch.cuda.Stream(), torch.cuda.Stream()], [torch.cuda.current_stream()] * 2):
+        ts = [threading.Thread(target=work, args=(i, s)) for i, s in enumerate(streams)]
+        for t in ts:
+            t.start()
+        for t in ts:
+            t.join()
+    assert not wrong
+
+
 # ------------------------------------------------------------ together
 
 def _dense(q, k, v, seen):
