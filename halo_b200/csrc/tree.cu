@@ -552,7 +552,8 @@ __device__ __forceinline__ void clean(const Params& p, Bars* bs, unsigned char* 
   while (ok && walk.next(p, s)) {
     if (lane == 0) bad[si % kBadSlots] = 0;
     __syncwarp();
-    if (!(ok = begin())) break;
+    ok = begin();
+    if (!ok) break;
     for (int t = s.t0; t < s.t1; ++t, ++g) {
       const int iv = g % SV;
       ok = __all_sync(0xffffffffu, wait_bar(&bs->v_full[iv], (g / SV) & 1, bs, p.err));
@@ -824,6 +825,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       const int ny = x ? (two ? n : (n + 1) / 2) : n1;   // of the other stream
       const int rowx = s.row0 + (two ? x * 128 : 0);     // request row of lane 0
       const int rows = min(s.row0 + s.rows - rowx, 128);
+      const int node = (rowx + r) / p.G;                 // of this thread's row
       float m = kNoMax, l = 0.f;
       for (int it = 0; it < nx; ++it, ++j) {
         const int p0 = (s.t0 + (two ? 0 : x) + it * step) * kBN + h * 64;
@@ -831,23 +833,39 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         const bool full = p0 + 64 <= ctx;
         uint32_t vis[2];
         if (!full) {
+          // a lane a position: positions of the context, and of the nodes
+          bool context[2], drafted[2];
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
-            const int b = p0 + 32 * w;
-            vis[w] = b + 32 <= ctx ? 0xffffffffu : 0u;
-            if (b + 32 > ctx && b < end) {
-              // one mask row at a time, a lane a position
-              const int jn = b + lane - ctx;
-              const bool node_ok = jn >= 0 && b + lane < end;
-              const uint8_t* mp = p.mask + (int64_t)cu0 * p.mask_stride + jn;
-#pragma unroll 8
-              for (int i = 0; i < 32; ++i) {
-                const int node = (rowx + sub * 32 + i) / p.G;
-                const bool v = jn < 0 || (node_ok && node < nodes &&
-                                          mp[(int64_t)node * p.mask_stride] != 0);
-                const uint32_t bits = __ballot_sync(0xffffffffu, v);
-                if (lane == i) vis[w] = bits;
+            const int pos = p0 + 32 * w + lane;
+            context[w] = pos < ctx;
+            drafted[w] = pos >= ctx && pos < end;
+            vis[w] = __ballot_sync(0xffffffffu, context[w]);
+          }
+          if (__any_sync(0xffffffffu, drafted[0] || drafted[1])) {
+            // the warp's rows are those of a few consecutive nodes: one mask
+            // row at a time, eight in flight
+            const int n0 = __shfl_sync(0xffffffffu, node, 0);
+            const int n1 = min(__shfl_sync(0xffffffffu, node, 31) + 1, nodes);
+            const uint8_t* mp = p.mask + (int64_t)(cu0 + n0) * p.mask_stride + (p0 + lane - ctx);
+#pragma unroll 1
+            for (int k = n0; k < n1; k += 8) {
+              uint8_t b[8][2];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+                  b[e][w] = drafted[w] && k + e < n1 ? mp[e * p.mask_stride + 32 * w] : 0;
               }
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                  const uint32_t bits = __ballot_sync(0xffffffffu, b[e][w] != 0);
+                  if (node == k + e) vis[w] |= bits;
+                }
+              }
+              mp += 8 * p.mask_stride;
             }
           }
         }
