@@ -21,7 +21,6 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
-
 #include <mutex>
 #include <type_traits>
 
@@ -645,6 +644,17 @@ __device__ __noinline__ float bad_sum(const Params& p, int r, int t, int ctx, in
 // Row groups of more than 128 rows (QT = 2): stream X takes query tile X and
 // both take every K/V tile.  Smaller ones: both streams share the query tile
 // and take every second K/V tile; the two are joined at the end of a segment.
+//
+// What bounds it: the chain of a tile (scores 0.6k clocks, weights 2.2k, PV and
+// the next QK 1.8k of queueing behind the other stream's, waits 0.8k) repeats
+// every 5.4k clocks a stream, the tensor pipe is busy 47 % of the time (its 48
+// MMAs take 3.1k) and the exponentials without the chain would fit into 2.0k.
+// 4 requests of 64 nodes on 65535 positions, 32 / 8 heads of 128, bf16: 450 us,
+// 611 TFLOP/s of the two products (917 with the remainders').  Steps, in us
+// there: 8 softmax warps polling issuer 583; 16 warps 552; turns 479; PV from
+// half of P 468; turn passed on halfway 453.  Tried: dropping the remainders
+// 380, but one bf16 P is 2^-9 off; exponentials taken out altogether 468: they
+// are not the limit; spinning instead of suspended waits 474.
 template <typename T, int D, int QT>
 __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ Params p) {
   using Gm = Geom<D, QT>;
@@ -1090,6 +1100,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
 // The row maximum lies across threads here, but it moves only past its
 // headroom of 2^8, so a tile costs one barrier with a vote; the reduction runs
 // in a segment's first tile and in the rare tile that raises it.
+//
+// What it reaches: 1M positions, 64 / 8 heads of 128, 4 nodes (4.3 GB): 616 to
+// 681 us by the clock that the power limit leaves, 6.3 to 7.0 TB/s (a plain copy
+// 6.5); with rows on the 128-row side 899.  8 requests of 16 nodes on 32768
+// positions (1.08 GB): 217 to 232 us, 4.6 to 5.0 TB/s: 192 us for the tiles of an
+// SM, 4 before the first, 3 for an epilogue, 4 for a second segment, 4 for the
+// merge and the launch.  One softmax group of all rows: 248; parts in rows of
+// 528 bytes: 225.  At 64 columns a tile's bytes take 1.4k clocks and its
+// softmax 1.55k: 1.3 times the bytes' time.  Small batches are latency: 10 us
+// for one token on 1000 positions (find the run 1.1, first rows and tables 1.5,
+// first tile 1.5, softmax and PV 1.9, epilogue 1.1, merge 3).
+
 // Sum or maximum over the warp of N (8, 16 or 32) columns, one a row: lane i
 // ends with row i % N in v[0].
 template <int N, class Op>
@@ -1532,9 +1554,11 @@ __global__ void __launch_bounds__(FewGeom<D, NR>::kThreads, 1) tree_few_kernel(c
 // ======================================================================
 // tree_merge_kernel: joins the parts of segments that were cut.  Block
 // (c - 1, y) looks at the cut between CTAs c - 1 and c; the first cut inside
-// a segment owns it, y takes 8 of its rows, a warp each.  Latency-bound: the
-// lanes find the CTAs that hold a part side by side.
+// a segment owns it, and its blocks share the rows, a warp a row.
+// Latency-bound (about 3 us behind the attention kernel): the lanes find the
+// CTAs that hold a part side by side; dividing for every cut took 8 us.
 constexpr int kMergeWarps = 8;
+constexpr int kMergeRowBlocks = 16;      // 8: 1 to 9 % slower with many rows, 32: empty blocks
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
@@ -1544,7 +1568,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
   grid_dep_trigger();                      // the next kernel may begin its set-up
   const int c = (int)blockIdx.x + 1;
   const Desc d = p.desc[c];
-  const int row = (int)blockIdx.y * kMergeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31;
+  int row = (int)blockIdx.y * kMergeWarps + (threadIdx.x >> 5);
   if (row >= d.rows) return;
   // the cut before CTA i, in tiles of this segment (a cut in its set-up units
   // or before it: 0); i U / n = i (U / n) + i (U mod n) / n
@@ -1555,76 +1580,78 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
   const int own = cut(c);
   if (own <= 0 || own >= d.nt || cut(c - 1) > 0) return;
   const int64_t before = (c - 1) * d.quot + (uint32_t)((c - 1) * d.rem) / (uint32_t)n_cta;
-  float M = -INFINITY, L = 0.f, acc[C];
+  for (; row < d.rows; row += (int)gridDim.y * kMergeWarps) {
+    float M = -INFINITY, L = 0.f, acc[C];
 #pragma unroll
-  for (int e = 0; e < C; ++e) acc[e] = 0.f;
-  for (int i0 = c - 1; i0 < n_cta && cut(i0) < d.nt; i0 += 32) {
-    const int a = cut(i0 + lane), b = cut(i0 + lane + 1);
-    uint32_t has = __ballot_sync(0xffffffffu, i0 + lane < n_cta && a < b);
-    while (has) {
-      constexpr int B = 4;
-      float2 ml[B];
-      float o[B][C];
+    for (int e = 0; e < C; ++e) acc[e] = 0.f;
+    for (int i0 = c - 1; i0 < n_cta && cut(i0) < d.nt; i0 += 32) {
+      const int a = cut(i0 + lane), b = cut(i0 + lane + 1);
+      uint32_t has = __ballot_sync(0xffffffffu, i0 + lane < n_cta && a < b);
+      while (has) {
+        constexpr int B = 4;
+        float2 ml[B];
+        float o[B][C];
 #pragma unroll
-      for (int u = 0; u < B; ++u) {
-        ml[u] = make_float2(-INFINITY, 0.f);
+        for (int u = 0; u < B; ++u) {
+          ml[u] = make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int e = 0; e < C; ++e) o[u][e] = 0.f;
-        if (has) {
-          const int i = i0 + __ffs(has) - 1;
-          has &= has - 1;
-          // CTA c - 1 may have begun before the segment's set-up units: then
-          // this is its second part
-          const int sl = i == c - 1 && before < d.start - (RG <= 64 ? kSetup<64> : kSetup<128>) ? 1 : 0;
-          const float* s = p.part + ((int64_t)i * 2 + sl) * part_floats<D>(RG);
-          ml[u] = *reinterpret_cast<const float2*>(s + RG * D + 2 * row);
-          s += row * D;
-          if constexpr (C == 4) {
-            const float4 y = *reinterpret_cast<const float4*>(s + lane * 4);
-            o[u][0] = y.x;
-            o[u][1] = y.y;
-            o[u][2] = y.z;
-            o[u][3] = y.w;
-          } else {
-            const float2 y = *reinterpret_cast<const float2*>(s + lane * 2);
-            o[u][0] = y.x;
-            o[u][1] = y.y;
+          for (int e = 0; e < C; ++e) o[u][e] = 0.f;
+          if (has) {
+            const int i = i0 + __ffs(has) - 1;
+            has &= has - 1;
+            // CTA c - 1 may have begun before the segment's set-up units: then
+            // this is its second part
+            const int sl = i == c - 1 && before < d.start - (RG <= 64 ? kSetup<64> : kSetup<128>) ? 1 : 0;
+            const float* s = p.part + ((int64_t)i * 2 + sl) * part_floats<D>(RG);
+            ml[u] = *reinterpret_cast<const float2*>(s + RG * D + 2 * row);
+            s += row * D;
+            if constexpr (C == 4) {
+              const float4 y = *reinterpret_cast<const float4*>(s + lane * 4);
+              o[u][0] = y.x;
+              o[u][1] = y.y;
+              o[u][2] = y.z;
+              o[u][3] = y.w;
+            } else {
+              const float2 y = *reinterpret_cast<const float2*>(s + lane * 2);
+              o[u][0] = y.x;
+              o[u][1] = y.y;
+            }
           }
         }
+        float Mn = M;
+#pragma unroll
+        for (int u = 0; u < B; ++u) Mn = fmaxf(Mn, ml[u].x);
+        // a part that saw only NaN has m = -inf and l = NaN: weight 1 keeps it
+        const float a0 = (M == -INFINITY) ? (L == L ? 0.f : 1.f) : ex2(M - Mn);
+        L *= a0;
+#pragma unroll
+        for (int e = 0; e < C; ++e) acc[e] *= a0;
+#pragma unroll
+        for (int u = 0; u < B; ++u) {
+          const float w = (ml[u].x == -INFINITY) ? (ml[u].y == ml[u].y ? 0.f : 1.f)
+                                                 : ex2(ml[u].x - Mn);
+          L = fmaf(ml[u].y, w, L);
+#pragma unroll
+          for (int e = 0; e < C; ++e) acc[e] = fmaf(o[u][e], w, acc[e]);
+        }
+        M = Mn;
       }
-      float Mn = M;
-#pragma unroll
-      for (int u = 0; u < B; ++u) Mn = fmaxf(Mn, ml[u].x);
-      // a part that saw only NaN has m = -inf and l = NaN: weight 1 keeps it
-      const float a0 = (M == -INFINITY) ? (L == L ? 0.f : 1.f) : ex2(M - Mn);
-      L *= a0;
-#pragma unroll
-      for (int e = 0; e < C; ++e) acc[e] *= a0;
-#pragma unroll
-      for (int u = 0; u < B; ++u) {
-        const float w = (ml[u].x == -INFINITY) ? (ml[u].y == ml[u].y ? 0.f : 1.f)
-                                               : ex2(ml[u].x - Mn);
-        L = fmaf(ml[u].y, w, L);
-#pragma unroll
-        for (int e = 0; e < C; ++e) acc[e] = fmaf(o[u][e], w, acc[e]);
-      }
-      M = Mn;
     }
-  }
-  const int rq = d.row0 + row, node = rq / p.G, hq = d.hk * p.G + rq - node * p.G;
-  const int64_t t = d.cu0 + node;
-  const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
-  if (lane == 0 && p.lse)
-    p.lse[t * p.H + hq] = L > 0.f ? (M + log2f(L)) * kLn2 : (L == L ? -INFINITY : L);
-  const int64_t at = t * p.out_st + hq * p.out_sh + lane * C;
-  if (p.out_f32) {
-    float* o = reinterpret_cast<float*>(p.out) + at;
+    const int rq = d.row0 + row, node = rq / p.G, hq = d.hk * p.G + rq - node * p.G;
+    const int64_t t = d.cu0 + node;
+    const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+    if (lane == 0 && p.lse)
+      p.lse[t * p.H + hq] = L > 0.f ? (M + log2f(L)) * kLn2 : (L == L ? -INFINITY : L);
+    const int64_t at = t * p.out_st + hq * p.out_sh + lane * C;
+    if (p.out_f32) {
+      float* o = reinterpret_cast<float*>(p.out) + at;
 #pragma unroll
-    for (int e = 0; e < C; ++e) o[e] = acc[e] * inv;
-  } else {
-    uint32_t* o = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + at);
+      for (int e = 0; e < C; ++e) o[e] = acc[e] * inv;
+    } else {
+      uint32_t* o = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + at);
 #pragma unroll
-    for (int e = 0; e < C; e += 2) o[e / 2] = Elem<T>::pack(acc[e] * inv, acc[e + 1] * inv);
+      for (int e = 0; e < C; e += 2) o[e / 2] = Elem<T>::pack(acc[e] * inv, acc[e + 1] * inv);
+    }
   }
 }
 
@@ -1782,7 +1809,7 @@ static int launch(const Params& p, int n_cta, cudaStream_t st) {
   count_launches();
   if (n_cta > 1) {
     e = launch_dependent(tree_merge_kernel<T, D>,
-                         dim3((unsigned)n_cta - 1, (RG + kMergeWarps - 1) / kMergeWarps),
+                         dim3((unsigned)n_cta - 1, std::min(RG / kMergeWarps, kMergeRowBlocks)),
                          dim3(kMergeWarps * 32), 0, st, p, n_cta, (int)RG);
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "tree_merge_kernel launch");
