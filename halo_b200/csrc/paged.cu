@@ -458,7 +458,8 @@ extern "C" int32_t halo_update_block_tables(int32_t* block_tables, int64_t table
   if (R < 0 || max_blocks < 0 || free_capacity < 0 || max_tokens < 0 || page_size <= 0)
     return fail(HALO_ERR_INVALID_ARG, "bad size (R=%d max_blocks=%d free=%d max_tokens=%d page_size=%d)",
                 R, max_blocks, free_capacity, max_tokens, page_size);
-  if (max_tokens > (1 << 30)) return fail(HALO_ERR_UNSUPPORTED, "%d tokens", max_tokens);
+  if (max_tokens > (1 << 30) || free_capacity > (1 << 30))
+    return fail(HALO_ERR_UNSUPPORTED, "%d tokens, %d pages", max_tokens, free_capacity);
   if (R > kTabMaxReq) return fail(HALO_ERR_UNSUPPORTED, "%d requests (at most %d)", R, kTabMaxReq);
   if ((int64_t)R * max_blocks > INT_MAX || ((int64_t)max_blocks + 1) * page_size > INT_MAX)
     return fail(HALO_ERR_UNSUPPORTED, "block tables of %d x %d pages of %d are too large", R,

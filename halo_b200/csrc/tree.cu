@@ -754,8 +754,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             umma::commit(&bs->s_full[x]);
             umma::commit(&bs->k_empty[ik]);
           };
+          // every segment is seen by both issuers, and its end waits for both:
+          // q_full cannot come round while one of them has yet to look
           ok = wait_bar(&bs->q_full[0], si & 1, bs, p.err);
-          if (ok && nx > 0 && (ok = k_landed(g))) {
+          if (nx == 0) umma::commit(&bs->pv_done[x]);
+          if (ok && nx > 0) ok = k_landed(g);
+          if (ok && nx > 0) {
             umma::fence_after_sync();
             qk(g);
           }
@@ -807,7 +811,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     const uint32_t scol = trow + x * 128 + h * 64;
     Walk<RG> walk(p, bs->r0, bs->req0, bs->base0, u0, u1);
     Seg s;
-    int j = 0, si = 0, s1 = 0;             // this stream's tiles; segments; those of stream 1
+    int j = 0, si = 0;                     // this stream's tiles; segments
     int turns = 0;                         // waited for
     bool ok = true;
     while (walk.next(p, s)) {
@@ -978,10 +982,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       // failed, so that no thread is left behind at one.  Both streams'
       // products are done before the query tile's space is scratch.
       ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->pv_done[0], si & 1, bs, p.err));
-      if (n1 > 0) {
-        ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->pv_done[1], s1 & 1, bs, p.err));
-        ++s1;
-      }
+      ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->pv_done[1], si & 1, bs, p.err));
       umma::fence_after_sync();
       float* sm_l = reinterpret_cast<float*>(smem + Gm::kOffQ);   // [stream][half][128]
       float* sm_m = sm_l + 512;                                   // [stream][128]
@@ -1839,15 +1840,19 @@ static int run(const halo_page_pool_t* pool, const halo_tree_problem_t* pb, void
     return fail(HALO_ERR_INVALID_ARG, "NULL pointer");
   if (pb->out_dtype != HALO_DTYPE_F32 && pb->out_dtype != pool->dtype)
     return fail(HALO_ERR_UNSUPPORTED, "out dtype must be fp32 or the pool's dtype");
-  if (!rows16(pool->k, pool->k_stride_p, pool->k_stride_h, pool->k_stride_t, 2) ||
-      !rows16(pool->v, pool->v_stride_p, pool->v_stride_h, pool->v_stride_t, 2) ||
+  // the stride of a dimension of one is never used
+  const bool many_p = pool->n_pages > 1, many_h = pool->H_kv > 1;
+  if (!rows16(pool->k, many_p ? pool->k_stride_p : 0, many_h ? pool->k_stride_h : 0,
+              pool->k_stride_t, 2) ||
+      !rows16(pool->v, many_p ? pool->v_stride_p : 0, many_h ? pool->v_stride_h : 0,
+              pool->v_stride_t, 2) ||
       pool->k_stride_t <= 0 || pool->v_stride_t <= 0 ||
-      (pool->H_kv > 1 && (pool->k_stride_h <= 0 || pool->v_stride_h <= 0)) ||
-      (pool->n_pages > 1 && (pool->k_stride_p <= 0 || pool->v_stride_p <= 0)))
+      (many_h && (pool->k_stride_h <= 0 || pool->v_stride_h <= 0)) ||
+      (many_p && (pool->k_stride_p <= 0 || pool->v_stride_p <= 0)))
     return fail(HALO_ERR_MISALIGNED, "page rows must be 16-byte aligned, strides positive");
-  if (!rows16(pb->q, pb->q_stride_t, pb->q_stride_h, 0, 2))
+  if (!rows16(pb->q, pb->T > 1 ? pb->q_stride_t : 0, pb->H > 1 ? pb->q_stride_h : 0, 0, 2))
     return fail(HALO_ERR_MISALIGNED, "q rows must be 16-byte aligned");
-  if (!rows16(pb->out, pb->out_stride_t, pb->out_stride_h, 0,
+  if (!rows16(pb->out, pb->T > 1 ? pb->out_stride_t : 0, pb->H > 1 ? pb->out_stride_h : 0, 0,
               pb->out_dtype == HALO_DTYPE_F32 ? 4 : 2))
     return fail(HALO_ERR_MISALIGNED, "out rows must be 16-byte aligned");
   const int64_t need = ws_bytes(pool, pb);

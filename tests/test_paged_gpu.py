@@ -289,11 +289,13 @@ def test_tree_attention_any_mask_and_rows_that_see_nothing(cuda_device):
 
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-@pytest.mark.parametrize("G", [2, 20])
-def test_hidden_rows_reach_no_output(cuda_device, bad, G):
+@pytest.mark.parametrize("G,D,dtype", [(2, 64, torch.bfloat16), (20, 64, torch.bfloat16),
+                                       (1, 128, torch.float16), (2, 128, torch.float16),
+                                       (4, 128, torch.bfloat16), (7, 128, torch.float16)])
+def test_hidden_rows_reach_no_output(cuda_device, bad, G, D, dtype):
     """A hidden node's K and V may hold anything; a node that sees it gets it."""
     n = 24
-    c = Case(3, [130, 0], [n, n], 2 * G, 2, 64, 16, torch.bfloat16)
+    c = Case(3, [130, 0], [n, n], 2 * G, 2, D, 16, dtype)
     c.mask[:, 5] = False
     c.mask[7, 5] = True                      # one row of request 0 sees node 5
     slots = [(c.table[0][(130 + 5) // 16], (130 + 5) % 16), (c.table[1][0], 5)]
