@@ -156,11 +156,11 @@ static_assert(sizeof(Bars) <= 1024, "barrier block");
 // Bounded wait that also ends when another role gave up.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Bars* bs,
                                          unsigned int* err) {
-  if (mbar_try_wait_hint(bar, parity, 1000)) return true;
+  if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
   while (true) {
     for (int i = 0; i < 8; ++i)
-      if (mbar_try_wait_hint(bar, parity, 1000)) return true;
+      if (mbar_try_wait(bar, parity)) return true;
     if (*reinterpret_cast<volatile int*>(&bs->abort_flag)) return false;
     if (globaltimer_ns() - t0 > kWaitLimitNs) {
       set_device_error(err, static_cast<unsigned int>(-HALO_ERR_TIMEOUT));
