@@ -1680,60 +1680,31 @@ static EncodeFn encode_fn() {
 }
 
 // The tensor map of a pool's K or V: {D, page, H_kv, n_pages}, boxes of 64
-// elements x `box` rows, 128-byte swizzle, zeros outside.  A map depends on
-// the description alone; the last ones made are kept.
-struct MapKey {
-  const void* ptr;
-  int64_t sp, sh, st;
-  int32_t n_pages, H_kv, page, D, dtype, box;
-};
-
-static int encode_pool(const MapKey& key, CUtensorMap* out) {
-  struct Slot {
-    MapKey key;
-    CUtensorMap map;
-    bool used;
-  };
-  constexpr int kSlots = 256;
-  static std::mutex mu;
-  static Slot cache[kSlots];
-  uint64_t h = reinterpret_cast<uint64_t>(key.ptr) >> 8;
-  for (uint64_t v : {(uint64_t)key.sp, (uint64_t)key.sh, (uint64_t)key.st, (uint64_t)key.n_pages,
-                     (uint64_t)key.page})
-    h = (h ^ v) * 0x9E3779B97F4A7C15ull;
-  Slot& s = cache[(h >> 32) % kSlots];
-  std::lock_guard<std::mutex> lk(mu);
-  const bool same = s.used && s.key.ptr == key.ptr && s.key.sp == key.sp && s.key.sh == key.sh &&
-                    s.key.st == key.st && s.key.n_pages == key.n_pages && s.key.H_kv == key.H_kv &&
-                    s.key.page == key.page && s.key.D == key.D && s.key.dtype == key.dtype &&
-                    s.key.box == key.box;
-  if (!same) {
-    EncodeFn fn = encode_fn();
-    if (!fn) return fail(HALO_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-    // the stride of a dimension of one is never used, but has to be legal
-    const int64_t st = key.st * 2;
-    const int64_t sh = key.H_kv > 1 ? key.sh * 2 : st;
-    const int64_t sp = key.n_pages > 1 ? key.sp * 2 : st;
-    cuuint64_t dims[4] = {(cuuint64_t)key.D, (cuuint64_t)key.page, (cuuint64_t)key.H_kv,
-                          (cuuint64_t)key.n_pages};
-    cuuint64_t str[3] = {(cuuint64_t)st, (cuuint64_t)sh, (cuuint64_t)sp};
-    cuuint32_t box[4] = {64, (cuuint32_t)key.box, 1, 1};
-    cuuint32_t estr[4] = {1, 1, 1, 1};
-    const CUresult r =
-        fn(&s.map, key.dtype == HALO_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-           4, const_cast<void*>(key.ptr), dims, str, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    s.used = r == CUDA_SUCCESS;
-    if (r != CUDA_SUCCESS)
-      return fail(HALO_ERR_INVALID_ARG,
-                  "page pool tensor map encode failed (%d): %d pages, page %d, strides %lld %lld "
-                  "%lld bytes", (int)r, key.n_pages, key.page, (long long)sp, (long long)sh,
-                  (long long)st);
-    s.key = key;
-  }
-  *out = s.map;
+// elements x `box` rows, 128-byte swizzle, zeros outside.
+static int encode_pool(const halo_page_pool_t* pool, const void* ptr, int64_t stride_p,
+                       int64_t stride_h, int64_t stride_t, int box, CUtensorMap* out) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return fail(HALO_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  // the stride of a dimension of one is never used, but has to be legal
+  const int64_t st = stride_t * 2;
+  const int64_t sh = pool->H_kv > 1 ? stride_h * 2 : st;
+  const int64_t sp = pool->n_pages > 1 ? stride_p * 2 : st;
+  cuuint64_t dims[4] = {(cuuint64_t)pool->D, (cuuint64_t)pool->page_size, (cuuint64_t)pool->H_kv,
+                        (cuuint64_t)pool->n_pages};
+  cuuint64_t str[3] = {(cuuint64_t)st, (cuuint64_t)sh, (cuuint64_t)sp};
+  cuuint32_t ext[4] = {64, (cuuint32_t)box, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r =
+      fn(out, pool->dtype == HALO_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+         4, const_cast<void*>(ptr), dims, str, ext, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(HALO_ERR_INVALID_ARG,
+                "page pool tensor map encode failed (%d): %d pages, page %d, strides %lld %lld "
+                "%lld bytes", (int)r, pool->n_pages, pool->page_size, (long long)sp, (long long)sh,
+                (long long)st);
   return HALO_OK;
 }
 
@@ -1865,11 +1836,11 @@ static int run(const halo_page_pool_t* pool, const halo_tree_problem_t* pb, void
   Params p{};
   p.box = 8;
   while (p.box < kBN && pool->page_size % (2 * p.box) == 0) p.box *= 2;
-  rc = encode_pool({pool->k, pool->k_stride_p, pool->k_stride_h, pool->k_stride_t, pool->n_pages,
-                    pool->H_kv, pool->page_size, pool->D, pool->dtype, p.box}, &p.kmap);
+  rc = encode_pool(pool, pool->k, pool->k_stride_p, pool->k_stride_h, pool->k_stride_t, p.box,
+                   &p.kmap);
   if (rc != HALO_OK) return rc;
-  rc = encode_pool({pool->v, pool->v_stride_p, pool->v_stride_h, pool->v_stride_t, pool->n_pages,
-                    pool->H_kv, pool->page_size, pool->D, pool->dtype, p.box}, &p.vmap);
+  rc = encode_pool(pool, pool->v, pool->v_stride_p, pool->v_stride_h, pool->v_stride_t, p.box,
+                   &p.vmap);
   if (rc != HALO_OK) return rc;
   p.q = static_cast<const char*>(pb->q);
   p.q_st = pb->q_stride_t;
