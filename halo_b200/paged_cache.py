@@ -72,12 +72,16 @@ class PagedKVCache:
 
     def accept(self, path: Optional[torch.Tensor], path_lens: torch.Tensor) -> None:
         """End the step: request ``r`` keeps the rows ``path[r, :path_lens[r]]``
-        of its step (``None``: its first ``path_lens[r]`` rows) and gives the
-        other pages back."""
+        of its step (``None``: its first ``path_lens[r]`` rows; never more than
+        the step gave it) and gives the other pages back."""
+        # no step of a path may reach behind held: table entries there name
+        # pages that another request may own by now
+        keep = torch.minimum(path_lens.clamp(0, None if path is None else path.shape[1]),
+                             self.held - self.lens)
         if path is not None:
             for k, v in zip(self.k, self.v):
-                ops.commit_tree_path(k, v, self.block_tables, self.lens, path, path_lens)
-        self._resize(torch.minimum(self.lens + path_lens.clamp(min=0), self.held))
+                ops.commit_tree_path(k, v, self.block_tables, self.lens, path, keep)
+        self._resize(self.lens + keep)
 
     def release(self, ended: torch.Tensor) -> None:
         """Empty the requests where ``ended (max_requests,)`` is true."""

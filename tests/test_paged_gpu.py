@@ -571,6 +571,69 @@ def test_tree_decoding_loop(cuda_device):
     assert cache.lens.tolist() == n
 
 
+def _small_cache(n_pages):
+    """Two requests of 10 and 6 rows on pages of 8, each row of K and V its
+    request's number."""
+    from halo_b200 import PagedKVCache
+    cache = PagedKVCache(1, n_pages, 1, 64, max_requests=2, max_len=64, page_size=8, device=DEV)
+    got = cache.extend(_i32([10, 6]), 16)
+    k = torch.ones(16, 1, 64, dtype=torch.bfloat16, device=DEV)
+    k[10:] = 2
+    cache.write(0, k, k, got)
+    cache.accept(None, _i32([10, 6]))
+    return cache
+
+
+def _rows_of(cache, r):
+    """The K rows of a request's context."""
+    n, page = int(cache.lens[r]), cache.page_size
+    pages = cache.block_tables[r, :-(-n // page)].long()
+    return cache.k[0][pages].transpose(1, 2).reshape(-1, *cache.k[0].shape[1::2])[:n, 0, 0].tolist()
+
+
+def _owners(cache):
+    page = cache.page_size
+    pages = [p for r, n in enumerate(cache.held.tolist())
+             for p in cache.block_tables[r, :-(-n // page)].tolist()]
+    return sorted(pages + cache.free_pages[:int(cache.n_free)].tolist())
+
+
+def test_accept_of_a_request_without_rows(cuda_device):
+    """A path given for a request that got no rows, or longer than its rows or
+    than the path tensor, keeps what there is and touches no other request."""
+    cache = _small_cache(4)
+    cache.accept(None, _i32([0, 0]))
+    cache.release(torch.tensor([True, False], device=DEV))       # its entries name old pages
+    got = cache.extend(_i32([0, 17]), 17)                        # 23 rows: these pages go to the other
+    cache.write(0, torch.full((17, 1, 64), 2., dtype=torch.bfloat16, device=DEV),
+                torch.full((17, 1, 64), 2., dtype=torch.bfloat16, device=DEV), got)
+    cache.accept(None, _i32([0, 17]))
+    got = cache.extend(_i32([12, 0]), 12)                        # 2 pages, 1 free
+    assert got.cu.tolist() == [0, 0, 0]
+    before = cache.k[0].clone()
+    before[:] = torch.arange(before.shape[0] * 8, device=DEV).view(-1, 1, 8, 1) % 250
+    cache.k[0].copy_(before)
+    cache.accept(_i32([[3, 9, 11], [0, 1, 2]]), _i32([3, 0]))
+    assert torch.equal(cache.k[0], before)
+    assert cache.lens.tolist() == [0, 23]
+    got = cache.extend(_i32([3, 0]), 3)
+    cache.accept(_i32([[1, 2], [0, 1]]), _i32([5, 0]))           # 3 rows, 2 steps
+    assert cache.lens.tolist() == [2, 23] and _owners(cache) == list(range(4))
+
+
+@pytest.mark.parametrize("n", [3, 40])
+def test_tree_attention_in_place(cuda_device, n):
+    """out may be q itself: a row is read by the CTA that writes it, or
+    written when all have been read."""
+    from halo_b200 import ops
+    c = Case(91, [5000, 130], [n, n], 8, 2, 128, 16, torch.bfloat16)
+    args = (c.k.to(DEV), c.v.to(DEV), _i32(c.table), _i32(c.ctx), _i32(c.cu), c.mask.to(DEV))
+    want, lse = ops.tree_attention(c.q.to(DEV), *args)
+    q = c.q.to(DEV)
+    out, lse2 = ops.tree_attention(q, *args, out=q)
+    assert out is q and torch.equal(out, want) and torch.equal(lse, lse2)
+
+
 # ------------------------------------------------------------ refusals
 
 def test_wrappers_refuse_what_does_not_fit(cuda_device):
