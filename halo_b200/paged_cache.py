@@ -55,7 +55,7 @@ class PagedKVCache:
         """Room for ``counts[r]`` (int32, at most ``max_tokens`` in all) rows
         behind each request's context."""
         slots, pos, cu, held = ops.update_block_tables(
-            self.block_tables, self.held, self.lens + counts, self.free_pages, self.n_free,
+            self.block_tables, self.held, self.lens + counts.clamp(min=0), self.free_pages, self.n_free,
             page_size=self.page_size, max_tokens=max_tokens)
         self.held.copy_(held)
         return PagedRows(slots, pos, cu)

@@ -621,6 +621,13 @@ def test_accept_of_a_request_without_rows(cuda_device):
     assert cache.lens.tolist() == [2, 23] and _owners(cache) == list(range(4))
 
 
+def test_extend_by_a_negative_count(cuda_device):
+    cache = _small_cache(8)
+    got = cache.extend(_i32([-9, 2]), 4)
+    assert got.cu.tolist() == [0, 0, 2] and cache.held.tolist() == [10, 8]
+    assert _owners(cache) == list(range(8)) and _rows_of(cache, 0) == [1.] * 10
+
+
 @pytest.mark.parametrize("n", [3, 40])
 def test_tree_attention_in_place(cuda_device, n):
     """out may be q itself: a row is read by the CTA that writes it, or
