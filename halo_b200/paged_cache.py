@@ -81,15 +81,17 @@ class PagedKVCache:
         if path is not None:
             for k, v in zip(self.k, self.v):
                 ops.commit_tree_path(k, v, self.block_tables, self.lens, path, keep)
-        self._resize(self.lens + keep)
+        self.lens.copy_(self._resize(self.lens + keep))
 
     def release(self, ended: torch.Tensor) -> None:
-        """Empty the requests where ``ended (max_requests,)`` is true."""
-        self._resize(torch.where(ended, torch.zeros_like(self.lens), self.lens))
+        """Empty the requests where ``ended (max_requests,)`` is true; others
+        keep their rows, those of a step under way too (an ended request's
+        rows of that step are nobody's: they may not be written any more)."""
+        self._resize(self.held.masked_fill(ended, 0))
+        self.lens.masked_fill_(ended, 0)
 
-    def _resize(self, lens: torch.Tensor) -> None:
+    def _resize(self, lens: torch.Tensor) -> torch.Tensor:
         _, _, _, held = ops.update_block_tables(
             self.block_tables, self.held, lens, self.free_pages, self.n_free,
             page_size=self.page_size, max_tokens=0)
-        self.held.copy_(held)
-        self.lens.copy_(held)
+        return self.held.copy_(held)

@@ -628,6 +628,19 @@ def test_extend_by_a_negative_count(cuda_device):
     assert _owners(cache) == list(range(8)) and _rows_of(cache, 0) == [1.] * 10
 
 
+def test_release_within_a_step(cuda_device):
+    """The other requests' rows of the step under way stay theirs."""
+    cache = _small_cache(8)
+    got = cache.extend(_i32([1, 5]), 6)
+    x = torch.full((6, 1, 64), 3., dtype=torch.bfloat16, device=DEV)
+    cache.release(torch.tensor([True, False], device=DEV))
+    assert cache.held.tolist() == [0, 11] and cache.lens.tolist() == [0, 6]
+    cache.write(0, x, x, got._replace(slots=torch.where(torch.arange(6, device=DEV) < 1, -1, got.slots)))
+    cache.accept(None, _i32([0, 5]))
+    assert cache.lens.tolist() == [0, 11] and _rows_of(cache, 1) == [2.] * 6 + [3.] * 5
+    assert _owners(cache) == list(range(8))
+
+
 @pytest.mark.parametrize("n", [3, 40])
 def test_tree_attention_in_place(cuda_device, n):
     """out may be q itself: a row is read by the CTA that writes it, or
