@@ -471,6 +471,9 @@ extern "C" int32_t halo_update_block_tables(int32_t* block_tables, int64_t table
   if (R > 1 && table_stride < max_blocks)
     return fail(HALO_ERR_INVALID_ARG, "block table rows overlap (stride %lld < %d)",
                 (long long)table_stride, max_blocks);
+  // several CTAs read the lengths, one writes them
+  if ((lens < old_lens + R && old_lens < lens + R) || (lens < new_lens + R && new_lens < lens + R))
+    return fail(HALO_ERR_INVALID_ARG, "lens overlaps the lengths it is made from");
   const size_t smem = (size_t)kTabArrays * R * sizeof(int32_t);
   static std::once_flag once[64];
   int dev = 0;
@@ -533,9 +536,9 @@ extern "C" int32_t halo_write_kv_pages(const halo_page_pool_t* pool, const void*
                            reinterpret_cast<uint64_t>(v) | (uint64_t)p.k_st | (uint64_t)p.k_sh |
                            (uint64_t)p.v_st | (uint64_t)p.v_sh | (uint64_t)row);
   p.vecs = row / vb;
-  if ((int64_t)2 * p.vecs * pool->H_kv * kWriteTok > INT_MAX)
+  if ((int64_t)2 * p.vecs * pool->H_kv * kWriteTok > INT_MAX / 2)
     return fail(HALO_ERR_UNSUPPORTED, "a token's rows are too large");
-  const unsigned grid = (unsigned)((T + kWriteTok - 1) / kWriteTok);
+  const unsigned grid = (unsigned)(((int64_t)T + kWriteTok - 1) / kWriteTok);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (vb == 16) write_kernel<uint4><<<grid, kWriteThreads, 0, st>>>(p);
   else if (vb == 8) write_kernel<uint2><<<grid, kWriteThreads, 0, st>>>(p);

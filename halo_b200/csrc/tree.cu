@@ -1826,6 +1826,9 @@ static int run(const halo_page_pool_t* pool, const halo_tree_problem_t* pb, void
   if (!rows16(pb->out, pb->T > 1 ? pb->out_stride_t : 0, pb->H > 1 ? pb->out_stride_h : 0, 0,
               pb->out_dtype == HALO_DTYPE_F32 ? 4 : 2))
     return fail(HALO_ERR_MISALIGNED, "out rows must be 16-byte aligned");
+  if ((pb->T > 1 && pb->out_stride_t < pool->D) || (pb->H > 1 && pb->out_stride_h < pool->D))
+    return fail(HALO_ERR_INVALID_ARG, "out rows overlap (strides %lld %lld)",
+                (long long)pb->out_stride_t, (long long)pb->out_stride_h);
   const int64_t need = ws_bytes(pool, pb);
   if (!workspace || workspace_bytes < need)
     return fail(HALO_ERR_WORKSPACE, "tree workspace has %lld bytes, needs %lld",

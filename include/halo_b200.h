@@ -450,7 +450,8 @@ typedef struct halo_page_pool {
  * free_pages are left as they were.  The new rows of all requests, packed in
  * request order (cu_tokens (R + 1): their running count), get their slot
  * and position in slots / positions (max_tokens); entries without a row get
- * -1, and rows beyond max_tokens no entry.  R <= 8192. */
+ * -1, and rows beyond max_tokens no entry.  lens overlaps neither old_lens
+ * nor new_lens.  R <= 8192. */
 int32_t halo_update_block_tables(int32_t* block_tables, int64_t table_stride, int32_t R,
                                  int32_t max_blocks, const int32_t* old_lens,
                                  const int32_t* new_lens, int32_t* free_pages,
@@ -492,7 +493,7 @@ typedef struct halo_tree_problem {
   const int32_t* cu_nodes;
   const uint8_t* mask;
   int64_t mask_stride;
-  void* out;                     /* (T, H, D) in out_dtype (the pool's, or fp32) */
+  void* out;                     /* (T, H, D) in out_dtype (the pool's, or fp32); may be q */
   int64_t out_stride_t, out_stride_h;
   int32_t out_dtype;
   float* lse;                    /* (T, H) contiguous, natural log; optional */

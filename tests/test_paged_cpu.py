@@ -94,6 +94,21 @@ def test_block_table_refusals():
         assert call(**kw) == L.HALO_ERR_UNSUPPORTED, kw
 
 
+def test_rows_that_overlap_are_refused():
+    from halo_b200 import _lib as L
+    lib = L.lib()
+    for old, new, lens in ((0x2000, 0x3000, 0x2000), (0x2000, 0x3000, 0x3000),
+                           (0x2000, 0x3000, 0x200c), (0x2000, 0x3000, 0x2ff4)):
+        assert lib.halo_update_block_tables(0x10000, 8, 4, 8, old, new, 0x12000, 10, 0x14000, 0x14000,
+                                            16, 5, 0x15000, 0x16000, 0x17000, lens,
+                                            None) == L.HALO_ERR_INVALID_ARG
+    po = _pool(L)
+    need = lib.halo_tree_workspace_bytes(ctypes.byref(po), ctypes.byref(_tree(L)))
+    for kw in ({"out_stride_t": 0}, {"out_stride_h": 0}, {"out_stride_h": po.D // 2}):
+        assert lib.halo_tree_attention(ctypes.byref(po), ctypes.byref(_tree(L, **kw)), 0x100000, need,
+                                       None) == L.HALO_ERR_INVALID_ARG
+
+
 def test_write_and_commit_refusals():
     from halo_b200 import _lib as L
     lib = L.lib()
