@@ -42,7 +42,7 @@ constexpr float kRescaleLog2 = 8.f;    // headroom of the running maximum
 constexpr int kBadSlots = 8;
 
 struct alignas(64) Params {
-  CUtensorMap kmap;                    // {D, page, H_kv, n_pages}
+  CUtensorMap kmap;                    // see encode_pool
   CUtensorMap vmap;
   const char* q;
   int64_t q_st, q_sh;                  // elements
@@ -81,11 +81,25 @@ __host__ __device__ constexpr int64_t part_floats(int RG) {
   return (int64_t)RG * (D + 2);
 }
 
-// tree_kernel: QT query tiles of 128 rows.
-template <int D, int QT>
-struct Geom {
-  static constexpr int kBlocks = D / 64;                  // 128-byte column blocks
+// A K/V tile in shared memory: 128 rows of D / 64 column blocks of 128 bytes,
+// swizzled.  A block is contiguous, or (PAIR) each 8 rows of both blocks are:
+// a copy cannot cross a page, so a tile of pages whose rows are an odd multiple
+// of 8 would take 32 copies of 8 rows and one block.
+template <int D, bool PAIR>
+struct Tile {
+  static_assert(!PAIR || D == 128, "pairs of column blocks");
+  static constexpr bool kPair = PAIR;
+  static constexpr int kBlocks = D / 64;
   static constexpr int kBlockBytes = kBN * 128;
+  static constexpr int kGroup = PAIR ? 2048 : 1024;       // from 8 rows to the next 8
+  static constexpr int kNextBlock = PAIR ? 1024 : kBlockBytes;
+};
+
+// tree_kernel: QT query tiles of 128 rows.
+template <int D, int QT, bool PAIR>
+struct Geom : Tile<D, PAIR> {
+  using Tile<D, PAIR>::kBlocks;
+  using Tile<D, PAIR>::kBlockBytes;
   static constexpr int kTileBytes = kBlocks * kBlockBytes;
   // as many K and V tiles in flight as 227 KB hold beside QT query tiles
   static constexpr int kStK = D == 64 ? 6 : 3;
@@ -100,12 +114,12 @@ struct Geom {
 };
 
 // tree_few_kernel: NR (16, 32 or 64) query rows.
-template <int D, int NR>
-struct FewGeom {
+template <int D, int NR, bool PAIR>
+struct FewGeom : Tile<D, PAIR> {
+  using Tile<D, PAIR>::kBlocks;
+  using Tile<D, PAIR>::kBlockBytes;
   // a warp more for V's copies where the registers of 64 rows leave room
   static constexpr int kThreads = NR == 64 ? 384 : 416;
-  static constexpr int kBlocks = D / 64;
-  static constexpr int kBlockBytes = kBN * 128;
   static constexpr int kTileBytes = kBlocks * kBlockBytes;
   static constexpr int kQBytes = NR * D * 2;
   static constexpr int kPBytes = (NR == 64 ? 2 : 1) * kBlockBytes;
@@ -122,10 +136,12 @@ struct FewGeom {
   static constexpr int kSmemBytes = kOffBar + 1024;
   static constexpr uint32_t kColO = 2 * NR;                    // S 2 x NR, O 2 NR
 };
-static_assert(FewGeom<128, 64>::kSmemBytes <= 232448 && FewGeom<128, 32>::kSmemBytes <= 232448 &&
-              FewGeom<64, 64>::kSmemBytes <= 232448 && FewGeom<64, 32>::kSmemBytes <= 232448 &&
-              Geom<128, 1>::kSmemBytes <= 232448 && Geom<128, 2>::kSmemBytes <= 232448 &&
-              Geom<64, 2>::kSmemBytes <= 232448, "227 KB of shared memory");
+static_assert(FewGeom<128, 64, true>::kSmemBytes <= 232448 &&
+              FewGeom<128, 32, true>::kSmemBytes <= 232448 &&
+              FewGeom<64, 64, false>::kSmemBytes <= 232448 &&
+              FewGeom<64, 32, false>::kSmemBytes <= 232448 &&
+              Geom<128, 1, true>::kSmemBytes <= 232448 && Geom<128, 2, true>::kSmemBytes <= 232448 &&
+              Geom<64, 2, false>::kSmemBytes <= 232448, "227 KB of shared memory");
 
 struct FewShared {
   float red[4][64];                    // per warp and row
@@ -346,6 +362,16 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
                : "memory");
 }
 
+__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, int c0, int c1,
+                                            int c2, int c3, int c4, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+      ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2),
+        "r"(c3), "r"(c4), "r"(smem_addr(bar))
+      : "memory");
+}
+
 // A value the compiler cannot see through: keeps it from holding every
 // unrolled MMA's descriptor in a register across the loop.
 __device__ __forceinline__ uint64_t opaque(uint64_t v) {
@@ -473,9 +499,9 @@ __device__ __forceinline__ void produce(const Params& p, Bars* bs, unsigned char
   constexpr int SK = Gm::kStK, SV = Gm::kStV;
   const int lane = threadIdx.x & 31;
   Seg s{};
-  const int n_box = kBN / p.box, n_iss = n_box * Gm::kBlocks;   // at most 32
+  const int n_box = kBN / p.box, n_iss = Gm::kPair ? n_box : n_box * Gm::kBlocks;   // at most 16
   const int blk = lane / n_box, bx = lane - blk * n_box;
-  const uint32_t dst = blk * Gm::kBlockBytes + bx * p.box * 128;
+  const uint32_t dst = blk * Gm::kBlockBytes + bx * (p.box >> 3) * Gm::kGroup;
   const int step_page = kBN / p.page, step_row = kBN - step_page * p.page;
   int nk = 0, nv = 0;             // K and V tiles issued
   bool ok = true;
@@ -490,8 +516,11 @@ __device__ __forceinline__ void produce(const Params& p, Bars* bs, unsigned char
       if (absent) mbar_arrive_n(&empty[i], absent);
     }
     __syncwarp();
-    if (lane < n_iss)
-      tma_load_4d(smem + off + i * Gm::kTileBytes + dst, map, blk * 64, row, s.hk, page, &full[i]);
+    if (lane < n_iss) {
+      unsigned char* to = smem + off + i * Gm::kTileBytes + dst;
+      if constexpr (Gm::kPair) tma_load_5d(to, map, 0, row, 0, s.hk, page, &full[i]);
+      else tma_load_4d(to, map, blk * 64, row, s.hk, page, &full[i]);
+    }
   };
   while (ok && walk.next(p, s)) {
     const int32_t* tab = p.table + (int64_t)walk.r * p.table_stride;
@@ -567,8 +596,8 @@ __device__ __forceinline__ void clean(const Params& p, Bars* bs, unsigned char* 
         for (int i = lane; i < n; i += 32) {
           const int row = lo + i / (D / 8), c = i % (D / 8);
           uint4* w = reinterpret_cast<uint4*>(smem + Gm::kOffV + iv * Gm::kTileBytes +
-                                              (c >> 3) * Gm::kBlockBytes + row * 128 +
-                                              (((c & 7) ^ (row & 7)) << 4));
+                                              (c >> 3) * Gm::kNextBlock + (row >> 3) * Gm::kGroup +
+                                              (row & 7) * 128 + (((c & 7) ^ (row & 7)) << 4));
           if (row >= end) {
             *w = make_uint4(0, 0, 0, 0);
             continue;
@@ -655,9 +684,9 @@ __device__ __noinline__ float bad_sum(const Params& p, int r, int t, int ctx, in
 // half of P 468; turn passed on halfway 453.  Tried: dropping the remainders
 // 380, but one bf16 P is 2^-9 off; exponentials taken out altogether 468: they
 // are not the limit; spinning instead of suspended waits 474.
-template <typename T, int D, int QT>
+template <typename T, int D, int QT, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ Params p) {
-  using Gm = Geom<D, QT>;
+  using Gm = Geom<D, QT, PAIR>;
   constexpr int RG = 128 * QT;             // rows of a group
   constexpr bool kBf16 = Elem<T>::kDtype == HALO_DTYPE_BF16;
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -728,8 +757,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         constexpr uint32_t kIdQK = umma::instr_desc_f16(128, kBN, kBf16, false, false);
         constexpr uint32_t kIdPV = umma::instr_desc_f16(128, D, kBf16, false, true);
         const uint64_t qdesc0 = umma::smem_desc_sw128(sQ, 16, 1024);
-        const uint64_t kdesc0 = umma::smem_desc_sw128(sK, 16, 1024);
-        const uint64_t vdesc0 = umma::smem_desc_sw128(sV, Gm::kBlockBytes, 1024);
+        const uint64_t kdesc0 = umma::smem_desc_sw128(sK, 16, Gm::kGroup);
+        const uint64_t vdesc0 = umma::smem_desc_sw128(sV, Gm::kNextBlock, Gm::kGroup);
         const uint32_t pc = tmem + x * 128, oc = tmem + Gm::kColO + x * D;
         int g0 = 0, si = 0, j = 0;            // tiles before the segment; segments; P waits
         bool ok = true;
@@ -748,8 +777,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             const uint64_t kd = opaque(kdesc0 + (uint64_t)((ik * Gm::kTileBytes) >> 4));
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off = ((kk >> 2) * Gm::kBlockBytes + (kk & 3) * 32) >> 4;
-              umma::mma_ss(pc, qd + off, kd + off, kIdQK, kk > 0);
+              umma::mma_ss(pc, qd + (((kk >> 2) * Gm::kBlockBytes + (kk & 3) * 32) >> 4),
+                           kd + (((kk >> 2) * Gm::kNextBlock + (kk & 3) * 32) >> 4), kIdQK, kk > 0);
             }
             umma::commit(&bs->s_full[x]);
             umma::commit(&bs->k_empty[ik]);
@@ -779,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
               for (int kk = 0; kk < 8; ++kk) {      // 16 positions: values, remainders
                 const int h = kk >> 2, b = (kk >> 1) & 1;
                 umma::mma_ts(oc, pc + h * 64 + c * 32 + (kk & 1) * 16 + b * 8,
-                             vd + (uint64_t)(((h * 4 + c * 2 + b) * 16 * 128) >> 4), kIdPV,
+                             vd + (uint64_t)(((h * 4 + c * 2 + b) * 2 * Gm::kGroup) >> 4), kIdPV,
                              it > 0 || c > 0 || kk > 0);
               }
             }
@@ -1134,9 +1163,10 @@ __device__ __forceinline__ void warp_columns(float (&v)[N], Op op) {
   }
 }
 
-template <typename T, int D, int NR>
-__global__ void __launch_bounds__(FewGeom<D, NR>::kThreads, 1) tree_few_kernel(const __grid_constant__ Params p) {
-  using Gm = FewGeom<D, NR>;
+template <typename T, int D, int NR, bool PAIR>
+__global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
+    tree_few_kernel(const __grid_constant__ Params p) {
+  using Gm = FewGeom<D, NR, PAIR>;
   constexpr int RG = NR;
   constexpr bool kBf16 = Elem<T>::kDtype == HALO_DTYPE_BF16;
   constexpr int SK = Gm::kStK, SV = Gm::kStV, PB = Gm::kPBuf;
@@ -1220,7 +1250,7 @@ __global__ void __launch_bounds__(FewGeom<D, NR>::kThreads, 1) tree_few_kernel(c
       // -------------------------------------------------------- QK issuer
       if (lane == 0) {
         constexpr uint32_t kIdQK = umma::instr_desc_f16(kBN, NR, kBf16, false, false);
-        const uint64_t kdesc0 = umma::smem_desc_sw128(sK, 16, 1024);
+        const uint64_t kdesc0 = umma::smem_desc_sw128(sK, 16, Gm::kGroup);
         int g = 0, si = 0;                  // tiles; segments
         bool ok = true;
         while (ok && walk.next(p, s)) {
@@ -1237,7 +1267,7 @@ __global__ void __launch_bounds__(FewGeom<D, NR>::kThreads, 1) tree_few_kernel(c
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk)
               umma::mma_ss(tmem + (g & 1) * NR,
-                           kd + (uint64_t)(((kk >> 2) * Gm::kBlockBytes + (kk & 3) * 32) >> 4),
+                           kd + (uint64_t)(((kk >> 2) * Gm::kNextBlock + (kk & 3) * 32) >> 4),
                            qd + (uint64_t)(((kk >> 2) * NR * 128 + (kk & 3) * 32) >> 4), kIdQK,
                            kk > 0);
             umma::commit(&bs->s_full[g & 1]);
@@ -1256,7 +1286,7 @@ __global__ void __launch_bounds__(FewGeom<D, NR>::kThreads, 1) tree_few_kernel(c
         // V^T has 128 rows; 64 columns of V fill them twice (the same block
         // again), and the second half of O^T is not read
         const uint64_t vdesc0 =
-            umma::smem_desc_sw128(sV, D == 64 ? 0 : Gm::kBlockBytes, 1024);
+            umma::smem_desc_sw128(sV, D == 64 ? 0 : Gm::kNextBlock, Gm::kGroup);
         const uint64_t pdesc0 = umma::smem_desc_sw128(sP, Gm::kBlockBytes, 1024);
         int g = 0;
         bool ok = true;
@@ -1271,7 +1301,7 @@ __global__ void __launch_bounds__(FewGeom<D, NR>::kThreads, 1) tree_few_kernel(c
             const uint64_t pd = opaque(pdesc0 + (uint64_t)(((g % PB) * Gm::kPBytes) >> 4));
 #pragma unroll
             for (int kk = 0; kk < kBN / 16; ++kk)
-              umma::mma_ss(tmem + Gm::kColO, vd + (uint64_t)((kk * 16 * 128) >> 4),
+              umma::mma_ss(tmem + Gm::kColO, vd + (uint64_t)((kk * 2 * Gm::kGroup) >> 4),
                            pd + (uint64_t)((kk * 16 * 128) >> 4), kIdPV, t > s.t0 || kk > 0);
             umma::commit(&bs->pv_done[g % PB]);
             umma::commit(&bs->v_empty[iv]);
@@ -1679,25 +1709,29 @@ static EncodeFn encode_fn() {
   return fn;
 }
 
-// The tensor map of a pool's K or V: {D, page, H_kv, n_pages}, boxes of 64
-// elements x `box` rows, 128-byte swizzle, zeros outside.
+// The tensor map of a pool's K or V: {D, page, H_kv, n_pages} with boxes of 64
+// columns x `box` rows or, for boxes of both column blocks, {64, page, 2,
+// H_kv, n_pages} (a swizzled box is at most 128 bytes wide); 128-byte swizzle,
+// zeros outside.
 static int encode_pool(const halo_page_pool_t* pool, const void* ptr, int64_t stride_p,
-                       int64_t stride_h, int64_t stride_t, int box, CUtensorMap* out) {
+                       int64_t stride_h, int64_t stride_t, int box, bool pair, CUtensorMap* out) {
   EncodeFn fn = encode_fn();
   if (!fn) return fail(HALO_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   // the stride of a dimension of one is never used, but has to be legal
-  const int64_t st = stride_t * 2;
-  const int64_t sh = pool->H_kv > 1 ? stride_h * 2 : st;
-  const int64_t sp = pool->n_pages > 1 ? stride_p * 2 : st;
-  cuuint64_t dims[4] = {(cuuint64_t)pool->D, (cuuint64_t)pool->page_size, (cuuint64_t)pool->H_kv,
-                        (cuuint64_t)pool->n_pages};
-  cuuint64_t str[3] = {(cuuint64_t)st, (cuuint64_t)sh, (cuuint64_t)sp};
-  cuuint32_t ext[4] = {64, (cuuint32_t)box, 1, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const cuuint64_t st = stride_t * 2;
+  const cuuint64_t sh = pool->H_kv > 1 ? stride_h * 2 : st;
+  const cuuint64_t sp = pool->n_pages > 1 ? stride_p * 2 : st;
+  const cuuint64_t page = pool->page_size, H_kv = pool->H_kv, n_pages = pool->n_pages;
+  const cuuint32_t rows = box;
+  const cuuint64_t dims4[4] = {(cuuint64_t)pool->D, page, H_kv, n_pages}, str4[3] = {st, sh, sp};
+  const cuuint64_t dims5[5] = {64, page, 2, H_kv, n_pages}, str5[4] = {st, 128, sh, sp};
+  const cuuint32_t box4[4] = {64, rows, 1, 1}, box5[5] = {64, rows, 2, 1, 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   const CUresult r =
       fn(out, pool->dtype == HALO_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-         4, const_cast<void*>(ptr), dims, str, ext, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         pair ? 5 : 4, const_cast<void*>(ptr), pair ? dims5 : dims4, pair ? str5 : str4,
+         pair ? box5 : box4, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
@@ -1754,17 +1788,17 @@ static int64_t ws_bytes(const halo_page_pool_t* pool, const halo_tree_problem_t*
   return desc_bytes(n) + (int64_t)n * 2 * group_rows(pool, pb) * (pool->D + 2) * sizeof(float);
 }
 
-template <typename T, int D, int RG>
+template <typename T, int D, int RG, bool PAIR>
 static int launch(const Params& p, int n_cta, cudaStream_t st) {
   void (*kernel)(const Params);
   int smem, threads;
   if constexpr (RG <= 64) {
-    kernel = tree_few_kernel<T, D, RG>;
-    smem = FewGeom<D, RG>::kSmemBytes;
-    threads = FewGeom<D, RG>::kThreads;
+    kernel = tree_few_kernel<T, D, RG, PAIR>;
+    smem = FewGeom<D, RG, PAIR>::kSmemBytes;
+    threads = FewGeom<D, RG, PAIR>::kThreads;
   } else {
-    kernel = tree_kernel<T, D, RG / 128>;
-    smem = Geom<D, RG / 128>::kSmemBytes;
+    kernel = tree_kernel<T, D, RG / 128, PAIR>;
+    smem = Geom<D, RG / 128, PAIR>::kSmemBytes;
     threads = kThreads;
   }
   static std::once_flag once[64];
@@ -1790,14 +1824,14 @@ static int launch(const Params& p, int n_cta, cudaStream_t st) {
   return HALO_OK;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool PAIR>
 static int dispatch(int rows, const Params& p, int n_cta, cudaStream_t st) {
   switch (rows) {
-    case 16: return launch<T, D, 16>(p, n_cta, st);
-    case 32: return launch<T, D, 32>(p, n_cta, st);
-    case 64: return launch<T, D, 64>(p, n_cta, st);
-    case 128: return launch<T, D, 128>(p, n_cta, st);
-    default: return launch<T, D, 256>(p, n_cta, st);
+    case 16: return launch<T, D, 16, PAIR>(p, n_cta, st);
+    case 32: return launch<T, D, 32, PAIR>(p, n_cta, st);
+    case 64: return launch<T, D, 64, PAIR>(p, n_cta, st);
+    case 128: return launch<T, D, 128, PAIR>(p, n_cta, st);
+    default: return launch<T, D, 256, PAIR>(p, n_cta, st);
   }
 }
 
@@ -1839,11 +1873,22 @@ static int run(const halo_page_pool_t* pool, const halo_tree_problem_t* pb, void
   Params p{};
   p.box = 8;
   while (p.box < kBN && pool->page_size % (2 * p.box) == 0) p.box *= 2;
+  const int rows = group_rows(pool, pb);
+  // Copies of 8 rows take both column blocks of 128 columns; groups of 64 rows,
+  // whose one producer warp is the busiest, also halve copies of 16 rows for
+  // that.  8 requests on 32768 positions, 32 / 8 heads of 128, us without and
+  // with pairs on pages of 8, 16, 24, 48 and 64:
+  //   16 nodes   327 212   242 217   336 230   253 233   204 236
+  //    4 nodes   217 176   173 183   199 173   174 176   176 176
+  // 4 requests of 64 nodes on 65535 positions: 456 434 and 516 444 on pages of 8
+  // and 24, within 1 % on others.
+  const bool pair = pool->D == 128 && (p.box == 8 || (p.box == 16 && rows == 64));
+  if (pair) p.box = 8;
   rc = encode_pool(pool, pool->k, pool->k_stride_p, pool->k_stride_h, pool->k_stride_t, p.box,
-                   &p.kmap);
+                   pair, &p.kmap);
   if (rc != HALO_OK) return rc;
   rc = encode_pool(pool, pool->v, pool->v_stride_p, pool->v_stride_h, pool->v_stride_t, p.box,
-                   &p.vmap);
+                   pair, &p.vmap);
   if (rc != HALO_OK) return rc;
   p.q = static_cast<const char*>(pb->q);
   p.q_st = pb->q_stride_t;
@@ -1878,12 +1923,13 @@ static int run(const halo_page_pool_t* pool, const halo_tree_problem_t* pb, void
   p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + desc_bytes(n_cta));
   p.err = device_error_ptr();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int rows = group_rows(pool, pb);
-  if (pool->dtype == HALO_DTYPE_BF16)
-    return pool->D == 128 ? dispatch<__nv_bfloat16, 128>(rows, p, n_cta, st)
-                          : dispatch<__nv_bfloat16, 64>(rows, p, n_cta, st);
-  return pool->D == 128 ? dispatch<__half, 128>(rows, p, n_cta, st)
-                        : dispatch<__half, 64>(rows, p, n_cta, st);
+  auto typed = [&](auto tag) {
+    using T = decltype(tag);
+    if (pool->D == 64) return dispatch<T, 64, false>(rows, p, n_cta, st);
+    return pair ? dispatch<T, 128, true>(rows, p, n_cta, st)
+                : dispatch<T, 128, false>(rows, p, n_cta, st);
+  };
+  return pool->dtype == HALO_DTYPE_BF16 ? typed(__nv_bfloat16{}) : typed(__half{});
 }
 
 }  // namespace tree
