@@ -118,15 +118,23 @@ template <int D, int NR, bool PAIR>
 struct FewGeom : Tile<D, PAIR> {
   using Tile<D, PAIR>::kBlocks;
   using Tile<D, PAIR>::kBlockBytes;
+  // Softmax groups of four warps.  Four where 64 rows' softmax is longer than a
+  // tile's bytes (64 columns): 64 requests of 16 nodes on 1200 positions 75 us
+  // and 84 with two, 8 on 32768 positions 154 to 160 and 173, but 23.2 and 20.8
+  // on 40 positions.  At 128 columns two: 202 and 204 us on 32768 positions, 54
+  // (four) and 51.5 on 300.  32 rows in four groups of 8 leave no registers for
+  // V's producer: 111 and 120 us on pages of 64, 226 and 148 on pages of 8.
+  static constexpr int kGroups = D == 64 && NR == 64 ? 4 : 2;
+  static constexpr int kSoft = kGroups * 128;                  // their threads
   // a warp more for V's copies where the registers of 64 rows leave room
-  static constexpr int kThreads = NR == 64 ? 384 : 416;
+  static constexpr int kThreads = 128 + kSoft + (NR == 64 ? 0 : 32);
   static constexpr int kTileBytes = kBlocks * kBlockBytes;
   static constexpr int kQBytes = NR * D * 2;
   static constexpr int kPBytes = (NR == 64 ? 2 : 1) * kBlockBytes;
   // two buffers of P where a tile's bytes take less than P V and its waits
-  static constexpr int kPBuf = D == 64 && NR <= 32 ? 2 : 1;
-  static constexpr int kStK = D == 64 ? 5 : 3;
-  static constexpr int kStV = D == 64 ? 5 : (NR == 64 ? 2 : 3);
+  static constexpr int kPBuf = D == 64 ? 2 : 1;
+  static constexpr int kStK = D == 64 ? (NR == 64 ? 4 : 5) : 3;
+  static constexpr int kStV = D == 64 ? (NR == 64 ? 4 : 5) : (NR == 64 ? 2 : 3);
   static constexpr int kOffK = 0;
   static constexpr int kOffV = kStK * kTileBytes;
   static constexpr int kOffP = kOffV + kStV * kTileBytes;
@@ -1108,15 +1116,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
 
 // ======================================================================
 // tree_few_kernel: groups of at most 64 rows (NR = 16, 32 or 64).  One CTA an
-// SM, 384 threads (NR = 64) or 416.
-//   warp 0      TMA producer (as in tree_kernel); warp 12, if there, V's
+// SM, 416 threads (NR < 64), 384 or 640.
+//   warp 0      TMA producer (as in tree_kernel); the last warp of 416 threads
+//               V's
 //   warps 1, 3  lane 0 issues the QK / PV MMAs (one thread for both took 1950
 //               clocks a tile, most of them in commits); warp 1 owns TMEM
 //   warp 2      cleans V; query rows of the next segment (two buffers; the
 //               first segment's are loaded by the softmax warps)
-//   warps 4-11  softmax (thread = position of the tile) and epilogue (thread =
-//               output column), warps 4-7 the first NR / 2 rows, warps 8-11 the
-//               others
+//   from 4      softmax (thread = position of the tile) and epilogue (thread =
+//               output column), four warps for each NR / kGroups rows
 // Both products have the K/V tile as the 128-row operand and the query rows
 // as the columns: S^T = K Q^T (M = positions, N = NR) and O^T += V^T P^T
 // (M = columns of V, N = 2 NR: the weights' 16-bit values and, beside them,
@@ -1137,8 +1145,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
 // positions (1.08 GB): 217 to 232 us, 4.6 to 5.0 TB/s: 192 us for the tiles of an
 // SM, 4 before the first, 3 for an epilogue, 4 for a second segment, 4 for the
 // merge and the launch.  One softmax group of all rows: 248; parts in rows of
-// 528 bytes: 225.  At 64 columns a tile's bytes take 1.4k clocks and its
-// softmax 1.55k: 1.3 times the bytes' time.  Small batches are latency: 10 us
+// 528 bytes: 225.  At 64 columns a tile's bytes take 1.4k clocks, the chain of
+// its softmax more: 8 requests on 32768 positions (82 us of bytes) take 97 us
+// with 16 rows, 119 with 32, 154 to 160 with 64.  Small batches are latency: 10 us
 // for one token on 1000 positions (find the run 1.1, first rows and tables 1.5,
 // first tile 1.5, softmax and PV 1.9, epilogue 1.1, merge 3).
 
@@ -1181,7 +1190,7 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
       mbar_init(&bs->q_full[i], 1);
       mbar_init(&bs->q_empty[i], 1);
       mbar_init(&bs->s_full[i], 1);
-      mbar_init(&bs->s_free[i], 8);
+      mbar_init(&bs->s_free[i], Gm::kSoft / 32);
     }
     for (int i = 0; i < 6; ++i) {
       mbar_init(&bs->k_full[i], 1);
@@ -1190,8 +1199,8 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
       mbar_init(&bs->v_ready[i], 1);
       mbar_init(&bs->v_empty[i], 1);
     }
-    mbar_init(&bs->p_full[0], 8);
-    mbar_init(&bs->p_full[1], 8);
+    mbar_init(&bs->p_full[0], Gm::kSoft / 32);
+    mbar_init(&bs->p_full[1], Gm::kSoft / 32);
     mbar_init(&bs->pv_done[0], 1);
     mbar_init(&bs->pv_done[1], 1);
     mbar_init(&bs->mma_done[0], 1);
@@ -1244,7 +1253,7 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
     };
     if (warp == 0) {
       produce<RG, Gm, false, NR == 64 ? 3 : 1>(p, bs, smem, walk);
-    } else if (NR < 64 && warp == 12) {
+    } else if (NR < 64 && warp == 4 + Gm::kSoft / 32) {
       produce<RG, Gm, false, 2>(p, bs, smem, walk);
     } else if (warp == 1) {
       // -------------------------------------------------------- QK issuer
@@ -1334,8 +1343,8 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
       });
     } else {
       // -------------------------------------------------------- softmax
-      // two groups of four warps, each RT of the NR rows; thread = position
-      constexpr int RT = NR / 2;
+      // groups of four warps, each RT of the NR rows; thread = position
+      constexpr int RT = NR / Gm::kGroups;
       const int sub = warp & 3, grp = (warp - 4) >> 2, bar = 1 + grp;
       const int tid = threadIdx.x & 127, r0 = grp * RT;
       const uint32_t trow = tmem + ((uint32_t)(sub * 32) << 16);
@@ -1347,10 +1356,10 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
       while (walk.next(p, s)) {
         const int ctx = walk.q.ctx, end = walk.q.end;
         if (si == 0) {                     // later ones come from warp 3, ahead
-          copy_q(walk, s, threadIdx.x - 128, 256, 0);
+          copy_q(walk, s, threadIdx.x - 128, Gm::kSoft, 0);
           asm volatile("cp.async.wait_all;" ::: "memory");
           fence_proxy_async_smem();
-          named_bar_sync(3, 256);
+          named_bar_sync(1 + Gm::kGroups, Gm::kSoft);
           if (threadIdx.x == 128) mbar_arrive(&bs->q_full[0]);
         }
         float l[RT];
