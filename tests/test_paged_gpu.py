@@ -319,6 +319,23 @@ def test_hidden_rows_reach_no_output(cuda_device, bad, G, D, dtype):
     assert torch.isfinite(out[rows]).all() and torch.isfinite(lse).all()
 
 
+@pytest.mark.parametrize("page", [8, 16, 24, 40])
+@pytest.mark.parametrize("nodes", [3, 7, 14, 30, 70])
+def test_small_pages_of_128_columns(cuda_device, page, nodes):
+    """12 to 280 rows a K/V head over tiles whose pages are a few rows long,
+    with a hidden node whose V is not finite in one column of each half."""
+    c = Case(page + nodes, [9003, 0, 261], [nodes, nodes, 1], 4, 1, 128, page,
+             torch.bfloat16 if page % 16 else torch.float16)
+    c.mask[:2 * nodes, 1] = False
+    hidden = [(c.table[r][(x + 1) // page], (x + 1) % page) for r, x in ((0, 9003), (1, 0))]
+    for pg, row in hidden:
+        c.v[pg, 0, row, 3], c.v[pg, 0, row, 100] = math.nan, -math.inf
+    out, lse = c.run(out_dtype=torch.float32)
+    for pg, row in hidden:                   # the oracle never reads what is hidden
+        c.v[pg, 0, row] = 0
+    c.check(out, lse)
+
+
 def test_tree_attention_large_scores_and_scale(cuda_device):
     """Scores of thousands: the running maximum keeps the weights in range."""
     c = Case(12, [700, 40], [9, 3], 8, 2, 128, 16, torch.bfloat16, spread=60.0)
