@@ -660,8 +660,8 @@ __device__ __noinline__ float bad_sum(const Params& p, int r, int t, int ctx, in
 // ======================================================================
 // tree_kernel: groups of more than 64 rows.  One CTA an SM, 640 threads.
 //   warp 0      TMA producer: K and V tiles of 128 positions, each made of
-//               boxes of p.box rows (the largest power of two, up to 128,
-//               that divides the page), through two rings; the lanes issue a
+//               boxes of p.box rows (a power of two up to 128 that divides
+//               the page), through two rings; the lanes issue a
 //               tile's boxes side by side.  Boxes behind the last position
 //               or without a page start outside the tensor: zeros.
 //   warps 1, 3  lane 0 issues the MMAs of stream 0 / 1; warp 1 owns TMEM.
@@ -686,12 +686,14 @@ __device__ __noinline__ float bad_sum(const Params& p, int r, int t, int ctx, in
 // the next QK 1.8k of queueing behind the other stream's, waits 0.8k) repeats
 // every 5.4k clocks a stream, the tensor pipe is busy 47 % of the time (its 48
 // MMAs take 3.1k) and the exponentials without the chain would fit into 2.0k.
-// 4 requests of 64 nodes on 65535 positions, 32 / 8 heads of 128, bf16: 450 us,
-// 611 TFLOP/s of the two products (917 with the remainders').  Steps, in us
+// 4 requests of 64 nodes on 65535 positions, 32 / 8 heads of 128, bf16: 428 to
+// 450 us, 611 to 642 TFLOP/s of the two products (half more with the remainders').  Steps, in us
 // there: 8 softmax warps polling issuer 583; 16 warps 552; turns 479; PV from
-// half of P 468; turn passed on halfway 453.  Tried: dropping the remainders
+// half of P 468; turn passed on halfway 453; waits
+// without a suspend hint 442 to 438.  Tried: dropping the remainders
 // 380, but one bf16 P is 2^-9 off; exponentials taken out altogether 468: they
-// are not the limit; spinning instead of suspended waits 474.
+// are not the limit; polling instead of suspended waits 474
+// (469 then).
 template <typename T, int D, int QT, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ Params p) {
   using Gm = Geom<D, QT, PAIR>;
@@ -1140,9 +1142,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
 // in a segment's first tile and in the rare tile that raises it.
 //
 // What it reaches: 1M positions, 64 / 8 heads of 128, 4 nodes (4.3 GB): 616 to
-// 681 us by the clock that the power limit leaves, 6.3 to 7.0 TB/s (a plain copy
+// 704 us by the clock that the power limit leaves, 6.1 to 7.0 TB/s (a plain copy
 // 6.5); with rows on the 128-row side 899.  8 requests of 16 nodes on 32768
-// positions (1.08 GB): 217 to 232 us, 4.6 to 5.0 TB/s: 192 us for the tiles of an
+// positions (1.08 GB): 213 to 233 us, 4.6 to 5.1 TB/s: 192 us for the tiles of an
 // SM, 4 before the first, 3 for an epilogue, 4 for a second segment, 4 for the
 // merge and the launch.  One softmax group of all rows: 248; parts in rows of
 // 528 bytes: 225.  At 64 columns a tile's bytes take 1.4k clocks, the chain of
