@@ -687,13 +687,12 @@ __device__ __noinline__ float bad_sum(const Params& p, int r, int t, int ctx, in
 // every 5.4k clocks a stream, the tensor pipe is busy 47 % of the time (its 48
 // MMAs take 3.1k) and the exponentials without the chain would fit into 2.0k.
 // 4 requests of 64 nodes on 65535 positions, 32 / 8 heads of 128, bf16: 428 to
-// 450 us, 611 to 642 TFLOP/s of the two products (half more with the remainders').  Steps, in us
-// there: 8 softmax warps polling issuer 583; 16 warps 552; turns 479; PV from
-// half of P 468; turn passed on halfway 453; waits
-// without a suspend hint 442 to 438.  Tried: dropping the remainders
-// 380, but one bf16 P is 2^-9 off; exponentials taken out altogether 468: they
-// are not the limit; polling instead of suspended waits 474
-// (469 then).
+// 450 us, 611 to 642 TFLOP/s of the two products (half more with the
+// remainders').  Steps, in us there: 8 softmax warps polling issuer 583; 16
+// warps 552; turns 479; PV from half of P 468; turn passed on halfway 453; waits
+// without a suspend hint 438 (442 with).  Tried: dropping the remainders 380,
+// but one bf16 P is 2^-9 off; exponentials taken out altogether 468 (469 then):
+// they are not the limit; polling instead of suspended waits 474 (469).
 template <typename T, int D, int QT, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ Params p) {
   using Gm = Geom<D, QT, PAIR>;
