@@ -658,6 +658,44 @@ def test_release_within_a_step(cuda_device):
     assert _owners(cache) == list(range(8))
 
 
+def test_a_whole_step_captured_and_replayed(cuda_device):
+    """extend, write, attend and accept in one graph, replayed on new inputs,
+    leave the cache as eager steps do, bit for bit."""
+    eager, cache = _small_cache(12), _small_cache(12)
+    g = torch.Generator().manual_seed(9)
+    counts, path, n = _i32([0, 0]), _i32([[0, 0, 0]] * 2), _i32([0, 0])
+    k, v = (torch.zeros(12, 1, 64, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    q = torch.zeros(12, 4, 64, dtype=torch.bfloat16, device=DEV)
+    mask = torch.zeros(12, 6, dtype=torch.bool, device=DEV)
+    out, lse = torch.zeros_like(q), torch.zeros(12, 4, device=DEV)
+
+    def step(c, out, lse):
+        rows = c.extend(counts, 12)
+        c.write(0, k, v, rows)
+        c.attend(0, q, rows, mask, out=out, lse=lse)
+        c.accept(path, n)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(cache, out, lse)
+    want, want_lse = torch.zeros_like(out), torch.zeros_like(lse)
+    for c, p, m in (([6, 3], [[0, 2, 5], [0, 1, 2]], [3, 1]), ([1, 6], [[0, 0, 0], [1, 3, 4]], [1, 3]),
+                    ([0, 5], [[0, 0, 0], [0, 4, 0]], [0, 2]), ([5, 70], [[2, 3, 0], [9, 9, 9]], [2, 3])):
+        for t, x in ((counts, c), (path, p), (n, m)):
+            t.copy_(_i32(x))
+        for t in (k, v, q):
+            t.copy_(torch.randn(t.shape, generator=g))
+        mask.copy_(torch.rand(mask.shape, generator=g) < 0.5)
+        graph.replay()
+        step(eager, want, want_lse)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+        for name in ("lens", "held", "n_free", "block_tables"):
+            assert torch.equal(getattr(cache, name), getattr(eager, name)), name
+        assert torch.equal(cache.k[0], eager.k[0]) and torch.equal(cache.v[0], eager.v[0])
+        assert _owners(cache) == list(range(12))
+    assert cache.lens.tolist() == [10 + 3 + 1 + 2, 6 + 1 + 3 + 2]
+
+
 @pytest.mark.parametrize("n", [3, 40])
 def test_tree_attention_in_place(cuda_device, n):
     """out may be q itself: a row is read by the CTA that writes it, or
