@@ -25,6 +25,7 @@
 #include <type_traits>
 
 #include "halo_common.cuh"
+#include "running_max.cuh"
 #include "umma.cuh"
 
 namespace halo {
@@ -38,7 +39,6 @@ namespace tree {
 constexpr int kBN = 128;               // positions of a tile (a unit)
 constexpr int kThreads = 640;          // tree_kernel
 constexpr uint32_t kTmemCols = 512;
-constexpr float kRescaleLog2 = 8.f;    // headroom of the running maximum
 constexpr int kBadSlots = 8;
 
 struct alignas(64) Params {
@@ -58,6 +58,7 @@ struct alignas(64) Params {
   int64_t out_st, out_sh;
   float* lse;
   float scale_log2;                    // softmax scale * log2(e)
+  float headroom;                      // of the running maximum, in raw scores
   int32_t out_f32;
   int32_t R, T, H, H_kv, G, max_nodes, max_blocks, n_pages, page, box;
   struct Desc* desc;                   // workspace: one a CTA
@@ -74,8 +75,8 @@ struct alignas(64) Desc {
   int32_t cu0, hk, row0, rows;         // row0: the group's first row of the request
 };
 
-// A part of a cut segment in the workspace: o [RG][D], then (m in log2 units,
-// l) [RG][2], fp32.
+// A part of a cut segment in the workspace: o [RG][D], then (m of the raw
+// scores, l) [RG][2], fp32.
 template <int D>
 __host__ __device__ constexpr int64_t part_floats(int RG) {
   return (int64_t)RG * (D + 2);
@@ -318,6 +319,11 @@ __device__ __forceinline__ uint64_t ffma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
+__device__ __forceinline__ uint64_t fmul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
@@ -329,13 +335,13 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return d;
 }
 
-// Weights of a pair of scores, e^(s - m) in log2 units: their 16-bit values
-// (hi) and remainders (lo); the fp32 pair is returned for the row sum.
+// Weights of a pair of raw scores, e^(scale (s - m)): their 16-bit values (hi)
+// and remainders (lo); the fp32 pair is returned for the row sum.
 template <typename T>
 __device__ __forceinline__ uint64_t weigh(float s0, float s1, uint64_t sc2, uint64_t nm2,
                                           uint32_t& hi, uint32_t& lo) {
   float x0, x1, h0, h1;
-  f2unpack(ffma2(f2pack(s0, s1), sc2, nm2), x0, x1);
+  f2unpack(fmul2(fadd2(f2pack(s0, s1), nm2), sc2), x0, x1);
   const float a = ex2(x0), b = ex2(x1);
   if constexpr (Elem<T>::kDtype == HALO_DTYPE_BF16) {   // truncated: one byte permute a pair
     hi = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
@@ -393,7 +399,10 @@ __device__ __forceinline__ bool bad16(uint32_t x) {   // inf or NaN in the low 1
   return (x & e) == e;
 }
 
-constexpr float kNoMax = -1e30f;           // nothing seen yet: any score raises it
+// ln of sum e^{scale s} from the maximum of the raw scores and the sum of weights.
+__device__ __forceinline__ float log_sum(float m, float l, float scale_log2) {
+  return l > 0.f ? fmaf(m, scale_log2, log2f(l)) * kLn2 : (l == l ? -INFINITY : l);
+}
 
 // Barrier `id` of N softmax threads that tells whether any of them voted.
 template <int N>
@@ -958,17 +967,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           }
           mx = fmaxf(mx, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
         }
-        mx *= p.scale_log2;
         // the maximum moves only past its headroom (weights are at most 2^8),
         // for both halves of a row at once
         bool rise = it == 0;
-        if (it > 0) rise = vote_bar<256>(2 + x, mx > m + kRescaleLog2);
+        if (it > 0) rise = vote_bar<256>(2 + x, rises(mx, m, p.headroom));
         if (rise) {
           sm_mx[(x * 2 + h) * 128 + r] = mx;
           named_bar_sync(2 + x, 256);
           mx = fmaxf(mx, sm_mx[(x * 2 + 1 - h) * 128 + r]);
-          const bool grow = mx > m + kRescaleLog2;
-          const float fac = grow ? ex2(m - mx) : 1.f;
+          const bool grow = rises(mx, m, p.headroom);
+          const float fac = grow ? ex2(excess(m, mx) * p.scale_log2) : 1.f;
           m = grow ? mx : m;
           l *= fac;
           if (it > 0) {
@@ -1039,7 +1047,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         constexpr int N = sizeof(o) / sizeof(float);
         if (fix)
           for (int e = 0; e < N; ++e) o[e] += bad(row, col + e);
-        M = M == kNoMax ? -INFINITY : M;
         if (!s.whole) {
           float4* d = reinterpret_cast<float4*>(part + row * D + col);
 #pragma unroll
@@ -1051,7 +1058,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         const int64_t t = cu0 + node;
         const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
         if (col == 0 && p.lse)
-          p.lse[t * p.H + hq] = L > 0.f ? (M + log2f(L)) * kLn2 : (L == L ? -INFINITY : L);
+          p.lse[t * p.H + hq] = log_sum(M, L, p.scale_log2);
         const int64_t at = t * p.out_st + hq * p.out_sh + col;
         if (p.out_f32) {
           float4* d = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at);
@@ -1080,13 +1087,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         }
       } else {
         // the two streams' states of a row are both in its TMEM lane: every
-        // thread joins a quarter of the columns.  A state that saw only NaN
-        // has no maximum and l = NaN: weight 1 keeps the NaN.
+        // thread joins a quarter of the columns.  A state that saw nothing has
+        // l = 0 and o = 0 beside kNoMax, one that saw only NaN l = NaN: either
+        // joins right with any weight.
         const float m0 = sm_m[r], m1 = n1 > 0 ? sm_m[128 + r] : kNoMax;
         const float l0 = sm_l[r] + sm_l[128 + r], l1 = n1 > 0 ? sm_l[256 + r] + sm_l[384 + r] : 0.f;
         const float M = fmaxf(m0, m1);
-        const float w0 = m0 == kNoMax ? (l0 == l0 ? 0.f : 1.f) : ex2(m0 - M);
-        const float w1 = m1 == kNoMax ? (l1 == l1 ? 0.f : 1.f) : ex2(m1 - M);
+        const float w0 = ex2(excess(m0, M) * p.scale_log2), w1 = ex2(excess(m1, M) * p.scale_log2);
         const float L = fmaf(l1, w1, l0 * w0);
         const int col = (x * 2 + h) * (D / 4);
 #pragma unroll 1
@@ -1404,11 +1411,12 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
           }
           ok = ok && __all_sync(0xffffffffu, wait_bar(&bs->s_full[g & 1], (g >> 1) & 1, bs, p.err));
           umma::fence_after_sync();
-          // Scores against the running maxima, in log2 units; where a row's
-          // maximum has to rise (always in the first tile) the raw scores are
-          // reduced and the loop runs again.
+          // Excess of the scores over the running maxima; where a row's maximum
+          // has to rise (always in the first tile) the raw scores are reduced
+          // and the loop runs again, at most once a tile: it ends after three
+          // passes whatever the scores are.
           float x[RT];
-          bool rise = t == s.t0;
+          bool rise = t == s.t0, risen = false;
           while (true) {
             tmem_ld(trow + (g & 1) * NR + r0, x);
             umma::tmem_wait_ld();
@@ -1419,17 +1427,20 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
             }
             if (!rise) {
               float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+              const uint64_t minus = f2pack(-1.f, -1.f);
 #pragma unroll
               for (int r = 0; r < RT; r += 4) {
+                // excess() of two rows at a time
                 const float4 m = *reinterpret_cast<const float4*>(&sh->m[r0 + r]);
-                x[r] = fmaf(x[r], p.scale_log2, -m.x);
-                x[r + 1] = fmaf(x[r + 1], p.scale_log2, -m.y);
-                x[r + 2] = fmaf(x[r + 2], p.scale_log2, -m.z);
-                x[r + 3] = fmaf(x[r + 3], p.scale_log2, -m.w);
+                f2unpack(ffma2(f2pack(m.x, m.y), minus, f2pack(x[r], x[r + 1])), x[r], x[r + 1]);
+                f2unpack(ffma2(f2pack(m.z, m.w), minus, f2pack(x[r + 2], x[r + 3])), x[r + 2],
+                         x[r + 3]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], x[r + e]);
               }
-              rise = vote_bar<128>(bar, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > kRescaleLog2);
+              if (risen) break;
+              rise = vote_bar<128>(
+                  bar, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > p.headroom);
               if (!rise) break;
               continue;
             }
@@ -1439,10 +1450,10 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
             if (tid < RT) {
               const int r = r0 + tid;
               const float mx = fmaxf(fmaxf(sh->red[0][r], sh->red[1][r]),
-                                     fmaxf(sh->red[2][r], sh->red[3][r])) * p.scale_log2;
+                                     fmaxf(sh->red[2][r], sh->red[3][r]));
               const float mo = t == s.t0 ? kNoMax : sh->m[r];
-              const bool grow = mx > mo + kRescaleLog2;
-              sh->fac[r] = grow ? ex2(mo - mx) : 1.f;
+              const bool grow = rises(mx, mo, p.headroom);
+              sh->fac[r] = grow ? ex2(excess(mo, mx) * p.scale_log2) : 1.f;
               sh->m[r] = grow ? mx : mo;
             }
             named_bar_sync(bar, 128);
@@ -1471,6 +1482,7 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
               umma::tmem_wait_st();
             }
             rise = false;
+            risen = true;
           }
           // the scores are in registers: S's buffer is free
           umma::fence_before_sync();
@@ -1479,7 +1491,10 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
           uint32_t hi[RT / 2], lo[RT / 2];
 #pragma unroll
           for (int r = 0; r < RT; r += 2) {
-            const float a = ex2(x[r]), b = ex2(x[r + 1]);
+            float a, b;
+            f2unpack(fmul2(f2pack(x[r], x[r + 1]), f2pack(p.scale_log2, p.scale_log2)), a, b);
+            a = ex2(a);
+            b = ex2(b);
             l[r] += a;
             l[r + 1] += b;
             float ah, bh;
@@ -1525,7 +1540,7 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
         if (tid < RT && r0 + tid < s.rows) {
           const int r = r0 + tid;
           const float L = (sh->red[0][r] + sh->red[1][r]) + (sh->red[2][r] + sh->red[3][r]);
-          const float M = sh->m[r] == kNoMax ? -INFINITY : sh->m[r];
+          const float M = sh->m[r];
           if (!s.whole) {
             *reinterpret_cast<float2*>(part + RG * D + 2 * r) = make_float2(M, L);
             sh->fac[r] = 1.f;
@@ -1534,8 +1549,7 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
             const int rq = s.row0 + r, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
             const int64_t row = walk.q.cu0 + node;
             if (p.lse)
-              p.lse[row * p.H + hq] =
-                  L > 0.f ? (M + log2f(L)) * kLn2 : (L == L ? -INFINITY : L);
+              p.lse[row * p.H + hq] = log_sum(M, L, p.scale_log2);
             sh->fac[r] = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
             sh->off[r] = row * p.out_st + hq * p.out_sh;
           }
@@ -1662,15 +1676,15 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
         float Mn = M;
 #pragma unroll
         for (int u = 0; u < B; ++u) Mn = fmaxf(Mn, ml[u].x);
-        // a part that saw only NaN has m = -inf and l = NaN: weight 1 keeps it
-        const float a0 = (M == -INFINITY) ? (L == L ? 0.f : 1.f) : ex2(M - Mn);
+        // a part that saw nothing or only NaN joins right with any weight (l and
+        // o are 0, or l is NaN), and Mn is at least kNoMax
+        const float a0 = ex2(excess(M, Mn) * p.scale_log2);
         L *= a0;
 #pragma unroll
         for (int e = 0; e < C; ++e) acc[e] *= a0;
 #pragma unroll
         for (int u = 0; u < B; ++u) {
-          const float w = (ml[u].x == -INFINITY) ? (ml[u].y == ml[u].y ? 0.f : 1.f)
-                                                 : ex2(ml[u].x - Mn);
+          const float w = ex2(excess(ml[u].x, Mn) * p.scale_log2);
           L = fmaf(ml[u].y, w, L);
 #pragma unroll
           for (int e = 0; e < C; ++e) acc[e] = fmaf(o[u][e], w, acc[e]);
@@ -1682,7 +1696,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
     const int64_t t = d.cu0 + node;
     const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
     if (lane == 0 && p.lse)
-      p.lse[t * p.H + hq] = L > 0.f ? (M + log2f(L)) * kLn2 : (L == L ? -INFINITY : L);
+      p.lse[t * p.H + hq] = log_sum(M, L, p.scale_log2);
     const int64_t at = t * p.out_st + hq * p.out_sh + lane * C;
     if (p.out_f32) {
       float* o = reinterpret_cast<float*>(p.out) + at;
@@ -1918,6 +1932,7 @@ static int run(const halo_page_pool_t* pool, const halo_tree_problem_t* pb, void
   p.out_sh = pb->out_stride_h;
   p.lse = pb->lse;
   p.scale_log2 = pb->scale * kLog2e;
+  p.headroom = raw_headroom(p.scale_log2);
   p.out_f32 = pb->out_dtype == HALO_DTYPE_F32;
   p.R = pb->R;
   p.T = pb->T;

@@ -1,0 +1,120 @@
+"""Tree attention where scores move the running maximum, against the plain
+restatement in 64 bits."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import running_max as M
+from test_paged_gpu import Case
+
+pytestmark = pytest.mark.gpu
+F = np.float32
+
+
+def _set_scores(c, r, scores):
+    """Raw scores of request ``r``'s positions, exactly: three parts of each in
+    three columns of K, against ones in q."""
+    page = c.k.shape[2]
+    rest = torch.from_numpy(np.asarray(scores, dtype=np.float64))
+    for col in range(3):
+        part = rest.to(c.k.dtype)
+        rest = rest - part.double()
+        for b in range(-(-len(scores) // page)):
+            rows = part[b * page:(b + 1) * page]
+            c.k[c.table[r][b], :, :len(rows), col] = rows
+    assert (rest == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("nodes", [1, 7, 14, 40])
+def test_scores_at_the_headroom(cuda_device, dtype, D, nodes):
+    """120 requests whose maximum rises several times, each time by a score
+    that lies within a few roundings of the headroom."""
+    R = 120
+    scale = F(F(1 / np.sqrt(D)) * M.LOG2E)
+    rng = np.random.default_rng(D + nodes)
+    c = Case(D + nodes, [1100 + int(x) for x in rng.integers(0, 200, R)],
+             [nodes if r % 8 == 0 else 1 for r in range(R)], 4, 1, D, 16, dtype)
+    c.k[:] = 0
+    c.q[:] = 0
+    c.q[:, :, :3] = 1
+    # fp16 holds 24 bits in three parts from 2^-2 up (its steps end at 2^-24)
+    for r in range(R):
+        n = c.ctx[r] + c.cu[r + 1] - c.cu[r]
+        s0 = F(rng.uniform(1, 100))
+        scores = (s0 - rng.uniform(2, 20, n) * 4).astype(F)
+        scores = np.where(np.abs(scores) < 1, F(1), scores)
+        scores[int(rng.integers(0, 100))] = s0
+        for at in (150, 300, 450, 700, 1000):
+            w = M.split_window(s0, scale) if rng.random() < 0.6 else None
+            s0 = M.at_headroom(s0, scale, int(rng.integers(-2, 3))) if w is None else w
+            scores[at + int(rng.integers(0, 60))] = s0
+        _set_scores(c, r, scores)
+    out, lse = c.run(out_dtype=torch.float32)
+    c.check(out, lse)
+
+
+@pytest.mark.parametrize("dtype,top", [(torch.bfloat16, 50), (torch.float16, 8)])
+@pytest.mark.parametrize("nodes", [1, 3, 12, 40, 70])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_any_finite_size(cuda_device, dtype, top, nodes, sign):
+    """Scores whose rounding is more than the headroom, up to 2^100: the
+    position with the largest one has all the weight (two have half each)."""
+    exps = [e for e in (4, 8, 12, 14, 17, 30, 50) if e <= top]
+    R, n_ctx, D = len(exps), 900, 64
+    c = Case(nodes, [n_ctx] * R, [nodes] * R, 4, 1, D, 16, dtype)
+    c.mask[:] = False
+    c.k[:] = 0
+    c.q[:] = 0
+    rng = np.random.default_rng(nodes)
+    best = []
+    for r, e in enumerate(exps):
+        c.q[c.cu[r]:c.cu[r + 1], :, 0] = sign * 2.0 ** e
+        a = rng.integers(1, 100, n_ctx)
+        first, second = 37 + 40 * r, 700
+        a[first], a[second] = (100, 100) if sign > 0 else (0, 0)
+        best.append((first, second))
+        page = c.k.shape[2]
+        for b in range(-(-n_ctx // page)):
+            rows = torch.from_numpy(a[b * page:(b + 1) * page]).to(dtype) * 2.0 ** e
+            c.k[c.table[r][b], :, :len(rows), 0] = rows
+    out, lse = c.run(out_dtype=torch.float32)
+    assert torch.isfinite(out).all()
+    for r, (x, y) in enumerate(best):
+        gap = 4.0 ** exps[r] / math.sqrt(D)        # to every other position
+        assert gap > 30
+        page = c.v.shape[2]
+        v = [c.v[c.table[r][p // page], 0, p % page].double() for p in (x, y)]
+        want = (v[0] + v[1]) / 2
+        got = out[c.cu[r]:c.cu[r + 1]].cpu().double()
+        # two weights of 16 bits each; n weights of at most e^-gap beside them
+        room = (v[0].abs() + v[1].abs()) * 2.0 ** -15 + n_ctx * 5 * math.exp(-gap)
+        assert ((got - want).abs() <= room).all()
+        wl = (100 * 4.0 ** exps[r] / math.sqrt(D) if sign > 0 else 0.0) + math.log(2)
+        room = abs(wl) * 2.0 ** -21 + n_ctx * math.exp(-gap) + 2.0 ** -20
+        assert ((lse[c.cu[r]:c.cu[r + 1]].cpu().double() - wl).abs() <= room).all()
+    from halo_b200 import _lib as L
+    assert L.device_error() == 0
+
+
+@pytest.mark.parametrize("seed", range(6))
+@pytest.mark.parametrize("D", [64, 128])
+def test_maxima_that_rise_often(cuda_device, seed, D):
+    """Contexts whose scores grow with the position, several rises a segment."""
+    rng = np.random.default_rng(seed)
+    nodes = [int(x) for x in rng.integers(1, 17, 40)]
+    c = Case(seed, [int(x) for x in rng.integers(100, 2500, 40)], nodes, 4, 1, D, 16,
+             torch.float16 if seed % 2 else torch.bfloat16)
+    page = c.k.shape[2]
+    for r, row in enumerate(c.table):
+        n = -(-(c.ctx[r] + nodes[r]) // page)
+        for b in range(n):
+            c.k[row[b], :, :, 0] = c.k[row[b], :, :, 0] * 0.2 + 40.0 * (b + 1) / n
+    c.q[:, :, 0] = 2.0 + rng.random()
+    out, lse = c.run(out_dtype=torch.float32)
+    c.check(out, lse)
