@@ -6,7 +6,7 @@
 // Whether it has to move is asked of single scores, and of a row's largest one
 // when it moves: both subtract first, with one rounding, and rounding keeps
 // order, so they cannot disagree.  The difference of near numbers is exact,
-// however large they are, so the largest score's weight stays between 1 and
+// however large they are, so the largest score's e^{..} stays between 1 and
 // 2^8 even where one step of m is more than that.
 #pragma once
 

@@ -319,11 +319,6 @@ __device__ __forceinline__ uint64_t ffma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
-__device__ __forceinline__ uint64_t fmul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 __device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
@@ -335,13 +330,21 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return d;
 }
 
-// Weights of a pair of raw scores, e^(scale (s - m)): their 16-bit values (hi)
-// and remainders (lo); the fp32 pair is returned for the row sum.
+// Weights are 2^kLift e^{scale (s - m)}.  fp16 has steps of 2^-24 below 2^-14,
+// so small weights would be lost from P V while the row sum counts them: lifted
+// by 7 they reach 2^15 beside a headroom of 2^8 (fp16 ends at 2^16) and are off
+// by 2^-32 of the largest at most.  bf16 has fp32's exponents.  The factor is in
+// l and o alike; only the log-sum-exp takes it out.
+template <typename T>
+constexpr float kLift = Elem<T>::kDtype == HALO_DTYPE_F16 ? 7.f : 0.f;
+
+// Weights of a pair of raw scores: their 16-bit values (hi) and remainders
+// (lo); the fp32 pair is returned for the row sum.
 template <typename T>
 __device__ __forceinline__ uint64_t weigh(float s0, float s1, uint64_t sc2, uint64_t nm2,
                                           uint32_t& hi, uint32_t& lo) {
   float x0, x1, h0, h1;
-  f2unpack(fmul2(fadd2(f2pack(s0, s1), nm2), sc2), x0, x1);
+  f2unpack(ffma2(fadd2(f2pack(s0, s1), nm2), sc2, f2pack(kLift<T>, kLift<T>)), x0, x1);
   const float a = ex2(x0), b = ex2(x1);
   if constexpr (Elem<T>::kDtype == HALO_DTYPE_BF16) {   // truncated: one byte permute a pair
     hi = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
@@ -400,8 +403,9 @@ __device__ __forceinline__ bool bad16(uint32_t x) {   // inf or NaN in the low 1
 }
 
 // ln of sum e^{scale s} from the maximum of the raw scores and the sum of weights.
+template <typename T>
 __device__ __forceinline__ float log_sum(float m, float l, float scale_log2) {
-  return l > 0.f ? fmaf(m, scale_log2, log2f(l)) * kLn2 : (l == l ? -INFINITY : l);
+  return l > 0.f ? fmaf(m, scale_log2, log2f(l) - kLift<T>) * kLn2 : (l == l ? -INFINITY : l);
 }
 
 // Barrier `id` of N softmax threads that tells whether any of them voted.
@@ -684,8 +688,8 @@ __device__ __noinline__ float bad_sum(const Params& p, int r, int t, int ctx, in
 // One thread issues a stream's MMAs, which execute in that order: the QK that
 // overwrites P_X follows the PV that reads it without waiting for its end.
 // P is split into a 16-bit value and a 16-bit remainder (two MMAs), ~16
-// significant bits: one 16-bit P would cost up to 2^-9 |v|, as much as the
-// output's own rounding.  Sums, maxima and O are fp32.
+// significant bits (fp16: down to 2^-32 of a row's largest, see kLift): one
+// 16-bit P would cost up to 2^-9 |v|, as much as the output's own rounding.  Sums, maxima and O are fp32.
 //
 // Row groups of more than 128 rows (QT = 2): stream X takes query tile X and
 // both take every K/V tile.  Smaller ones: both streams share the query tile
@@ -967,8 +971,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           }
           mx = fmaxf(mx, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
         }
-        // the maximum moves only past its headroom (weights are at most 2^8),
-        // for both halves of a row at once
+        // the maximum moves only past its headroom (weights are at most 2^8,
+        // lifted 2^15), for both halves of a row at once
         bool rise = it == 0;
         if (it > 0) rise = vote_bar<256>(2 + x, rises(mx, m, p.headroom));
         if (rise) {
@@ -1058,7 +1062,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         const int64_t t = cu0 + node;
         const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
         if (col == 0 && p.lse)
-          p.lse[t * p.H + hq] = log_sum(M, L, p.scale_log2);
+          p.lse[t * p.H + hq] = log_sum<T>(M, L, p.scale_log2);
         const int64_t at = t * p.out_st + hq * p.out_sh + col;
         if (p.out_f32) {
           float4* d = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at);
@@ -1492,7 +1496,8 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
 #pragma unroll
           for (int r = 0; r < RT; r += 2) {
             float a, b;
-            f2unpack(fmul2(f2pack(x[r], x[r + 1]), f2pack(p.scale_log2, p.scale_log2)), a, b);
+            f2unpack(ffma2(f2pack(x[r], x[r + 1]), f2pack(p.scale_log2, p.scale_log2),
+                           f2pack(kLift<T>, kLift<T>)), a, b);
             a = ex2(a);
             b = ex2(b);
             l[r] += a;
@@ -1549,7 +1554,7 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
             const int rq = s.row0 + r, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
             const int64_t row = walk.q.cu0 + node;
             if (p.lse)
-              p.lse[row * p.H + hq] = log_sum(M, L, p.scale_log2);
+              p.lse[row * p.H + hq] = log_sum<T>(M, L, p.scale_log2);
             sh->fac[r] = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
             sh->off[r] = row * p.out_st + hq * p.out_sh;
           }
@@ -1696,7 +1701,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
     const int64_t t = d.cu0 + node;
     const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
     if (lane == 0 && p.lse)
-      p.lse[t * p.H + hq] = log_sum(M, L, p.scale_log2);
+      p.lse[t * p.H + hq] = log_sum<T>(M, L, p.scale_log2);
     const int64_t at = t * p.out_st + hq * p.out_sh + lane * C;
     if (p.out_f32) {
       float* o = reinterpret_cast<float*>(p.out) + at;

@@ -128,7 +128,8 @@ def allowed(reach, vmax, D, n, lse):
     may truncate).  A weight e^(s - m) is off by that factor twice (its own
     score and the maximum) plus 2^-21 from the exponential.  Weights enter
     P V as two 16-bit parts, the second rounded: off by at most 2^-16 of
-    themselves.  The sums over n keys add (n / 8 + 64) * 2^-23: eight or more
+    themselves in bf16; in fp16 by 2^-22 of themselves and 2^-32 of the largest
+    weight, which for n up to 65536 keys is less than 2^-16 of their sum.  The sums over n keys add (n / 8 + 64) * 2^-23: eight or more
     keys a step of the matrix pipe, and at most 64 partial results joined."""
     e = 2.0 * D * 2.0 ** -23 * reach + 2.0 ** -21
     sums = (n / 8 + 64) * 2.0 ** -23

@@ -118,3 +118,33 @@ def test_maxima_that_rise_often(cuda_device, seed, D):
     c.q[:, :, 0] = 2.0 + rng.random()
     out, lse = c.run(out_dtype=torch.float32)
     c.check(out, lse)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("nodes", [1, 7, 14, 20, 40])
+def test_many_small_weights_beside_a_large_one(cuda_device, dtype, nodes):
+    """One position 25.1 log2 units above 300000 equal ones whose V is 1 where
+    its own is 0: their share, 0.8 % together, has to come out whole."""
+    from halo_b200 import ops
+    n, H, H_kv, D, page = 300_000, 32, 8, 64, 64
+    dev = torch.device("cuda")
+    n_pages = -(-(n + nodes) // page)
+    k = torch.zeros(n_pages, H_kv, page, D, dtype=dtype, device=dev)
+    v = torch.ones_like(k)
+    table = torch.randperm(n_pages, generator=torch.Generator().manual_seed(1)).int()
+    k[table[0], :, 5, 0] = 139.0
+    v[table[0], :, 5] = 0
+    q = torch.zeros(nodes, H, D, dtype=dtype, device=dev)
+    q[:, :, 0] = 1
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)      # noqa: E731
+    out, lse = ops.tree_attention(q, k, v, table[None].to(dev), i32([n]), i32([0, nodes]),
+                                  torch.zeros(nodes, nodes, dtype=torch.bool, device=dev),
+                                  out_dtype=torch.float32)
+    w = math.exp(-139 / math.sqrt(D))                      # 2^-25.07 of the large one
+    mass = (n - 1) * w
+    want = mass / (1 + mass)
+    # a weight is off by 2^-32 of the largest (fp16) and by 2^-16 of itself, an
+    # exponential by 2^-21, sums of n keys as oracle.paged.allowed has them
+    room = n * 2.0 ** -32 + mass * (2.0 ** -16 + 2.0 ** -20) + 2 * want * (n / 8 + 64) * 2.0 ** -23
+    assert float((out.double() - want).abs().max()) <= room
+    assert float((lse.double() - (139 / math.sqrt(D) + math.log1p(mass))).abs().max()) <= 1e-5
