@@ -822,7 +822,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
                  (it + 1 == nx || k_landed(g + step));
             const uint64_t vd = opaque(vdesc0 + (uint64_t)((iv * Gm::kTileBytes) >> 4));
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {           // O_X += P_X V(g), as the halves of P come
+            for (int c = 1; c >= 0; --c) {          // O_X += P_X V(g), as the halves of P come
               ok = ok && wait_bar(&bs->p_full[2 * x + c], j & 1, bs, p.err);
               if (!ok) break;
               umma::fence_after_sync();
@@ -831,7 +831,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
                 const int h = kk >> 2, b = (kk >> 1) & 1;
                 umma::mma_ts(oc, pc + h * 64 + c * 32 + (kk & 1) * 16 + b * 8,
                              vd + (uint64_t)(((h * 4 + c * 2 + b) * 2 * Gm::kGroup) >> 4), kIdPV,
-                             it > 0 || c > 0 || kk > 0);
+                             it > 0 || c == 0 || kk > 0);
               }
             }
             if (!ok) break;
@@ -947,7 +947,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         }
         umma::fence_after_sync();
         // 32 positions at a time, read once for the maximum and again for the
-        // weights: 64 of them held would spill
+        // weights: 64 of them held would spill.  The second 32 are weighed
+        // first, from the registers that their maximum left.
         float sv[32];
         auto scores = [&](int c) {
           umma::tmem_ld32(scol + c * 32, sv);
@@ -1002,8 +1003,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         const uint64_t sc2 = f2pack(p.scale_log2, p.scale_log2), nm2 = f2pack(-m, -m);
         uint64_t rs2 = 0;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {      // 16 columns of values, 16 of remainders
-          scores(c);
+        for (int c = 1; c >= 0; --c) {     // 16 columns of values, 16 of remainders
+          if (c == 0) scores(0);
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
             uint32_t hi[8], lo[8];
@@ -1020,7 +1021,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           if (lane == 0) {
             mbar_arrive(&bs->p_full[2 * x + c]);
             // passed on halfway: the other stream's scores are read meanwhile
-            if (c == 0 && (x == 0 ? it < ny : it + 1 < ny)) mbar_arrive(&bs->turn[1 - x]);
+            if (c == 1 && (x == 0 ? it < ny : it + 1 < ny)) mbar_arrive(&bs->turn[1 - x]);
           }
         }
         float rs0, rs1;
