@@ -43,6 +43,12 @@ namespace paged {
 // new tokens: 15.4 us (22.5 us with a binary search a thread; 1.8 us each for
 // the two passes over the requests, 1.7 us for the new entries, 4 us for the
 // pages given back, 5 us for the tokens).
+//
+// STEP is a cache's next step: request r has a context of ctx rows, holds pages
+// for old >= ctx of them (more than ctx where a step was given up) and is to
+// hold ctx + max(count, 0).  Its new rows begin at ctx, in pages it holds
+// already or takes.  old is updated in place: behind the cluster barrier, when
+// every CTA has read it.
 constexpr int kTabThreads = 1024;
 constexpr int kTabMaxReq = 8192;
 constexpr int kTabArrays = 7;      // shared int arrays of R entries
@@ -51,7 +57,10 @@ struct TablesParams {
   int32_t* table;
   int64_t table_stride;
   const int32_t* old_lens;
-  const int32_t* new_lens;
+  const int32_t* new_lens;               // STEP: counts
+  const int32_t* ctx;                    // STEP alone, as rows and held
+  int32_t* rows;                         // new rows granted
+  int32_t* held;                         // old_lens, to be updated
   int32_t* free_pages;
   const int32_t* n_free;
   int32_t* n_free_out;
@@ -91,6 +100,27 @@ __device__ __forceinline__ int blocks(int n, int page) {
   return (int)(b + ((uint32_t)n - b * (uint32_t)page != 0 ? 1u : 0u));
 }
 
+// What request r has and wants: pages for `old` rows now and `want` rows then,
+// new rows from `from` on.  False where that cannot be (a negative length, one
+// that the table cannot hold): the request stays as it is.
+template <bool STEP>
+__device__ __forceinline__ bool load_lens(const TablesParams& p, int r, int& old, int& want,
+                                          int& from) {
+  old = p.old_lens[r];
+  if constexpr (STEP) {
+    from = p.ctx[r];
+    const int64_t n = (int64_t)from + max(p.new_lens[r], 0);
+    want = (int)min(n, (int64_t)INT_MAX);
+    return from >= 0 && from <= old && blocks(old, p.page) <= p.max_blocks &&
+           blocks(want, p.page) <= p.max_blocks;
+  } else {
+    from = old;
+    want = p.new_lens[r];
+    return old >= 0 && want >= 0 && blocks(old, p.page) <= p.max_blocks &&
+           blocks(want, p.page) <= p.max_blocks;
+  }
+}
+
 // First i in [0, n) with a[i] > k (running sums, k < a[n - 1]) for the warp's
 // smallest k, found by all lanes together: 32 probes a step.
 __device__ __forceinline__ int warp_find(const int32_t* a, int n, int k) {
@@ -106,6 +136,7 @@ __device__ __forceinline__ int warp_find(const int32_t* a, int n, int k) {
   return lo;
 }
 
+template <bool STEP>
 __global__ void __launch_bounds__(kTabThreads) tables_kernel(const TablesParams p) {
   extern __shared__ int32_t sm[];
   __shared__ int64_t s_warp[32];
@@ -113,7 +144,7 @@ __global__ void __launch_bounds__(kTabThreads) tables_kernel(const TablesParams 
   int32_t* s_need = sm;                  // inclusive running sums
   int32_t* s_give = sm + p.R;
   int32_t* s_tok = sm + 2 * p.R;
-  int32_t* s_old = sm + 3 * p.R;
+  int32_t* s_old = sm + 3 * p.R;         // positions of its new rows: from, to
   int32_t* s_new = sm + 4 * p.R;
   int32_t* s_ob = sm + 5 * p.R;          // pages held before, and asked for
   int32_t* s_nb = sm + 6 * p.R;
@@ -130,16 +161,14 @@ __global__ void __launch_bounds__(kTabThreads) tables_kernel(const TablesParams 
     const int r = base + threadIdx.x;
     int64_t v = 0;
     if (r < p.R) {
-      const int o = p.old_lens[r], n = p.new_lens[r];
+      int o, n, from;
+      const bool ok = load_lens<STEP>(p, r, o, n, from);
       const int ob = blocks(o, p.page), nb = blocks(n, p.page);
-      // a length that is negative or that the table cannot hold is refused:
-      // the request stays as it is (new = old)
-      const bool ok = o >= 0 && n >= 0 && ob <= p.max_blocks && nb <= p.max_blocks;
       if (ok) v = nb > ob ? nb - ob : (int64_t)(ob - nb) << 32;
-      s_old[r] = o;
+      s_old[r] = from;
       s_ob[r] = ob;
       s_nb[r] = nb;
-      s_new[r] = ok ? n : o;
+      s_new[r] = ok ? n : from;
     }
     const int64_t s = carry + block_scan(v, s_warp, &total);
     carry += total;
@@ -172,7 +201,8 @@ __global__ void __launch_bounds__(kTabThreads) tables_kernel(const TablesParams 
       s_tok[r] = c;
       if (rank == 0) {
         p.cu[r + 1] = c;
-        p.lens[r] = s_new[r];
+        if constexpr (STEP) p.rows[r] = (int32_t)v;
+        else p.lens[r] = s_new[r];
       }
     }
   }
@@ -216,6 +246,14 @@ __global__ void __launch_bounds__(kTabThreads) tables_kernel(const TablesParams 
 
   cl.sync();                             // all table entries are written, n_free was read
   if (rank == 0 && threadIdx.x == 0) *p.n_free_out = left;
+  if constexpr (STEP) {
+    for (int r = i0; r < p.R; r += di) {
+      int o, n, from;
+      if (!load_lens<STEP>(p, r, o, n, from)) continue;
+      const bool needs = s_need[r] > (r > 0 ? s_need[r - 1] : 0);
+      if (!needs || s_need[r] <= have) p.held[r] = n;
+    }
+  }
 
   // the slots of the new tokens (a row without a token gets -1), two of them
   // kTabThreads apart in flight
@@ -441,6 +479,62 @@ static int vec_bytes(uint64_t bits) {
   return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
 }
 
+// Launch of either form; lengths, tables and outputs are checked by the callers.
+template <bool STEP>
+static int launch_tables(const TablesParams& p, halo_stream_t stream) {
+  const size_t smem = (size_t)kTabArrays * p.R * sizeof(int32_t);
+  static std::once_flag once[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  cudaError_t e = cudaSuccess;
+  std::call_once(once[dev & 63], [&] {
+    e = cudaFuncSetAttribute(tables_kernel<STEP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kTabArrays * kTabMaxReq * (int)sizeof(int32_t));
+  });
+  if (e != cudaSuccess) return cuda_fail(e, "tables_kernel shared-memory attribute");
+  // two tokens a thread before another CTA joins
+  const int n_cta = std::min(8, std::max(1, p.T / (2 * kTabThreads)));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)n_cta);
+  cfg.blockDim = dim3(kTabThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)n_cta;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, tables_kernel<STEP>, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "tables_kernel launch");
+  count_launches();
+  return HALO_OK;
+}
+
+// Sizes that both forms have in common.
+static int check_tables(int64_t table_stride, int32_t R, int32_t max_blocks, int32_t free_capacity,
+                        int32_t page_size, int32_t max_tokens) {
+  if (R < 0 || max_blocks < 0 || free_capacity < 0 || max_tokens < 0 || page_size <= 0)
+    return fail(HALO_ERR_INVALID_ARG, "bad size (R=%d max_blocks=%d free=%d max_tokens=%d page_size=%d)",
+                R, max_blocks, free_capacity, max_tokens, page_size);
+  if (max_tokens > (1 << 30) || free_capacity > (1 << 30))
+    return fail(HALO_ERR_UNSUPPORTED, "%d tokens, %d pages", max_tokens, free_capacity);
+  if (R > kTabMaxReq) return fail(HALO_ERR_UNSUPPORTED, "%d requests (at most %d)", R, kTabMaxReq);
+  if ((int64_t)R * max_blocks > INT_MAX || ((int64_t)max_blocks + 1) * page_size > INT_MAX)
+    return fail(HALO_ERR_UNSUPPORTED, "block tables of %d x %d pages of %d are too large", R,
+                max_blocks, page_size);
+  if (R > 1 && table_stride < max_blocks)
+    return fail(HALO_ERR_INVALID_ARG, "block table rows overlap (stride %lld < %d)",
+                (long long)table_stride, max_blocks);
+  return HALO_OK;
+}
+
+static uint32_t magic(int32_t page_size) {
+  return (uint32_t)(((1ull << 32) + page_size - 1) / page_size);
+}
+
 }  // namespace paged
 }  // namespace halo
 
@@ -455,58 +549,45 @@ extern "C" int32_t halo_update_block_tables(int32_t* block_tables, int64_t table
                                             int32_t* cu_tokens, int32_t* lens,
                                             halo_stream_t stream) {
   using namespace halo::paged;
-  if (R < 0 || max_blocks < 0 || free_capacity < 0 || max_tokens < 0 || page_size <= 0)
-    return fail(HALO_ERR_INVALID_ARG, "bad size (R=%d max_blocks=%d free=%d max_tokens=%d page_size=%d)",
-                R, max_blocks, free_capacity, max_tokens, page_size);
-  if (max_tokens > (1 << 30) || free_capacity > (1 << 30))
-    return fail(HALO_ERR_UNSUPPORTED, "%d tokens, %d pages", max_tokens, free_capacity);
-  if (R > kTabMaxReq) return fail(HALO_ERR_UNSUPPORTED, "%d requests (at most %d)", R, kTabMaxReq);
-  if ((int64_t)R * max_blocks > INT_MAX || ((int64_t)max_blocks + 1) * page_size > INT_MAX)
-    return fail(HALO_ERR_UNSUPPORTED, "block tables of %d x %d pages of %d are too large", R,
-                max_blocks, page_size);
+  const int rc = check_tables(table_stride, R, max_blocks, free_capacity, page_size, max_tokens);
+  if (rc != HALO_OK) return rc;
   if ((R > 0 && (!old_lens || !new_lens || !lens || (max_blocks > 0 && !block_tables))) ||
       (free_capacity > 0 && !free_pages) || !n_free || !n_free_out || !cu_tokens ||
       (max_tokens > 0 && (!slots || !positions)))
     return fail(HALO_ERR_INVALID_ARG, "NULL pointer");
-  if (R > 1 && table_stride < max_blocks)
-    return fail(HALO_ERR_INVALID_ARG, "block table rows overlap (stride %lld < %d)",
-                (long long)table_stride, max_blocks);
   // several CTAs read the lengths, one writes them
   if ((lens < old_lens + R && old_lens < lens + R) || (lens < new_lens + R && new_lens < lens + R))
     return fail(HALO_ERR_INVALID_ARG, "lens overlaps the lengths it is made from");
-  const size_t smem = (size_t)kTabArrays * R * sizeof(int32_t);
-  static std::once_flag once[64];
-  int dev = 0;
-  cudaGetDevice(&dev);
-  cudaError_t e = cudaSuccess;
-  std::call_once(once[dev & 63], [&] {
-    e = cudaFuncSetAttribute(tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kTabArrays * kTabMaxReq * (int)sizeof(int32_t));
-  });
-  if (e != cudaSuccess) return cuda_fail(e, "tables_kernel shared-memory attribute");
-  const TablesParams p{block_tables, table_stride, old_lens, new_lens, free_pages, n_free,
-                       n_free_out, slots, positions, cu_tokens, lens, R, max_blocks, page_size,
-                       free_capacity, max_tokens,
-                       (uint32_t)(((1ull << 32) + page_size - 1) / page_size)};
-  // two tokens a thread before another CTA joins
-  const int n_cta = std::min(8, std::max(1, max_tokens / (2 * kTabThreads)));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)n_cta);
-  cfg.blockDim = dim3(kTabThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)n_cta;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, tables_kernel, p);
-  if (e == cudaSuccess) e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "tables_kernel launch");
-  count_launches();
-  return HALO_OK;
+  return launch_tables<false>(
+      TablesParams{block_tables, table_stride, old_lens, new_lens, nullptr, nullptr, nullptr,
+                   free_pages, n_free, n_free_out, slots, positions, cu_tokens, lens, R, max_blocks,
+                   page_size, free_capacity, max_tokens, magic(page_size)}, stream);
+}
+
+extern "C" int32_t halo_extend_block_tables(int32_t* block_tables, int64_t table_stride, int32_t R,
+                                            int32_t max_blocks, int32_t* held_lens,
+                                            const int32_t* context_lens, const int32_t* counts,
+                                            int32_t* free_pages, int32_t free_capacity,
+                                            int32_t* n_free, int32_t page_size, int32_t max_tokens,
+                                            int64_t* slots, int64_t* positions, int32_t* cu_tokens,
+                                            int32_t* rows, halo_stream_t stream) {
+  using namespace halo::paged;
+  const int rc = check_tables(table_stride, R, max_blocks, free_capacity, page_size, max_tokens);
+  if (rc != HALO_OK) return rc;
+  if ((R > 0 && (!held_lens || !context_lens || !counts || !rows ||
+                 (max_blocks > 0 && !block_tables))) ||
+      (free_capacity > 0 && !free_pages) || !n_free || !cu_tokens ||
+      (max_tokens > 0 && (!slots || !positions)))
+    return fail(HALO_ERR_INVALID_ARG, "NULL pointer");
+  // several CTAs read the lengths, one writes rows early and held late
+  const auto overlap = [&](const int32_t* a, const int32_t* b) { return a < b + R && b < a + R; };
+  if (overlap(rows, held_lens) || overlap(rows, context_lens) || overlap(rows, counts) ||
+      overlap(held_lens, context_lens) || overlap(held_lens, counts))
+    return fail(HALO_ERR_INVALID_ARG, "rows or held_lens overlaps the lengths it is made from");
+  return launch_tables<true>(
+      TablesParams{block_tables, table_stride, held_lens, counts, context_lens, rows, held_lens,
+                   free_pages, n_free, n_free, slots, positions, cu_tokens, nullptr, R, max_blocks,
+                   page_size, free_capacity, max_tokens, magic(page_size)}, stream);
 }
 
 extern "C" int32_t halo_write_kv_pages(const halo_page_pool_t* pool, const void* k,

@@ -626,6 +626,39 @@ def update_block_tables(block_tables: torch.Tensor, old_lens: torch.Tensor, new_
     return slots, positions, cu, lens
 
 
+def extend_block_tables(block_tables: torch.Tensor, held_lens: torch.Tensor,
+                        context_lens: torch.Tensor, counts: torch.Tensor, rows: torch.Tensor,
+                        free_pages: torch.Tensor, n_free: torch.Tensor, *, page_size: int,
+                        max_tokens: int):
+    """``update_block_tables`` for a cache's next step
+    (``halo_extend_block_tables``): room for ``counts (R,)`` rows (none where
+    negative) behind contexts of ``context_lens`` rows, in pages that
+    ``held_lens`` rows hold already or off the free list.  ``held_lens`` is
+    updated in place and ``rows (R,)`` gets the rows granted to each request,
+    0 for one whose rows do not fit.  Returns ``(slots, positions,
+    cu_tokens)`` of the granted rows."""
+    if not block_tables.is_cuda:
+        _refuse("block_tables must be a CUDA tensor (no CPU path)")
+    dev = block_tables.device
+    index = dev.index
+    R, max_blocks, tstride = _table(block_tables, index)
+    _int32s(index, {"held_lens": (held_lens, R), "context_lens": (context_lens, R),
+                    "counts": (counts, R), "rows": (rows, R),
+                    "free_pages": (free_pages, free_pages.numel()), "n_free": (n_free, 1)})
+    if max_tokens < 0:
+        _refuse("max_tokens must not be negative")
+    slots = torch.empty(max_tokens, dtype=torch.int64, device=dev)
+    positions = torch.empty(max_tokens, dtype=torch.int64, device=dev)
+    cu = torch.empty(R + 1, dtype=torch.int32, device=dev)
+    rc = _call(L.lib().halo_extend_block_tables, index, block_tables.data_ptr(), tstride, R,
+               max_blocks, held_lens.data_ptr(), context_lens.data_ptr(), counts.data_ptr(),
+               free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(), page_size, max_tokens,
+               slots.data_ptr(), positions.data_ptr(), cu.data_ptr(), rows.data_ptr())
+    if rc:
+        L.check(rc, "halo_extend_block_tables")
+    return slots, positions, cu
+
+
 def write_kv_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                    slots: torch.Tensor) -> None:
     """Copy K/V rows ``(T, H_kv, D)`` into the slots ``(T,)`` (int64) of page

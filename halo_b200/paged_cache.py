@@ -47,18 +47,19 @@ class PagedKVCache:
         self.block_tables = torch.zeros(max_requests, blocks, dtype=torch.int32, device=dev)
         self.free_pages = torch.arange(n_pages, dtype=torch.int32, device=dev)
         self.n_free = torch.full((1,), n_pages, dtype=torch.int32, device=dev)
-        # rows of each request's context, and with the rows of the step under way
+        # rows of each request's context, of the step under way, and rows whose
+        # pages the request holds
         self.lens = torch.zeros(max_requests, dtype=torch.int32, device=dev)
+        self.step = torch.zeros(max_requests, dtype=torch.int32, device=dev)
         self.held = torch.zeros(max_requests, dtype=torch.int32, device=dev)
 
     def extend(self, counts: torch.Tensor, max_tokens: int) -> PagedRows:
-        """Room for ``counts[r]`` (int32, at most ``max_tokens`` in all) rows
-        behind each request's context."""
-        slots, pos, cu, held = ops.update_block_tables(
-            self.block_tables, self.held, self.lens + counts.clamp(min=0), self.free_pages, self.n_free,
-            page_size=self.page_size, max_tokens=max_tokens)
-        self.held.copy_(held)
-        return PagedRows(slots, pos, cu)
+        """Begin a step: room for ``counts[r]`` (int32, at most ``max_tokens`` in
+        all) rows behind each request's context.  A step that was begun before
+        and not accepted is given up: its rows are room again."""
+        return PagedRows(*ops.extend_block_tables(
+            self.block_tables, self.held, self.lens, counts.contiguous(), self.step, self.free_pages,
+            self.n_free, page_size=self.page_size, max_tokens=max_tokens))
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, rows: PagedRows) -> None:
         """Store the step's K/V rows ``(max_tokens, H_kv, D)``."""
@@ -74,14 +75,14 @@ class PagedKVCache:
         """End the step: request ``r`` keeps the rows ``path[r, :path_lens[r]]``
         of its step (``None``: its first ``path_lens[r]`` rows; never more than
         the step gave it) and gives the other pages back."""
-        # no step of a path may reach behind held: table entries there name
-        # pages that another request may own by now
-        keep = torch.minimum(path_lens.clamp(0, None if path is None else path.shape[1]),
-                             self.held - self.lens)
+        # no step of a path may reach behind the rows of its step: table entries
+        # there name pages that another request may own by now
+        keep = torch.minimum(path_lens.clamp(0, None if path is None else path.shape[1]), self.step)
         if path is not None:
             for k, v in zip(self.k, self.v):
                 ops.commit_tree_path(k, v, self.block_tables, self.lens, path, keep)
         self.lens.copy_(self._resize(self.lens + keep))
+        self.step.zero_()
 
     def release(self, ended: torch.Tensor) -> None:
         """Empty the requests where ``ended (max_requests,)`` is true; others
@@ -89,6 +90,7 @@ class PagedKVCache:
         rows of that step are nobody's: they may not be written any more)."""
         self._resize(self.held.masked_fill(ended, 0))
         self.lens.masked_fill_(ended, 0)
+        self.step.masked_fill_(ended, 0)
 
     def _resize(self, lens: torch.Tensor) -> torch.Tensor:
         _, _, _, held = ops.update_block_tables(

@@ -460,6 +460,23 @@ int32_t halo_update_block_tables(int32_t* block_tables, int64_t table_stride, in
                                  int64_t* slots, int64_t* positions, int32_t* cu_tokens,
                                  int32_t* lens, halo_stream_t stream);
 
+/* The same for a cache's next step, in one launch: request r has a context of
+ * context_lens[r] rows and pages for held_lens[r] >= context_lens[r] of them
+ * (more than its context where a step was begun and given up).  It asks for
+ * max(counts[r], 0) rows behind its context, in pages it holds or takes;
+ * pages it holds beyond them are given back.  Granted, held_lens[r] becomes
+ * the context and those rows (in place) and rows[r] their number; refused
+ * (as above), it stays as it is and rows[r] is 0.  slots, positions and
+ * cu_tokens (the running count of rows) describe the granted rows.  held_lens
+ * and rows overlap neither one another nor context_lens or counts. */
+int32_t halo_extend_block_tables(int32_t* block_tables, int64_t table_stride, int32_t R,
+                                 int32_t max_blocks, int32_t* held_lens,
+                                 const int32_t* context_lens, const int32_t* counts,
+                                 int32_t* free_pages, int32_t free_capacity, int32_t* n_free,
+                                 int32_t page_size, int32_t max_tokens, int64_t* slots,
+                                 int64_t* positions, int32_t* cu_tokens, int32_t* rows,
+                                 halo_stream_t stream);
+
 /* Copy K and V rows k, v (T, H_kv, D) (element strides *_stride_t,
  * *_stride_h) into the slots (T) of the pool.  Rows whose slot is negative
  * or beyond the pool are skipped.  Slots are distinct: of two rows with one
