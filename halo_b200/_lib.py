@@ -115,13 +115,13 @@ class TreeProblem(ctypes.Structure):
                 ("mask", ctypes.c_void_p), ("mask_stride", ctypes.c_int64),
                 ("out", ctypes.c_void_p), ("out_stride_t", ctypes.c_int64),
                 ("out_stride_h", ctypes.c_int64), ("out_dtype", ctypes.c_int32),
-                ("lse", ctypes.c_void_p)]
+                ("lse", ctypes.c_void_p), ("node_starts", ctypes.c_void_p)]
 
 
 # The two descriptions above as packed bytes, which cost a call a fraction of
 # what filling the ctypes structures does; entry points take either.
 pack_page_pool = struct.Struct("=QQ6q5i4x").pack
-pack_tree_problem = struct.Struct("=5ifQ2qQqQQQqQ2qi4xQ").pack
+pack_tree_problem = struct.Struct("=5ifQ2qQqQQQqQ2qi4x2Q").pack
 
 
 # name -> (restype, argtypes); must match include/halo_b200.h
@@ -204,7 +204,8 @@ SIGNATURES = {
                                                   ctypes.c_void_p, ctypes.c_int32,
                                                   ctypes.c_int32, ctypes.c_void_p,
                                                   ctypes.c_void_p, ctypes.c_void_p,
-                                                  ctypes.c_void_p, ctypes.c_void_p]),
+                                                  ctypes.c_void_p, ctypes.c_void_p,
+                                                  ctypes.c_void_p]),
     "halo_write_kv_pages": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_void_p,
                                              ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
                                              ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,

@@ -47,8 +47,10 @@ namespace paged {
 // STEP is a cache's next step: request r has a context of ctx rows, holds pages
 // for old >= ctx of them (more than ctx where a step was given up) and is to
 // hold ctx + max(count, 0).  Its new rows begin at ctx, in pages it holds
-// already or takes.  old is updated in place: behind the cluster barrier, when
-// every CTA has read it.
+// already or takes.  The caller has packed its rows by the counts and does not
+// know who is refused, so every request has its count's places in the slots,
+// refused ones filled with -1.  old is updated in place: behind the cluster
+// barrier, when every CTA has read it.
 constexpr int kTabThreads = 1024;
 constexpr int kTabMaxReq = 8192;
 constexpr int kTabArrays = 7;      // shared int arrays of R entries
@@ -60,6 +62,7 @@ struct TablesParams {
   const int32_t* new_lens;               // STEP: counts
   const int32_t* ctx;                    // STEP alone, as rows and held
   int32_t* rows;                         // new rows granted
+  int32_t* starts;                       // places of its rows
   int32_t* held;                         // old_lens, to be updated
   int32_t* free_pages;
   const int32_t* n_free;
@@ -181,7 +184,9 @@ __global__ void __launch_bounds__(kTabThreads) tables_kernel(const TablesParams 
   const int have = (int)min((int64_t)n_free + n_give, (int64_t)p.cap);
   __syncthreads();
 
-  // pass 2: who is granted, and the running count of new tokens
+  // pass 2: who is granted, and the running count of new tokens (STEP: of
+  // those granted, and of those asked for, which the places go by)
+  int64_t asked = 0;
   carry = 0;
   int used = 0;
   for (int base = 0; base < p.R; base += kTabThreads) {
@@ -198,11 +203,20 @@ __global__ void __launch_bounds__(kTabThreads) tables_kernel(const TablesParams 
     carry += total;
     if (r < p.R) {
       const int32_t c = (int32_t)min(s, (int64_t)INT_MAX);
-      s_tok[r] = c;
+      if constexpr (!STEP) s_tok[r] = c;
       if (rank == 0) {
         p.cu[r + 1] = c;
         if constexpr (STEP) p.rows[r] = (int32_t)v;
         else p.lens[r] = s_new[r];
+      }
+    }
+    if constexpr (STEP) {
+      const int64_t n = r < p.R ? max(p.new_lens[r], 0) : 0;
+      const int64_t end = asked + block_scan(n, s_warp, &total);
+      asked += total;
+      if (r < p.R) {
+        s_tok[r] = (int32_t)min(end, (int64_t)INT_MAX);
+        if (rank == 0) p.starts[r] = (int32_t)min(end - n, (int64_t)INT_MAX);
       }
     }
   }
@@ -210,7 +224,7 @@ __global__ void __launch_bounds__(kTabThreads) tables_kernel(const TablesParams 
   __syncthreads();
   used = s_used;
   if (rank == 0 && threadIdx.x == 0) p.cu[0] = 0;
-  const int n_tok = (int)min(carry, (int64_t)p.T);
+  const int n_tok = (int)min(STEP ? asked : carry, (int64_t)p.T);
   const int i0 = rank * kTabThreads + threadIdx.x, di = n_cta * kTabThreads;
   const int lane = threadIdx.x & 31;
   // Entry k of the stack: the free list, then the pages given back.  `low` is
@@ -269,12 +283,15 @@ __global__ void __launch_bounds__(kTabThreads) tables_kernel(const TablesParams 
         const int t = (int)te + lane;
         if (t < n_tok) {
           while (t >= s_tok[r]) ++r;
-          pos[e] = s_old[r] + (t - (r > 0 ? s_tok[r - 1] : 0));
-          int b = (int)__umulhi((uint32_t)pos[e], p.page_magic);   // exact or one more
-          if (p.page == 1) b = pos[e];
-          b -= (uint32_t)b * (uint32_t)p.page > (uint32_t)pos[e] ? 1 : 0;
-          slot[e] = (int64_t)p.table[(int64_t)r * p.table_stride + b] * p.page +
-                    (pos[e] - b * p.page);
+          const int i = t - (r > 0 ? s_tok[r - 1] : 0);
+          if (!STEP || i < s_new[r] - s_old[r]) {   // not one that was refused
+            pos[e] = s_old[r] + i;
+            int b = (int)__umulhi((uint32_t)pos[e], p.page_magic);   // exact or one more
+            if (p.page == 1) b = pos[e];
+            b -= (uint32_t)b * (uint32_t)p.page > (uint32_t)pos[e] ? 1 : 0;
+            slot[e] = (int64_t)p.table[(int64_t)r * p.table_stride + b] * p.page +
+                      (pos[e] - b * p.page);
+          }
         }
       }
     }
@@ -560,7 +577,7 @@ extern "C" int32_t halo_update_block_tables(int32_t* block_tables, int64_t table
     return fail(HALO_ERR_INVALID_ARG, "lens overlaps the lengths it is made from");
   return launch_tables<false>(
       TablesParams{block_tables, table_stride, old_lens, new_lens, nullptr, nullptr, nullptr,
-                   free_pages, n_free, n_free_out, slots, positions, cu_tokens, lens, R, max_blocks,
+                   nullptr, free_pages, n_free, n_free_out, slots, positions, cu_tokens, lens, R, max_blocks,
                    page_size, free_capacity, max_tokens, magic(page_size)}, stream);
 }
 
@@ -570,23 +587,27 @@ extern "C" int32_t halo_extend_block_tables(int32_t* block_tables, int64_t table
                                             int32_t* free_pages, int32_t free_capacity,
                                             int32_t* n_free, int32_t page_size, int32_t max_tokens,
                                             int64_t* slots, int64_t* positions, int32_t* cu_tokens,
-                                            int32_t* rows, halo_stream_t stream) {
+                                            int32_t* rows, int32_t* starts,
+                                            halo_stream_t stream) {
   using namespace halo::paged;
   const int rc = check_tables(table_stride, R, max_blocks, free_capacity, page_size, max_tokens);
   if (rc != HALO_OK) return rc;
-  if ((R > 0 && (!held_lens || !context_lens || !counts || !rows ||
+  if ((R > 0 && (!held_lens || !context_lens || !counts || !rows || !starts ||
                  (max_blocks > 0 && !block_tables))) ||
       (free_capacity > 0 && !free_pages) || !n_free || !cu_tokens ||
       (max_tokens > 0 && (!slots || !positions)))
     return fail(HALO_ERR_INVALID_ARG, "NULL pointer");
-  // several CTAs read the lengths, one writes rows early and held late
+  // several CTAs read the lengths, one writes rows and starts early and held late
   const auto overlap = [&](const int32_t* a, const int32_t* b) { return a < b + R && b < a + R; };
   if (overlap(rows, held_lens) || overlap(rows, context_lens) || overlap(rows, counts) ||
-      overlap(held_lens, context_lens) || overlap(held_lens, counts))
-    return fail(HALO_ERR_INVALID_ARG, "rows or held_lens overlaps the lengths it is made from");
+      overlap(held_lens, context_lens) || overlap(held_lens, counts) ||
+      overlap(starts, held_lens) || overlap(starts, context_lens) || overlap(starts, counts) ||
+      overlap(starts, rows))
+    return fail(HALO_ERR_INVALID_ARG, "held_lens, rows or starts overlap one another or what they "
+                "are made from");
   return launch_tables<true>(
-      TablesParams{block_tables, table_stride, held_lens, counts, context_lens, rows, held_lens,
-                   free_pages, n_free, n_free, slots, positions, cu_tokens, nullptr, R, max_blocks,
+      TablesParams{block_tables, table_stride, held_lens, counts, context_lens, rows, starts,
+                   held_lens, free_pages, n_free, n_free, slots, positions, cu_tokens, nullptr, R, max_blocks,
                    page_size, free_capacity, max_tokens, magic(page_size)}, stream);
 }
 

@@ -52,6 +52,7 @@ struct alignas(64) Params {
   int64_t table_stride;
   const int32_t* ctx;
   const int32_t* cu;
+  const int32_t* starts;               // where a request's rows begin: cu itself unless given
   const uint8_t* mask;
   int64_t mask_stride;
   char* out;
@@ -207,8 +208,8 @@ template <int RG>
 __device__ __forceinline__ Req load_req(const Params& p, int r) {
   Req q;
   const int lim = p.max_blocks * p.page;
-  q.cu0 = min(max(p.cu[r], 0), p.T);
-  q.nodes = min(min(max(p.cu[r + 1] - q.cu0, 0), p.max_nodes), p.T - q.cu0);
+  q.cu0 = min(max(p.starts[r], 0), p.T);
+  q.nodes = min(min(max(p.cu[r + 1] - max(p.cu[r], 0), 0), p.max_nodes), p.T - q.cu0);
   q.ctx = min(max(p.ctx[r], 0), lim);
   q.end = min(q.ctx + q.nodes, lim);
   q.ng = (q.nodes * p.G + RG - 1) / RG;
@@ -1931,6 +1932,7 @@ static int run(const halo_page_pool_t* pool, const halo_tree_problem_t* pb, void
   p.table_stride = pb->table_stride;
   p.ctx = pb->context_lens;
   p.cu = pb->cu_nodes;
+  p.starts = pb->node_starts ? pb->node_starts : pb->cu_nodes;
   p.mask = pb->mask;
   p.mask_stride = pb->mask_stride;
   p.out = static_cast<char*>(pb->out);

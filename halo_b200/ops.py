@@ -628,22 +628,25 @@ def update_block_tables(block_tables: torch.Tensor, old_lens: torch.Tensor, new_
 
 def extend_block_tables(block_tables: torch.Tensor, held_lens: torch.Tensor,
                         context_lens: torch.Tensor, counts: torch.Tensor, rows: torch.Tensor,
-                        free_pages: torch.Tensor, n_free: torch.Tensor, *, page_size: int,
-                        max_tokens: int):
+                        starts: torch.Tensor, free_pages: torch.Tensor, n_free: torch.Tensor,
+                        *, page_size: int, max_tokens: int):
     """``update_block_tables`` for a cache's next step
     (``halo_extend_block_tables``): room for ``counts (R,)`` rows (none where
     negative) behind contexts of ``context_lens`` rows, in pages that
     ``held_lens`` rows hold already or off the free list.  ``held_lens`` is
     updated in place and ``rows (R,)`` gets the rows granted to each request,
-    0 for one whose rows do not fit.  Returns ``(slots, positions,
-    cu_tokens)`` of the granted rows."""
+    0 for one whose rows do not fit.
+
+    Returns ``(slots, positions, cu_tokens)``: places for all rows asked for,
+    those of request ``r`` from ``starts[r]`` on (also written, ``(R,)``), -1
+    where it is refused, and the running count of rows granted."""
     if not block_tables.is_cuda:
         _refuse("block_tables must be a CUDA tensor (no CPU path)")
     dev = block_tables.device
     index = dev.index
     R, max_blocks, tstride = _table(block_tables, index)
     _int32s(index, {"held_lens": (held_lens, R), "context_lens": (context_lens, R),
-                    "counts": (counts, R), "rows": (rows, R),
+                    "counts": (counts, R), "rows": (rows, R), "starts": (starts, R),
                     "free_pages": (free_pages, free_pages.numel()), "n_free": (n_free, 1)})
     if max_tokens < 0:
         _refuse("max_tokens must not be negative")
@@ -653,7 +656,8 @@ def extend_block_tables(block_tables: torch.Tensor, held_lens: torch.Tensor,
     rc = _call(L.lib().halo_extend_block_tables, index, block_tables.data_ptr(), tstride, R,
                max_blocks, held_lens.data_ptr(), context_lens.data_ptr(), counts.data_ptr(),
                free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(), page_size, max_tokens,
-               slots.data_ptr(), positions.data_ptr(), cu.data_ptr(), rows.data_ptr())
+               slots.data_ptr(), positions.data_ptr(), cu.data_ptr(), rows.data_ptr(),
+               starts.data_ptr())
     if rc:
         L.check(rc, "halo_extend_block_tables")
     return slots, positions, cu
@@ -712,7 +716,8 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                    block_tables: torch.Tensor, context_lens: torch.Tensor, cu_nodes: torch.Tensor,
                    tree_mask: torch.Tensor, *, scale: Optional[float] = None,
                    out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None,
-                   lse: Optional[torch.Tensor] = None, want_lse: bool = True):
+                   lse: Optional[torch.Tensor] = None, want_lse: bool = True,
+                   node_starts: Optional[torch.Tensor] = None):
     """Attention of drafted token trees over a paged K/V cache
     (``halo_tree_attention``).
 
@@ -722,11 +727,13 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     before.  A node sees every position of its context and the nodes ``j``
     with ``tree_mask[row, j]`` (bool ``(T, max_nodes)``); one that sees
     nothing gets zeros and a log-sum-exp of -inf.  With one node a request
-    and a mask of ones this is a decode step over the paged cache.
+    and a mask of ones this is a decode step over the paged cache.  With
+    ``node_starts (R,)`` request ``r``'s ``cu_nodes[r + 1] - cu_nodes[r]`` rows
+    begin there instead of at ``cu_nodes[r]``.
 
     Returns ``(out (T, H, D), lse (T, H))``; ``lse`` is ``None`` with
-    ``want_lse=False`` and none given.  Rows from ``cu_nodes[R]`` on are not
-    written.  bf16/fp16, head dim 64 or 128, a page size that is a multiple
+    ``want_lse=False`` and none given.  Rows that are no request's (those
+    from ``cu_nodes[R]`` on) are not written.  bf16/fp16, head dim 64 or 128, a page size that is a multiple
     of 8."""
     if not q.is_cuda:
         _refuse("q must be a CUDA tensor (no CPU path)")
@@ -741,6 +748,8 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
             context_lens.numel() == R and cu_nodes.numel() == R + 1 and
             context_lens.is_contiguous() and cu_nodes.is_contiguous()):
         _int32s(index, {"context_lens": (context_lens, R), "cu_nodes": (cu_nodes, R + 1)})
+    if node_starts is not None:
+        _int32s(index, {"node_starts": (node_starts, R)})
     mshape, mstride = tree_mask.shape, tree_mask.stride()
     if len(mshape) != 2 or mshape[0] != T or tree_mask.get_device() != index or \
             tree_mask.dtype not in (torch.bool, torch.uint8) or (mshape[1] > 1 and mstride[1] != 1):
@@ -766,14 +775,16 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     if _get_device() != index:
         with torch.cuda.device(index):
             return tree_attention(q, k_pages, v_pages, block_tables, context_lens, cu_nodes,
-                                  tree_mask, scale=scale, out=out, lse=lse, want_lse=want_lse)
+                                  tree_mask, scale=scale, out=out, lse=lse, want_lse=want_lse,
+                                  node_starts=node_starts)
     max_nodes = mshape[1]
     prob = L.pack_tree_problem(R, T, H, max_nodes, max_blocks,
                                scale if scale is not None else 1.0 / math.sqrt(D), q.data_ptr(), qt,
                                qh, block_tables.data_ptr(), tstride, context_lens.data_ptr(),
                                cu_nodes.data_ptr(), tree_mask.data_ptr(), mstride[0],
                                out.data_ptr(), ot, oh, L.halo_dtype(out.dtype),
-                               lse.data_ptr() if lse is not None else 0)
+                               lse.data_ptr() if lse is not None else 0,
+                               node_starts.data_ptr() if node_starts is not None else 0)
     lib, stream = L.lib(), L.stream_handle_of(index)
     key = (index, D, H_kv, H, max_nodes, R > 0 and T > 0)
     need = _TREE_BYTES.get(key)

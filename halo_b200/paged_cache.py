@@ -25,10 +25,13 @@ from halo_b200 import ops
 
 
 class PagedRows(NamedTuple):
-    """Rows of one step, packed in request order (``ops.update_block_tables``).
-    ``cu[r + 1] - cu[r]`` is 0 for a request whose rows the pool cannot hold."""
-    slots: torch.Tensor        # int64 (max_tokens,), -1 behind the last row
-    positions: torch.Tensor    # int64 (max_tokens,), -1 behind the last row
+    """Rows of one step, in the places of the counts they were asked by:
+    request ``r``'s begin at ``counts[:r].sum()``, whether or not the requests
+    before it were granted theirs.  ``cu`` counts those granted:
+    ``cu[r + 1] - cu[r]`` is 0 for a request whose rows the pool cannot hold,
+    whose places hold -1 and are neither written nor attended."""
+    slots: torch.Tensor        # int64 (max_tokens,), -1 for a row that is not there
+    positions: torch.Tensor    # int64 (max_tokens,), -1 for a row that is not there
     cu: torch.Tensor           # int32 (max_requests + 1,)
 
 
@@ -47,10 +50,11 @@ class PagedKVCache:
         self.block_tables = torch.zeros(max_requests, blocks, dtype=torch.int32, device=dev)
         self.free_pages = torch.arange(n_pages, dtype=torch.int32, device=dev)
         self.n_free = torch.full((1,), n_pages, dtype=torch.int32, device=dev)
-        # rows of each request's context, of the step under way, and rows whose
-        # pages the request holds
+        # rows of each request's context, of the step under way (and where they
+        # begin in it), and rows whose pages the request holds
         self.lens = torch.zeros(max_requests, dtype=torch.int32, device=dev)
         self.step = torch.zeros(max_requests, dtype=torch.int32, device=dev)
+        self.starts = torch.zeros(max_requests, dtype=torch.int32, device=dev)
         self.held = torch.zeros(max_requests, dtype=torch.int32, device=dev)
 
     def extend(self, counts: torch.Tensor, max_tokens: int) -> PagedRows:
@@ -58,8 +62,8 @@ class PagedKVCache:
         all) rows behind each request's context.  A step that was begun before
         and not accepted is given up: its rows are room again."""
         return PagedRows(*ops.extend_block_tables(
-            self.block_tables, self.held, self.lens, counts.contiguous(), self.step, self.free_pages,
-            self.n_free, page_size=self.page_size, max_tokens=max_tokens))
+            self.block_tables, self.held, self.lens, counts.contiguous(), self.step, self.starts,
+            self.free_pages, self.n_free, page_size=self.page_size, max_tokens=max_tokens))
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, rows: PagedRows) -> None:
         """Store the step's K/V rows ``(max_tokens, H_kv, D)``."""
@@ -67,9 +71,10 @@ class PagedKVCache:
 
     def attend(self, layer: int, q: torch.Tensor, rows: PagedRows, tree_mask: torch.Tensor,
                **kwargs):
-        """``ops.tree_attention`` of the step's rows over ``layer``."""
+        """``ops.tree_attention`` of the step's rows over ``layer``; rows of a
+        request that was refused are not written."""
         return ops.tree_attention(q, self.k[layer], self.v[layer], self.block_tables, self.lens,
-                                  rows.cu, tree_mask, **kwargs)
+                                  rows.cu, tree_mask, node_starts=self.starts, **kwargs)
 
     def accept(self, path: Optional[torch.Tensor], path_lens: torch.Tensor) -> None:
         """End the step: request ``r`` keeps the rows ``path[r, :path_lens[r]]``

@@ -466,16 +466,18 @@ int32_t halo_update_block_tables(int32_t* block_tables, int64_t table_stride, in
  * max(counts[r], 0) rows behind its context, in pages it holds or takes;
  * pages it holds beyond them are given back.  Granted, held_lens[r] becomes
  * the context and those rows (in place) and rows[r] their number; refused
- * (as above), it stays as it is and rows[r] is 0.  slots, positions and
- * cu_tokens (the running count of rows) describe the granted rows.  held_lens
- * and rows overlap neither one another nor context_lens or counts. */
+ * (as above), it stays as it is and rows[r] is 0.  cu_tokens is the running
+ * count of granted rows.  slots and positions have a place for every row asked
+ * for, in request order: request r's begin at starts[r], the running count of
+ * the others' before it, and hold -1 where r is refused.  held_lens, rows and
+ * starts overlap neither one another nor context_lens or counts. */
 int32_t halo_extend_block_tables(int32_t* block_tables, int64_t table_stride, int32_t R,
                                  int32_t max_blocks, int32_t* held_lens,
                                  const int32_t* context_lens, const int32_t* counts,
                                  int32_t* free_pages, int32_t free_capacity, int32_t* n_free,
                                  int32_t page_size, int32_t max_tokens, int64_t* slots,
                                  int64_t* positions, int32_t* cu_tokens, int32_t* rows,
-                                 halo_stream_t stream);
+                                 int32_t* starts, halo_stream_t stream);
 
 /* Copy K and V rows k, v (T, H_kv, D) (element strides *_stride_t,
  * *_stride_h) into the slots (T) of the pool.  Rows whose slot is negative
@@ -514,6 +516,9 @@ typedef struct halo_tree_problem {
   int64_t out_stride_t, out_stride_h;
   int32_t out_dtype;
   float* lse;                    /* (T, H) contiguous, natural log; optional */
+  const int32_t* node_starts;    /* (R), optional: request r's rows begin at node_starts[r]
+                                  * instead of cu_nodes[r], which then only count them; rows of
+                                  * no request are not written */
 } halo_tree_problem_t;
 
 /* Bytes of workspace for halo_tree_attention (256-byte aligned; no

@@ -46,19 +46,19 @@ def update_block_tables(table, old, new, free, n_free, page, max_tokens):
 
 
 def extend_block_tables(table, held, ctx, counts, free, n_free, page, max_tokens):
-    """Returns ``(table, free, n_free, slots, positions, cu, rows, held)``."""
+    """Returns ``(table, free, n_free, slots, positions, cu, rows, starts, held)``."""
     want = [c + max(n, 0) if 0 <= c <= h else -1 for h, c, n in zip(held, ctx, counts)]
     table, free, n_free, _, _, _, lens = update_block_tables(table, held, want, free, n_free, page, 0)
     rows = [max(n, 0) if 0 <= w == got else 0 for n, w, got in zip(counts, want, lens)]
-    slots, pos, cu = [], [], [0]
+    slots, pos, cu, starts, at = [-1] * max_tokens, [-1] * max_tokens, [0], [], 0
     for r, n in enumerate(rows):
-        for t in range(ctx[r], ctx[r] + n):
-            slots.append(table[r][t // page] * page + t % page)
-            pos.append(t)
-        cu.append(len(slots))
-    slots = (slots + [-1] * max_tokens)[:max_tokens]
-    pos = (pos + [-1] * max_tokens)[:max_tokens]
-    return table, free, n_free, slots, pos, cu, rows, lens
+        starts.append(min(at, 2 ** 31 - 1))
+        for i in range(min(n, max(0, max_tokens - at))):
+            t = ctx[r] + i
+            slots[at + i], pos[at + i] = table[r][t // page] * page + t % page, t
+        cu.append(cu[-1] + n)
+        at += max(counts[r], 0)
+    return table, free, n_free, slots, pos, cu, rows, starts, lens
 
 
 def write_kv_pages(k, v, k_pages, v_pages, slots):

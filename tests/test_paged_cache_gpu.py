@@ -45,12 +45,13 @@ def test_extend_block_tables(cuda_device, R, width, page, spare, top, seed):
     table, held, ctx, counts, free, n_free = _case(rng, R, width, page, spare)
     want = O.extend_block_tables(table, held, ctx, counts, free, n_free, page, top)
     t, h, f, n, rows = _i32(table), _i32(held), _i32(free), _i32([n_free]), _i32([-5] * R)
-    slots, pos, cu = ops.extend_block_tables(t, h, _i32(ctx), _i32(counts), rows, f, n,
+    starts = _i32([-5] * R)
+    slots, pos, cu = ops.extend_block_tables(t, h, _i32(ctx), _i32(counts), rows, starts, f, n,
                                              page_size=page, max_tokens=top)
     got = (t.tolist(), f.tolist(), int(n), slots.tolist(), pos.tolist(), cu.tolist(), rows.tolist(),
-           h.tolist())
-    for name, a, b in zip(("table", "free", "n_free", "slots", "positions", "cu", "rows", "held"),
-                          got, want):
+           starts.tolist(), h.tolist())
+    for name, a, b in zip(("table", "free", "n_free", "slots", "positions", "cu", "rows", "starts",
+                           "held"), got, want):
         assert a == b, name
 
 
@@ -92,3 +93,68 @@ def test_a_step_refused_after_one_given_up(cuda_device):
     assert got.cu.tolist() == [0, 6, 6]
     cache.accept(None, _i32([6, 2]))
     assert cache.lens.tolist() == [16, 6] and _owners(cache) == list(range(6))
+
+
+@pytest.mark.parametrize("refused", ["table", "pool"])
+@pytest.mark.parametrize("nodes", [3, 20])
+@pytest.mark.parametrize("captured", [False, True])
+def test_requests_behind_a_refused_one_keep_their_rows(cuda_device, refused, nodes, captured):
+    """K, V and q are packed by the counts; a request in the middle is refused.
+    The others' rows are stored, attended and accepted as theirs."""
+    from halo_b200 import PagedKVCache
+    H, H_kv, D, page, n0 = 8, 2, 64, 16, [20, 35, 3, 50]
+    cache = PagedKVCache(1, 12 if refused == "pool" else 60, H_kv, D, max_requests=4,
+                         max_len=400 if refused == "pool" else 80, page_size=page,
+                         dtype=torch.float16, device=DEV)
+    g = torch.Generator().manual_seed(nodes)
+    rand = lambda *s: torch.randn(*s, generator=g).half()          # noqa: E731
+    k0, v0 = rand(sum(n0), H_kv, D), rand(sum(n0), H_kv, D)
+    cache.write(0, k0.to(DEV), v0.to(DEV), cache.extend(_i32(n0), sum(n0)))
+    cache.accept(None, _i32(n0))
+    # pages held: 2, 3, 1, 4; the last needs no page
+    counts = [4, 200 if refused == "pool" else 50, nodes, min(nodes, 14)]
+    granted = [True, False, nodes <= 13 or refused == "table", True]
+    T = sum(counts) + 2
+    k, v, q = rand(T, H_kv, D), rand(T, H_kv, D), rand(T, H, D)
+    mask = (torch.rand(T, max(counts), generator=g) < 0.6) | torch.eye(T, max(counts)).bool()
+    path, lens = _i32([[1, 2, 3], [0, 1, 2], [0, 2, 0], [2, 0, 0]]), _i32([3, 3, 2, 1])
+    kd, vd, qd, md, cd = (x.to(DEV) for x in (k, v, q, mask, torch.tensor(counts, dtype=torch.int32)))
+    out = torch.full((T, H, D), 7.0, device=DEV)
+    lse = torch.full((T, H), 7.0, device=DEV)
+
+    def step():
+        rows = cache.extend(cd, T)
+        cache.write(0, kd, vd, rows)
+        cache.attend(0, qd, rows, md, out=out, lse=lse)
+        cache.accept(path, lens)
+        return rows
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            rows = step()
+        graph.replay()
+    else:
+        rows = step()
+    assert (rows.cu[1:] - rows.cu[:-1]).tolist() == [c if ok else 0 for c, ok in zip(counts, granted)]
+    at, old, kept = 0, 0, []
+    for r, (n, c) in enumerate(zip(n0, counts)):
+        kk, vv = k0[old:old + n], v0[old:old + n]
+        if granted[r]:
+            seen = torch.cat([torch.ones(c, n, dtype=torch.bool), mask[at:at + c, :c]], 1)
+            want = _dense(q[at:at + c], torch.cat([kk, k[at:at + c]]), torch.cat([vv, v[at:at + c]]),
+                          seen)
+            assert float((out[at:at + c].cpu() - want).abs().max()) < 1e-3
+            pick = path[r, :int(lens[r])].tolist()
+            kept.append((torch.cat([kk, k[at:at + c][pick]]), torch.cat([vv, v[at:at + c][pick]])))
+        else:
+            assert (out[at:at + c] == 7).all() and (lse[at:at + c] == 7).all()
+            assert (rows.slots[at:at + c] == -1).all() and (rows.positions[at:at + c] == -1).all()
+            kept.append((kk, vv))
+        at, old = at + c, old + n
+    assert (out[at:] == 7).all() and rows.slots[at:].tolist() == [-1, -1]
+    assert cache.lens.tolist() == [x.shape[0] for x, _ in kept] == cache.held.tolist()
+    for r, (kk, vv) in enumerate(kept):
+        pages = cache.block_tables[r, :-(-kk.shape[0] // page)].tolist()
+        assert torch.equal(O.gather_rows(cache.k[0].cpu(), pages, kk.shape[0]), kk.double().transpose(0, 1))
+        assert torch.equal(O.gather_rows(cache.v[0].cpu(), pages, kk.shape[0]), vv.double().transpose(0, 1))
+    assert _owners(cache) == list(range(cache.k[0].shape[0]))

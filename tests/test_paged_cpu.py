@@ -196,13 +196,14 @@ def test_extend_refusals():
     lib = L.lib()
 
     def call(table=0x1000, stride=8, R=4, blocks=8, held=0x2000, ctx=0x2400, counts=0x2800, cap=10,
-             n=0x4000, page=16, tok=5, slots=0x5000, cu=0x7000, rows=0x8000):
+             n=0x4000, page=16, tok=5, slots=0x5000, cu=0x7000, rows=0x8000, starts=0x8800):
         return lib.halo_extend_block_tables(table, stride, R, blocks, held, ctx, counts, 0x3000, cap,
-                                            n, page, tok, slots, 0x6000, cu, rows, None)
+                                            n, page, tok, slots, 0x6000, cu, rows, starts, None)
     for kw in ({"table": None}, {"held": None}, {"ctx": None}, {"counts": None}, {"n": None},
                {"slots": None}, {"cu": None}, {"rows": None}, {"R": -1}, {"blocks": -1}, {"cap": -1},
                {"page": 0}, {"tok": -1}, {"stride": 7}, {"rows": 0x2000}, {"rows": 0x2408},
-               {"rows": 0x27fc}, {"ctx": 0x2000}, {"counts": 0x200c}):
+               {"rows": 0x27fc}, {"ctx": 0x2000}, {"counts": 0x200c}, {"starts": None}, {"starts": 0x2000},
+               {"starts": 0x2408}, {"starts": 0x27fc}, {"starts": 0x800c}):
         assert call(**kw) == L.HALO_ERR_INVALID_ARG, kw
     for kw in ({"R": 8193}, {"blocks": 2 ** 28, "stride": 2 ** 28}):
         assert call(**kw) == L.HALO_ERR_UNSUPPORTED, kw
@@ -211,9 +212,18 @@ def test_extend_refusals():
 def test_oracle_extend_by_hand():
     # page 4: request 0 gave up a step (9 rows held, context 3), asks for 2 rows
     # and gives page 9 back; request 1 takes it and page 6
-    t, f, n, s, p, cu, rows, held = O.extend_block_tables(
+    t, f, n, s, p, cu, rows, starts, held = O.extend_block_tables(
         [[7, 8, 9], [1, 0, 0]], [9, 3], [3, 3], [2, 9], [5, 6, 0, 0, 0], 2, 4, 12)
+    assert starts == [0, 2]
     assert t == [[7, 8, 9], [1, 9, 6]] and held == [5, 12] and rows == [2, 9]
     assert n == 1 and f == [5, 6, 0, 0, 0] and cu == [0, 2, 11]
     assert p == [3, 4, 3, 4, 5, 6, 7, 8, 9, 10, 11, -1]
     assert s == [31, 32, 7, 36, 37, 38, 39, 24, 25, 26, 27, -1]
+
+
+def test_oracle_extend_keeps_the_places_of_refused_rows():
+    t, f, n, s, p, cu, rows, starts, held = O.extend_block_tables(
+        [[3, 0], [4, 0], [5, 0]], [2, 2, 2], [2, 2, 2], [1, 50, 2], [6, 7], 2, 4, 60)
+    assert starts == [0, 1, 51] and cu == [0, 1, 1, 3] and rows == [1, 0, 2] and held == [3, 2, 4]
+    assert s[0] == 14 and s[1:51] == [-1] * 50 and s[51:] == [22, 23] + [-1] * 7
+    assert p[0] == 2 and p[51:53] == [2, 3]
