@@ -79,11 +79,13 @@ class PagedKVCache:
     def accept(self, path: Optional[torch.Tensor], path_lens: torch.Tensor) -> None:
         """End the step: request ``r`` keeps the rows ``path[r, :path_lens[r]]``
         of its step (``None``: its first ``path_lens[r]`` rows; never more than
-        the step gave it) and gives the other pages back."""
-        # no step of a path may reach behind the rows of its step: table entries
-        # there name pages that another request may own by now
+        the step gave it) and gives the other pages back.  A node that is not
+        of the step moves nothing: row ``i`` of the step stays in its place."""
+        # neither a path's steps nor its nodes may reach behind the rows of the
+        # step: table entries there name pages that another request may own by now
         keep = torch.minimum(path_lens.clamp(0, None if path is None else path.shape[1]), self.step)
         if path is not None:
+            path = path.masked_fill(path >= self.step[:, None], 0)
             for k, v in zip(self.k, self.v):
                 ops.commit_tree_path(k, v, self.block_tables, self.lens, path, keep)
         self.lens.copy_(self._resize(self.lens + keep))

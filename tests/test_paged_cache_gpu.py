@@ -158,3 +158,28 @@ def test_requests_behind_a_refused_one_keep_their_rows(cuda_device, refused, nod
         assert torch.equal(O.gather_rows(cache.k[0].cpu(), pages, kk.shape[0]), kk.double().transpose(0, 1))
         assert torch.equal(O.gather_rows(cache.v[0].cpu(), pages, kk.shape[0]), vv.double().transpose(0, 1))
     assert _owners(cache) == list(range(cache.k[0].shape[0]))
+
+
+@pytest.mark.parametrize("node", [3, 7, 10, 13, 53, 2 ** 31 - 1, -1, -2 ** 31])
+def test_accept_of_nodes_that_are_not_of_the_step(cuda_device, node):
+    """The entries behind a request's rows still name pages it gave back, which
+    are another's now: none of their rows comes into its context."""
+    cache = _small_cache(8)
+    cache.extend(_i32([30, 0]), 30)                        # 5 pages of request 0
+    cache.accept(None, _i32([0, 0]))                       # given back, entries stay
+    got = cache.extend(_i32([0, 30]), 30)
+    x = torch.full((30, 1, 64), 9., dtype=torch.bfloat16, device=DEV)
+    cache.write(0, x, x, got)
+    cache.accept(None, _i32([0, 30]))
+    stale = cache.block_tables[0, 2:5].tolist()
+    assert set(stale) & set(cache.block_tables[1, :5].tolist())
+    got = cache.extend(_i32([3, 0]), 3)
+    y = torch.tensor([4., 5., 6.], device=DEV)[:, None, None].expand(3, 1, 64).bfloat16()
+    cache.write(0, y, y, got)
+    cache.accept(_i32([[0, node, 2], [0, 0, 0]]), _i32([3, 0]))
+    assert _rows_of(cache, 0) == [1.] * 10 + [4., 5., 6.]
+    assert _rows_of(cache, 1) == [2.] * 6 + [9.] * 30 and _owners(cache) == list(range(8))
+    got = cache.extend(_i32([3, 0]), 3)
+    cache.write(0, y, y, got)
+    cache.accept(_i32([[2, node, 0], [0, 0, 0]]), _i32([2, 0]))
+    assert _rows_of(cache, 0) == [1.] * 10 + [4., 5., 6., 6., 5.]
