@@ -1778,6 +1778,21 @@ static bool rows16(const void* p, int64_t a, int64_t b, int64_t c, int elt) {
            (uint64_t)(c * elt)) & 15) == 0;
 }
 
+// Whether two of the rows of D elements at t * st + h * sh (t < T, h < H) share
+// an element: two heads dh apart and two tokens dt apart whose distances differ
+// by less than D.  dt next to dh * sh / st is the nearest.
+static bool rows_overlap(int64_t T, int64_t st, int64_t H, int64_t sh, int64_t D) {
+  if ((T > 1 && st < D) || (H > 1 && sh < D)) return true;
+  if (T <= 1 || H <= 1) return false;
+  if (st / H >= sh || sh / T >= st) return false;         // one inside the other, as in a tensor
+  for (int64_t dh = 1; dh < H; ++dh) {
+    const int64_t dt = dh * sh / st, over = dh * sh - dt * st;   // 0 <= over < st
+    if (dt >= T) return false;
+    if (over < D || (dt + 1 < T && st - over < D)) return true;
+  }
+  return false;
+}
+
 static int check(const halo_page_pool_t* pool, const halo_tree_problem_t* pb) {
   if (!pool || !pb) return fail(HALO_ERR_INVALID_ARG, "page pool/problem is NULL");
   if (pool->dtype != HALO_DTYPE_BF16 && pool->dtype != HALO_DTYPE_F16)
@@ -1891,7 +1906,7 @@ static int run(const halo_page_pool_t* pool, const halo_tree_problem_t* pb, void
   if (!rows16(pb->out, pb->T > 1 ? pb->out_stride_t : 0, pb->H > 1 ? pb->out_stride_h : 0, 0,
               pb->out_dtype == HALO_DTYPE_F32 ? 4 : 2))
     return fail(HALO_ERR_MISALIGNED, "out rows must be 16-byte aligned");
-  if ((pb->T > 1 && pb->out_stride_t < pool->D) || (pb->H > 1 && pb->out_stride_h < pool->D))
+  if (rows_overlap(pb->T, pb->out_stride_t, pb->H, pb->out_stride_h, pool->D))
     return fail(HALO_ERR_INVALID_ARG, "out rows overlap (strides %lld %lld)",
                 (long long)pb->out_stride_t, (long long)pb->out_stride_h);
   const int64_t need = ws_bytes(pool, pb);

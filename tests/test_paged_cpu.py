@@ -227,3 +227,30 @@ def test_oracle_extend_keeps_the_places_of_refused_rows():
     assert starts == [0, 1, 51] and cu == [0, 1, 1, 3] and rows == [1, 0, 2] and held == [3, 2, 4]
     assert s[0] == 14 and s[1:51] == [-1] * 50 and s[51:] == [22, 23] + [-1] * 7
     assert p[0] == 2 and p[51:53] == [2, 3]
+
+
+def test_out_rows_that_share_elements_are_refused():
+    """Any strides of out, against the rows spelled out.  A workspace that is
+    too small is refused behind them, so nothing is launched."""
+    import random
+    from halo_b200 import _lib as L
+    lib = L.lib()
+    rng = random.Random(5)
+    po = _pool(L, D=64, H_kv=1)
+    seen = {True: 0, False: 0}
+    for _ in range(3000):
+        T, H = rng.randint(1, 6), rng.randint(1, 6)
+        st, sh = (rng.choice((0, 8, 56, 64, 72, 128, 192, 256, 320, 448)) + 64 * rng.randint(0, 3)
+                  for _ in range(2))
+        at = sorted(t * st + h * sh for t in range(T) for h in range(H))
+        overlap = any(b - a < 64 for a, b in zip(at, at[1:]))
+        pr = _tree(L, T=T, H=H, out_stride_t=st, out_stride_h=sh)
+        rc = lib.halo_tree_attention(ctypes.byref(po), ctypes.byref(pr), 0x100000, 1, None)
+        assert rc == (L.HALO_ERR_INVALID_ARG if overlap else L.HALO_ERR_WORKSPACE), (T, H, st, sh)
+        seen[overlap] += 1
+    assert min(seen.values()) > 500
+    # two dimensions of one stride, and rows of a wide tensor
+    for st, sh, rc in ((64, 64, L.HALO_ERR_INVALID_ARG), (2 ** 40, 64, L.HALO_ERR_WORKSPACE),
+                       (64, 2 ** 40, L.HALO_ERR_WORKSPACE)):
+        pr = _tree(L, T=1000, H=65535, out_stride_t=st, out_stride_h=sh)
+        assert lib.halo_tree_attention(ctypes.byref(po), ctypes.byref(pr), 0x100000, 1, None) == rc
