@@ -591,7 +591,7 @@ __device__ __forceinline__ void produce(const Params& p, Bars* bs, unsigned char
 // Cleaner warp: passes every V tile on, cleaned where it reaches behind the
 // context: rows behind the last node and elements that are not finite become
 // zero (a weight of zero would turn them into NaN).  bs->bad[segment] tells
-// whether a node's element was taken out; bad_sum gives it back.
+// whether a node's element was taken out; restore gives it back.
 // `begin` runs at the start of every segment.
 template <typename T, int D, int RG, class Gm, class F>
 __device__ __forceinline__ void clean(const Params& p, Bars* bs, unsigned char* smem,
@@ -669,6 +669,52 @@ __device__ __noinline__ float bad_sum(const Params& p, int r, int t, int ctx, in
     if (!isfinite(y)) o += y;
   }
   return o;
+}
+
+// The same of the context's positions [a, b), which every row sees; NaN once it
+// is NaN.
+template <typename T>
+__device__ __noinline__ float context_sum(const Params& p, int r, int a, int b, int hk, int col) {
+  float o = 0.f;
+  for (int pos = a; pos < b && o == o;) {
+    const int idx = pos / p.page, row = pos - idx * p.page, n = min(p.page - row, b - pos);
+    const int pg = p.table[(int64_t)r * p.table_stride + idx];
+    pos += n;
+    if ((uint32_t)pg >= (uint32_t)p.n_pages) continue;
+    const T* v = reinterpret_cast<const T*>(p.v) + pg * p.v_sp + hk * p.v_sh + row * p.v_st + col;
+#pragma unroll 1
+    for (int i = 0; i < n; i += 8) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = i + e < n ? Elem<T>::to_f32(v[(i + e) * p.v_st]) : 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (!isfinite(y[e])) o += y[e];
+    }
+  }
+  return o;
+}
+
+// Gives a row the non-finite V elements that it sees among positions [a, b):
+// those of nodes, which were cleaned out, and of the context, which is not
+// cleaned, so that an infinity of it times a remainder of zero or of the other
+// sign made the output NaN.  Columns [col, col + n) of query row t, stored at `at`
+// of a part or (part null) of the output.  Rows whose sum of weights is NaN do
+// not come here.
+template <typename T>
+__device__ __noinline__ void restore(const Params& p, int r, int t, int ctx, int a, int b, int hk,
+                                     int col, int n, float* part, int64_t at) {
+  float* f = part ? part : p.out_f32 ? reinterpret_cast<float*>(p.out) : nullptr;
+  T* h = reinterpret_cast<T*>(p.out);
+  for (int e = 0; e < n; ++e, ++at) {
+    const float x = f ? f[at] : Elem<T>::to_f32(h[at]);
+    float y = bad_sum<T>(p, r, t, ctx, max(a, ctx), b, hk, col + e);
+    if (x == x) y += x;
+    else y += context_sum<T>(p, r, a, min(b, ctx), hk, col + e);
+    if (isfinite(y)) continue;             // nothing of the kind
+    if (f) f[at] = y;
+    else h[at] = Elem<T>::from_f32(y);
+  }
 }
 
 // ======================================================================
@@ -1043,16 +1089,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       named_bar_sync(1, 512);
       const bool fix = *reinterpret_cast<volatile int*>(&bs->bad[si % kBadSlots]) != 0;
       float* part = p.part + ((int64_t)blockIdx.x * 2 + (s.first ? 0 : 1)) * part_floats<D>(RG);
-      auto bad = [&](int row, int col) {
-        return bad_sum<T>(p, walk.r, cu0 + (s.row0 + row) / p.G, ctx, max(ctx, s.t0 * kBN),
-                          min(end, s.t1 * kBN), s.hk, col);
-      };
+      bool sound = false;                  // the row's weights are no NaN
+      float odd = fix ? NAN : 0.f;         // NaN if any element is not finite
       // N columns from col of a row of the group: o scaled by 1 / L, or as it
       // is to the workspace
       auto store = [&](int row, int col, float M, float L, auto& o) {
         constexpr int N = sizeof(o) / sizeof(float);
-        if (fix)
-          for (int e = 0; e < N; ++e) o[e] += bad(row, col + e);
+        sound = L == L;
+#pragma unroll
+        for (int e = 0; e < N; ++e) odd = fmaf(o[e], 0.f, odd);
         if (!s.whole) {
           float4* d = reinterpret_cast<float4*>(part + row * D + col);
 #pragma unroll
@@ -1112,6 +1157,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           for (int e = 0; e < 16; ++e) a[e] = n1 > 0 ? fmaf(b[e], w1, a[e] * w0) : a[e] * w0;
           if (r < rows && ok) store(r, col + c, M, L, a);
         }
+      }
+      if (__builtin_expect(odd != odd && sound, 0)) {
+        const int row = r + (two ? x * 128 : 0), n = two ? D / 2 : D / 4;
+        const int col = (two ? h : x * 2 + h) * n;
+        const int rq = s.row0 + row, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
+        restore<T>(p, walk.r, cu0 + node, ctx, s.t0 * kBN, min(end, s.t1 * kBN), s.hk, col, n,
+                   s.whole ? nullptr : part,
+                   s.whole ? (int64_t)(cu0 + node) * p.out_st + hq * p.out_sh + col
+                           : (int64_t)row * D + col);
       }
       umma::fence_before_sync();
       ++si;
@@ -1550,7 +1604,7 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
           const float M = sh->m[r];
           if (!s.whole) {
             *reinterpret_cast<float2*>(part + RG * D + 2 * r) = make_float2(M, L);
-            sh->fac[r] = 1.f;
+            sh->fac[r] = L == L ? 1.f : L;
             sh->off[r] = r * D;
           } else {
             const int rq = s.row0 + r, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
@@ -1564,6 +1618,7 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
         named_bar_sync(bar, 128);
         const bool fix = *reinterpret_cast<volatile int*>(&bs->bad[si % kBadSlots]) != 0;
         float* of = !s.whole ? part : p.out_f32 ? reinterpret_cast<float*>(p.out) : nullptr;
+        float odd = fix ? NAN : 0.f;       // NaN if any element is not finite
 #pragma unroll 1
         for (int c = r0; c < min(r0 + RT, s.rows); c += 8) {
           float a[8], b[8];
@@ -1579,13 +1634,9 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
           umma::tmem_wait_ld();
           if (tid >= D || !ok) continue;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) a[e] += b[e];
-          if (fix) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (c + e < s.rows)
-                a[e] += bad_sum<T>(p, walk.r, walk.q.cu0 + (s.row0 + c + e) / p.G, ctx,
-                                   max(ctx, s.t0 * kBN), min(end, s.t1 * kBN), s.hk, tid);
+          for (int e = 0; e < 8; ++e) {
+            a[e] += b[e];
+            odd = fmaf(a[e], 0.f, odd);
           }
           if (of) {
 #pragma unroll
@@ -1597,6 +1648,14 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
               if (c + e < s.rows)
                 reinterpret_cast<T*>(p.out)[off[e]] = Elem<T>::from_f32(a[e] * fac[e]);
           }
+        }
+        if (__builtin_expect(odd != odd && tid < D && ok, 0)) {
+#pragma unroll 1
+          for (int r = r0; r < min(r0 + RT, s.rows); ++r)
+            if (sh->fac[r] == sh->fac[r])
+              restore<T>(p, walk.r, walk.q.cu0 + (s.row0 + r) / p.G, ctx, s.t0 * kBN,
+                         min(end, s.t1 * kBN), s.hk, tid, 1, s.whole ? nullptr : part,
+                         sh->off[r] + tid);
         }
         umma::fence_before_sync();
         ++si;
@@ -1642,6 +1701,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
   const int own = cut(c);
   if (own <= 0 || own >= d.nt || cut(c - 1) > 0) return;
   const int64_t before = (c - 1) * d.quot + (uint32_t)((c - 1) * d.rem) / (uint32_t)n_cta;
+  // CTA i's part of the segment.  CTA c - 1 may have begun before the segment's
+  // set-up units: then this is its second part.
+  auto part = [&](int i) {
+    const int sl = i == c - 1 && before < d.start - (RG <= 64 ? kSetup<64> : kSetup<128>) ? 1 : 0;
+    return p.part + ((int64_t)i * 2 + sl) * part_floats<D>(RG);
+  };
   for (; row < d.rows; row += (int)gridDim.y * kMergeWarps) {
     float M = -INFINITY, L = 0.f, acc[C];
 #pragma unroll
@@ -1661,10 +1726,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
           if (has) {
             const int i = i0 + __ffs(has) - 1;
             has &= has - 1;
-            // CTA c - 1 may have begun before the segment's set-up units: then
-            // this is its second part
-            const int sl = i == c - 1 && before < d.start - (RG <= 64 ? kSetup<64> : kSetup<128>) ? 1 : 0;
-            const float* s = p.part + ((int64_t)i * 2 + sl) * part_floats<D>(RG);
+            const float* s = part(i);
             ml[u] = *reinterpret_cast<const float2*>(s + RG * D + 2 * row);
             s += row * D;
             if constexpr (C == 4) {
@@ -1698,6 +1760,24 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
         }
         M = Mn;
       }
+    }
+    // an infinity whose part's weight ended as 0 came out NaN: the infinities
+    // of the parts again
+    float odd = 0.f;
+#pragma unroll
+    for (int e = 0; e < C; ++e) odd = fmaf(acc[e], 0.f, odd);
+    if (__builtin_expect(odd != odd && L == L, 0)) {
+      float y[C];
+#pragma unroll
+      for (int e = 0; e < C; ++e) y[e] = 0.f;
+      for (int i = c - 1; i < n_cta && cut(i) < d.nt; ++i) {
+        if (cut(i) >= cut(i + 1)) continue;
+        const float* s = part(i) + row * D + lane * C;
+#pragma unroll
+        for (int e = 0; e < C; ++e) y[e] += isfinite(s[e]) ? 0.f : s[e];
+      }
+#pragma unroll
+      for (int e = 0; e < C; ++e) acc[e] = acc[e] == acc[e] || y[e] == 0.f ? acc[e] : y[e];
     }
     const int rq = d.row0 + row, node = rq / p.G, hq = d.hk * p.G + rq - node * p.G;
     const int64_t t = d.cu0 + node;

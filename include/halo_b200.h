@@ -496,8 +496,8 @@ int32_t halo_write_kv_pages(const halo_page_pool_t* pool, const void* k, int64_t
  * (mask (T, max_nodes) bytes, rows mask_stride apart).  A node that sees
  * nothing gets zeros and lse -inf.  A K/V row that a node does not see (a
  * hidden node's, one behind the last node) never reaches its output, whatever
- * the row holds; a non-finite V element of the context, which every node
- * sees, makes its column NaN.  Rows of out and lse from cu_nodes[R] on are
+ * the row holds; a non-finite V element that it does see makes its column that
+ * element, or NaN where such elements differ.  Rows of out and lse from cu_nodes[R] on are
  * not written.  A request has at most max_nodes nodes (others are not
  * written) and at most max_blocks pages (positions behind them are not
  * there); a table entry that names no page reads as rows of zeros. */

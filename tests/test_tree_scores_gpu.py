@@ -148,3 +148,67 @@ def test_many_small_weights_beside_a_large_one(cuda_device, dtype, nodes):
     room = n * 2.0 ** -32 + mass * (2.0 ** -16 + 2.0 ** -20) + 2 * want * (n / 8 + 64) * 2.0 ** -23
     assert float((out.double() - want).abs().max()) <= room
     assert float((lse.double() - (139 / math.sqrt(D) + math.log1p(mass))).abs().max()) <= 1e-5
+
+
+@pytest.mark.parametrize("nodes", [1, 5, 14, 20, 40, 70])
+@pytest.mark.parametrize("D,dtype", [(64, torch.bfloat16), (128, torch.float16),
+                                     (128, torch.bfloat16), (64, torch.float16)])
+@pytest.mark.parametrize("ctx", [130, 2000, 40000])
+def test_infinities_of_the_context(cuda_device, nodes, D, dtype, ctx):
+    """An infinity that a node sees is its column's value wherever it lies and
+    however small its weight, as one of a drafted row is; other columns are as
+    they were."""
+    c = Case(ctx + nodes, [ctx, 70], [nodes, 2], 4, 1, D, 16, dtype)
+    page = 16
+
+    def put(r, pos, col, x):
+        c.v[c.table[r][pos // page], 0, pos % page, col] = x
+    low = ctx // 2                           # a position whose weight ends as zero
+    c.k[c.table[0][low // page], 0, low % page] = 0
+    c.k[c.table[0][low // page], 0, low % page, 1] = -300
+    c.q[:, :, 1] = 60.0
+    c.k[:, :, :, 1].clamp_(max=1)
+    bad = {0: math.inf, 3: -math.inf, 5: math.nan, 31: math.nan, 40: math.inf, D - 1: -math.inf}
+    spots = {0: [(0, math.inf)], 3: [(ctx - 1, -math.inf)], 5: [(127, math.nan)],
+             31: [(2, math.inf), (ctx - 3, -math.inf)], 40: [(low, math.inf)],
+             D - 1: [(at, -math.inf) for at in range(1, ctx, 7)]}
+    for col, at in spots.items():
+        for pos, x in at:
+            put(0, pos, col, x)
+    out, lse = c.run(out_dtype=torch.float32)
+    half, _ = c.run()
+    for o in (out.cpu(), half.float().cpu()):
+        for col, x in bad.items():
+            got = o[:nodes, :, col]
+            assert torch.isnan(got).all() if math.isnan(x) else (got == x).all(), col
+        for col in spots:
+            assert torch.isfinite(o[nodes:]).all()
+    for col, at in spots.items():            # the oracle's other columns
+        for pos, _ in at:
+            put(0, pos, col, 0.0)
+        out[:nodes, :, col] = 0
+    keep = [x for x in range(D) if x not in spots]
+    c.v[:, :, :, list(spots)] = 0
+    out[:, :, list(spots)] = 0
+    assert torch.isfinite(out).all() and len(keep) == D - len(spots)
+    c.check(out, lse)
+
+
+def test_accepting_an_infinity_keeps_the_answer(cuda_device):
+    """A node's infinity gives the same output drafted and accepted."""
+    from test_paged_gpu import _i32, _small_cache
+    cache = _small_cache(12)
+    got = cache.extend(_i32([2, 0]), 2)
+    k = torch.ones(2, 1, 64, dtype=torch.bfloat16, device="cuda")
+    v = k.clone()
+    v[0, 0, 9] = math.inf
+    q = torch.rand(2, 4, 64, device="cuda").bfloat16()
+    mask = torch.ones(2, 2, dtype=torch.bool, device="cuda")
+    cache.write(0, k, v, got)
+    drafted = cache.attend(0, q, got, mask)[0][1]
+    cache.accept(None, _i32([1, 0]))
+    got = cache.extend(_i32([1, 0]), 1)
+    cache.write(0, k[1:], v[1:], got)
+    accepted = cache.attend(0, q[1:], got, mask[1:, :1])[0][0]
+    assert (drafted[:, 9] == math.inf).all()
+    assert torch.equal(drafted, accepted)
