@@ -696,18 +696,23 @@ def write_kv_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
 # workspaces of calls outside a capture, which need no initial contents
 _TREE_BYTES: dict = {}
 _TREE_LOCAL = threading.local()
+_TREE_KEPT = 4          # buffers a thread keeps: up to 39 MB each
 
 
 def _tree_workspace(index: int, stream: int, need: int) -> torch.Tensor:
     """``need`` bytes for a call on ``stream``.  A thread's calls on one stream
-    follow one another and share a buffer that grows; a captured call gets one
-    of its own from the graph's pool, so that no two graphs share one."""
+    follow one another and share a buffer that grows, kept for the last
+    ``_TREE_KEPT`` streams it came to; a captured call gets one of its own from
+    the graph's pool, so that no two graphs share one."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(need, dtype=torch.uint8, device=f"cuda:{index}")
     bufs = _TREE_LOCAL.__dict__
     ws = bufs.get((index, stream))
     if ws is None or ws.numel() < need:
         ws = torch.empty(need, dtype=torch.uint8, device=f"cuda:{index}")
+        if len(bufs) >= _TREE_KEPT and (index, stream) not in bufs:
+            # the memory goes back to its own stream, behind the calls that use it
+            del bufs[next(iter(bufs))]
         bufs[index, stream] = ws
     return ws
 
