@@ -36,17 +36,29 @@ class PagedRows(NamedTuple):
 
 
 class PagedKVCache:
+    """``n_pages`` pages of ``page_size`` rows a layer, shared by up to
+    ``max_requests`` (8192) requests of up to ``max_len`` rows.  Rows of any
+    ``head_dim``, page size and floating type can be written, moved and given
+    back; ``attend`` takes bf16 and fp16, a ``head_dim`` of 64 or 128 and a
+    page size that is a multiple of 8."""
+
     def __init__(self, n_layers: int, n_pages: int, n_kv_heads: int, head_dim: int, *,
                  max_requests: int, max_len: int, page_size: int = 64,
                  dtype: torch.dtype = torch.bfloat16, device="cuda"):
         if min(n_layers, n_pages, n_kv_heads, head_dim, max_requests, max_len, page_size) < 1:
             raise L.HaloError("cache dimensions must be positive", L.HALO_ERR_INVALID_ARG)
+        blocks = -(-max_len // page_size)
+        # what no step could be begun in is refused before the pools are allocated
+        if max_requests > 8192 or n_pages > 2 ** 30 or max_requests * blocks >= 2 ** 31 or \
+                (blocks + 1) * page_size >= 2 ** 31:
+            raise L.HaloError(f"{max_requests} requests of {max_len} rows on {n_pages} pages of "
+                              f"{page_size} are too many", L.HALO_ERR_UNSUPPORTED)
+        L.halo_dtype(dtype)
         self.page_size = page_size
         shape = (n_pages, n_kv_heads, page_size, head_dim)
         self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(n_layers)]
         self.v = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(n_layers)]
         dev = self.k[0].device
-        blocks = -(-max_len // page_size)
         self.block_tables = torch.zeros(max_requests, blocks, dtype=torch.int32, device=dev)
         self.free_pages = torch.arange(n_pages, dtype=torch.int32, device=dev)
         self.n_free = torch.full((1,), n_pages, dtype=torch.int32, device=dev)

@@ -254,3 +254,24 @@ def test_out_rows_that_share_elements_are_refused():
                        (64, 2 ** 40, L.HALO_ERR_WORKSPACE)):
         pr = _tree(L, T=1000, H=65535, out_stride_t=st, out_stride_h=sh)
         assert lib.halo_tree_attention(ctypes.byref(po), ctypes.byref(pr), 0x100000, 1, None) == rc
+
+
+@pytest.mark.parametrize("bad,code", [
+    ({"max_requests": 8193}, "UNSUPPORTED"), ({"max_len": 2 ** 31}, "UNSUPPORTED"),
+    ({"max_len": 2 ** 31 - 64}, "UNSUPPORTED"), ({"n_pages": 2 ** 30 + 1}, "UNSUPPORTED"),
+    ({"max_requests": 8192, "max_len": 2 ** 24}, "UNSUPPORTED"), ({"page_size": 0}, "INVALID_ARG"),
+    ({"max_requests": 0}, "INVALID_ARG"), ({"dtype": torch.float64}, "UNSUPPORTED")])
+def test_caches_that_could_begin_no_step_are_refused(bad, code):
+    from halo_b200 import PagedKVCache
+    from halo_b200 import _lib as L
+    kw = {"n_pages": 2, "max_requests": 2, "max_len": 64, "page_size": 64, **bad}
+    with pytest.raises(L.HaloError) as e:
+        PagedKVCache(1, kw.pop("n_pages"), 1, 64, device="cpu", **kw)
+    assert e.value.code == getattr(L, "HALO_ERR_" + code)
+
+
+def test_the_largest_tables_are_not_refused():
+    from halo_b200 import PagedKVCache
+    for kw in ({"max_requests": 8192, "max_len": 64}, {"max_requests": 1, "max_len": 2 ** 31 - 129},
+               {"max_requests": 2, "max_len": 64, "dtype": torch.float32, "page_size": 5}):
+        PagedKVCache(1, 2, 1, 8, device="cpu", **kw)
