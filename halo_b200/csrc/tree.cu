@@ -683,12 +683,12 @@ __device__ __noinline__ float context_sum(const Params& p, int r, int a, int b, 
     if ((uint32_t)pg >= (uint32_t)p.n_pages) continue;
     const T* v = reinterpret_cast<const T*>(p.v) + pg * p.v_sp + hk * p.v_sh + row * p.v_st + col;
 #pragma unroll 1
-    for (int i = 0; i < n; i += 8) {
-      float y[8];
+    for (int i = 0; i < n; i += 4) {
+      float y[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = i + e < n ? Elem<T>::to_f32(v[(i + e) * p.v_st]) : 0.f;
+      for (int e = 0; e < 4; ++e) y[e] = i + e < n ? Elem<T>::to_f32(v[(i + e) * p.v_st]) : 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+      for (int e = 0; e < 4; ++e)
         if (!isfinite(y[e])) o += y[e];
     }
   }
@@ -699,18 +699,23 @@ __device__ __noinline__ float context_sum(const Params& p, int r, int a, int b, 
 // those of nodes, which were cleaned out, and of the context, which is not
 // cleaned, so that an infinity of it times a remainder of zero or of the other
 // sign made the output NaN.  Columns [col, col + n) of query row t, stored at `at`
-// of a part or (part null) of the output.  Rows whose sum of weights is NaN do
-// not come here.
+// of a part or (part null) of the output.  `context` keeps the context's sum of
+// the last column (kUnknown: not formed yet) for further rows of one column.
+// Rows whose sum of weights is NaN do not come here.
+constexpr float kUnknown = 1.f;            // no sum of non-finite elements
 template <typename T>
 __device__ __noinline__ void restore(const Params& p, int r, int t, int ctx, int a, int b, int hk,
-                                     int col, int n, float* part, int64_t at) {
+                                     int col, int n, float* part, int64_t at, float& context) {
   float* f = part ? part : p.out_f32 ? reinterpret_cast<float*>(p.out) : nullptr;
   T* h = reinterpret_cast<T*>(p.out);
   for (int e = 0; e < n; ++e, ++at) {
     const float x = f ? f[at] : Elem<T>::to_f32(h[at]);
     float y = bad_sum<T>(p, r, t, ctx, max(a, ctx), b, hk, col + e);
     if (x == x) y += x;
-    else y += context_sum<T>(p, r, a, min(b, ctx), hk, col + e);
+    else {
+      if (e > 0 || context == kUnknown) context = context_sum<T>(p, r, a, min(b, ctx), hk, col + e);
+      y += context;
+    }
     if (isfinite(y)) continue;             // nothing of the kind
     if (f) f[at] = y;
     else h[at] = Elem<T>::from_f32(y);
@@ -1162,10 +1167,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         const int row = r + (two ? x * 128 : 0), n = two ? D / 2 : D / 4;
         const int col = (two ? h : x * 2 + h) * n;
         const int rq = s.row0 + row, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
+        float context = kUnknown;
         restore<T>(p, walk.r, cu0 + node, ctx, s.t0 * kBN, min(end, s.t1 * kBN), s.hk, col, n,
                    s.whole ? nullptr : part,
                    s.whole ? (int64_t)(cu0 + node) * p.out_st + hq * p.out_sh + col
-                           : (int64_t)row * D + col);
+                           : (int64_t)row * D + col, context);
       }
       umma::fence_before_sync();
       ++si;
@@ -1650,12 +1656,13 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
           }
         }
         if (__builtin_expect(odd != odd && tid < D && ok, 0)) {
+          float context = kUnknown;
 #pragma unroll 1
           for (int r = r0; r < min(r0 + RT, s.rows); ++r)
             if (sh->fac[r] == sh->fac[r])
               restore<T>(p, walk.r, walk.q.cu0 + (s.row0 + r) / p.G, ctx, s.t0 * kBN,
                          min(end, s.t1 * kBN), s.hk, tid, 1, s.whole ? nullptr : part,
-                         sh->off[r] + tid);
+                         sh->off[r] + tid, context);
         }
         umma::fence_before_sync();
         ++si;

@@ -212,3 +212,23 @@ def test_accepting_an_infinity_keeps_the_answer(cuda_device):
     accepted = cache.attend(0, q[1:], got, mask[1:, :1])[0][0]
     assert (drafted[:, 9] == math.inf).all()
     assert torch.equal(drafted, accepted)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("nodes", [2, 30])
+@pytest.mark.parametrize("scale", [1e-40, 1e-38, 1e-30, 1e-6])
+def test_scales_that_leave_a_mean(cuda_device, dtype, nodes, scale):
+    """Weights that are all one: the headroom of a raw score may be infinite."""
+    c = Case(nodes, [700, 50], [nodes, 1], 4, 1, 64, 16, dtype)
+    out, lse = c.run(out_dtype=torch.float32, scale=scale)
+    c.check(out, lse, scale=scale)
+
+
+@pytest.mark.parametrize("nodes", [3, 30])
+def test_infinities_everywhere(cuda_device, nodes):
+    """Every column of a long context holds infinities: no wait runs out."""
+    from halo_b200 import _lib as L
+    c = Case(nodes, [100000], [nodes], 4, 1, 128, 64, torch.bfloat16)
+    c.v[c.table[0][::3]] = math.inf
+    out, lse = c.run(out_dtype=torch.float32)
+    assert (out == math.inf).all() and torch.isfinite(lse).all() and L.device_error() == 0
