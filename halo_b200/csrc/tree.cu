@@ -57,7 +57,7 @@ struct alignas(64) Params {
   int64_t mask_stride;
   char* out;
   int64_t out_st, out_sh;
-  float* lse;
+  float* lse;                          // never null: in the workspace if not asked for
   float scale_log2;                    // softmax scale * log2(e)
   float headroom;                      // of the running maximum, in raw scores
   int32_t out_f32;
@@ -171,9 +171,9 @@ struct Bars {
   uint64_t k_full[6], k_empty[6], v_full[6], v_ready[6], v_empty[6];
   uint64_t s_full[2], s_free[2], p_full[4], pv_done[2], mma_done[2], turn[2];
   int64_t scan[20];
-  int64_t base0, total;
+  int64_t base0, u0, u1;
   uint32_t tmem_base;
-  int abort_flag, r0;
+  int abort_flag, r0, odd;             // odd: an output element is not finite
   Req req0;
   int bad[kBadSlots];
 };
@@ -409,6 +409,12 @@ __device__ __forceinline__ float log_sum(float m, float l, float scale_log2) {
   return l > 0.f ? fmaf(m, scale_log2, log2f(l) - kLift<T>) * kLn2 : (l == l ? -INFINITY : l);
 }
 
+// Weight of a state in a join.  Where it would end as 0 it stays the smallest
+// normal number, which is as near to it: an infinity of the state stays one.
+__device__ __forceinline__ float join_weight(float m, float top, float scale_log2) {
+  return fmaxf(ex2(excess(m, top) * scale_log2), 1.17549435e-38f);
+}
+
 // Barrier `id` of N softmax threads that tells whether any of them voted.
 template <int N>
 __device__ __forceinline__ bool vote_bar(int id, bool vote) {
@@ -492,7 +498,10 @@ __device__ __forceinline__ void find_run(const Params& p, Bars* bs, int64_t& u0,
 
 // One thread: the segment that holds the run's first unit, for the merge.
 template <int RG>
-__device__ __forceinline__ void write_desc(const Params& p, const Bars* bs, int64_t u0, int64_t U) {
+__device__ __forceinline__ void write_desc(const Params& p, Bars* bs, int64_t u0, int64_t u1,
+                                           int64_t U) {
+  bs->u0 = u0;                             // for restore, which comes last
+  bs->u1 = u1;
   Desc d{};
   d.quot = U / gridDim.x;
   d.rem = (int32_t)(U - d.quot * gridDim.x);
@@ -591,7 +600,7 @@ __device__ __forceinline__ void produce(const Params& p, Bars* bs, unsigned char
 // Cleaner warp: passes every V tile on, cleaned where it reaches behind the
 // context: rows behind the last node and elements that are not finite become
 // zero (a weight of zero would turn them into NaN).  bs->bad[segment] tells
-// whether a node's element was taken out; restore gives it back.
+// whether a node's element was taken out; bad_sum gives it back.
 // `begin` runs at the start of every segment.
 template <typename T, int D, int RG, class Gm, class F>
 __device__ __forceinline__ void clean(const Params& p, Bars* bs, unsigned char* smem,
@@ -671,54 +680,66 @@ __device__ __noinline__ float bad_sum(const Params& p, int r, int t, int ctx, in
   return o;
 }
 
-// The same of the context's positions [a, b), which every row sees; NaN once it
-// is NaN.
+// ---- infinities of the context.  The context is not cleaned, so an infinity of
+// it times a remainder of zero, or of the other sign, makes the output element
+// NaN, where the definition gives the infinity.  Such elements are formed again
+// when the CTA's run is done: calls in the epilogues cost up to 27 % (16 rows of 64
+// columns 97 -> 123 us), calls in the merge 0.7 us of every call.
+
+// Warp: sum of the V elements that are not finite, in column `col`, of the
+// positions in [a, b) that query row t sees.
 template <typename T>
-__device__ __noinline__ float context_sum(const Params& p, int r, int a, int b, int hk, int col) {
+__device__ __noinline__ float seen_sum(const Params& p, int r, int t, int ctx, int a, int b, int hk,
+                                       int col) {
+  const T* v = reinterpret_cast<const T*>(p.v) + hk * p.v_sh + col;
+  const uint8_t* mask = p.mask + (int64_t)t * p.mask_stride;
   float o = 0.f;
-  for (int pos = a; pos < b && o == o;) {
-    const int idx = pos / p.page, row = pos - idx * p.page, n = min(p.page - row, b - pos);
-    const int pg = p.table[(int64_t)r * p.table_stride + idx];
-    pos += n;
-    if ((uint32_t)pg >= (uint32_t)p.n_pages) continue;
-    const T* v = reinterpret_cast<const T*>(p.v) + pg * p.v_sp + hk * p.v_sh + row * p.v_st + col;
 #pragma unroll 1
-    for (int i = 0; i < n; i += 4) {
-      float y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = i + e < n ? Elem<T>::to_f32(v[(i + e) * p.v_st]) : 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (!isfinite(y[e])) o += y[e];
-    }
+  for (int pos = a + (int)(threadIdx.x & 31); pos < b; pos += 32) {
+    const int idx = pos / p.page, row = pos - idx * p.page;
+    const int pg = p.table[(int64_t)r * p.table_stride + idx];
+    if ((uint32_t)pg >= (uint32_t)p.n_pages || (pos >= ctx && !mask[pos - ctx])) continue;
+    const float y = Elem<T>::to_f32(v[pg * p.v_sp + row * p.v_st]);
+    if (!isfinite(y)) o += y;
   }
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) o += __shfl_xor_sync(0xffffffffu, o, d);
   return o;
 }
 
-// Gives a row the non-finite V elements that it sees among positions [a, b):
-// those of nodes, which were cleaned out, and of the context, which is not
-// cleaned, so that an infinity of it times a remainder of zero or of the other
-// sign made the output NaN.  Columns [col, col + n) of query row t, stored at `at`
-// of a part or (part null) of the output.  `context` keeps the context's sum of
-// the last column (kUnknown: not formed yet) for further rows of one column.
-// Rows whose sum of weights is NaN do not come here.
-constexpr float kUnknown = 1.f;            // no sum of non-finite elements
-template <typename T>
-__device__ __noinline__ void restore(const Params& p, int r, int t, int ctx, int a, int b, int hk,
-                                     int col, int n, float* part, int64_t at, float& context) {
-  float* f = part ? part : p.out_f32 ? reinterpret_cast<float*>(p.out) : nullptr;
-  T* h = reinterpret_cast<T*>(p.out);
-  for (int e = 0; e < n; ++e, ++at) {
-    const float x = f ? f[at] : Elem<T>::to_f32(h[at]);
-    float y = bad_sum<T>(p, r, t, ctx, max(a, ctx), b, hk, col + e);
-    if (x == x) y += x;
-    else {
-      if (e > 0 || context == kUnknown) context = context_sum<T>(p, r, a, min(b, ctx), hk, col + e);
-      y += context;
+// Warp `warp` of n: the run's stored elements (of the output or of a part) that
+// are NaN though their row's weights are not become what the non-finite elements
+// that the row sees sum to, if there are any.
+template <typename T, int D, int RG>
+__device__ __noinline__ void restore(const Params& p, const Bars* bs, int warp, int n) {
+  const int lane = threadIdx.x & 31;
+  Walk<RG> walk(p, bs->r0, bs->req0, bs->base0, bs->u0, bs->u1);
+  Seg s;
+  while (walk.next(p, s)) {
+    float* part = p.part + ((int64_t)blockIdx.x * 2 + (s.first ? 0 : 1)) * part_floats<D>(RG);
+    for (int row = warp; row < s.rows; row += n) {
+      const int rq = s.row0 + row, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
+      const int t = walk.q.cu0 + node;
+      const float l = s.whole ? p.lse[(int64_t)t * p.H + hq] : part[RG * D + 2 * row + 1];
+      if (l != l) continue;
+      const int64_t at = (int64_t)t * p.out_st + hq * p.out_sh;
+      float* f = !s.whole ? part + row * D : p.out_f32 ? reinterpret_cast<float*>(p.out) + at : nullptr;
+      T* h = reinterpret_cast<T*>(p.out) + at;
+#pragma unroll 1
+      for (int c = lane; c < D; c += 32) {
+        const float x = f ? f[c] : Elem<T>::to_f32(h[c]);
+        uint32_t lost = __ballot_sync(0xffffffffu, x != x);
+        while (lost) {
+          const int k = __ffs(lost) - 1;
+          lost &= lost - 1;
+          const float y = seen_sum<T>(p, walk.r, t, walk.q.ctx, s.t0 * kBN,
+                                      min(walk.q.end, s.t1 * kBN), s.hk, c - lane + k);
+          if (lane != k || isfinite(y)) continue;
+          if (f) f[c] = y;
+          else h[c] = Elem<T>::from_f32(y);
+        }
+      }
     }
-    if (isfinite(y)) continue;             // nothing of the kind
-    if (f) f[at] = y;
-    else h[at] = Elem<T>::from_f32(y);
   }
 }
 
@@ -785,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       mbar_init(&bs->pv_done[x], 1);
       mbar_init(&bs->mma_done[x], 1);
     }
-    bs->abort_flag = 0;
+    bs->abort_flag = bs->odd = 0;
     fence_mbar_init();
     prefetch_map(&p.kmap);
     prefetch_map(&p.vmap);
@@ -802,7 +823,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   __syncthreads();
   umma::fence_after_sync();
   const uint32_t tmem = bs->tmem_base;
-  if (threadIdx.x == 0) write_desc<RG>(p, bs, u0, U);
+  if (threadIdx.x == 0) write_desc<RG>(p, bs, u0, u1, U);
   grid_dep_trigger();
 
   const uint32_t sQ = smem_addr(smem + Gm::kOffQ);
@@ -1094,13 +1115,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       named_bar_sync(1, 512);
       const bool fix = *reinterpret_cast<volatile int*>(&bs->bad[si % kBadSlots]) != 0;
       float* part = p.part + ((int64_t)blockIdx.x * 2 + (s.first ? 0 : 1)) * part_floats<D>(RG);
-      bool sound = false;                  // the row's weights are no NaN
-      float odd = fix ? NAN : 0.f;         // NaN if any element is not finite
+      auto bad = [&](int row, int col) {
+        return bad_sum<T>(p, walk.r, cu0 + (s.row0 + row) / p.G, ctx, max(ctx, s.t0 * kBN),
+                          min(end, s.t1 * kBN), s.hk, col);
+      };
+      float odd = 0.f;                     // NaN if any element is not finite
       // N columns from col of a row of the group: o scaled by 1 / L, or as it
       // is to the workspace
       auto store = [&](int row, int col, float M, float L, auto& o) {
         constexpr int N = sizeof(o) / sizeof(float);
-        sound = L == L;
+        if (fix)
+          for (int e = 0; e < N; ++e) o[e] += bad(row, col + e);
 #pragma unroll
         for (int e = 0; e < N; ++e) odd = fmaf(o[e], 0.f, odd);
         if (!s.whole) {
@@ -1113,7 +1138,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         const int rq = s.row0 + row, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
         const int64_t t = cu0 + node;
         const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
-        if (col == 0 && p.lse)
+        if (col == 0)
           p.lse[t * p.H + hq] = log_sum<T>(M, L, p.scale_log2);
         const int64_t at = t * p.out_st + hq * p.out_sh + col;
         if (p.out_f32) {
@@ -1149,7 +1174,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         const float m0 = sm_m[r], m1 = n1 > 0 ? sm_m[128 + r] : kNoMax;
         const float l0 = sm_l[r] + sm_l[128 + r], l1 = n1 > 0 ? sm_l[256 + r] + sm_l[384 + r] : 0.f;
         const float M = fmaxf(m0, m1);
-        const float w0 = ex2(excess(m0, M) * p.scale_log2), w1 = ex2(excess(m1, M) * p.scale_log2);
+        const float w0 = join_weight(m0, M, p.scale_log2), w1 = join_weight(m1, M, p.scale_log2);
         const float L = fmaf(l1, w1, l0 * w0);
         const int col = (x * 2 + h) * (D / 4);
 #pragma unroll 1
@@ -1163,19 +1188,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           if (r < rows && ok) store(r, col + c, M, L, a);
         }
       }
-      if (__builtin_expect(odd != odd && sound, 0)) {
-        const int row = r + (two ? x * 128 : 0), n = two ? D / 2 : D / 4;
-        const int col = (two ? h : x * 2 + h) * n;
-        const int rq = s.row0 + row, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
-        float context = kUnknown;
-        restore<T>(p, walk.r, cu0 + node, ctx, s.t0 * kBN, min(end, s.t1 * kBN), s.hk, col, n,
-                   s.whole ? nullptr : part,
-                   s.whole ? (int64_t)(cu0 + node) * p.out_st + hq * p.out_sh + col
-                           : (int64_t)row * D + col, context);
-      }
+      if (odd != odd) bs->odd = 1;
       umma::fence_before_sync();
       ++si;
     }
+    named_bar_sync(1, 512);
+    if (bs->odd) restore<T, D, RG>(p, bs, warp - 4, 16);
   }
   }
 
@@ -1279,7 +1297,7 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
     mbar_init(&bs->pv_done[1], 1);
     mbar_init(&bs->mma_done[0], 1);
     mbar_init(&bs->mma_done[1], 1);
-    bs->abort_flag = 0;
+    bs->abort_flag = bs->odd = 0;
     fence_mbar_init();
     prefetch_map(&p.kmap);
     prefetch_map(&p.vmap);
@@ -1295,7 +1313,7 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
   __syncthreads();
   umma::fence_after_sync();
   const uint32_t tmem = bs->tmem_base;
-  if (threadIdx.x == 64) write_desc<RG>(p, bs, u0, U);
+  if (threadIdx.x == 64) write_desc<RG>(p, bs, u0, u1, U);
   grid_dep_trigger();
 
   const uint32_t sQ = smem_addr(smem + Gm::kOffQ);
@@ -1610,13 +1628,12 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
           const float M = sh->m[r];
           if (!s.whole) {
             *reinterpret_cast<float2*>(part + RG * D + 2 * r) = make_float2(M, L);
-            sh->fac[r] = L == L ? 1.f : L;
+            sh->fac[r] = 1.f;
             sh->off[r] = r * D;
           } else {
             const int rq = s.row0 + r, node = rq / p.G, hq = s.hk * p.G + rq - node * p.G;
             const int64_t row = walk.q.cu0 + node;
-            if (p.lse)
-              p.lse[row * p.H + hq] = log_sum<T>(M, L, p.scale_log2);
+            p.lse[row * p.H + hq] = log_sum<T>(M, L, p.scale_log2);
             sh->fac[r] = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
             sh->off[r] = row * p.out_st + hq * p.out_sh;
           }
@@ -1624,7 +1641,7 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
         named_bar_sync(bar, 128);
         const bool fix = *reinterpret_cast<volatile int*>(&bs->bad[si % kBadSlots]) != 0;
         float* of = !s.whole ? part : p.out_f32 ? reinterpret_cast<float*>(p.out) : nullptr;
-        float odd = fix ? NAN : 0.f;       // NaN if any element is not finite
+        float odd = 0.f;                   // NaN if any element is not finite
 #pragma unroll 1
         for (int c = r0; c < min(r0 + RT, s.rows); c += 8) {
           float a[8], b[8];
@@ -1640,10 +1657,16 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
           umma::tmem_wait_ld();
           if (tid >= D || !ok) continue;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            a[e] += b[e];
-            odd = fmaf(a[e], 0.f, odd);
+          for (int e = 0; e < 8; ++e) a[e] += b[e];
+          if (fix) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (c + e < s.rows)
+                a[e] += bad_sum<T>(p, walk.r, walk.q.cu0 + (s.row0 + c + e) / p.G, ctx,
+                                   max(ctx, s.t0 * kBN), min(end, s.t1 * kBN), s.hk, tid);
           }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) odd = fmaf(a[e], 0.f, odd);
           if (of) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -1655,18 +1678,12 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
                 reinterpret_cast<T*>(p.out)[off[e]] = Elem<T>::from_f32(a[e] * fac[e]);
           }
         }
-        if (__builtin_expect(odd != odd && tid < D && ok, 0)) {
-          float context = kUnknown;
-#pragma unroll 1
-          for (int r = r0; r < min(r0 + RT, s.rows); ++r)
-            if (sh->fac[r] == sh->fac[r])
-              restore<T>(p, walk.r, walk.q.cu0 + (s.row0 + r) / p.G, ctx, s.t0 * kBN,
-                         min(end, s.t1 * kBN), s.hk, tid, 1, s.whole ? nullptr : part,
-                         sh->off[r] + tid, context);
-        }
+        if (odd != odd) bs->odd = 1;
         umma::fence_before_sync();
         ++si;
       }
+      named_bar_sync(1 + Gm::kGroups, Gm::kSoft);
+      if (bs->odd) restore<T, D, NR>(p, bs, warp - 4, Gm::kSoft / 32);
     }
   }
 
@@ -1708,12 +1725,6 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
   const int own = cut(c);
   if (own <= 0 || own >= d.nt || cut(c - 1) > 0) return;
   const int64_t before = (c - 1) * d.quot + (uint32_t)((c - 1) * d.rem) / (uint32_t)n_cta;
-  // CTA i's part of the segment.  CTA c - 1 may have begun before the segment's
-  // set-up units: then this is its second part.
-  auto part = [&](int i) {
-    const int sl = i == c - 1 && before < d.start - (RG <= 64 ? kSetup<64> : kSetup<128>) ? 1 : 0;
-    return p.part + ((int64_t)i * 2 + sl) * part_floats<D>(RG);
-  };
   for (; row < d.rows; row += (int)gridDim.y * kMergeWarps) {
     float M = -INFINITY, L = 0.f, acc[C];
 #pragma unroll
@@ -1733,7 +1744,10 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
           if (has) {
             const int i = i0 + __ffs(has) - 1;
             has &= has - 1;
-            const float* s = part(i);
+            // CTA c - 1 may have begun before the segment's set-up units: then
+            // this is its second part
+            const int sl = i == c - 1 && before < d.start - (RG <= 64 ? kSetup<64> : kSetup<128>) ? 1 : 0;
+            const float* s = p.part + ((int64_t)i * 2 + sl) * part_floats<D>(RG);
             ml[u] = *reinterpret_cast<const float2*>(s + RG * D + 2 * row);
             s += row * D;
             if constexpr (C == 4) {
@@ -1754,13 +1768,13 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
         for (int u = 0; u < B; ++u) Mn = fmaxf(Mn, ml[u].x);
         // a part that saw nothing or only NaN joins right with any weight (l and
         // o are 0, or l is NaN), and Mn is at least kNoMax
-        const float a0 = ex2(excess(M, Mn) * p.scale_log2);
+        const float a0 = join_weight(M, Mn, p.scale_log2);
         L *= a0;
 #pragma unroll
         for (int e = 0; e < C; ++e) acc[e] *= a0;
 #pragma unroll
         for (int u = 0; u < B; ++u) {
-          const float w = ex2(excess(ml[u].x, Mn) * p.scale_log2);
+          const float w = join_weight(ml[u].x, Mn, p.scale_log2);
           L = fmaf(ml[u].y, w, L);
 #pragma unroll
           for (int e = 0; e < C; ++e) acc[e] = fmaf(o[u][e], w, acc[e]);
@@ -1768,29 +1782,10 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(
         M = Mn;
       }
     }
-    // an infinity whose part's weight ended as 0 came out NaN: the infinities
-    // of the parts again
-    float odd = 0.f;
-#pragma unroll
-    for (int e = 0; e < C; ++e) odd = fmaf(acc[e], 0.f, odd);
-    if (__builtin_expect(odd != odd && L == L, 0)) {
-      float y[C];
-#pragma unroll
-      for (int e = 0; e < C; ++e) y[e] = 0.f;
-      for (int i = c - 1; i < n_cta && cut(i) < d.nt; ++i) {
-        if (cut(i) >= cut(i + 1)) continue;
-        const float* s = part(i) + row * D + lane * C;
-#pragma unroll
-        for (int e = 0; e < C; ++e) y[e] += isfinite(s[e]) ? 0.f : s[e];
-      }
-#pragma unroll
-      for (int e = 0; e < C; ++e) acc[e] = acc[e] == acc[e] || y[e] == 0.f ? acc[e] : y[e];
-    }
     const int rq = d.row0 + row, node = rq / p.G, hq = d.hk * p.G + rq - node * p.G;
     const int64_t t = d.cu0 + node;
     const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
-    if (lane == 0 && p.lse)
-      p.lse[t * p.H + hq] = log_sum<T>(M, L, p.scale_log2);
+    if (lane == 0) p.lse[t * p.H + hq] = log_sum<T>(M, L, p.scale_log2);
     const int64_t at = t * p.out_st + hq * p.out_sh + lane * C;
     if (p.out_f32) {
       float* o = reinterpret_cast<float*>(p.out) + at;
@@ -1916,9 +1911,14 @@ static int group_rows(const halo_page_pool_t* pool, const halo_tree_problem_t* p
 
 static int64_t desc_bytes(int n_cta) { return ((int64_t)n_cta * sizeof(Desc) + 255) & ~int64_t(255); }
 
+static int64_t part_bytes(const halo_page_pool_t* pool, const halo_tree_problem_t* pb, int n_cta) {
+  return (int64_t)n_cta * 2 * group_rows(pool, pb) * (pool->D + 2) * sizeof(float);
+}
+
 static int64_t ws_bytes(const halo_page_pool_t* pool, const halo_tree_problem_t* pb) {
   const int n = device_sms();
-  return desc_bytes(n) + (int64_t)n * 2 * group_rows(pool, pb) * (pool->D + 2) * sizeof(float);
+  return desc_bytes(n) + part_bytes(pool, pb, n) +
+         (pb->lse ? 0 : (int64_t)pb->T * pb->H * sizeof(float));
 }
 
 template <typename T, int D, int RG, bool PAIR>
@@ -2040,7 +2040,6 @@ static int run(const halo_page_pool_t* pool, const halo_tree_problem_t* pb, void
   p.out = static_cast<char*>(pb->out);
   p.out_st = pb->out_stride_t;
   p.out_sh = pb->out_stride_h;
-  p.lse = pb->lse;
   p.scale_log2 = pb->scale * kLog2e;
   p.headroom = raw_headroom(p.scale_log2);
   p.out_f32 = pb->out_dtype == HALO_DTYPE_F32;
@@ -2054,8 +2053,11 @@ static int run(const halo_page_pool_t* pool, const halo_tree_problem_t* pb, void
   p.n_pages = pool->n_pages;
   p.page = pool->page_size;
   const int n_cta = device_sms();
-  p.desc = static_cast<Desc*>(workspace);
-  p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + desc_bytes(n_cta));
+  char* ws = static_cast<char*>(workspace);
+  p.desc = reinterpret_cast<Desc*>(ws);
+  p.part = reinterpret_cast<float*>(ws + desc_bytes(n_cta));
+  p.lse = pb->lse ? pb->lse
+                  : reinterpret_cast<float*>(ws + desc_bytes(n_cta) + part_bytes(pool, pb, n_cta));
   p.err = device_error_ptr();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto typed = [&](auto tag) {

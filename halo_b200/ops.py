@@ -792,12 +792,13 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                                node_starts.data_ptr() if node_starts is not None else 0)
     lib, stream = L.lib(), L.stream_handle_of(index)
     key = (index, D, H_kv, H, max_nodes, R > 0 and T > 0)
-    need = _TREE_BYTES.get(key)
+    need = _TREE_BYTES.get(key) if lse is not None else None
     if need is None:
         need = int(lib.halo_tree_workspace_bytes(pool, prob))
         if need < 0:
             L.check(need, "halo_tree_workspace_bytes")
-        _TREE_BYTES[key] = need
+        if lse is not None:            # one that is not asked for is kept there, of T rows
+            _TREE_BYTES[key] = need
     ws = _tree_workspace(index, stream, need) if need else None
     rc = lib.halo_tree_attention(pool, prob, ws.data_ptr() if need else None, need, stream)
     if rc:

@@ -523,7 +523,7 @@ typedef struct halo_tree_problem {
 
 /* Bytes of workspace for halo_tree_attention (256-byte aligned; no
  * initialisation, overwritten by the call; one call in flight per
- * workspace).  Negative status on bad arguments. */
+ * workspace), T * H floats more where lse is NULL.  Negative status on bad arguments. */
 int64_t halo_tree_workspace_bytes(const halo_page_pool_t* pool,
                                   const halo_tree_problem_t* problem);
 

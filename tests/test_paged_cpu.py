@@ -275,3 +275,14 @@ def test_the_largest_tables_are_not_refused():
     for kw in ({"max_requests": 8192, "max_len": 64}, {"max_requests": 1, "max_len": 2 ** 31 - 129},
                {"max_requests": 2, "max_len": 64, "dtype": torch.float32, "page_size": 5}):
         PagedKVCache(1, 2, 1, 8, device="cpu", **kw)
+
+
+def test_workspace_holds_a_log_sum_exp_that_is_not_asked_for():
+    from halo_b200 import _lib as L
+    lib = L.lib()
+    po = _pool(L)
+    need = lib.halo_tree_workspace_bytes(ctypes.byref(po), ctypes.byref(_tree(L)))
+    more = lib.halo_tree_workspace_bytes(ctypes.byref(po), ctypes.byref(_tree(L, lse=None)))
+    assert more == need + 8 * 8 * 4
+    assert lib.halo_tree_attention(ctypes.byref(po), ctypes.byref(_tree(L, lse=None)), 0x100000,
+                                   more - 1, None) == L.HALO_ERR_WORKSPACE

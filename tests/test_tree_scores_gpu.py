@@ -232,3 +232,37 @@ def test_infinities_everywhere(cuda_device, nodes):
     c.v[c.table[0][::3]] = math.inf
     out, lse = c.run(out_dtype=torch.float32)
     assert (out == math.inf).all() and torch.isfinite(lse).all() and L.device_error() == 0
+
+
+@pytest.mark.parametrize("nodes", [1, 6, 16, 33])
+@pytest.mark.parametrize("want_lse", [True, False])
+def test_infinities_of_many_requests(cuda_device, nodes, want_lse):
+    """Segments that one CTA finishes by itself, every third request with
+    infinities in some columns and every seventh with K that is NaN as well."""
+    R, D, page = 330, 64, 16
+    rng = np.random.default_rng(nodes)
+    ctx = [int(x) for x in rng.integers(1, 500, R)]
+    c = Case(nodes, ctx, [nodes if r % 5 else 1 for r in range(R)], 4, 1, D, page, torch.bfloat16)
+    keep_v, keep_k = c.v.clone(), c.k.clone()
+    bad, dead = list(range(0, R, 3)), list(range(0, R, 21))
+    for r in bad:
+        pos = int(rng.integers(0, ctx[r]))
+        c.v[c.table[r][pos // page], 0, pos % page, 7] = math.inf
+        c.v[c.table[r][0], 0, 0, 8] = -math.inf
+    for r in dead:
+        c.k[c.table[r][0], 0, 0, 3] = math.nan
+    out, lse = c.run(out_dtype=torch.float32, want_lse=want_lse)
+    assert (lse is not None) == want_lse
+    out = out.cpu()
+    for r in bad:
+        rows = slice(c.cu[r], c.cu[r + 1])
+        if r in dead:
+            assert torch.isnan(out[rows]).all() and (lse is None or torch.isnan(lse[rows]).all())
+        else:
+            assert (out[rows, :, 7] == math.inf).all() and (out[rows, :, 8] == -math.inf).all()
+        out[rows, :, 7:9] = 0
+        # its own pages: entries behind them name other requests' pages
+        keep_v[c.table[r][:-(-(ctx[r] + c.cu[r + 1] - c.cu[r]) // page)], :, :, 7:9] = 0
+    c.v, c.k = keep_v, keep_k
+    rows = [t for r in range(R) if r not in dead for t in range(c.cu[r], c.cu[r + 1])]
+    c.check(out, lse if want_lse else c.run()[1], rows=rows)
