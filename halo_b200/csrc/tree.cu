@@ -477,6 +477,10 @@ __device__ __forceinline__ void find_run(const Params& p, Bars* bs, int64_t& u0,
     u0 = (int64_t)blockIdx.x * U / gridDim.x;
     u1 = (int64_t)(blockIdx.x + 1) * U / gridDim.x;
   }
+  if (threadIdx.x == 0) {              // for restore, which comes last
+    bs->u0 = u0;
+    bs->u1 = u1;
+  }
   {
     int64_t before = 0;
     for (int r0 = 0; r0 < p.R; r0 += NT) {
@@ -498,10 +502,7 @@ __device__ __forceinline__ void find_run(const Params& p, Bars* bs, int64_t& u0,
 
 // One thread: the segment that holds the run's first unit, for the merge.
 template <int RG>
-__device__ __forceinline__ void write_desc(const Params& p, Bars* bs, int64_t u0, int64_t u1,
-                                           int64_t U) {
-  bs->u0 = u0;                             // for restore, which comes last
-  bs->u1 = u1;
+__device__ __forceinline__ void write_desc(const Params& p, const Bars* bs, int64_t u0, int64_t U) {
   Desc d{};
   d.quot = U / gridDim.x;
   d.rem = (int32_t)(U - d.quot * gridDim.x);
@@ -823,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   __syncthreads();
   umma::fence_after_sync();
   const uint32_t tmem = bs->tmem_base;
-  if (threadIdx.x == 0) write_desc<RG>(p, bs, u0, u1, U);
+  if (threadIdx.x == 0) write_desc<RG>(p, bs, u0, U);
   grid_dep_trigger();
 
   const uint32_t sQ = smem_addr(smem + Gm::kOffQ);
@@ -1313,7 +1314,7 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
   __syncthreads();
   umma::fence_after_sync();
   const uint32_t tmem = bs->tmem_base;
-  if (threadIdx.x == 64) write_desc<RG>(p, bs, u0, u1, U);
+  if (threadIdx.x == 64) write_desc<RG>(p, bs, u0, U);
   grid_dep_trigger();
 
   const uint32_t sQ = smem_addr(smem + Gm::kOffQ);
@@ -1447,7 +1448,7 @@ __global__ void __launch_bounds__(FewGeom<D, NR, PAIR>::kThreads, 1)
       };
       while (walk.next(p, s)) {
         const int ctx = walk.q.ctx, end = walk.q.end;
-        if (si == 0) {                     // later ones come from warp 3, ahead
+        if (si == 0) {                     // later ones come from warp 2, ahead
           copy_q(walk, s, threadIdx.x - 128, Gm::kSoft, 0);
           asm volatile("cp.async.wait_all;" ::: "memory");
           fence_proxy_async_smem();
