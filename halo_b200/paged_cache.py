@@ -71,8 +71,11 @@ class PagedKVCache:
 
     def extend(self, counts: torch.Tensor, max_tokens: int) -> PagedRows:
         """Begin a step: room for ``counts[r]`` (int32, at most ``max_tokens`` in
-        all) rows behind each request's context.  A step that was begun before
-        and not accepted is given up: its rows are room again."""
+        all; a single count is every request's) rows behind each request's
+        context.  A step that was begun before and not accepted is given up:
+        its rows are room again."""
+        if counts.numel() == 1:
+            counts = counts.expand(self.lens.shape)
         return PagedRows(*ops.extend_block_tables(
             self.block_tables, self.held, self.lens, counts.contiguous(), self.step, self.starts,
             self.free_pages, self.n_free, page_size=self.page_size, max_tokens=max_tokens))

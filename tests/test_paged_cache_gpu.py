@@ -183,3 +183,21 @@ def test_accept_of_nodes_that_are_not_of_the_step(cuda_device, node):
     cache.write(0, y, y, got)
     cache.accept(_i32([[2, node, 0], [0, 0, 0]]), _i32([2, 0]))
     assert _rows_of(cache, 0) == [1.] * 10 + [4., 5., 6., 6., 5.]
+
+
+def test_extend_by_one_count_for_all(cuda_device):
+    for one in (torch.tensor(3, dtype=torch.int32, device=DEV), _i32([3])):
+        cache = _small_cache(8)
+        got = cache.extend(one, 6)
+        assert got.cu.tolist() == [0, 3, 6] and got.positions.tolist() == [10, 11, 12, 6, 7, 8]
+
+
+def test_extend_refuses_other_counts(cuda_device):
+    from halo_b200._lib import HaloError
+    cache = _small_cache(8)
+    for bad in (_i32([1, 2, 3]), torch.tensor([1, 2], device=DEV), torch.tensor([1, 2], dtype=torch.int32)):
+        with pytest.raises(HaloError):
+            cache.extend(bad, 6)
+    with pytest.raises(HaloError):
+        cache.extend(_i32([1, 2]), -1)
+    assert cache.extend(_i32([1, 0, 2, 0])[::2], 3).cu.tolist() == [0, 1, 3]
