@@ -1193,6 +1193,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       umma::fence_before_sync();
       ++si;
     }
+    // by these warps alone: the others gave registers away that the call may use
     named_bar_sync(1, 512);
     if (bs->odd) restore<T, D, RG>(p, bs, warp - 4, 16);
   }
@@ -1239,8 +1240,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
 // SM, 4 before the first, 3 for an epilogue, 4 for a second segment, 4 for the
 // merge and the launch.  One softmax group of all rows: 248; parts in rows of
 // 528 bytes: 225.  At 64 columns a tile's bytes take 1.4k clocks, the chain of
-// its softmax more: 8 requests on 32768 positions (82 us of bytes) take 97 us
-// with 16 rows, 119 with 32, 154 to 160 with 64.  Small batches are latency: 10 us
+// its softmax more: 8 requests on 32768 positions (82 us of bytes) take 99 us
+// with 16 rows, 120 with 32, 145 to 154 with 64.  Small batches are latency: 10 us
 // for one token on 1000 positions (find the run 1.1, first rows and tables 1.5,
 // first tile 1.5, softmax and PV 1.9, epilogue 1.1, merge 3).
 

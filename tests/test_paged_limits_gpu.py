@@ -96,3 +96,68 @@ def test_a_table_row_of_a_million_positions(cuda_device):
             old = lens
         used = [p for r, x in enumerate(old.tolist()) for p in tab[r, :-(-x // page)].tolist()]
         assert sorted(used + free[:int(n_free)].tolist()) == list(range(n))
+
+
+@pytest.mark.parametrize("nodes", [[3, 0, 5, 1], [40, 2, 0, 33]])
+@pytest.mark.parametrize("captured", [False, True])
+def test_rows_that_begin_elsewhere(cuda_device, nodes, captured):
+    """node_starts: requests' rows in another order and with gaps between them;
+    cu_nodes then only counts them."""
+    from halo_b200 import ops
+    c = Case(sum(nodes), [300, 40, 9, 2000], nodes, 8, 2, 64, 16, torch.bfloat16)
+    T, starts = c.cu[-1], [0] * 4
+    at = 2
+    for r in (2, 0, 3, 1):
+        starts[r] = at
+        at += nodes[r] + 3
+    rows = [starts[r] + i for r in range(4) for i in range(nodes[r])]
+    q = torch.full((at, 8, 64), float("nan"), dtype=torch.bfloat16)
+    mask = torch.ones(at, c.mask.shape[1], dtype=torch.bool)
+    q[rows], mask[rows] = c.q, c.mask
+    out = torch.full((at, 8, 64), 7.0, device=DEV)
+    lse = torch.full((at, 8), 7.0, device=DEV)
+    args = (q.to(DEV), c.k.to(DEV), c.v.to(DEV), _i32(c.table), _i32(c.ctx), _i32(c.cu),
+            mask.to(DEV))
+    st = _i32(starts)
+    if captured:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ops.tree_attention(*args, out=out, lse=lse, node_starts=st)
+            other, none = ops.tree_attention(*args, out_dtype=torch.float32, node_starts=st,
+                                             want_lse=False)
+        g.replay()
+        assert none is None and torch.equal(other[rows], out[rows])
+    else:
+        ops.tree_attention(*args, out=out, lse=lse, node_starts=st)
+    c.check(out[rows], lse[rows])
+    rest = [t for t in range(at) if t not in rows]
+    assert (out[rest] == 7).all() and (lse[rest] == 7).all()
+    assert T == len(rows)
+
+
+def test_node_starts_that_do_not_fit_are_refused(cuda_device):
+    from halo_b200 import ops
+    from halo_b200._lib import HaloError
+    c = Case(2, [30, 5], [2, 2], 2, 1, 64, 8, torch.float16)
+    args = (c.q.to(DEV), c.k.to(DEV), c.v.to(DEV), _i32(c.table), _i32(c.ctx), _i32(c.cu),
+            c.mask.to(DEV))
+    ops.tree_attention(*args, node_starts=_i32([0, 2]))
+    for bad in (_i32([0]), _i32([0, 2, 4]), torch.tensor([0, 2], device=DEV), _i32([0, 2]).cpu(),
+                _i32([0, 0, 2, 0])[::2]):
+        with pytest.raises(HaloError):
+            ops.tree_attention(*args, node_starts=bad)
+    # rows that would leave the tensors are not there
+    out = torch.full((4, 2, 64), 7.0, dtype=torch.float16, device=DEV)
+    lse = torch.full((4, 2), 7.0, device=DEV)
+    ops.tree_attention(*args, node_starts=_i32([2, 2 ** 31 - 1]), out=out, lse=lse)
+    assert (out[:2] == 7).all() and (lse[:2] == 7).all() and torch.isfinite(out).all()
+
+
+def test_extend_of_no_requests(cuda_device):
+    from halo_b200 import ops
+    e, n = _i32([]), _i32([2])
+    slots, pos, cu = ops.extend_block_tables(torch.empty(0, 4, dtype=I32, device=DEV), e, e, e,
+                                             torch.empty_like(e), torch.empty_like(e), _i32([4, 5]), n,
+                                             page_size=16, max_tokens=3)
+    assert slots.tolist() == [-1] * 3 and pos.tolist() == [-1] * 3 and cu.tolist() == [0]
+    assert n.tolist() == [2]
