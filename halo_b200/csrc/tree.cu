@@ -763,7 +763,8 @@ __device__ __noinline__ void restore(const Params& p, const Bars* bs, int warp, 
 // overwrites P_X follows the PV that reads it without waiting for its end.
 // P is split into a 16-bit value and a 16-bit remainder (two MMAs), ~16
 // significant bits (fp16: down to 2^-32 of a row's largest, see kLift): one
-// 16-bit P would cost up to 2^-9 |v|, as much as the output's own rounding.  Sums, maxima and O are fp32.
+// 16-bit P would cost up to 2^-9 |v|, as much as the output's own rounding.
+// Sums, maxima and O are fp32.
 //
 // Row groups of more than 128 rows (QT = 2): stream X takes query tile X and
 // both take every K/V tile.  Smaller ones: both streams share the query tile

@@ -201,3 +201,63 @@ def test_extend_refuses_other_counts(cuda_device):
     with pytest.raises(HaloError):
         cache.extend(_i32([1, 2]), -1)
     assert cache.extend(_i32([1, 0, 2, 0])[::2], 3).cu.tolist() == [0, 1, 3]
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_any_order_of_calls(cuda_device, seed):
+    """Steps begun, given up, refused, accepted by any path and requests ended,
+    at random: every row and every page against a list of rows a request."""
+    from halo_b200 import PagedKVCache
+    rng = np.random.default_rng(seed)
+    R, page, n_pages, top = 5, (1, 4, 8, 7)[seed], (60, 20, 9, 12)[seed], 40
+    cache = PagedKVCache(1, n_pages, 1, 8, max_requests=R, max_len=top, page_size=page,
+                         dtype=torch.float32, device=DEV)
+    kept, step, mark = [[] for _ in range(R)], None, 0
+    refused = 0
+    for _ in range(120):
+        what = rng.random()
+        if what < 0.5 or step is None:
+            counts = [int(x) for x in rng.integers(-1, (3, 12, 45)[int(rng.integers(3))], R)]
+            T = sum(max(c, 0) for c in counts) + int(rng.integers(0, 3))
+            rows = cache.extend(_i32(counts), T)
+            got = (rows.cu[1:] - rows.cu[:-1]).tolist()
+            assert all(g in (0, max(c, 0)) for g, c in zip(got, counts))
+            assert all(len(k) + g <= -(-top // page) * page for k, g in zip(kept, got))
+            refused += sum(g == 0 < c for g, c in zip(got, counts))
+            k = torch.arange(mark, mark + T, device=DEV, dtype=torch.float32)[:, None, None]
+            cache.write(0, k.expand(T, 1, 8), -k.expand(T, 1, 8), rows)
+            step, at = [], 0
+            for c, g in zip(counts, got):
+                step.append([mark + at + i for i in range(g)])
+                at += max(c, 0)
+            mark += T
+        elif what < 0.85:
+            depth = int(rng.integers(1, 14))
+            lens = [int(x) for x in rng.integers(-1, depth + 3, R)]
+            path = None
+            if rng.random() < 0.7:
+                path = rng.integers(-2, 20, (R, depth))
+                if rng.random() < 0.6:
+                    path = np.sort(path, 1)
+            for r in range(R):
+                n = min(max(lens[r], 0), len(step[r]), 10 ** 9 if path is None else depth)
+                p = list(range(n)) if path is None else path[r, :n].tolist()
+                kept[r] += [step[r][x if i < x < len(step[r]) else i] for i, x in enumerate(p)]
+            cache.accept(None if path is None else _i32(path.tolist()), _i32(lens))
+            step = None
+        else:
+            ended = rng.random(R) < 0.3
+            cache.release(torch.from_numpy(ended).to(DEV))
+            for r in np.nonzero(ended)[0]:
+                kept[r], step[r] = [], []
+        assert cache.lens.tolist() == [len(x) for x in kept]
+        held = [len(x) + (len(step[r]) if step else 0) for r, x in enumerate(kept)]
+        assert all(h >= n for h, n in zip(cache.held.tolist(), held))
+        assert _owners(cache) == list(range(n_pages))
+        for r in range(R):
+            want = kept[r] + (step[r] if step else [])
+            pages = cache.block_tables[r, :-(-len(want) // page)].long()
+            for x, sign in ((cache.k[0], 1.0), (cache.v[0], -1.0)):
+                rows_r = x[pages].transpose(1, 2).reshape(-1, 8)[:len(want)]
+                assert (rows_r * sign == torch.tensor(want, device=DEV)[:, None]).all()
+    assert refused > 0 and mark > 500
